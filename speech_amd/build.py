@@ -15,7 +15,9 @@ LIB = os.path.join(HERE, "libspeech_hip.so")
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
-         "-fno-gpu-sanitize"]
+         "-fno-gpu-sanitize",
+         # no packed FP32 instructions: some of their operand forms have returned wrong values on this hardware
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
@@ -41,8 +43,10 @@ def _compile(src):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src}:\n{r.stdout}\n{r.stderr}")
-    if r.stderr.strip():
-        sys.stderr.write(r.stderr)
+    # (the host pass does not know the device feature named in FLAGS and says so)
+    err = "\n".join(l for l in r.stderr.splitlines() if "packed-fp32-ops" not in l).strip()
+    if err:
+        sys.stderr.write(err + "\n")
     return obj
 
 

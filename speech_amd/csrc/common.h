@@ -31,6 +31,13 @@ inline int check_launch(const char* what) {
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+// f32 -> f16 as a rounding of its own.  Without the barrier the compiler may fold the conversion into the multiplication before it
+// (v_fma_mixlo_f16: the exact product rounded once), and an f16 output is then no longer the f32 output rounded.
+__device__ __forceinline__ __half f32_to_f16(float v) {
+    asm("" : "+v"(v));
+    return __float2half(v);
+}
+
 // ---- activation element types -------------------------------------------------------
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -48,7 +55,7 @@ template <> struct Elem<__hip_bfloat16> {
 template <> struct Elem<__half> {
     static __device__ __forceinline__ float f(__half v) { return __half2float(v); }
     static __device__ __forceinline__ float ld(const __half* p) { return __half2float(*p); }
-    static __device__ __forceinline__ void st(__half* p, float v) { *p = __float2half(v); }
+    static __device__ __forceinline__ void st(__half* p, float v) { *p = f32_to_f16(v); }
 };
 
 // ---- wave-level primitives (64 lanes) -----------------------------------------------

@@ -626,10 +626,10 @@ __device__ __forceinline__ void store4(__hip_bfloat16* g, int c, float a, float 
 
 __device__ __forceinline__ void store4(__half* g, int c, float a, float b, float x, float y) {
     uint2 o;
-    o.x = (uint32_t)__builtin_bit_cast(unsigned short, __float2half(a)) |
-          ((uint32_t)__builtin_bit_cast(unsigned short, __float2half(b)) << 16);
-    o.y = (uint32_t)__builtin_bit_cast(unsigned short, __float2half(x)) |
-          ((uint32_t)__builtin_bit_cast(unsigned short, __float2half(y)) << 16);
+    o.x = (uint32_t)__builtin_bit_cast(unsigned short, f32_to_f16(a)) |
+          ((uint32_t)__builtin_bit_cast(unsigned short, f32_to_f16(b)) << 16);
+    o.y = (uint32_t)__builtin_bit_cast(unsigned short, f32_to_f16(x)) |
+          ((uint32_t)__builtin_bit_cast(unsigned short, f32_to_f16(y)) << 16);
     reinterpret_cast<uint2*>(g)[c] = o;
 }
 

@@ -15,8 +15,7 @@
 //            frames per tile, only over the 4-bin blocks where the tile's filters are non-zero; the five tiles
 //            are dealt to the pair's two waves by block count
 //   phase 5  masked / padded store, [B][80][T_max], 64 bytes per mel row and tile
-// Complex arithmetic is packed (one v_pk_*_f32 per butterfly, see below): at three waves per SIMD the kernel
-// pays per instruction issued, not per flop.
+// At three waves per SIMD the kernel pays per instruction issued, not per flop.
 // HBM traffic: every sample is read once from HBM (neighbouring waves' 240-sample overlap comes from L2),
 // every output element written once.  LDS: 12.9 KB per wave (samples, intermediates and magnitudes alias),
 // 3 blocks per CU.
@@ -77,40 +76,22 @@ constexpr int kWaveLdsBytes = kF * kZStride * 8 + 64;   // + 16 banks: the pair'
 static_assert(2 * kZStride * 8 >= (kHop + kNfft) * 4, "pass 1 writes above the samples pass 0 still needs");
 static_assert(kWaveLdsBytes % 16 == 0, "16-byte staging stores");
 
-// ---- packed complex arithmetic ------------------------------------------------------------------------
-// A complex number is a register pair (re, im) and every butterfly is ONE v_pk_*_f32: a wave issues an
-// instruction every ~5 cycles whatever it is (tools/ubench/valu_tput.hip), so at the three waves per SIMD the
-// LDS footprint allows, the instruction count, not the flop count, is what the transform costs.  The compiler
-// packs plain adds and scalar multiples by itself; multiplications by +-i and conjugations need the
-// op_sel / neg modifiers, which it does not fold (it emits v_xor + v_mov), hence the asm helpers.  The scalar
-// forms of the same transforms live in mel_math.h (host replay: tests/host/mel_emulate.cpp).
+// ---- complex arithmetic -------------------------------------------------------------------------------
+// A complex number is a register pair (re, im).  The library is compiled without packed FP32 instructions (some of
+// their operand-select forms have returned wrong values on this hardware), so these are plain scalar operations; the
+// products are written as mul + fma so that every host and device build rounds them alike.  The same transforms for
+// the host live in mel_math.h (host replay: tests/host/mel_emulate.cpp).
 using c2 = f32x2;
-#define SP_PK2(name, text)                                        \
-    __device__ __forceinline__ c2 name(c2 a, c2 b) {              \
-        c2 d;                                                     \
-        asm(text : "=v"(d) : "v"(a), "v"(b));                     \
-        return d;                                                 \
-    }
-SP_PK2(add_mi, "v_pk_add_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[1,0] neg_hi:[0,1]")     // a + (-i) b
-SP_PK2(add_pi, "v_pk_add_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[1,0] neg_lo:[0,1]")     // a + i b
-SP_PK2(add_conj, "v_pk_add_f32 %0, %1, %2 neg_hi:[0,1]")                                // a + conj(b)
-SP_PK2(sub_conj, "v_pk_add_f32 %0, %1, %2 neg_lo:[0,1]")                                // a - conj(b)
-#undef SP_PK2
+__device__ __forceinline__ c2 add_mi(c2 a, c2 b) { return {a.x + b.y, a.y - b.x}; }       // a + (-i) b
+__device__ __forceinline__ c2 add_pi(c2 a, c2 b) { return {a.x - b.y, a.y + b.x}; }       // a + i b
+__device__ __forceinline__ c2 add_conj(c2 a, c2 b) { return {a.x + b.x, a.y - b.y}; }     // a + conj(b)
+__device__ __forceinline__ c2 sub_conj(c2 a, c2 b) { return {a.x - b.x, a.y + b.y}; }     // a - conj(b)
 // a * w: (a.im w.im, a.im w.re), then (a.re w.re - ., a.re w.im + .)
 __device__ __forceinline__ c2 cmul(c2 a, c2 w) {
-    c2 t, d;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[1,1] op_sel_hi:[1,0]" : "=v"(t) : "v"(a), "v"(w));
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1] neg_lo:[0,0,1]" : "=v"(d) : "v"(a), "v"(w), "v"(t));
-    return d;
+    return {fmaf(a.x, w.x, -(a.y * w.y)), fmaf(a.x, w.y, a.y * w.x)};
 }
-// the same with a compile-time constant w held in a scalar register pair
-__device__ __forceinline__ c2 cmul_k(c2 a, float wre, float wim) {
-    const c2 w = {wre, wim};
-    c2 t, d;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[1,1] op_sel_hi:[1,0]" : "=v"(t) : "v"(a), "s"(w));
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1] neg_lo:[0,0,1]" : "=v"(d) : "v"(a), "s"(w), "v"(t));
-    return d;
-}
+// the same with a compile-time constant w
+__device__ __forceinline__ c2 cmul_k(c2 a, float wre, float wim) { return cmul(a, c2{wre, wim}); }
 
 // forward 8-point DFT in place (mel_math.h dft8)
 __device__ __forceinline__ void dft8_pk(c2 (&z)[8]) {
