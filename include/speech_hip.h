@@ -35,6 +35,11 @@ extern "C" {
 #define SP_F16 1
 #define SP_BF16 2
 
+/* activations of sp_groupnorm_* */
+#define SP_ACT_NONE 0
+#define SP_ACT_RELU 1
+#define SP_ACT_SILU 2
+
 const char* sp_last_error(void);
 int sp_version(void);
 
@@ -348,6 +353,42 @@ int sp_layernorm_fwd(const void* x, const float* gamma, const float* beta, int64
 int sp_layernorm_bwd(const void* gy, const void* x, const float* mean, const float* rstd,
                      const float* gamma, const void* gres, int64_t M, int N, int dtype, void* gx,
                      float* dgamma, float* dbeta, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Group normalisation with an activation, channels last (no counterpart in the reference, whose blocks use BatchNorm,
+ * net.py:24-25, :36-41): y = act((x - mean) * rstd * gamma[c] + beta[c] + residual), mean and rstd (biased variance + eps)
+ * over the F * T positions and C / G channels of one sample and group.
+ * Tensors are [N][F][T][C] of dtype (SP_F32 / SP_F16 / SP_BF16), element (n, f, t, c) at n*s0 + f*s1 + t*s2 + c; strides (HOST
+ * array, elements): fwd x, residual, y; bwd gy, x, residual, gx, gres (three each; those of a NULL tensor are ignored).
+ * gamma, beta f32 [C]; C % G == 0, C <= 2048, N <= 2^22.  residual may be NULL.  act: SP_ACT_*.  lengths: DEVICE int32 [N] or NULL;
+ * frames t >= lengths[n] are outside: not counted, not read, written as 0 (values outside [0, T] are clamped).  A sample of length
+ * 0 is all zeros.  mean, rstd: f32 [N][G], both or neither NULL (the backward needs them).
+ * Backward: gx, gres = d loss / d x, d residual (gres may be NULL), dgamma / dbeta f32
+ * [C], overwritten or (accumulate != 0) added to.  All reductions are in a fixed order: results are bit-reproducible.
+ * Any vector width the addresses and strides allow is used; alignment to 8 elements is fastest.
+ * --------------------------------------------------------------------------------------- */
+size_t sp_groupnorm_workspace_bytes(int64_t N, int F, int T, int C, int G, int backward);
+int sp_groupnorm_fwd(const void* x, const void* residual, const float* gamma, const float* beta, const int32_t* lengths,
+                     const int64_t* strides, int64_t N, int F, int T, int C, int G, float eps, int act, int dtype, void* y,
+                     float* mean, float* rstd, void* workspace, size_t workspace_bytes, void* stream);
+int sp_groupnorm_bwd(const void* gy, const void* x, const void* residual, const float* gamma, const float* beta,
+                     const float* mean, const float* rstd, const int32_t* lengths, const int64_t* strides, int64_t N, int F,
+                     int T, int C, int G, int act, int accumulate, int dtype, void* gx, void* gres, float* dgamma,
+                     float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Dropout from a counter-based generator; the mask is never stored, the backward call forms it again.
+ *   y[i] = keep(i mod period) ? x[i] * 65536 / (65536 - thr) : 0   (+ residual[i]),   thr = round(65536 p), 0 <= i < rows * period
+ * keep(j) is draw number j % 8 of counter j / 8 >= thr: Philox4x32-10 (Salmon, Moraes, Dror, Shaw, SC'11) with key = rng[0] (64-bit
+ * seed) and counter words (j / 8 low, j / 8 high, rng[1] low word = the step, site); a counter's four words give eight 16-bit draws,
+ * low half first.  rows = 1 is elementwise dropout; rows = T, period = B * C shares one mask among all frames of a [T][B][C] tensor
+ * (the variational form, net.py:61-72).  p is honoured to 2^-17 and the scale matches the honoured rate; p = 1 drops everything.  A
+ * dropped element is 0 whatever x holds.  rng: DEVICE int64[2], read by the kernel (a captured graph follows its updates).
+ * used: DEVICE int64[2] or NULL: receives the pair that was used, for the backward call (which passes x = gy, residual = NULL,
+ * rng = used).  x, residual, y: contiguous, any alignment of their element; y may be x or residual.
+ * --------------------------------------------------------------------------------------- */
+int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period, double p, const int64_t* rng, int site,
+               int dtype, void* y, int64_t* used, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * General GEMM on the matrix cores, f32 accumulation:

@@ -10,6 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspeech_hip.so")
 
 SP_F32, SP_F16, SP_BF16 = 0, 1, 2
+ACT_CODES = {"none": 0, "relu": 1, "silu": 2}   # SP_ACT_*
 SUMSQ_WORDS = 1025   # SP_SUMSQ_WORDS of include/speech_hip.h
 ADAM8_BLOCK = 2048   # SP_ADAM8_BLOCK
 CONV_WGRAD_WS_WORDS = 512 * 15 * 32 * 32   # SP_CONV_WGRAD_WS_WORDS: one slab per persistent workgroup
@@ -69,6 +70,11 @@ SIGNATURES = {
     "sp_linear_pack": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "sp_layernorm_fwd": (_i, [_vp, _vp, _vp, _i64, _i, _f, _i, _vp, _i64, _vp, _vp, _vp]),
     "sp_layernorm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp]),
+    "sp_groupnorm_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),
+    "sp_groupnorm_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "sp_groupnorm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp,
+                              _vp, _sz, _vp]),
+    "sp_dropout": (_i, [_vp, _vp, _i64, _i64, _c.c_double, _vp, _i, _i, _vp, _vp, _vp]),
 }
 
 _lib = None

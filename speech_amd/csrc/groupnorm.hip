@@ -1,0 +1,729 @@
+// Group normalisation with an activation, channels last, forward and backward:
+//     y = act( (x - mean) * rstd * gamma[c] + beta[c] + residual ),   act = identity, ReLU or SiLU,
+// mean and rstd over the positions and the C / G channels of one (sample, group).  x is [N][F][T][C] with unit channel stride; with
+// `lengths` only frames t < lengths[n] count and are written as values, the others become zero.  The batch-independent normalisation of
+// the conv stack's blocks (the reference normalises those over the batch, net.py:24-25) and of a recurrent layer's output.
+//
+// HBM-bound: forward reads x (and the residual) and writes y; the statistics need x before the first output, so x is read twice -- the
+// second time from the Infinity Cache at the conv stack's size (61 MB).  Two routes, chosen by the shape alone:
+//   rows    one position a sample (F * T == 1): a (sample, group) is a contiguous segment that a team of lanes holds in registers; one
+//           read, one write, two-pass statistics.
+//   blocks  everything else: a statistics kernel over (sample, split) and an apply kernel that merges the splits' partials itself.
+// Statistics: every thread sums differences to its own first value, (count, mean, M2) triples are merged as sums of w * mean and of
+// M2 + w * (mean - mean_all)^2: a large mean or a click in the first frame costs no digits.  All sums are f32 in a fixed order.
+#include "common.h"
+
+namespace sp {
+
+constexpr int kGnMaxC = 2048;
+constexpr int kGnThreads = 256;
+constexpr int kGnMaxSplit = 64;
+
+struct GnShape {
+    int N, F, T, C, G, Cg, act;
+    const int32_t* lengths;
+};
+struct GnStr { int64_t n, f, t; };
+
+template <typename T, int VW> struct alignas(sizeof(T) * VW) GnRaw { T e[VW]; };
+
+template <typename T, int VW> __device__ __forceinline__ void gn_ld(const T* p, float (&f)[VW]) {
+    const GnRaw<T, VW> r = *reinterpret_cast<const GnRaw<T, VW>*>(p);
+#pragma unroll
+    for (int i = 0; i < VW; ++i) f[i] = Elem<T>::f(r.e[i]);
+}
+template <typename T, int VW> __device__ __forceinline__ void gn_st(T* p, const float (&f)[VW]) {
+    GnRaw<T, VW> r;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) Elem<T>::st(&r.e[i], f[i]);
+    *reinterpret_cast<GnRaw<T, VW>*>(p) = r;
+}
+
+__device__ __forceinline__ float gn_act(float v, int act) {
+    if (act == SP_ACT_RELU) return v <= 0.f ? 0.f : v;   // NaN stays NaN
+    if (act == SP_ACT_SILU) return v / (1.f + __expf(-v));
+    return v;
+}
+__device__ __forceinline__ float gn_act_grad(float v, int act) {
+    if (act == SP_ACT_RELU) return v > 0.f ? 1.f : 0.f;
+    if (act == SP_ACT_SILU) {
+        const float s = 1.f / (1.f + __expf(-v));
+        return s * (1.f + v * (1.f - s));
+    }
+    return 1.f;
+}
+
+// Positions [lo, hi) of a sample walked by rows of threads: (f, t) advance without a division per step.
+struct GnWalk {
+    int f, t, df, dt;
+    __device__ __forceinline__ GnWalk(int p, int step, int T) : f(p / T), t(p % T), df(step / T), dt(step % T) {}
+    __device__ __forceinline__ void next(int T) {
+        f += df; t += dt;
+        if (t >= T) { t -= T; ++f; }
+    }
+};
+
+// ---- block route --------------------------------------------------------------------------------------
+// thread = (row, chunk of VW channels); a chunk lies inside a group or holds whole groups
+template <typename T, int VW>
+__global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restrict__ x, GnStr xs, GnShape s, int nsplit,
+                                                              float* __restrict__ part) {
+    __shared__ float red[kGnThreads * VW];
+    __shared__ float gmean[kGnMaxC];
+    const int n = blockIdx.x / nsplit, split = blockIdx.x % nsplit;
+    const int P = s.F * s.T, nch = s.C / VW;
+    const int per = (P + nsplit - 1) / nsplit, lo = split * per, hi = min(P, lo + per);
+    const int len = s.lengths ? min(max(s.lengths[n], 0), s.T) : s.T;
+    const int cpb = min(nch, kGnThreads);                 // chunks walked at a time
+    const int rows = kGnThreads / cpb, row = threadIdx.x / cpb;
+    for (int cb = 0; cb < nch; cb += cpb) {
+        const int chunk = cb + threadIdx.x % cpb;
+        const bool on = row < rows && chunk < nch;
+        float k[VW], sm[VW], sq[VW];
+        int cnt = 0;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) { k[i] = 0.f; sm[i] = 0.f; sq[i] = 0.f; }
+        if (on) {
+            const T* base = x + n * xs.n + chunk * VW;
+            GnWalk w(lo + row, rows, s.T);
+            for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
+                if (w.t >= len) continue;
+                float v[VW];
+                gn_ld<T, VW>(base + w.f * xs.f + w.t * xs.t, v);
+                if (cnt == 0) {
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) k[i] = v[i];
+                }
+                ++cnt;
+#pragma unroll
+                for (int i = 0; i < VW; ++i) { const float d = v[i] - k[i]; sm[i] += d; sq[i] += d * d; }
+            }
+        }
+        const float inv = cnt ? 1.f / (float)cnt : 0.f;
+        float c_all;
+        if (s.lengths) {
+            __syncthreads();
+            red[threadIdx.x] = (threadIdx.x % cpb == 0 && row < rows) ? (float)cnt : 0.f;
+            __syncthreads();
+            for (int o = kGnThreads / 2; o > 0; o >>= 1) {
+                if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+                __syncthreads();
+            }
+            c_all = red[0];
+        } else {
+            c_all = (float)max(0, hi - lo);
+        }
+        __syncthreads();
+        float mean[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            mean[i] = k[i] + sm[i] * inv;
+            red[threadIdx.x * VW + i] = (float)cnt * mean[i];
+            sq[i] -= sm[i] * sm[i] * inv;
+            if (sq[i] < 0.f) sq[i] = 0.f;
+        }
+        auto tree = [&]() {                                    // sums over the rows, left in row 0's slots
+            __syncthreads();
+            for (int o = 128; o > 0; o >>= 1) {
+                if (row < o && row + o < rows) {
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) red[threadIdx.x * VW + i] += red[(threadIdx.x + o * cpb) * VW + i];
+                }
+                __syncthreads();
+            }
+        };
+        tree();
+        // channels of this pass: [cb * VW, cb * VW + cpb * VW); a group may span passes only when VW == 1 (C > 256): see below
+        const int c0 = cb * VW, c1 = min(s.C, c0 + cpb * VW);
+        const int g0 = c0 / s.Cg, g1 = (c1 - 1) / s.Cg;
+        const float winv = c_all > 0.f ? 1.f / c_all : 0.f;
+        for (int g = g0 + threadIdx.x; g <= g1; g += kGnThreads) {
+            const int a = max(c0, g * s.Cg), b = min(c1, (g + 1) * s.Cg);
+            float m = 0.f;
+            for (int c = a; c < b; ++c) m += red[c - c0];
+            gmean[g - g0] = m * winv / (float)(b - a);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const int c = chunk * VW + i;
+            const float d = on ? mean[i] - gmean[c / s.Cg - g0] : 0.f;
+            red[threadIdx.x * VW + i] = on && cnt ? sq[i] + (float)cnt * d * d : 0.f;
+        }
+        tree();
+        for (int g = g0 + threadIdx.x; g <= g1; g += kGnThreads) {
+            const int a = max(c0, g * s.Cg), b = min(c1, (g + 1) * s.Cg);
+            float m2 = 0.f;
+            for (int c = a; c < b; ++c) m2 += red[c - c0];
+            // slot: one per (sample, split, pass-part of the group)
+            const int sub = cb / cpb;
+            const int nsub = (nch + cpb - 1) / cpb;
+            float* o = part + (((int64_t)n * nsplit + split) * nsub + sub) * s.G * 3 + g * 3;
+            o[0] = c_all * (float)(b - a); o[1] = gmean[g - g0]; o[2] = m2;
+        }
+        if (nch > cpb) {   // groups that this pass does not touch hold no weight
+            const int sub = cb / cpb, nsub = (nch + cpb - 1) / cpb;
+            for (int g = threadIdx.x; g < s.G; g += kGnThreads)
+                if (g < g0 || g > g1) part[(((int64_t)n * nsplit + split) * nsub + sub) * s.G * 3 + g * 3] = 0.f;
+        }
+        __syncthreads();
+    }
+}
+
+// mean and rstd of every group of sample n from the splits' triples, into LDS
+__device__ __forceinline__ void gn_merge(const float* __restrict__ part, int n, int nparts, int G, float eps, float* mean, float* rstd) {
+    for (int g = threadIdx.x; g < G; g += kGnThreads) {
+        const float* p = part + (int64_t)n * nparts * G * 3 + g * 3;
+        float w = 0.f, m = 0.f, m2 = 0.f;
+        for (int i = 0; i < nparts; ++i) {
+            const float wi = p[(int64_t)i * G * 3];
+            if (wi > 0.f) { w += wi; m += wi * p[(int64_t)i * G * 3 + 1]; }
+        }
+        const float inv = w > 0.f ? 1.f / w : 0.f;
+        m *= inv;
+        for (int i = 0; i < nparts; ++i) {
+            const float wi = p[(int64_t)i * G * 3];
+            if (wi > 0.f) { const float d = p[(int64_t)i * G * 3 + 1] - m; m2 += p[(int64_t)i * G * 3 + 2] + wi * d * d; }
+        }
+        mean[g] = m;
+        rstd[g] = rsqrtf(m2 * inv + eps);
+    }
+    __syncthreads();
+}
+
+template <typename T, int VW>
+__global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(const T* __restrict__ x, GnStr xs, const T* __restrict__ res, GnStr rs,
+                                                              const float* __restrict__ gamma, const float* __restrict__ beta, GnShape s,
+                                                              float eps, const float* __restrict__ part, int nsplit, int nparts, T* __restrict__ y,
+                                                              GnStr ys, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    __shared__ float mean[kGnMaxC], rstd[kGnMaxC];
+    const int n = blockIdx.x / nsplit, split = blockIdx.x % nsplit;
+    gn_merge(part, n, nparts, s.G, eps, mean, rstd);
+    if (split == 0 && mean_out)
+        for (int g = threadIdx.x; g < s.G; g += kGnThreads) { mean_out[(int64_t)n * s.G + g] = mean[g]; rstd_out[(int64_t)n * s.G + g] = rstd[g]; }
+    const int P = s.F * s.T, nch = s.C / VW;
+    const int len = s.lengths ? min(max(s.lengths[n], 0), s.T) : s.T;
+    const int cpb = min(nch, kGnThreads), rows = kGnThreads / cpb, row = threadIdx.x / cpb;
+    const int per = (P + nsplit - 1) / nsplit, lo = split * per, hi = min(P, lo + per);
+    for (int cb = 0; cb < nch; cb += cpb) {
+        const int chunk = cb + threadIdx.x % cpb;
+        if (row >= rows || chunk >= nch) continue;
+        float mu[VW], a[VW], b[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const int c = chunk * VW + i;
+            mu[i] = mean[c / s.Cg];
+            a[i] = rstd[c / s.Cg] * gamma[c];
+            b[i] = beta[c];
+        }
+        GnWalk w(lo + row, rows, s.T);
+        for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
+            float o[VW];
+            if (w.t < len) {
+                float v[VW];
+                gn_ld<T, VW>(x + n * xs.n + w.f * xs.f + w.t * xs.t + chunk * VW, v);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] = (v[i] - mu[i]) * a[i] + b[i];
+                if (res) {
+                    gn_ld<T, VW>(res + n * rs.n + w.f * rs.f + w.t * rs.t + chunk * VW, v);
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) o[i] += v[i];
+                }
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] = gn_act(o[i], s.act);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] = 0.f;
+            }
+            gn_st<T, VW>(y + n * ys.n + w.f * ys.f + w.t * ys.t + chunk * VW, o);
+        }
+    }
+}
+
+// Backward, first pass: g = gy * act'(pre) (written as the residual's gradient), per (sample, split): channel sums of g and of g * xhat,
+// and the same weighted with gamma per group.
+template <typename T, int VW>
+__global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __restrict__ gy, GnStr gs, const T* __restrict__ x, GnStr xs,
+                                                                  const T* __restrict__ res, GnStr rs, const float* __restrict__ gamma,
+                                                                  const float* __restrict__ beta, const float* __restrict__ mean,
+                                                                  const float* __restrict__ rstd, GnShape s, int nsplit,
+                                                                  T* __restrict__ gres, GnStr grs, float* __restrict__ cpart,
+                                                                  float* __restrict__ gpart) {
+    __shared__ float red[kGnThreads * VW * 2];
+    const int n = blockIdx.x / nsplit, split = blockIdx.x % nsplit;
+    const int P = s.F * s.T, nch = s.C / VW;
+    const int per = (P + nsplit - 1) / nsplit, lo = split * per, hi = min(P, lo + per);
+    const int len = s.lengths ? min(max(s.lengths[n], 0), s.T) : s.T;
+    const int cpb = min(nch, kGnThreads), rows = kGnThreads / cpb, row = threadIdx.x / cpb;
+    float* cp = cpart + ((int64_t)n * nsplit + split) * s.C * 2;
+    for (int cb = 0; cb < nch; cb += cpb) {
+        const int chunk = cb + threadIdx.x % cpb;
+        const bool on = row < rows && chunk < nch;
+        float sb[VW], sx[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) { sb[i] = 0.f; sx[i] = 0.f; }
+        if (on) {
+            float mu[VW], r[VW], gm[VW], bt[VW];
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const int c = chunk * VW + i;
+                mu[i] = mean[(int64_t)n * s.G + c / s.Cg];
+                r[i] = rstd[(int64_t)n * s.G + c / s.Cg];
+                gm[i] = gamma[c];
+                bt[i] = beta[c];
+            }
+            GnWalk w(lo + row, rows, s.T);
+            for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
+                float g[VW], v[VW], z[VW];
+                if (w.t < len) {
+                    gn_ld<T, VW>(gy + n * gs.n + w.f * gs.f + w.t * gs.t + chunk * VW, g);
+                    gn_ld<T, VW>(x + n * xs.n + w.f * xs.f + w.t * xs.t + chunk * VW, v);
+                    if (res) gn_ld<T, VW>(res + n * rs.n + w.f * rs.f + w.t * rs.t + chunk * VW, z);
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) {
+                        const float xh = (v[i] - mu[i]) * r[i];
+                        if (s.act != SP_ACT_NONE) g[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (res ? z[i] : 0.f), s.act);
+                        sb[i] += g[i];
+                        sx[i] += g[i] * xh;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) g[i] = 0.f;
+                }
+                if (gres) gn_st<T, VW>(gres + n * grs.n + w.f * grs.f + w.t * grs.t + chunk * VW, g);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            red[threadIdx.x * VW * 2 + i] = sb[i];
+            red[threadIdx.x * VW * 2 + VW + i] = sx[i];
+        }
+        __syncthreads();
+        for (int o = 128; o > 0; o >>= 1) {
+            if (row < o && row + o < rows) {
+#pragma unroll
+                for (int i = 0; i < 2 * VW; ++i) red[threadIdx.x * VW * 2 + i] += red[(threadIdx.x + o * cpb) * VW * 2 + i];
+            }
+            __syncthreads();
+        }
+        if (on && row == 0) {
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                cp[(chunk * VW + i) * 2] = red[threadIdx.x * VW * 2 + i];
+                cp[(chunk * VW + i) * 2 + 1] = red[threadIdx.x * VW * 2 + VW + i];
+            }
+        }
+    }
+    __syncthreads();   // this workgroup's own global writes are visible to it behind the barrier
+    for (int g = threadIdx.x; g < s.G; g += kGnThreads) {
+        float a = 0.f, b = 0.f;
+        for (int c = g * s.Cg; c < (g + 1) * s.Cg; ++c) { a += gamma[c] * cp[c * 2]; b += gamma[c] * cp[c * 2 + 1]; }
+        float* o = gpart + (((int64_t)n * nsplit + split) * s.G + g) * 2;
+        o[0] = a; o[1] = b;
+    }
+}
+
+// out[c] (+)= sum over parts of part[r][c][0 / 1]; a workgroup takes 32 channels, eight rows of threads walk the parts
+__device__ __forceinline__ void gn_param_reduce(const float* __restrict__ cpart, int64_t nrows, int C, int c0, int accumulate,
+                                                float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    __shared__ float red[8][32][2];
+    const int c = c0 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
+    float a = 0.f, b = 0.f;
+    if (c < C) {
+#pragma unroll 4
+        for (int64_t r = r0; r < nrows; r += 8) { a += cpart[(r * C + c) * 2]; b += cpart[(r * C + c) * 2 + 1]; }
+    }
+    red[r0][threadIdx.x & 31][0] = a;
+    red[r0][threadIdx.x & 31][1] = b;
+    __syncthreads();
+    if (r0 == 0 && c < C) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) { a += red[i][threadIdx.x][0]; b += red[i][threadIdx.x][1]; }
+        dbeta[c] = accumulate ? dbeta[c] + a : a;
+        dgamma[c] = accumulate ? dgamma[c] + b : b;
+    }
+}
+
+// Backward, second pass: gx = rstd * (gamma g - mean(gamma g) - xhat mean(gamma g xhat)); the workgroups behind the N * nsplit that do so
+// add up the parameter gradients instead, 32 channels each.  g is formed again from gy, x and the residual: reading the written gres back
+// would save a read in three but carry its 16-bit rounding into gx.
+template <typename T, int VW>
+__global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(const T* __restrict__ gy, GnStr gs, const T* __restrict__ x, GnStr xs,
+                                                                  const T* __restrict__ res, GnStr rs, const float* __restrict__ gamma,
+                                                                  const float* __restrict__ beta, const float* __restrict__ mean,
+                                                                  const float* __restrict__ rstd, GnShape s, const float* __restrict__ cpart, const float* __restrict__ gpart,
+                                                                  int nsplit, int accumulate, T* __restrict__ gx, GnStr gxs,
+                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    __shared__ float c1[kGnMaxC], c2[kGnMaxC];
+    const int n = blockIdx.x / nsplit, split = blockIdx.x % nsplit;
+    if (n >= s.N) {
+        gn_param_reduce(cpart, (int64_t)s.N * nsplit, s.C, (blockIdx.x - s.N * nsplit) * 32, accumulate, dgamma, dbeta);
+        return;
+    }
+    const int len = s.lengths ? min(max(s.lengths[n], 0), s.T) : s.T;
+    const float cinv = len > 0 ? 1.f / ((float)len * (float)s.F * (float)s.Cg) : 0.f;
+    for (int g = threadIdx.x; g < s.G; g += kGnThreads) {
+        float a = 0.f, b = 0.f;
+        for (int i = 0; i < nsplit; ++i) {
+            const float* p = gpart + (((int64_t)n * nsplit + i) * s.G + g) * 2;
+            a += p[0]; b += p[1];
+        }
+        c1[g] = a * cinv; c2[g] = b * cinv;
+    }
+    __syncthreads();
+    const int P = s.F * s.T, nch = s.C / VW;
+    const int cpb = min(nch, kGnThreads), rows = kGnThreads / cpb, row = threadIdx.x / cpb;
+    const int per = (P + nsplit - 1) / nsplit, lo = split * per, hi = min(P, lo + per);
+    for (int cb = 0; cb < nch; cb += cpb) {
+        const int chunk = cb + threadIdx.x % cpb;
+        if (row >= rows || chunk >= nch) continue;
+        float mu[VW], r[VW], gm[VW], bt[VW], k1[VW], k2[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const int c = chunk * VW + i, g = c / s.Cg;
+            mu[i] = mean[(int64_t)n * s.G + g];
+            r[i] = rstd[(int64_t)n * s.G + g];
+            gm[i] = gamma[c];
+            bt[i] = beta[c];
+            k1[i] = c1[g];
+            k2[i] = c2[g];
+        }
+        GnWalk w(lo + row, rows, s.T);
+        for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
+            float o[VW];
+            if (w.t < len) {
+                float g[VW], v[VW], z[VW];
+                gn_ld<T, VW>(gy + n * gs.n + w.f * gs.f + w.t * gs.t + chunk * VW, g);
+                gn_ld<T, VW>(x + n * xs.n + w.f * xs.f + w.t * xs.t + chunk * VW, v);
+                if (res) gn_ld<T, VW>(res + n * rs.n + w.f * rs.f + w.t * rs.t + chunk * VW, z);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    const float xh = (v[i] - mu[i]) * r[i];
+                    if (s.act != SP_ACT_NONE) g[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (res ? z[i] : 0.f), s.act);
+                    o[i] = r[i] * (gm[i] * g[i] - k1[i] - xh * k2[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] = 0.f;
+            }
+            gn_st<T, VW>(gx + n * gxs.n + w.f * gxs.f + w.t * gxs.t + chunk * VW, o);
+        }
+    }
+}
+
+// ---- rows route ---------------------------------------------------------------------------------------
+// Unit u = (sample u / G, group u % G): Cg contiguous channels held by `team` lanes (a power of two), NCH chunks of VW each.
+template <typename T, int VW, int NCH>
+__global__ __launch_bounds__(kGnThreads) void gn_rows_fwd_kernel(const T* __restrict__ x, int64_t xsn, const T* __restrict__ res, int64_t rsn,
+                                                                 const float* __restrict__ gamma, const float* __restrict__ beta, GnShape s,
+                                                                 float eps, int team, T* __restrict__ y, int64_t ysn,
+                                                                 float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    const int64_t units = (int64_t)s.N * s.G;
+    const int upb = kGnThreads / team, lane = threadIdx.x & (team - 1);
+    const float inv = 1.f / (float)s.Cg;
+    for (int64_t u = (int64_t)blockIdx.x * upb + threadIdx.x / team; u < units; u += (int64_t)gridDim.x * upb) {
+        const int64_t n = u / s.G;
+        const int g = (int)(u - n * s.G), c0 = g * s.Cg;
+        const bool dead = s.lengths && s.lengths[n] <= 0;
+        float v[NCH][VW], sm = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int c = (k * team + lane) * VW;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) v[k][i] = 0.f;
+            if (c < s.Cg && !dead) gn_ld<T, VW>(x + n * xsn + c0 + c, v[k]);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) sm += v[k][i];
+        }
+        for (int o = team >> 1; o > 0; o >>= 1) sm += __shfl_xor(sm, o);
+        const float mean = sm * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+            if ((k * team + lane) * VW < s.Cg) {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) { v[k][i] -= mean; q += v[k][i] * v[k][i]; }
+            }
+        for (int o = team >> 1; o > 0; o >>= 1) q += __shfl_xor(q, o);
+        const float rstd = rsqrtf(q * inv + eps);
+        if (lane == 0 && mean_out) { mean_out[u] = mean; rstd_out[u] = rstd; }
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int c = (k * team + lane) * VW;
+            if (c < s.Cg) {
+                float gm[VW], bt[VW], o[VW];
+                gn_ld<float, VW>(gamma + c0 + c, gm);
+                gn_ld<float, VW>(beta + c0 + c, bt);
+                if (res && !dead) gn_ld<T, VW>(res + n * rsn + c0 + c, o);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    const float pre = v[k][i] * (rstd * gm[i]) + bt[i] + (res && !dead ? o[i] : 0.f);
+                    o[i] = dead ? 0.f : gn_act(pre, s.act);
+                }
+                gn_st<T, VW>(y + n * ysn + c0 + c, o);
+            }
+        }
+    }
+}
+
+// The grid steps by a multiple of G units, so a lane keeps its channels and sums its parameter gradients in registers; slot = unit slot of
+// the grid, cpart [slots / G][C][2] because slot % G is the group.
+template <typename T, int VW, int NCH>
+__global__ __launch_bounds__(kGnThreads) void gn_rows_bwd_kernel(const T* __restrict__ gy, int64_t gsn, const T* __restrict__ x, int64_t xsn,
+                                                                 const T* __restrict__ res, int64_t rsn, const float* __restrict__ gamma,
+                                                                 const float* __restrict__ beta, const float* __restrict__ mean_in,
+                                                                 const float* __restrict__ rstd_in, GnShape s, int team, T* __restrict__ gx,
+                                                                 int64_t gxsn, T* __restrict__ gres, int64_t grsn, float* __restrict__ cpart) {
+    const int64_t units = (int64_t)s.N * s.G;
+    const int upb = kGnThreads / team, lane = threadIdx.x & (team - 1);
+    const float inv = 1.f / (float)s.Cg;
+    const int64_t slot = (int64_t)blockIdx.x * upb + threadIdx.x / team;
+    const int g = (int)(slot % s.G), c0 = g * s.Cg;
+    float gm[NCH][VW], bt[NCH][VW], dg[NCH][VW], db[NCH][VW];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+        const int c = (k * team + lane) * VW;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) { gm[k][i] = bt[k][i] = dg[k][i] = db[k][i] = 0.f; }
+        if (c < s.Cg) { gn_ld<float, VW>(gamma + c0 + c, gm[k]); gn_ld<float, VW>(beta + c0 + c, bt[k]); }
+    }
+    for (int64_t u = slot; u < units; u += (int64_t)gridDim.x * upb) {
+        const int64_t n = u / s.G;
+        const bool dead = s.lengths && s.lengths[n] <= 0;
+        const float mean = mean_in[u], rstd = rstd_in[u];
+        float w[NCH][VW], xh[NCH][VW], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int c = (k * team + lane) * VW;
+            const bool on = c < s.Cg && !dead;
+            float z[VW];
+#pragma unroll
+            for (int i = 0; i < VW; ++i) { w[k][i] = 0.f; xh[k][i] = 0.f; z[i] = 0.f; }
+            if (on) {
+                gn_ld<T, VW>(gy + n * gsn + c0 + c, w[k]);
+                gn_ld<T, VW>(x + n * xsn + c0 + c, xh[k]);
+                if (res) gn_ld<T, VW>(res + n * rsn + c0 + c, z);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    xh[k][i] = (xh[k][i] - mean) * rstd;
+                    if (s.act != SP_ACT_NONE) w[k][i] *= gn_act_grad(xh[k][i] * gm[k][i] + bt[k][i] + z[i], s.act);
+                }
+            }
+            if (gres && c < s.Cg) gn_st<T, VW>(gres + n * grsn + c0 + c, w[k]);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                dg[k][i] += w[k][i] * xh[k][i];
+                db[k][i] += w[k][i];
+                w[k][i] *= gm[k][i];
+                s1 += w[k][i];
+                s2 += w[k][i] * xh[k][i];
+            }
+        }
+        for (int o = team >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o); s2 += __shfl_xor(s2, o); }
+        s1 *= inv; s2 *= inv;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int c = (k * team + lane) * VW;
+            if (c < s.Cg) {
+                float o[VW];
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] = dead ? 0.f : rstd * (w[k][i] - s1 - xh[k][i] * s2);
+                gn_st<T, VW>(gx + n * gxsn + c0 + c, o);
+            }
+        }
+    }
+    float* cp = cpart + (slot / s.G) * s.C * 2 + c0 * 2;
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+        const int c = (k * team + lane) * VW;
+        if (c < s.Cg) {
+#pragma unroll
+            for (int i = 0; i < VW; ++i) { cp[(c + i) * 2] = db[k][i]; cp[(c + i) * 2 + 1] = dg[k][i]; }
+        }
+    }
+}
+
+__global__ __launch_bounds__(kGnThreads) void gn_param_kernel(const float* __restrict__ cpart, int64_t nrows, int C, int accumulate,
+                                                              float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    gn_param_reduce(cpart, nrows, C, blockIdx.x * 32, accumulate, dgamma, dbeta);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------
+struct GnPlan {
+    bool rows;
+    int vw;                  // channels a chunk
+    int nch, team;           // rows route: chunks a lane, lanes a unit
+    int splits, nsub;        // block route
+    int grid;                // rows route, backward
+};
+
+// `vw`: the widest vector that the tensors' addresses and strides allow
+static GnPlan gn_plan(int64_t N, int F, int T, int C, int G, int vw) {
+    GnPlan p{};
+    const int Cg = C / G;
+    if ((int64_t)F * T == 1) {
+        p.vw = vw;
+        while (Cg % p.vw) p.vw >>= 1;
+        const int chunks = Cg / p.vw;
+        int team = 1;
+        while (team < 64 && team < chunks) team *= 2;
+        const int nch = (chunks + team - 1) / team;
+        if (nch <= 4) {
+            p.rows = true; p.team = team; p.nch = nch == 3 ? 4 : nch;
+            const int upb = kGnThreads / team;
+            // one persistent grid; its step is a multiple of G units, so that a lane keeps its channels
+            int64_t blocks = (N * G + upb - 1) / upb;
+            if (blocks > 1024) blocks = 1024;
+            int step = 1;
+            while ((int64_t)step * upb % G) ++step;
+            p.grid = (int)((blocks + step - 1) / step * step);
+            return p;
+        }
+    }
+    // a chunk of channels lies inside one group or holds whole groups
+    p.vw = vw;
+    while (p.vw > 1 && !(C % p.vw == 0 && (Cg % p.vw == 0 || p.vw % Cg == 0))) p.vw >>= 1;
+    const int64_t P = (int64_t)F * T;
+    // ~2048 workgroups on the chip, at least 32 positions each
+    int64_t sp = N > 0 ? 2048 / N : 1;
+    if (sp > kGnMaxSplit) sp = kGnMaxSplit;
+    if (sp > (P + 31) / 32) sp = (P + 31) / 32;
+    if (sp < 1) sp = 1;
+    p.splits = (int)sp;
+    const int nch = C / p.vw, cpb = nch < kGnThreads ? nch : kGnThreads;
+    p.nsub = (nch + cpb - 1) / cpb;
+    return p;
+}
+
+static size_t gn_bytes(const GnPlan& p, int64_t N, int C, int G, int backward) {
+    if (p.rows) return backward ? align_up((size_t)p.grid * (kGnThreads / p.team) / G * C * 2 * sizeof(float), 256) : 0;
+    const size_t parts = (size_t)N * p.splits;
+    if (!backward) return align_up(parts * p.nsub * G * 3 * sizeof(float), 256);
+    return align_up(parts * C * 2 * sizeof(float), 256) + align_up(parts * G * 2 * sizeof(float), 256);
+}
+
+static int gn_check(const char* who, int64_t N, int F, int T, int C, int G, int act, int dtype) {
+    SP_CHECK_ARG(N >= 0 && N <= (1 << 22) && F >= 0 && T >= 0 && (int64_t)F * T < (1ll << 31) - 4096,
+                 "%s: bad shape N=%lld (at most 2^22) F=%d T=%d", who, (long long)N, F, T);
+    SP_CHECK_ARG(C >= 1 && C <= kGnMaxC && G >= 1 && C % G == 0, "%s: C=%d must be a multiple of G=%d and at most %d", who, C, G, kGnMaxC);
+    SP_CHECK_ARG(act == SP_ACT_NONE || act == SP_ACT_RELU || act == SP_ACT_SILU, "%s: act %d unknown", who, act);
+    SP_CHECK_ARG(dtype == SP_F32 || dtype == SP_BF16 || dtype == SP_F16, "%s: dtype %d not supported (f32, bf16, f16)", who, dtype);
+    return SP_OK;
+}
+
+// widest vector (8 at most) that addresses and strides allow; gamma and beta are read as f32 vectors
+static int gn_align(int esize, const void* const* p, const int64_t* st, int k, const float* gamma, const float* beta) {
+    int vw = 8;
+    const uintptr_t par = reinterpret_cast<uintptr_t>(gamma) | reinterpret_cast<uintptr_t>(beta);
+    for (; vw > 1; vw >>= 1) {
+        bool ok = par % (vw * sizeof(float)) == 0;
+        for (int i = 0; i < k; ++i) {
+            if (!p[i]) continue;
+            if (reinterpret_cast<uintptr_t>(p[i]) % (vw * esize)) ok = false;
+            for (int j = 0; j < 3; ++j) if (st[3 * i + j] % vw) ok = false;
+        }
+        if (ok) break;
+    }
+    return vw;
+}
+
+}  // namespace sp
+
+using namespace sp;
+
+#define SP_GN_TYPES(DT, CALL)                                     \
+    if (DT == SP_F32) { using T_ = float; CALL }                  \
+    else if (DT == SP_F16) { using T_ = __half; CALL }            \
+    else { using T_ = __hip_bfloat16; CALL }
+#define SP_GN_VW(V, CALL)                          \
+    if (V == 8) { constexpr int VW_ = 8; CALL }    \
+    else if (V == 4) { constexpr int VW_ = 4; CALL } \
+    else if (V == 2) { constexpr int VW_ = 2; CALL } \
+    else { constexpr int VW_ = 1; CALL }
+#define SP_GN_NCH(K, CALL)                          \
+    if (K == 1) { constexpr int NC_ = 1; CALL }     \
+    else if (K == 2) { constexpr int NC_ = 2; CALL } \
+    else { constexpr int NC_ = 4; CALL }
+
+extern "C" size_t sp_groupnorm_workspace_bytes(int64_t N, int F, int T, int C, int G, int backward) {
+    if (gn_check("sp_groupnorm_workspace_bytes", N, F, T, C, G, 0, SP_F32)) return 0;
+    size_t most = 0;        // whatever vector width the tensors will allow
+    for (int vw = 8; vw; vw >>= 1) {
+        const size_t b = gn_bytes(gn_plan(N, F, T, C, G, vw), N, C, G, backward);
+        if (b > most) most = b;
+    }
+    return most;
+}
+
+extern "C" int sp_groupnorm_fwd(const void* x, const void* residual, const float* gamma, const float* beta, const int32_t* lengths,
+                                const int64_t* strides, int64_t N, int F, int T, int C, int G, float eps, int act, int dtype, void* y,
+                                float* mean, float* rstd, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = gn_check("sp_groupnorm_fwd", N, F, T, C, G, act, dtype);
+    if (rc) return rc;
+    SP_CHECK_ARG(strides, "sp_groupnorm_fwd: null strides");
+    SP_CHECK_ARG((mean == nullptr) == (rstd == nullptr), "sp_groupnorm_fwd: mean and rstd are given together or not at all");
+    if (N == 0 || F == 0 || T == 0) return SP_OK;
+    SP_CHECK_ARG(x && gamma && beta && y, "sp_groupnorm_fwd: null pointer");
+    const size_t need = sp_groupnorm_workspace_bytes(N, F, T, C, G, 0);
+    if (workspace_bytes < need || (need && !workspace)) return fail(SP_EWORKSPACE, "sp_groupnorm_fwd: workspace %zu < %zu bytes", workspace_bytes, need);
+    const GnShape s{(int)N, F, T, C, G, C / G, act, lengths};
+    const void* ptrs[3] = {x, residual, y};
+    const GnPlan p = gn_plan(N, F, T, C, G, gn_align(dtype == SP_F32 ? 4 : 2, ptrs, strides, 3, gamma, beta));
+    const GnStr xs{strides[0], strides[1], strides[2]}, rs{strides[3], strides[4], strides[5]}, ys{strides[6], strides[7], strides[8]};
+    hipStream_t st = (hipStream_t)stream;
+    if (p.rows) {
+        const int upb = kGnThreads / p.team;
+        int64_t blocks = (N * G + upb - 1) / upb;
+        if (blocks > 65536) blocks = 65536;
+        SP_GN_TYPES(dtype, SP_GN_VW(p.vw, SP_GN_NCH(p.nch, {
+            hipLaunchKernelGGL((gn_rows_fwd_kernel<T_, VW_, NC_>), dim3((unsigned)blocks), dim3(kGnThreads), 0, st, (const T_*)x, xs.n,
+                               (const T_*)residual, rs.n, gamma, beta, s, eps, p.team, (T_*)y, ys.n, mean, rstd); })))
+        return check_launch("gn_rows_fwd_kernel");
+    }
+    SP_GN_TYPES(dtype, SP_GN_VW(p.vw, {
+        hipLaunchKernelGGL((gn_stats_kernel<T_, VW_>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)x, xs, s, p.splits,
+                           (float*)workspace);
+        hipLaunchKernelGGL((gn_apply_kernel<T_, VW_>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)x, xs,
+                           (const T_*)residual, rs, gamma, beta, s, eps, (const float*)workspace, p.splits, p.splits * p.nsub, (T_*)y, ys, mean, rstd); }))
+    return check_launch("gn_apply_kernel");
+}
+
+extern "C" int sp_groupnorm_bwd(const void* gy, const void* x, const void* residual, const float* gamma, const float* beta,
+                                const float* mean, const float* rstd, const int32_t* lengths, const int64_t* strides, int64_t N, int F,
+                                int T, int C, int G, int act, int accumulate, int dtype, void* gx, void* gres, float* dgamma,
+                                float* dbeta, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = gn_check("sp_groupnorm_bwd", N, F, T, C, G, act, dtype);
+    if (rc) return rc;
+    SP_CHECK_ARG(strides, "sp_groupnorm_bwd: null strides");
+    SP_CHECK_ARG(dgamma && dbeta, "sp_groupnorm_bwd: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    if (N == 0 || F == 0 || T == 0) {       // no positions: the parameter gradients are zero
+        hipLaunchKernelGGL(gn_param_kernel, dim3((C + 31) / 32), dim3(kGnThreads), 0, st, nullptr, (int64_t)0, C, accumulate, dgamma, dbeta);
+        return check_launch("gn_param_kernel");
+    }
+    SP_CHECK_ARG(gy && x && gamma && beta && mean && rstd && gx, "sp_groupnorm_bwd: null pointer");
+    const size_t need = sp_groupnorm_workspace_bytes(N, F, T, C, G, 1);
+    if (workspace_bytes < need || !workspace) return fail(SP_EWORKSPACE, "sp_groupnorm_bwd: workspace %zu < %zu bytes", workspace_bytes, need);
+    const GnShape s{(int)N, F, T, C, G, C / G, act, lengths};
+    const void* ptrs[5] = {gy, x, residual, gx, gres};
+    const GnPlan p = gn_plan(N, F, T, C, G, gn_align(dtype == SP_F32 ? 4 : 2, ptrs, strides, 5, gamma, beta));
+    const GnStr gs{strides[0], strides[1], strides[2]}, xs{strides[3], strides[4], strides[5]}, rs{strides[6], strides[7], strides[8]},
+        gxs{strides[9], strides[10], strides[11]}, grs{strides[12], strides[13], strides[14]};
+    float* cpart = (float*)workspace;
+    if (p.rows) {
+        SP_GN_TYPES(dtype, SP_GN_VW(p.vw, SP_GN_NCH(p.nch, {
+            hipLaunchKernelGGL((gn_rows_bwd_kernel<T_, VW_, NC_>), dim3(p.grid), dim3(kGnThreads), 0, st, (const T_*)gy, gs.n, (const T_*)x,
+                               xs.n, (const T_*)residual, rs.n, gamma, beta, mean, rstd, s, p.team, (T_*)gx, gxs.n, (T_*)gres, grs.n, cpart); })))
+        hipLaunchKernelGGL(gn_param_kernel, dim3((C + 31) / 32), dim3(kGnThreads), 0, st, cpart, (int64_t)p.grid * (kGnThreads / p.team) / G, C,
+                           accumulate, dgamma, dbeta);
+        return check_launch("gn_rows_bwd_kernel");
+    }
+    float* gpart = (float*)((char*)workspace + align_up((size_t)N * p.splits * C * 2 * sizeof(float), 256));
+    SP_GN_TYPES(dtype, SP_GN_VW(p.vw, {
+        hipLaunchKernelGGL((gn_bwd_stats_kernel<T_, VW_>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)gy, gs, (const T_*)x,
+                           xs, (const T_*)residual, rs, gamma, beta, mean, rstd, s, p.splits, (T_*)gres, grs, cpart, gpart);
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T_, VW_>), dim3((unsigned)N * p.splits + (C + 31) / 32), dim3(kGnThreads), 0, st,
+                           (const T_*)gy, gs, (const T_*)x, xs, (const T_*)residual, rs, gamma, beta, mean, rstd, s, cpart, gpart, p.splits, accumulate, (T_*)gx, gxs, dgamma, dbeta); }))
+    return check_launch("gn_bwd_apply_kernel");
+}

@@ -879,3 +879,181 @@ def matmul(a, w):
 def sru_layer(x, ln_w, ln_b, weight, wc, bias, mask, d, k, C=1, eps=1e-5, pre=None):
     """pre: this layer's entry of sru_prepack (its weights already packed), or None."""
     return _SRULayerFn.apply(x, ln_w, ln_b, weight, wc, bias, mask, d, k, C, eps, pre)
+
+
+# ------------------------------------------------------------------------------------------
+# Group normalisation with an activation, channels last
+# ------------------------------------------------------------------------------------------
+def _same_device(x, **others):
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
+
+
+def _act_tensor(t, name):
+    _need_cuda(t, name)
+    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+
+
+def _unit_last(t):
+    """t, or a contiguous copy where its last dimension is not contiguous."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _host_i64(values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def _gn_strides(tensors):
+    return _host_i64([s for t in tensors for s in (t.stride()[:3] if t is not None else (0, 0, 0))])
+
+
+class _GroupNormFn(torch.autograd.Function):
+    """x, residual [N,F,T,C] views with unit channel stride."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, lengths, groups, eps, act, time_major):
+        N, F, T, C = x.shape
+        w32, b32 = weight.detach().float().contiguous(), bias.detach().float().contiguous()
+        if time_major:
+            y = torch.empty((T, N, F, C), dtype=x.dtype, device=x.device).permute(1, 2, 0, 3)
+        else:
+            y = torch.empty((N, F, T, C), dtype=x.dtype, device=x.device)
+        train = any(ctx.needs_input_grad)
+        mean = torch.empty((2, N, groups), dtype=torch.float32, device=x.device) if train else None
+        with torch.cuda.device(x.device):
+            n = lib().sp_groupnorm_workspace_bytes(N, F, T, C, groups, 0)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            check(lib().sp_groupnorm_fwd(ptr(x), ptr(residual), ptr(w32), ptr(b32), ptr(lengths), _gn_strides((x, residual, y)), N, F, T,
+                                         C, groups, eps, act, _lib.dtype_code(x), ptr(y), ptr(mean[0]) if train else None,
+                                         ptr(mean[1]) if train else None, ptr(ws), n, stream_ptr()), "sp_groupnorm_fwd")
+        if train:
+            ctx.save_for_backward(x, residual, w32, b32, mean, lengths)
+        ctx.cfg = (groups, act, weight.dtype, bias.dtype)
+        ctx.params = (weight, bias)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, residual, w32, b32, mean, lengths = ctx.saved_tensors
+        groups, act, wdt, bdt = ctx.cfg
+        N, F, T, C = x.shape
+        gy = _unit_last(gy.to(x.dtype))
+        gx = torch.empty((N, F, T, C), dtype=x.dtype, device=x.device)
+        # without an activation (and without frames to clear) the residual's gradient is gy itself
+        own = ctx.needs_input_grad[3] and (act != 0 or lengths is not None)
+        gres = torch.empty_like(gx) if own else None
+        sink = _sink
+        direct = sink is not None and sink.ok(*ctx.params)
+        if direct:
+            dw, db = ctx.params[0].grad, ctx.params[1].grad
+        else:
+            dw, db = torch.empty_like(w32), torch.empty_like(b32)
+        with torch.cuda.device(x.device):
+            n = lib().sp_groupnorm_workspace_bytes(N, F, T, C, groups, 1)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            check(lib().sp_groupnorm_bwd(ptr(gy), ptr(x), ptr(residual), ptr(w32), ptr(b32), ptr(mean[0]), ptr(mean[1]), ptr(lengths),
+                                         _gn_strides((gy, x, residual, gx, gres)), N, F, T, C, groups, act, int(direct),
+                                         _lib.dtype_code(x), ptr(gx), ptr(gres), ptr(dw), ptr(db), ptr(ws), n, stream_ptr()),
+                  "sp_groupnorm_bwd")
+        if ctx.needs_input_grad[3] and not own:
+            gres = gy
+        if direct:
+            sink.ready(*ctx.params)
+            return gx, None, None, gres, None, None, None, None, None
+        return gx, dw.to(wdt), db.to(bdt), gres, None, None, None, None, None
+
+
+def group_norm(x, weight, bias, groups, eps=1e-5, act="none", residual=None, lengths=None, time_major=False):
+    """act(GroupNorm(x) * weight + bias + residual), channels last, differentiable in x, weight, bias and residual.
+
+    x [N, C], [N, T, C] or [N, F, T, C] (float32 / bfloat16 / float16); statistics per sample and group over all positions and the
+    C / groups channels (f32, biased variance).  act: "none", "relu" or "silu".  residual: like x.  lengths int [N]: only frames
+    t < lengths[n] of the T dimension belong to sample n; the others are not read and come out (and back) as zeros.  Any strides are
+    taken as they are, the channel dimension excepted.  time_major=True: the result is the same tensor, laid out in memory as
+    [T, N, F, C] (the order the recurrent layers read)."""
+    _act_tensor(x, "x")
+    if x.dim() not in (2, 3, 4):
+        raise ValueError(f"x must be [N, C], [N, T, C] or [N, F, T, C], got {tuple(x.shape)}")
+    if act not in _lib.ACT_CODES:
+        raise ValueError(f"act must be one of {sorted(_lib.ACT_CODES)}, got {act!r}")
+    C = x.shape[-1]
+    if groups < 1 or C % groups:
+        raise ValueError(f"{C} channels do not divide into {groups} groups")
+    if tuple(weight.shape) != (C,) or tuple(bias.shape) != (C,):
+        raise ValueError(f"weight and bias must be [{C}]")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have x's shape and dtype")
+    _same_device(x, weight=weight, bias=bias, residual=residual, lengths=lengths)
+    shape = x.shape
+
+    def four(t):
+        return None if t is None else t.view(t.shape[0], 1, 1, C) if t.dim() == 2 else t.unsqueeze(1) if t.dim() == 3 else t
+    if lengths is not None:
+        if tuple(lengths.shape) != (shape[0],) or lengths.is_floating_point():
+            raise ValueError(f"lengths must be whole numbers [{shape[0]}]")
+        lengths = lengths.to(torch.int32).contiguous()
+    y = _GroupNormFn.apply(four(_unit_last(x)), weight, bias, four(_unit_last(residual)), lengths, int(groups), float(eps),
+                           _lib.ACT_CODES[act], bool(time_major))
+    return y if len(shape) == 4 else y.squeeze(1) if len(shape) == 3 else y.reshape(shape)
+
+
+# ------------------------------------------------------------------------------------------
+# Dropout from a counter-based generator
+# ------------------------------------------------------------------------------------------
+def _dropout(x, residual, rows, p, rng, site, used):
+    y = torch.empty_like(x)
+    with torch.cuda.device(x.device):
+        check(lib().sp_dropout(ptr(x), ptr(residual), rows, x.numel() // max(rows, 1), p, ptr(rng), site, _lib.dtype_code(x), ptr(y),
+                               ptr(used), stream_ptr()), "sp_dropout")
+    return y
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, rng, site, rows):
+        # the pair that this call used: `rng` may have moved on (one step further, in place) when the backward runs
+        used = torch.empty(2, dtype=torch.int64, device=x.device) if any(ctx.needs_input_grad) else None
+        y = _dropout(x, residual, rows, p, rng, site, used)
+        if used is not None:
+            ctx.save_for_backward(used)
+        ctx.cfg = (p, site, rows)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        (used,) = ctx.saved_tensors
+        p, site, rows = ctx.cfg
+        gx = _dropout(gy.contiguous(), None, rows, p, used, site, None) if ctx.needs_input_grad[0] else None
+        return gx, gy if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def dropout_rng(seed, device, step=0):
+    """The generator state of ops.dropout: int64 [2] = (seed, step) on the device.  Advance the step in place once per training step
+    (``rng[1] += 1``, which a captured graph may do too); data-parallel ranks take different seeds."""
+    return torch.tensor([int(seed), int(step)], dtype=torch.int64, device=device)
+
+
+def dropout(x, p, rng, site=0, residual=None, shared=False):
+    """Dropout with rate p (honoured to 2^-17), scaled by 1 / (1 - p), plus an optional residual; differentiable in x and residual.
+
+    The mask comes from a counter-based generator over (element index, rng step, site) and is never stored.  rng: see dropout_rng.
+    site: a whole number that tells the dropouts of one step apart.  shared=True: x [T, ...] drops the same elements in every frame
+    t (the variational form).  The rate is not tied to a training flag: do not call it in evaluation."""
+    _act_tensor(x, "x")
+    if not 0.0 <= float(p) <= 1.0:
+        raise ValueError(f"p must lie in [0, 1], got {p}")
+    if not torch.is_tensor(rng) or rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous():
+        raise ValueError("rng must be an int64 tensor [2] (see dropout_rng)")
+    if not 0 <= int(site) < 2 ** 31:
+        raise ValueError("site must lie in [0, 2^31)")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have x's shape and dtype")
+    if shared and x.dim() < 2:
+        raise ValueError("shared dropout needs x [T, ...]")
+    _same_device(x, rng=rng, residual=residual)
+    return _DropoutFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), float(p), rng, int(site),
+                            x.shape[0] if shared else 1)
