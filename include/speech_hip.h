@@ -391,6 +391,36 @@ int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period
                int dtype, void* y, int64_t* used, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Gated delta rule: a recurrent layer's state update beside sp_sru_* (no counterpart in the reference, whose layers are SRU,
+ * net.py:61-72).  Per utterance b and value head h, with a state S [dk][dv] (f32):
+ *   S_t = e^{g_t} S_{t-1} + kh_t u_t^T,  u_t = beta_t (v_t - e^{g_t} S_{t-1}^T kh_t),  o_t = S_t^T qh_t
+ * qh = scale * q, kh = k; with SP_GDR_NORMALIZE q and k are first divided by sqrt(|.|^2 + 1e-6).
+ * q, k: [T][B][Hk][dk], v: [T][B][H][dv] of dtype (SP_F32 / SP_F16 / SP_BF16); H % Hk == 0, value head h reads key head h / (H / Hk).
+ * g, beta: f32 [T][B][H] (g = log decay; anything below -200 decays to zero).  dk, dv: multiples of 8 up to 128.  state, state_out: f32
+ * [B][H][dk][dv] dense, state NULL = zeros, state_out may be state (updated in place).  lengths: DEVICE int32 [B] or NULL (values outside
+ * [0, T] are clamped): frames behind an utterance's end are not read, leave the state alone and come out as zeros.  SP_GDR_BIDIRECTIONAL:
+ * value heads h >= H / 2 walk each utterance's own frames backwards (Hk even).  o: [T][B][H][dv] dense.
+ * strides: HOST array of element strides (t, b, h): fwd q, k, v, g, beta (15); bwd the same and go's (18).  q, k, v, go: unit stride inside
+ * a head, addresses and strides aligned to 16 bytes (a forward of up to 32 frames without `saved` takes any).
+ * saved: NULL (inference), or sp_gdr_saved_bytes() device bytes that the forward fills and the backward reads; workspace:
+ * sp_gdr_workspace_bytes(.., backward), for an inference forward and for the backward (a forward with `saved` needs none).
+ * Backward: go = d loss / d o, gstate_out = d loss / d state_out or NULL; writes gq, gk [T][B][Hk][dk], gv [T][B][H][dv] (dense, dtype), gg,
+ * gbeta f32 [T][B][H] dense, gstate f32 or NULL; frames behind an utterance's end get zeros.  T >= 1.  Results are bit-reproducible.
+ * --------------------------------------------------------------------------------------- */
+#define SP_GDR_NORMALIZE 1
+#define SP_GDR_BIDIRECTIONAL 2
+size_t sp_gdr_workspace_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype, int backward);
+size_t sp_gdr_saved_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype);
+int sp_gdr_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const float* state,
+               const int32_t* lengths, const int64_t* strides, int T, int B, int Hk, int H, int dk, int dv, float scale, int flags,
+               int dtype, void* o, float* state_out, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+               void* stream);
+int sp_gdr_bwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const int32_t* lengths,
+               const int64_t* strides, int T, int B, int Hk, int H, int dk, int dv, float scale, int flags, int dtype, const void* o,
+               const void* saved, size_t saved_bytes, const void* go, const float* gstate_out, void* gq, void* gk, void* gv, float* gg,
+               float* gbeta, float* gstate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * General GEMM on the matrix cores, f32 accumulation:
  *     C[m][n] (+)= sum_k A(m,k) B(n,k),   A(m,k) = A[m*sam + k*sak],   B(n,k) = B[n*sbn + k*sbk]
  * Replaces every matmul the reference reaches through net.py:61-76: sru.SRU's `x.mm(weight)` and the

@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libspeech_hip.so")
 
 SP_F32, SP_F16, SP_BF16 = 0, 1, 2
 ACT_CODES = {"none": 0, "relu": 1, "silu": 2}   # SP_ACT_*
+GDR_NORMALIZE, GDR_BIDIRECTIONAL = 1, 2         # SP_GDR_*
 SUMSQ_WORDS = 1025   # SP_SUMSQ_WORDS of include/speech_hip.h
 ADAM8_BLOCK = 2048   # SP_ADAM8_BLOCK
 CONV_WGRAD_WS_WORDS = 512 * 15 * 32 * 32   # SP_CONV_WGRAD_WS_WORDS: one slab per persistent workgroup
@@ -74,6 +75,10 @@ SIGNATURES = {
     "sp_groupnorm_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
     "sp_groupnorm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp,
                               _vp, _sz, _vp]),
+    "sp_gdr_workspace_bytes": (_sz, [_i] * 8),
+    "sp_gdr_saved_bytes": (_sz, [_i] * 7),
+    "sp_gdr_fwd": (_i, [_vp] * 8 + [_i] * 6 + [_f, _i, _i] + [_vp] * 3 + [_sz, _vp, _sz, _vp]),
+    "sp_gdr_bwd": (_i, [_vp] * 7 + [_i] * 6 + [_f, _i, _i] + [_vp, _vp, _sz] + [_vp] * 9 + [_sz, _vp]),
     "sp_dropout": (_i, [_vp, _vp, _i64, _i64, _c.c_double, _vp, _i, _i, _vp, _vp, _vp]),
 }
 

@@ -1057,3 +1057,155 @@ def dropout(x, p, rng, site=0, residual=None, shared=False):
     _same_device(x, rng=rng, residual=residual)
     return _DropoutFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), float(p), rng, int(site),
                             x.shape[0] if shared else 1)
+
+
+# ------------------------------------------------------------------------------------------
+# Gated delta rule
+# ------------------------------------------------------------------------------------------
+def _head_rows(t, gates=False):
+    """t as the kernels take it: unit stride inside a head, 16-byte aligned rows (gates: any strides); a copy where it is not."""
+    if gates:
+        return t
+    ve = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % ve == 0 for s in t.stride()[:-1]):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _gdr_strides(tensors):
+    return _host_i64([s for t in tensors for s in t.stride()[:3]])
+
+
+def _gdr_fwd(q, k, v, g, beta, state, state_out, lengths, scale, flags, train):
+    T, B, Hk, dk = q.shape
+    H, dv = v.shape[2:]
+    dims = (T, B, Hk, H, dk, dv)
+    code = _lib.dtype_code(q)
+    o = torch.empty((T, B, H, dv), dtype=v.dtype, device=v.device)
+    saved = ws = None
+    ns = nw = 0
+    with torch.cuda.device(q.device):
+        if train:
+            ns = lib().sp_gdr_saved_bytes(*dims, code)
+            saved = torch.empty(ns, dtype=torch.uint8, device=q.device)
+        else:
+            nw = lib().sp_gdr_workspace_bytes(*dims, code, 0)
+            ws = torch.empty(nw, dtype=torch.uint8, device=q.device)
+        check(lib().sp_gdr_fwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(state), ptr(lengths), _gdr_strides((q, k, v, g, beta)), *dims,
+                               scale, flags, code, ptr(o), ptr(state_out), ptr(saved), ns, ptr(ws), nw, stream_ptr()), "sp_gdr_fwd")
+    return o, saved
+
+
+class _GatedDeltaFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, lengths, scale, flags):
+        train = any(ctx.needs_input_grad)
+        T, B, Hk, dk = q.shape
+        H, dv = v.shape[2:]
+        final = torch.empty((B, H, dk, dv), dtype=torch.float32, device=v.device)
+        o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, scale, flags, train)
+        if train:
+            ctx.save_for_backward(q, k, v, g, beta, lengths, o, saved)
+        ctx.cfg = (scale, flags)
+        ctx.set_materialize_grads(False)
+        return o, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go, gstate):
+        q, k, v, g, beta, lengths, o, saved = ctx.saved_tensors
+        scale, flags = ctx.cfg
+        T, B, Hk, dk = q.shape
+        H, dv = v.shape[2:]
+        dims = (T, B, Hk, H, dk, dv)
+        dev, code = q.device, _lib.dtype_code(q)
+        go = _head_rows(go) if go is not None else torch.zeros_like(o)
+        gstate = gstate.contiguous() if gstate is not None else None
+        gq = torch.empty((T, B, Hk, dk), dtype=q.dtype, device=dev)
+        gk = torch.empty_like(gq)
+        gv = torch.empty((T, B, H, dv), dtype=v.dtype, device=dev)
+        gg, gb = torch.empty((2, T, B, H), dtype=torch.float32, device=dev).unbind(0)
+        gs0 = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
+        with torch.cuda.device(dev):
+            nw = lib().sp_gdr_workspace_bytes(*dims, code, 1)
+            ws = torch.empty(nw, dtype=torch.uint8, device=dev)
+            check(lib().sp_gdr_bwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(lengths), _gdr_strides((q, k, v, g, beta, go)), *dims, scale,
+                                   flags, code, ptr(o), ptr(saved), saved.numel(), ptr(go), ptr(gstate), ptr(gq), ptr(gk), ptr(gv), ptr(gg),
+                                   ptr(gb), ptr(gs0), ptr(ws), nw, stream_ptr()), "sp_gdr_bwd")
+        return gq, gk, gv, gg, gb, gs0, None, None, None
+
+
+def _gdr_check(q, k, v, g, beta, state, lead):
+    _act_tensor(q, "q")
+    if q.dim() != len(lead) + 2 or k.shape != q.shape or v.dim() != q.dim() or v.shape[:-2] != q.shape[:-2]:
+        raise ValueError(f"q and k must be [{', '.join(lead)}, Hk, dk] and v [{', '.join(lead)}, H, dv], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one dtype")
+    Hk, dk = q.shape[-2:]
+    H, dv = v.shape[-2:]
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{H} value heads do not share {Hk} key heads evenly")
+    if not (8 <= dk <= 128 and dk % 8 == 0 and 8 <= dv <= 128 and dv % 8 == 0):
+        raise ValueError(f"head widths must be multiples of 8 up to 128, got dk={dk}, dv={dv}")
+    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1] or not g.is_floating_point() or not beta.is_floating_point():
+        raise ValueError(f"g and beta must be floating point [{', '.join(lead)}, H]")
+    B = q.shape[-3]
+    if state is not None and (tuple(state.shape) != (B, H, dk, dv) or state.dtype != torch.float32):
+        raise ValueError(f"state must be float32 {(B, H, dk, dv)}")
+    _same_device(q, k=k, v=v, g=g, beta=beta, state=state)
+    return B, Hk, dk, H, dv
+
+
+def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, normalize=False, bidirectional=False):
+    """The gated delta rule over a sequence -> (o [T, B, H, dv] in v's dtype, final state f32 [B, H, dk, dv]), differentiable in q, k, v,
+    g, beta and state:
+
+        S_t = exp(g_t) S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),   o_t = S_t^T (scale q_t)
+
+    q, k [T, B, Hk, dk] and v [T, B, H, dv] (time-major like the SRU stack; float32 / bfloat16 / float16; dk, dv multiples of 8 up to
+    128): H a multiple of Hk, H / Hk consecutive value heads share a key head.  g (log decay) and beta [T, B, H] are taken in float32.
+    state: the state before the first frame (zeros).  lengths int [B]: frames t >= lengths[b] are not read, leave the state alone and come
+    out (and back) as zeros.  scale: default dk ** -0.5.  normalize=True divides q and k by sqrt(|.|^2 + 1e-6) first.  bidirectional=True:
+    the second half of the heads walks each utterance's own frames backwards (Hk even)."""
+    B, Hk, dk, H, dv = _gdr_check(q, k, v, g, beta, state, ("T", "B"))
+    if bidirectional and Hk % 2:
+        raise ValueError(f"both directions need an even number of key heads, not {Hk}")
+    if lengths is not None:
+        _same_device(q, lengths=lengths)
+        if tuple(lengths.shape) != (B,) or lengths.is_floating_point():
+            raise ValueError(f"lengths must be whole numbers [{B}]")
+        lengths = lengths.to(torch.int32).contiguous()
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if scale == 0.0 or not math.isfinite(scale):
+        raise ValueError(f"scale must be finite and not zero, got {scale}")
+    if state is not None:
+        state = state.contiguous()
+        if state.data_ptr() % 16:
+            state = state.clone()
+    if q.shape[0] == 0 or B == 0:
+        final = torch.zeros((B, H, dk, dv), dtype=torch.float32, device=q.device) if state is None else state.clone()
+        return torch.zeros_like(v), final
+    flags = (_lib.GDR_NORMALIZE if normalize else 0) | (_lib.GDR_BIDIRECTIONAL if bidirectional else 0)
+    return _GatedDeltaFn.apply(_head_rows(q), _head_rows(k), _head_rows(v), g.float(), beta.float(), state, lengths, scale, flags)
+
+
+@torch.no_grad()
+def gated_delta_step(q, k, v, g, beta, state, scale=None, normalize=False):
+    """One frame of gated_delta_rule for serving: q, k [B, Hk, dk], v [B, H, dv], g, beta [B, H] -> o [B, H, dv]; `state` (float32,
+    contiguous [B, H, dk, dv]) is updated in place.  Not differentiable."""
+    B, Hk, dk, H, dv = _gdr_check(q, k, v, g, beta, state, ("B",))
+    if state is None or not state.is_contiguous() or state.data_ptr() % 16:
+        raise ValueError("state must be a contiguous, 16-byte aligned tensor: it is updated in place")
+    if state.requires_grad:
+        raise ValueError("state requires a gradient: gated_delta_step updates it in place and is not differentiable")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if scale == 0.0 or not math.isfinite(scale):
+        raise ValueError(f"scale must be finite and not zero, got {scale}")
+    if B == 0:
+        return torch.zeros_like(v)
+    q, k, v, g, beta = (_unit_last(t) if t.dim() == 3 else t for t in (q, k, v, g.float(), beta.float()))
+    o, _ = _gdr_fwd(q[None], k[None], v[None], g[None], beta[None], state, state, None, scale,
+                    _lib.GDR_NORMALIZE if normalize else 0, False)
+    return o[0]
