@@ -15,9 +15,10 @@
 //     dg = suffix sums of dO_i.O_i - dV_i.V_i, plus <dS, S_C> at the chunk's end (every other dependence on G cancels)
 //
 // Arithmetic: the state, the chunk matrices and every sum are f32.  Products run on v_mfma_f32_16x16x32_bf16 with operands split into
-// bf16 parts (x = hi + lo [+ lo2]): an input of type bf16 is one exact part, f16 two, f32 three; what is derived (S, U, X, ...) two, for
-// f32 inputs three.  Two parts carry 2^-17, so that the f32 results (states, dg, dbeta) keep about 1e-6; one part of everything would be
-// four times cheaper on the matrix cores and leave 1e-3.  Outputs of 16-bit type are rounded once.
+// bf16 parts (x = hi + mid + lo): an input of type bf16 is one exact part, f16 two, f32 three; what is derived (S, U, X, ...) three, which
+// is all of an f32's mantissa, wherever a result of 32 bits (states, dg, dbeta) hangs on it.  With two parts those results were off by
+// 3e-6 to 1e-5 instead of 3e-7; the f32 matrix instruction costs 5.3 times a bf16 one, three to six bf16 products at most as much.  What
+// only reaches a 16-bit output (o, dq, dk) takes two parts.  Outputs of 16-bit type are rounded once.
 //
 // Kernels: prep (N, P, X of a chunk; all chunks at once) -> scan (walks the chunks with S in registers; a wave owns 32 columns of dv and
 // never talks to the others: the accumulator layout of one product is the B operand of the next) ; backward: rscan (the same walk in
@@ -30,9 +31,11 @@ constexpr int kC = 64;              // frames a chunk
 constexpr int kRecurrentMax = 32;   // frames up to which the recurrent kernel runs (inference)
 constexpr int kLdm = 72;            // row pitch (elements) of a 64 x 64 matrix plane in LDS: 16 rows of 8 bytes fall on distinct banks
 constexpr int kVec = 8;             // per-chunk vectors of 64 floats: aq, ak, kb, beta, rk, sq, G (as 64 doubles)
+constexpr int kTri = 10 * 256;      // a lower triangular 64 x 64 matrix: ten 16 x 16 blocks (row block major), f32
 enum { kAq = 0, kAk = 1, kKb = 2, kBe = 3, kRk = 4, kSq = 5, kG64 = 6 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -47,21 +50,21 @@ struct GdrArgs {
     const float *g, *beta, *s0;
     const int32_t* lengths;
     int64_t qs[3], ks[3], vs[3], gs[3], bs[3];       // element strides (t, b, h)
-    int T, B, Hk, H, r, dk, dv, nc, nsl;             // nsl: slices of 32 columns
+    int T, B, Hk, H, r, dk, dv, nc, nsl;             // nsl: slices of 16 columns of dv
     float scale;
     int norm, bidir;
     void* o;
     float* sT;
     // kept between the kernels (and, in training, for the backward)
     float* vec;              // [bh][nc][kVec][64]
-    __bf16 *X, *P;           // [bh][nc][planes][64][64]
-    float *S0, *E;           // [bh][nc][dk][dv], [bh][nc][64][dv]
-    __bf16* olo;             // [T][B][H][dv]: what o's 16-bit rounding dropped
+    float *X, *P;            // [bh][nc][kTri]
+    float* S0;               // [bh][nc][dk][dv]: the state at the chunk's start
     // backward
     const void* go;
     const float* gsT;
-    float* dS;               // [bh][nc][dk][dv]
-    float *xpart, *bpart;    // [nsl][bh][nc][64]
+    float* dS;               // [bh][nc][dk][dv]: the state's gradient at the chunk's end
+    void* E;                 // [bh][nc][64][dv] (bf16 for bf16 inputs, else f32)
+    float *zpart, *bpart;    // [nsl][bh][nc][64]: dO.O - dV.V and E.F over 16 columns
     float* apart;            // [nsl][bh][nc]
     void *gq, *gk, *gv;
     float *gg, *gbeta, *gs0;
@@ -69,10 +72,11 @@ struct GdrArgs {
 };
 
 // ---- operand fragments --------------------------------------------------------------------------------
+// PT: parts of an input; OP: parts that reach a 16-bit output; EP: parts of P in o's product; ET: type that E is kept in for dq and dk
 template <typename T> struct Gd;
-template <> struct Gd<__hip_bfloat16> { static constexpr int PT = 1, PD = 2; };
-template <> struct Gd<__half> { static constexpr int PT = 2, PD = 2; };
-template <> struct Gd<float> { static constexpr int PT = 3, PD = 3; };
+template <> struct Gd<__hip_bfloat16> { static constexpr int PT = 1, OP = 2, EP = 1; using ET = __hip_bfloat16; };
+template <> struct Gd<__half> { static constexpr int PT = 2, OP = 2, EP = 2; using ET = float; };
+template <> struct Gd<float> { static constexpr int PT = 3, OP = 3, EP = 3; using ET = float; };
 
 template <int P> struct Frag { bf16x8 p[P]; };
 
@@ -250,30 +254,90 @@ __device__ __forceinline__ void stage(T* dst, int ld, const T* src, int64_t ts, 
         for (int j = 0; j < Q; ++j) d[j] = v[j];
     }
 }
-// dense [planes][64][64] bf16 -> LDS planes of pitch kLdm
-__device__ __forceinline__ void stage_planes(__bf16* dst, const __bf16* src, int planes, int tid, int nt) {
-    for (int i = tid; i < planes * kC * 8; i += nt) {
-        const int row = i >> 3, c = (i & 7) * 8;
-        *reinterpret_cast<u32x4a*>(dst + row * kLdm + c) = *reinterpret_cast<const u32x4a*>(src + row * kC + c);
+// A thread's share of a tile of 64 frames x COLS columns on its way from global memory to LDS: requested a chunk ahead, in registers.
+template <typename T, int COLS, int NT> struct TileRegs {
+    static constexpr int Q = sizeof(T) / 2, N = (kC * COLS / 8 + NT - 1) / NT;
+    u32x4a v[N][Q];
+    __device__ __forceinline__ void load(const T* src, int64_t ts, int ncol, int pos0, Walk w) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8, p = pos0 + row;
+#pragma unroll
+            for (int j = 0; j < Q; ++j) v[n][j] = u32x4a{0, 0, 0, 0};
+            if (row < kC && p < w.len && c < ncol) {
+                const u32x4a* s = reinterpret_cast<const u32x4a*>(src + w.frame(p) * ts + c);
+#pragma unroll
+                for (int j = 0; j < Q; ++j) v[n][j] = s[j];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* dst, int ld) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
+            if (row < kC) {
+                u32x4a* d = reinterpret_cast<u32x4a*>(dst + row * ld + c);
+#pragma unroll
+                for (int j = 0; j < Q; ++j) d[j] = v[n][j];
+            }
+        }
+    }
+};
+// the same for a lower triangular matrix, split into bf16 planes when it is stored
+template <int NT> struct TriRegs {
+    static constexpr int N = (kTri / 4 + NT - 1) / NT;
+    f32x4a v[N];
+    __device__ __forceinline__ void load(const float* src) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x + n * NT;
+            if (i < kTri / 4) v[n] = reinterpret_cast<const f32x4a*>(src)[i];
+        }
+    }
+    template <int P> __device__ __forceinline__ void store(__bf16* dst) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x + n * NT, blk = i >> 6;
+            if (i < kTri / 4) {
+                const int bi = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, bj = blk - bi * (bi + 1) / 2;
+                __bf16* d = dst + (16 * bi + ((i >> 2) & 15)) * kLdm + 16 * bj + 4 * (i & 3);
+                f32x4 x = v[n];
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                    const bf16x4 h = __builtin_convertvector(x, bf16x4);
+                    *reinterpret_cast<u32x2a*>(d + e * kC * kLdm) = __builtin_bit_cast(u32x2a, h);
+                    x -= __builtin_convertvector(h, f32x4);
+                }
+            }
+        }
+    }
+};
+// the blocks right of the diagonal that products over 32 columns touch: (0, 1) and (2, 3)
+__device__ __forceinline__ void clear_upper(__bf16* t, int planes, int tid, int nt) {
+    for (int i = tid; i < planes * 64; i += nt) {
+        const int pl = i >> 6, row = (i >> 1) & 31, half = i & 1;
+        const int r = row & 15, blk = (row >> 4) * 2;
+        *reinterpret_cast<u32x4a*>(t + pl * kC * kLdm + (16 * blk + r) * kLdm + 16 * (blk + 1) + 8 * half) = u32x4a{0, 0, 0, 0};
     }
 }
 
 // ---- prep -----------------------------------------------------------------------------------------------
 template <typename T, int DK> struct PrepLds {
     static constexpr int LDK = DK + 8, LDN = kC + 4;
-    static constexpr size_t bytes = (size_t)2 * kC * LDK * sizeof(T) + (size_t)2 * kC * LDN * 4 + 4 * 16 * 20 * 4 + kVec * kC * 4;
+    static constexpr size_t in = (size_t)2 * kC * LDK * sizeof(T), mat = (size_t)2 * kC * LDN * 4;
+    static constexpr size_t bytes = (in > mat ? in : mat) + 4 * 16 * 20 * 4 + kVec * kC * 4;
 };
 
-template <typename T, int DK, int NP>
+template <typename T, int DK>
 __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = PrepLds<T, DK>;
-    constexpr int PD = Gd<T>::PD, LDK = L::LDK, LDN = L::LDN;
+    constexpr int LDK = L::LDK, LDN = L::LDN;
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
-    float* N = reinterpret_cast<float*>(Ql + kC * LDK);
+    float* N = reinterpret_cast<float*>(smem);    // over K and Q once their products are done
     float* P = N + kC * LDN;
-    float* Tb = P + kC * LDN;                 // [4][16][20]
+    float* Tb = reinterpret_cast<float*>(smem + (L::in > L::mat ? L::in : L::mat));   // [4][16][20]
     float* vec = Tb + 4 * 16 * 20;
     double* G = reinterpret_cast<double*>(vec + kG64 * kC);
     const int c = blockIdx.x % a.nc, bh = blockIdx.x / a.nc, b = bh / a.H, h = bh % a.H, hk = h / a.r;
@@ -317,28 +381,36 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     }
     __syncthreads();
     // wave = block column of N and P
-    for (int m = 0; m < 4; ++m) {
-        f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
-        if (m >= wave) {
+    f32x4 kk[4], qk[4];
 #pragma unroll
-            for (int kb = 0; kb < DK / 32; ++kb) {
-                const auto bf = row_frag(Kl, LDK, 16 * wave, 32 * kb);
-                kk = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), bf, kk);
-                qk = mma(row_frag(Ql, LDK, 16 * m, 32 * kb), bf, qk);
-            }
-            const int j = 16 * wave + (l & 15);
-            const float rkj = vec[kRk * kC + j];
-            const double gj = G[j];
+    for (int m = 0; m < 4; ++m) { kk[m] = f32x4{0, 0, 0, 0}; qk[m] = kk[m]; }
+#pragma unroll
+    for (int kb = 0; kb < DK / 32; ++kb) {
+        const auto bf = row_frag(Kl, LDK, 16 * wave, 32 * kb);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if (m < wave) continue;
+            kk[m] = mma<Gd<T>::PT, Gd<T>::PT, 3>(row_frag(Kl, LDK, 16 * m, 32 * kb), bf, kk[m]);
+            qk[m] = mma<Gd<T>::PT, Gd<T>::PT, 3>(row_frag(Ql, LDK, 16 * m, 32 * kb), bf, qk[m]);
+        }
+    }
+    __syncthreads();
+    {
+        const int j = 16 * wave + (l & 15);
+        const float rkj = vec[kRk * kC + j];
+        const double gj = G[j];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 16 * m + 4 * (l >> 4) + e;
                 const float d = i >= j ? __expf((float)(G[i] - gj)) * rkj : 0.f;
-                kk[e] = i > j ? kk[e] * d * vec[kRk * kC + i] : 0.f;
-                qk[e] = i >= j ? qk[e] * d * vec[kSq * kC + i] : 0.f;
+                kk[m][e] = i > j ? kk[m][e] * d * vec[kRk * kC + i] : 0.f;
+                qk[m][e] = i >= j ? qk[m][e] * d * vec[kSq * kC + i] : 0.f;
             }
+            tile_write(N, LDN, 16 * m, 16 * wave, kk[m]);
+            tile_write(P, LDN, 16 * m, 16 * wave, qk[m]);
         }
-        tile_write(N, LDN, 16 * m, 16 * wave, kk);
-        tile_write(P, LDN, 16 * m, 16 * wave, qk);
     }
     __syncthreads();
     {   // diagonal block `wave` of (I + N diag(beta))^-1 by substitution: lane = column, all lane groups alike
@@ -387,32 +459,26 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     for (int i = 0; i < 4; ++i) tile_write(N, LDN, 16 * i, 16 * wave, X[i]);
     __syncthreads();
     const int64_t at = (int64_t)bh * a.nc + c;
-    __bf16* Xo = a.X + at * PD * kC * kC;
-    __bf16* Po = a.P + at * NP * kC * kC;
-    for (int i = tid; i < kC * 8; i += 256) {
-        const int row = i >> 3, col = (i & 7) * 8;
-        const float* x = N + row * LDN + col;
-        const float* p = P + row * LDN + col;
-        const Frag<PD> xf = split<PD>(*reinterpret_cast<const f32x4a*>(x), *reinterpret_cast<const f32x4a*>(x + 4));
-        const Frag<NP> pf = split<NP>(*reinterpret_cast<const f32x4a*>(p), *reinterpret_cast<const f32x4a*>(p + 4));
-#pragma unroll
-        for (int e = 0; e < PD; ++e) *reinterpret_cast<bf16x8*>(Xo + e * kC * kC + row * kC + col) = xf.p[e];
-#pragma unroll
-        for (int e = 0; e < NP; ++e) *reinterpret_cast<bf16x8*>(Po + e * kC * kC + row * kC + col) = pf.p[e];
+    for (int i = tid; i < kTri / 4; i += 256) {
+        const int blk = i >> 6, bi = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, bj = blk - bi * (bi + 1) / 2;
+        const int src = (16 * bi + ((i >> 2) & 15)) * LDN + 16 * bj + 4 * (i & 3);
+        reinterpret_cast<f32x4a*>(a.X + at * kTri)[i] = *reinterpret_cast<const f32x4a*>(N + src);
+        reinterpret_cast<f32x4a*>(a.P + at * kTri)[i] = *reinterpret_cast<const f32x4a*>(P + src);
     }
     float* vo = a.vec + at * kVec * kC;
     for (int i = tid; i < kVec * kC; i += 256) vo[i] = vec[i];
 }
 
 // ---- scan -----------------------------------------------------------------------------------------------
-// rows [64][32 columns of this wave] from LDS to frames of a [T][B][H][dv] tensor, 16 bytes a lane; frames behind the end get nothing
-template <typename T>
-__device__ __forceinline__ void store_rows(const T* src, int ld, T* dst, int64_t ts, int ncol, int pos0, Walk w) {
+// rows [64][16 columns of this wave] from LDS to global rows, 16 bytes a lane
+template <typename T, typename F>
+__device__ __forceinline__ void store_rows(const T* src, int ld, int ncol, int rows, F&& dst) {
     const int l = threadIdx.x & 63;
-    constexpr int VE = 16 / sizeof(T), LPR = 32 / VE;       // elements a lane, lanes a row
+    constexpr int VE = 16 / sizeof(T), LPR = 16 / VE;       // elements a lane, lanes a row
+#pragma unroll
     for (int r = l / LPR; r < kC; r += 64 / LPR) {
-        const int p = pos0 + r, c = (l % LPR) * VE;
-        if (p < w.len && c < ncol) *reinterpret_cast<u32x4a*>(dst + w.frame(p) * ts + c) = *reinterpret_cast<const u32x4a*>(src + r * ld + c);
+        const int c = (l % LPR) * VE;
+        if (r < rows && c < ncol) *reinterpret_cast<u32x4a*>(dst(r) + c) = *reinterpret_cast<const u32x4a*>(src + r * ld + c);
     }
 }
 template <typename T>
@@ -423,430 +489,411 @@ __device__ __forceinline__ void zero_rows(T* dst, int64_t ts, int ncol, int from
         *reinterpret_cast<u32x4a*>(dst + (from + i / vpr) * ts + (i % vpr) * VE) = u32x4a{0, 0, 0, 0};
 }
 
-template <typename T, int DK, int NW, int NP> struct ScanLds {
-    static constexpr int LDK = DK + 8, LDV = NW * 32 + 8;
-    static constexpr size_t bytes = (size_t)kC * (2 * LDK + LDV) * sizeof(T) + (size_t)(Gd<T>::PD + NP) * kC * kLdm * 2 + kVec * kC * 4;
+template <typename T, int DK, int NW> struct ScanLds {
+    static constexpr int LDK = DK + 8, LDV = NW * 16 + 8;
+    static constexpr size_t bytes = (size_t)kC * (2 * LDK + LDV) * sizeof(T) + (size_t)(3 + Gd<T>::EP) * kC * kLdm * 2 + kVec * kC * 4;
 };
 
-template <typename T, int DK, int NW, int NP, bool TRAIN>
+// B operands (inner index = rows of the accumulators) of 64 frames: row tiles 2 kb and 2 kb + 1, each scaled by a vector
+template <int P> __device__ __forceinline__ void row_operands(Frag<P> (&f)[2], const float* scale, const f32x4 (&t)[4]) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) f[kb] = split<P>(vec4(scale, 32 * kb) * t[2 * kb], vec4(scale, 32 * kb + 16) * t[2 * kb + 1]);
+}
+
+// A wave owns 16 columns of dv: the state's columns, U's, O's.  Only K, Q, X, P and the vectors are shared (LDS, filled a chunk ahead
+// through registers); two barriers a chunk.
+template <typename T, int DK, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
-    using L = ScanLds<T, DK, NW, NP>;
-    constexpr int PD = Gd<T>::PD, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    using L = ScanLds<T, DK, NW>;
+    constexpr int NT = NW * 64, EP = Gd<T>::EP, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
     T* Vl = Ql + kC * LDK;
     __bf16* Xl = reinterpret_cast<__bf16*>(Vl + kC * LDV);
-    __bf16* Pl = Xl + PD * kC * kLdm;
-    float* vec = reinterpret_cast<float*>(Pl + NP * kC * kLdm);
+    __bf16* Pl = Xl + 3 * kC * kLdm;
+    float* vec = reinterpret_cast<float*>(Pl + EP * kC * kLdm);
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
     const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6, g = l >> 4, i16 = l & 15;
-    const int col0 = (sg * NW + wave) * 32;                 // this wave's columns of dv
-    const int vcols = min(a.dv - sg * NW * 32, NW * 32), mycols = a.dv - col0;
+    const int col0 = (sg * NW + wave) * 16, col = col0 + i16;     // this wave's columns of dv
+    const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv;
-    f32x4 S[KT][2];
+    f32x4 S[KT];
 #pragma unroll
     for (int m = 0; m < KT; ++m)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * m + 4 * g + e, col = col0 + 16 * ct + i16;
-                S[m][ct][e] = a.s0 && row < a.dk && col < a.dv ? a.s0[state + (int64_t)row * a.dv + col] : 0.f;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * m + 4 * g + e;
+            S[m][e] = a.s0 && row < a.dk && col < a.dv ? a.s0[state + (int64_t)row * a.dv + col] : 0.f;
+        }
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
-    const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 32;
+    const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 16;
     const int64_t ots = (int64_t)a.B * a.H * a.dv;
     T* op = (T*)a.o + ((int64_t)b * a.H + h) * a.dv;
     const int ncl = (w.len + kC - 1) / kC;
+    TileRegs<T, DK, NT> rk, rq;
+    TileRegs<T, NW * 16, NT> rv;
+    TriRegs<NT> rx, rp;
+    float rvec[kVec * kC / NT];
+    auto fetch = [&](int c) {
+        const int64_t at = (int64_t)bh * a.nc + c;
+        rk.load(kp, a.ks[0], a.dk, c * kC, w);
+        rq.load(qp, a.qs[0], a.dk, c * kC, w);
+        rv.load(vp, a.vs[0], vcols, c * kC, w);
+        rx.load(a.X + at * kTri);
+        rp.load(a.P + at * kTri);
+#pragma unroll
+        for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
+    };
+    clear_upper(Xl, 3 + EP, tid, NT);
+    if (ncl > 0) fetch(0);
     for (int c = 0; c < ncl; ++c) {
         const int64_t at = (int64_t)bh * a.nc + c;
         __syncthreads();
-        stage(Kl, LDK, kp, a.ks[0], a.dk, DK, c * kC, w, tid, NW * 64);
-        stage(Ql, LDK, qp, a.qs[0], a.dk, DK, c * kC, w, tid, NW * 64);
-        stage(Vl, LDV, vp, a.vs[0], vcols, NW * 32, c * kC, w, tid, NW * 64);
-        stage_planes(Xl, a.X + at * PD * kC * kC, PD, tid, NW * 64);
-        stage_planes(Pl, a.P + at * NP * kC * kC, NP, tid, NW * 64);
-        for (int i = tid; i < kVec * kC; i += NW * 64) vec[i] = a.vec[at * kVec * kC + i];
+        rk.store(Kl, LDK);
+        rq.store(Ql, LDK);
+        rv.store(Vl, LDV);
+        rx.template store<3>(Xl);
+        rp.template store<EP>(Pl);
+#pragma unroll
+        for (int i = 0; i < kVec * kC / NT; ++i) vec[i * NT + tid] = rvec[i];
         __syncthreads();
+        if (c + 1 < ncl) fetch(c + 1);
         if (mycols <= 0) continue;
-        if (TRAIN) {      // the state at the chunk's start, for the backward
+        if (TRAIN) {      // for the backward
             float* so = a.S0 + at * a.dk * a.dv;
 #pragma unroll
             for (int m = 0; m < KT; ++m)
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = 16 * m + 4 * g + e, col = col0 + 16 * ct + i16;
-                        if (row < a.dk && col < a.dv) so[(int64_t)row * a.dv + col] = S[m][ct][e];
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 16 * m + 4 * g + e;
+                    if (row < a.dk && col < a.dv) so[(int64_t)row * a.dv + col] = S[m][e];
+                }
         }
-        f32x4 ks[4][2], qs[4][2];
+        f32x4 ks[4], qs[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) { ks[m][ct] = f32x4{0, 0, 0, 0}; qs[m][ct] = f32x4{0, 0, 0, 0}; }
+        for (int m = 0; m < 4; ++m) { ks[m] = f32x4{0, 0, 0, 0}; qs[m] = ks[m]; }
 #pragma unroll
         for (int kb = 0; kb < DK / 32; ++kb) {
-            Frag<PD> sb[2];
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) sb[ct] = split<PD>(S[2 * kb][ct], S[2 * kb + 1][ct]);
+            const Frag<3> sb = split<3>(S[2 * kb], S[2 * kb + 1]);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const auto kf = row_frag(Kl, LDK, 16 * m, 32 * kb);
-                const auto qf = row_frag(Ql, LDK, 16 * m, 32 * kb);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) { ks[m][ct] = mma(kf, sb[ct], ks[m][ct]); qs[m][ct] = mma(qf, sb[ct], qs[m][ct]); }
+                ks[m] = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), sb, ks[m]);
+                qs[m] = mma<Gd<T>::PT, 3, OP>(row_frag(Ql, LDK, 16 * m, 32 * kb), sb, qs[m]);
             }
         }
         // Vt in ks; O's first part in qs
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const f32x4 ak = vec4(vec + kAk * kC, 16 * m), aq = vec4(vec + kAq * kC, 16 * m);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                ks[m][ct] = tile_read(Vl, LDV, 16 * m, wave * 32 + 16 * ct) - ak * ks[m][ct];
-                qs[m][ct] *= aq;
-            }
+            ks[m] = tile_read(Vl, LDV, 16 * m, wave * 16) - vec4(vec + kAk * kC, 16 * m) * ks[m];
+            qs[m] *= vec4(vec + kAq * kC, 16 * m);
         }
-        Frag<PD> uf[2][2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const f32x4 b0 = vec4(vec + kBe * kC, 32 * kb), b1 = vec4(vec + kBe * kC, 32 * kb + 16);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) uf[kb][ct] = split<PD>(b0 * ks[2 * kb][ct], b1 * ks[2 * kb + 1][ct]);
-        }
+        Frag<3> uf[2];
+        row_operands(uf, vec + kBe * kC, ks);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {      // E = Vt - X (beta Vt); X is lower triangular: row tiles 0, 1 need the first 32 columns only
-            f32x4 xs[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+            f32x4 xs = {0, 0, 0, 0};
 #pragma unroll
-            for (int kb = 0; kb <= m / 2; ++kb) {
-                const Frag<PD> xf = plane_rows<PD>(Xl, 16 * m, 32 * kb);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) xs[ct] = mma(xf, uf[kb][ct], xs[ct]);
-            }
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) ks[m][ct] -= xs[ct];
-        }
-        if (TRAIN) {
-            float* eo = a.E + at * kC * a.dv;
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int col = col0 + 16 * ct + i16;
-                        if (col < a.dv) eo[(int64_t)(16 * m + 4 * g + e) * a.dv + col] = ks[m][ct][e];
-                    }
+            for (int kb = 0; kb <= m / 2; ++kb) xs = mma(plane_rows<3>(Xl, 16 * m, 32 * kb), uf[kb], xs);
+            ks[m] = (ks[m] - xs) * vec4(vec + kBe * kC, 16 * m);      // U
         }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const f32x4 b0 = vec4(vec + kBe * kC, 32 * kb), b1 = vec4(vec + kBe * kC, 32 * kb + 16);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                ks[2 * kb][ct] *= b0;
-                ks[2 * kb + 1][ct] *= b1;
-                uf[kb][ct] = split<PD>(ks[2 * kb][ct], ks[2 * kb + 1][ct]);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-#pragma unroll
-            for (int kb = 0; kb <= m / 2; ++kb) {
-                const Frag<NP> pf = plane_rows<NP>(Pl, 16 * m, 32 * kb);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) qs[m][ct] = mma(pf, uf[kb][ct], qs[m][ct]);
-            }
-        }
-        // O leaves through this wave's own columns of the V tile, which it has read
-        lds_order();
-        T* my = Vl + wave * 32;
+        for (int kb = 0; kb < 2; ++kb) uf[kb] = split<3>(ks[2 * kb], ks[2 * kb + 1]);
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) tile_write(my, LDV, 16 * m, 16 * ct, qs[m][ct]);
+            for (int kb = 0; kb <= m / 2; ++kb) qs[m] = mma<EP, 3, OP>(plane_rows<EP>(Pl, 16 * m, 32 * kb), uf[kb], qs[m]);
+        // O leaves through this wave's own columns of the V tile, which it has read
         lds_order();
-        store_rows(my, LDV, op + col0, ots, mycols, c * kC, w);
-        if (TRAIN && sizeof(T) == 2) {      // what the rounding dropped (dO . O needs O in 32 bits)
+        T* my = Vl + wave * 16;
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) qs[m][ct] -= tile_read(my, LDV, 16 * m, 16 * ct);
-            lds_order();
-            __hip_bfloat16* lo = reinterpret_cast<__hip_bfloat16*>(my);
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) tile_write(lo, LDV, 16 * m, 16 * ct, qs[m][ct]);
-            lds_order();
-            store_rows(lo, LDV, reinterpret_cast<__hip_bfloat16*>(a.olo) + ((int64_t)b * a.H + h) * a.dv + col0, ots, mycols, c * kC, w);
-        }
+        for (int m = 0; m < 4; ++m) tile_write(my, LDV, 16 * m, 0, qs[m]);
+        lds_order();
+        store_rows(my, LDV, mycols, w.len - c * kC, [&](int r) { return op + w.frame(c * kC + r) * ots + col0; });
         // S = e^{G_C} S + K^T (kb U)
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const f32x4 b0 = vec4(vec + kKb * kC, 32 * kb), b1 = vec4(vec + kKb * kC, 32 * kb + 16);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) uf[kb][ct] = split<PD>(b0 * ks[2 * kb][ct], b1 * ks[2 * kb + 1][ct]);
-        }
+        row_operands(uf, vec + kKb * kC, ks);
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
+            S[m] *= dec;
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) S[m][ct] *= dec;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const auto kf = col_frag(Kl, LDK, 32 * kb, 16 * m);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) S[m][ct] = mma(kf, uf[kb][ct], S[m][ct]);
-            }
+            for (int kb = 0; kb < 2; ++kb) S[m] = mma(col_frag(Kl, LDK, 32 * kb, 16 * m), uf[kb], S[m]);
         }
     }
 #pragma unroll
     for (int m = 0; m < KT; ++m)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * m + 4 * g + e, col = col0 + 16 * ct + i16;
-                if (row < a.dk && col < a.dv) a.sT[state + (int64_t)row * a.dv + col] = S[m][ct][e];
-            }
-    if (vcols > 0) zero_rows(op + sg * NW * 32, ots, vcols, w.len, a.T, tid, NW * 64);
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * m + 4 * g + e;
+            if (row < a.dk && col < a.dv) a.sT[state + (int64_t)row * a.dv + col] = S[m][e];
+        }
+    if (vcols > 0) zero_rows(op + sg * NW * 16, ots, vcols, w.len, a.T, tid, NT);
 }
 
 // ---- reverse scan ---------------------------------------------------------------------------------------
 template <typename T, int DK, int NW> struct RscanLds {
-    static constexpr int LDK = DK + 8, LDV = NW * 32 + 8;
-    static constexpr size_t bytes = (size_t)kC * (2 * LDK + 2 * LDV) * sizeof(T) + (size_t)2 * Gd<T>::PD * kC * kLdm * 2 + kVec * kC * 4;
+    static constexpr int LDK = DK + 8, LDV = NW * 16 + 8;
+    static constexpr size_t bytes = (size_t)kC * (2 * LDK + 2 * LDV) * sizeof(T) + (size_t)6 * kC * kLdm * 2 + kVec * kC * 4;
 };
 
+// E and O are formed again from the state at the chunk's start: 36 + 84 more matrix instructions a wave and chunk instead of 100 KB more
+// traffic a chunk (E in f32 and the rest of O that its rounding dropped, written by the forward and read back).
 template <typename T, int DK, int NW>
 __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = RscanLds<T, DK, NW>;
-    constexpr int PD = Gd<T>::PD, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    using ET = typename Gd<T>::ET;
+    constexpr int NT = NW * 64, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
     T* Vl = Ql + kC * LDK;
     T* Ol = Vl + kC * LDV;                                  // dO
     __bf16* Xl = reinterpret_cast<__bf16*>(Ol + kC * LDV);
-    __bf16* Pl = Xl + PD * kC * kLdm;
-    float* vec = reinterpret_cast<float*>(Pl + PD * kC * kLdm);
+    __bf16* Pl = Xl + 3 * kC * kLdm;
+    float* vec = reinterpret_cast<float*>(Pl + 3 * kC * kLdm);
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
     const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6, g = l >> 4, i16 = l & 15;
-    const int col0 = (sg * NW + wave) * 32;
-    const int vcols = min(a.dv - sg * NW * 32, NW * 32), mycols = a.dv - col0;
-    const int64_t state = (int64_t)bh * a.dk * a.dv;
-    f32x4 S[KT][2];                                         // dS
+    const int slice = sg * NW + wave, col0 = slice * 16, col = col0 + i16;
+    const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
+    const int64_t state = (int64_t)bh * a.dk * a.dv, nat = (int64_t)a.B * a.H * a.nc;
+    f32x4 S[KT], s0n[KT];                                   // dS; the next chunk's starting state
 #pragma unroll
     for (int m = 0; m < KT; ++m)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * m + 4 * g + e, col = col0 + 16 * ct + i16;
-                S[m][ct][e] = a.gsT && row < a.dk && col < a.dv ? a.gsT[state + (int64_t)row * a.dv + col] : 0.f;
-            }
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * m + 4 * g + e;
+            S[m][e] = a.gsT && row < a.dk && col < a.dv ? a.gsT[state + (int64_t)row * a.dv + col] : 0.f;
+        }
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
-    const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 32;
-    const T* gp = (const T*)a.go + b * a.gos[1] + h * a.gos[2] + sg * NW * 32;
+    const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 16;
+    const T* gp = (const T*)a.go + b * a.gos[1] + h * a.gos[2] + sg * NW * 16;
     const int64_t ots = (int64_t)a.B * a.H * a.dv;
     T* gvp = (T*)a.gv + ((int64_t)b * a.H + h) * a.dv;
     const int ncl = (w.len + kC - 1) / kC;
-    const int slice = sg * NW + wave;
+    TileRegs<T, DK, NT> rk, rq;
+    TileRegs<T, NW * 16, NT> rv, ro;
+    TriRegs<NT> rx, rp;
+    float rvec[kVec * kC / NT];
+    auto fetch = [&](int c) {
+        const int64_t at = (int64_t)bh * a.nc + c;
+        rk.load(kp, a.ks[0], a.dk, c * kC, w);
+        rq.load(qp, a.qs[0], a.dk, c * kC, w);
+        rv.load(vp, a.vs[0], vcols, c * kC, w);
+        ro.load(gp, a.gos[0], vcols, c * kC, w);
+        rx.load(a.X + at * kTri);
+        rp.load(a.P + at * kTri);
+#pragma unroll
+        for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
+        const float* so = a.S0 + at * a.dk * a.dv;
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * m + 4 * g + e;
+                s0n[m][e] = row < a.dk && col < a.dv ? so[(int64_t)row * a.dv + col] : 0.f;
+            }
+    };
+    clear_upper(Xl, 6, tid, NT);
+    if (ncl > 0) fetch(ncl - 1);
     for (int c = ncl - 1; c >= 0; --c) {
         const int64_t at = (int64_t)bh * a.nc + c;
         __syncthreads();
-        stage(Kl, LDK, kp, a.ks[0], a.dk, DK, c * kC, w, tid, NW * 64);
-        stage(Ql, LDK, qp, a.qs[0], a.dk, DK, c * kC, w, tid, NW * 64);
-        stage(Vl, LDV, vp, a.vs[0], vcols, NW * 32, c * kC, w, tid, NW * 64);
-        stage(Ol, LDV, gp, a.gos[0], vcols, NW * 32, c * kC, w, tid, NW * 64);
-        stage_planes(Xl, a.X + at * PD * kC * kC, PD, tid, NW * 64);
-        stage_planes(Pl, a.P + at * PD * kC * kC, PD, tid, NW * 64);
-        for (int i = tid; i < kVec * kC; i += NW * 64) vec[i] = a.vec[at * kVec * kC + i];
+        rk.store(Kl, LDK);
+        rq.store(Ql, LDK);
+        rv.store(Vl, LDV);
+        ro.store(Ol, LDV);
+        rx.template store<3>(Xl);
+        rp.template store<3>(Pl);
+#pragma unroll
+        for (int i = 0; i < kVec * kC / NT; ++i) vec[i * NT + tid] = rvec[i];
+        f32x4 s0[KT];
+#pragma unroll
+        for (int m = 0; m < KT; ++m) s0[m] = s0n[m];
         __syncthreads();
+        if (c > 0) fetch(c - 1);
         if (mycols <= 0) continue;
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
         float anchor = 0.f;
         {   // dS at the chunk's end is what the gradient kernel needs; <dS, S_C> = dec <dS, S0> + sum_j dU2_j . U_j
             float* so = a.dS + at * a.dk * a.dv;
-            const float* s0 = a.S0 + at * a.dk * a.dv;
 #pragma unroll
-            for (int m = 0; m < KT; ++m)
+            for (int m = 0; m < KT; ++m) {
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = 16 * m + 4 * g + e, col = col0 + 16 * ct + i16;
-                        if (row < a.dk && col < a.dv) {
-                            so[(int64_t)row * a.dv + col] = S[m][ct][e];
-                            anchor += S[m][ct][e] * s0[(int64_t)row * a.dv + col];
-                        }
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const int row = 16 * m + 4 * g + e;
+                    if (row < a.dk && col < a.dv) so[(int64_t)row * a.dv + col] = S[m][e];
+                    anchor += S[m][e] * s0[m][e];
+                }
+            }
             anchor *= dec;
         }
-        f32x4 du[4][2];
+        f32x4 E[4], O[4], du[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) du[m][ct] = f32x4{0, 0, 0, 0};
+        for (int m = 0; m < 4; ++m) { E[m] = f32x4{0, 0, 0, 0}; O[m] = E[m]; du[m] = E[m]; }
 #pragma unroll
         for (int kb = 0; kb < DK / 32; ++kb) {
-            Frag<PD> sb[2];
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) sb[ct] = split<PD>(S[2 * kb][ct], S[2 * kb + 1][ct]);
+            const Frag<3> sb = split<3>(s0[2 * kb], s0[2 * kb + 1]), db = split<3>(S[2 * kb], S[2 * kb + 1]);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const auto kf = row_frag(Kl, LDK, 16 * m, 32 * kb);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) du[m][ct] = mma(kf, sb[ct], du[m][ct]);
+                E[m] = mma(kf, sb, E[m]);
+                du[m] = mma(kf, db, du[m]);
+                O[m] = mma(row_frag(Ql, LDK, 16 * m, 32 * kb), sb, O[m]);
             }
         }
-        f32x4 E[4][2];
-        {
-            const float* eo = a.E + at * kC * a.dv;
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const f32x4 kb = vec4(vec + kKb * kC, 16 * m), be = vec4(vec + kBe * kC, 16 * m);
+        for (int m = 0; m < 4; ++m) {
+            E[m] = tile_read(Vl, LDV, 16 * m, wave * 16) - vec4(vec + kAk * kC, 16 * m) * E[m];      // Vt
+            O[m] *= vec4(vec + kAq * kC, 16 * m);
+        }
+        Frag<3> f[2];
+        row_operands(f, vec + kBe * kC, E);
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) {
-                    const int col = col0 + 16 * ct + i16;
+        for (int m = 0; m < 4; ++m) {
+            f32x4 xs = {0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) E[m][ct][e] = col < a.dv ? eo[(int64_t)(16 * m + 4 * g + e) * a.dv + col] : 0.f;
-                    du[m][ct] *= kb;
-                    const f32x4 p = du[m][ct] * be * E[m][ct];
-                    anchor += p[0] + p[1] + p[2] + p[3];
-                }
-            }
+            for (int kb = 0; kb <= m / 2; ++kb) xs = mma(plane_rows<3>(Xl, 16 * m, 32 * kb), f[kb], xs);
+            E[m] -= xs;
+        }
+        row_operands(f, vec + kBe * kC, E);                 // U
+        f32x4 z[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+#pragma unroll
+            for (int kb = 0; kb <= m / 2; ++kb) O[m] = mma(plane_rows<3>(Pl, 16 * m, 32 * kb), f[kb], O[m]);
+            z[m] = O[m] * tile_read(Ol, LDV, 16 * m, wave * 16);
+            du[m] *= vec4(vec + kKb * kC, 16 * m);
+            const f32x4 p = du[m] * vec4(vec + kBe * kC, 16 * m) * E[m];
+            anchor += (p[0] + p[1]) + (p[2] + p[3]);
         }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {      // + P^T dO: column tile m of P has rows >= 16 m
-            Frag<Gd<T>::PT> of[2];
+            const auto of = col_frag(Ol, LDV, 32 * kb, wave * 16);
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) of[ct] = col_frag(Ol, LDV, 32 * kb, wave * 32 + 16 * ct);
-#pragma unroll
-            for (int m = 0; m < 2 * kb + 2; ++m) {
-                const Frag<PD> pf = plane_cols<PD>(Pl, 32 * kb, 16 * m);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) du[m][ct] = mma(pf, of[ct], du[m][ct]);
-            }
+            for (int m = 0; m < 2 * kb + 2; ++m) du[m] = mma(plane_cols<3>(Pl, 32 * kb, 16 * m), of, du[m]);
         }
-        Frag<PD> wf[2][2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const f32x4 b0 = vec4(vec + kBe * kC, 32 * kb), b1 = vec4(vec + kBe * kC, 32 * kb + 16);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) wf[kb][ct] = split<PD>(b0 * du[2 * kb][ct], b1 * du[2 * kb + 1][ct]);
-        }
-        float* xo = a.xpart + ((int64_t)slice * a.B * a.H * a.nc + at) * kC;
-        float* bo = a.bpart + ((int64_t)slice * a.B * a.H * a.nc + at) * kC;
+        row_operands(f, vec + kBe * kC, du);
+        float* zo = a.zpart + (slice * nat + at) * kC;
+        float* bo = a.bpart + (slice * nat + at) * kC;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {      // F = dU - X^T (beta dU), dV = beta F
-            f32x4 xs[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+            f32x4 xs = {0, 0, 0, 0};
 #pragma unroll
-            for (int kb = m / 2; kb < 2; ++kb) {
-                const Frag<PD> xf = plane_cols<PD>(Xl, 32 * kb, 16 * m);
+            for (int kb = m / 2; kb < 2; ++kb) xs = mma(plane_cols<3>(Xl, 32 * kb, 16 * m), f[kb], xs);
+            du[m] -= xs;
+            f32x4 sb = E[m] * du[m];
+            du[m] *= vec4(vec + kBe * kC, 16 * m);
+            z[m] -= du[m] * tile_read(Vl, LDV, 16 * m, wave * 16);
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) xs[ct] = mma(xf, wf[kb][ct], xs[ct]);
-            }
-            const f32x4 be = vec4(vec + kBe * kC, 16 * m);
-            f32x4 sb = {0, 0, 0, 0}, sx = {0, 0, 0, 0};
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                du[m][ct] -= xs[ct];
-                sb += E[m][ct] * du[m][ct];
-                du[m][ct] *= be;
-                sx += du[m][ct] * tile_read(Vl, LDV, 16 * m, wave * 32 + 16 * ct);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { sb[e] = row16_sum(sb[e]); sx[e] = row16_sum(sx[e]); }
+            for (int e = 0; e < 4; ++e) { sb[e] = row16_sum(sb[e]); z[m][e] = row16_sum(z[m][e]); }
             if (i16 == 0) {
                 *reinterpret_cast<f32x4a*>(bo + 16 * m + 4 * g) = sb;
-                *reinterpret_cast<f32x4a*>(xo + 16 * m + 4 * g) = sx;
+                *reinterpret_cast<f32x4a*>(zo + 16 * m + 4 * g) = z[m];
             }
         }
         anchor = wave_sum(anchor);
-        if (l == 0) a.apart[(int64_t)slice * a.B * a.H * a.nc + at] = anchor;
-        lds_order();
-        T* my = Vl + wave * 32;
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) tile_write(my, LDV, 16 * m, 16 * ct, du[m][ct]);
-        lds_order();
-        store_rows(my, LDV, gvp + col0, ots, mycols, c * kC, w);
+        if (l == 0) a.apart[slice * nat + at] = anchor;
         // dS = dec dS + Q^T (aq dO) - K^T (ak dV)
-        Frag<PD> qf[2][2];
+        Frag<3> qf[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const f32x4 k0 = vec4(vec + kAk * kC, 32 * kb), k1 = vec4(vec + kAk * kC, 32 * kb + 16);
-            const f32x4 q0 = vec4(vec + kAq * kC, 32 * kb), q1 = vec4(vec + kAq * kC, 32 * kb + 16);
+            f[kb] = split<3>(-vec4(vec + kAk * kC, 32 * kb) * du[2 * kb], -vec4(vec + kAk * kC, 32 * kb + 16) * du[2 * kb + 1]);
+            qf[kb] = split<3>(vec4(vec + kAq * kC, 32 * kb) * tile_read(Ol, LDV, 32 * kb, wave * 16),
+                              vec4(vec + kAq * kC, 32 * kb + 16) * tile_read(Ol, LDV, 32 * kb + 16, wave * 16));
+        }
+        // dV and E leave through this wave's own columns of the V and dO tiles, which it has read
+        lds_order();
+        T* my = Vl + wave * 16;
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                wf[kb][ct] = split<PD>(-k0 * du[2 * kb][ct], -k1 * du[2 * kb + 1][ct]);
-                qf[kb][ct] = split<PD>(q0 * tile_read(Ol, LDV, 32 * kb, wave * 32 + 16 * ct), q1 * tile_read(Ol, LDV, 32 * kb + 16, wave * 32 + 16 * ct));
-            }
+        for (int m = 0; m < 4; ++m) tile_write(my, LDV, 16 * m, 0, du[m]);
+        lds_order();
+        store_rows(my, LDV, mycols, w.len - c * kC, [&](int r) { return gvp + w.frame(c * kC + r) * ots + col0; });
+        ET* eo = (ET*)a.E + at * kC * a.dv;
+        if constexpr (sizeof(ET) == sizeof(T)) {
+            ET* me = reinterpret_cast<ET*>(Ol + wave * 16);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) tile_write(me, LDV, 16 * m, 0, E[m]);
+            lds_order();
+            store_rows(me, LDV, mycols, kC, [&](int r) { return eo + (int64_t)r * a.dv + col0; });
+        } else {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (col < a.dv) eo[(int64_t)(16 * m + 4 * g + e) * a.dv + col] = E[m][e];
         }
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
+            S[m] *= dec;
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) S[m][ct] *= dec;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                const auto kf = col_frag(Kl, LDK, 32 * kb, 16 * m);
-                const auto qa = col_frag(Ql, LDK, 32 * kb, 16 * m);
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) S[m][ct] = mma(qa, qf[kb][ct], mma(kf, wf[kb][ct], S[m][ct]));
-            }
+            for (int kb = 0; kb < 2; ++kb)
+                S[m] = mma(col_frag(Ql, LDK, 32 * kb, 16 * m), qf[kb], mma(col_frag(Kl, LDK, 32 * kb, 16 * m), f[kb], S[m]));
         }
     }
     if (a.gs0) {
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = 16 * m + 4 * g + e, col = col0 + 16 * ct + i16;
-                    if (row < a.dk && col < a.dv) a.gs0[state + (int64_t)row * a.dv + col] = S[m][ct][e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * m + 4 * g + e;
+                if (row < a.dk && col < a.dv) a.gs0[state + (int64_t)row * a.dv + col] = S[m][e];
+            }
     }
-    if (vcols > 0) zero_rows(gvp + sg * NW * 32, ots, vcols, w.len, a.T, tid, NW * 64);
+    if (vcols > 0) zero_rows(gvp + sg * NW * 16, ots, vcols, w.len, a.T, tid, NT);
 }
 
 // ---- gradients of a chunk ---------------------------------------------------------------------------------
-template <typename T> struct MatT { using type = float; };
-template <> struct MatT<__hip_bfloat16> { using type = __hip_bfloat16; };
-
 template <typename T, int DK> struct GradLds {
-    using M = typename MatT<T>::type;
-    static constexpr int LDK = DK + 8, LDV = 136, LDM = sizeof(M) == 2 ? 72 : 68;
-    static constexpr size_t tiles = (size_t)3 * kC * LDV > (size_t)2 * kC * LDK ? (size_t)3 * kC * LDV : (size_t)2 * kC * LDK;
-    static constexpr size_t bytes = tiles * sizeof(T) + (size_t)2 * kC * LDM * sizeof(M) + (kVec + 8 + 1) * kC * 4;
+    static constexpr int LDK = DK + 8, LDV = sizeof(T) == 4 ? 132 : 136, LDE = sizeof(typename Gd<T>::ET) == 4 ? 132 : 136;
+    static constexpr size_t one = (size_t)2 * kC * LDV * sizeof(T) + (size_t)kC * LDE * sizeof(typename Gd<T>::ET), two = (size_t)2 * kC * LDK * sizeof(T);
+    static constexpr size_t tiles = one > two ? one : two, mat = (size_t)Gd<T>::OP * kC * kLdm * 2;
+    static constexpr size_t bytes = tiles + mat + (kVec + 8) * kC * 4;
 };
 
+template <int P> __device__ __forceinline__ void plane_write(__bf16* t, int r0, int c0, f32x4 v) {
+    const int l = threadIdx.x & 63;
+    __bf16* p = t + (r0 + 4 * (l >> 4)) * kLdm + c0 + (l & 15);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const bf16x4 h = __builtin_convertvector(v, bf16x4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[i * kC * kLdm + e * kLdm] = h[e];
+        v -= __builtin_convertvector(h, f32x4);
+    }
+}
+// the transpose of a tile: rows and columns exchanged
+template <int P> __device__ __forceinline__ void plane_write_t(__bf16* t, int r0, int c0, f32x4 v) {
+    const int l = threadIdx.x & 63;
+    __bf16* p = t + (c0 + (l & 15)) * kLdm + r0 + 4 * (l >> 4);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const bf16x4 h = __builtin_convertvector(v, bf16x4);
+        *reinterpret_cast<u32x2a*>(p + i * kC * kLdm) = __builtin_bit_cast(u32x2a, h);
+        v -= __builtin_convertvector(h, f32x4);
+    }
+}
+
+// Two workgroups a CU (16-bit types): one loads while the other multiplies.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = GradLds<T, DK>;
-    using M = typename L::M;
-    constexpr int PT = Gd<T>::PT, LDK = L::LDK, LDV = L::LDV, LDM = L::LDM, NT = DK / 64;
-    T* tile = reinterpret_cast<T*>(smem);
-    T *Ol = tile, *Dl = tile + kC * LDV, *Ul = tile + 2 * kC * LDV;      // dO, dV, U
-    T *Kl = tile, *Ql = tile + kC * LDK;                                  // later
-    M* M1 = reinterpret_cast<M*>(tile + L::tiles);
-    M* M2 = M1 + kC * LDM;
-    float* vec = reinterpret_cast<float*>(M2 + kC * LDM);
+    using ET = typename Gd<T>::ET;
+    constexpr int PT = Gd<T>::PT, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, LDE = L::LDE, NT = DK / 64;
+    constexpr int PE = sizeof(ET) == 2 ? 1 : 3;
+    T *Ol = reinterpret_cast<T*>(smem), *Dl = Ol + kC * LDV;              // dO, dV
+    ET* El = reinterpret_cast<ET*>(Dl + kC * LDV);
+    T *Kl = reinterpret_cast<T*>(smem), *Ql = Kl + kC * LDK;              // later
+    __bf16* M = reinterpret_cast<__bf16*>(smem + L::tiles);
+    float* vec = reinterpret_cast<float*>(smem + L::tiles + L::mat);
     const double* G = reinterpret_cast<const double*>(vec + kG64 * kC);
     float* dots = vec + kVec * kC;                                        // [2][4][64]
-    float* ys = dots + 8 * kC;
     const int c = blockIdx.x % a.nc, bk = blockIdx.x / a.nc, b = bk / a.Hk, hk = bk % a.Hk;
     const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6, g = l >> 4, i16 = l & 15;
     const Walk w = walk_of(a, b, hk * a.r);
@@ -871,43 +918,25 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
     for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) { tq[m][n] = f32x4{0, 0, 0, 0}; tk[m][n] = f32x4{0, 0, 0, 0}; }
-    const int64_t ots = (int64_t)a.B * a.H * a.dv, nbh = (int64_t)a.B * a.H;
+    const int64_t ots = (int64_t)a.B * a.H * a.dv, nat = (int64_t)a.B * a.H * a.nc;
     for (int hh = 0; hh < a.r; ++hh) {
         const int h = hk * a.r + hh, bh = b * a.H + h;
         const int64_t at = (int64_t)bh * a.nc + c;
         __syncthreads();
-        for (int i = tid; i < kVec * kC; i += 256) vec[i] = a.vec[at * kVec * kC + i];
-        stage(Ol, LDV, (const T*)a.go + b * a.gos[1] + h * a.gos[2], a.gos[0], a.dv, 128, p0, w, tid, 256);
-        stage(Dl, LDV, (const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, 128, p0, w, tid, 256);
         {
-            const float* e = a.E + at * kC * a.dv;
-            for (int i = tid; i < kC * 32; i += 256) {
-                const int row = i >> 5, col = (i & 31) * 4;
-                const float be = a.vec[at * kVec * kC + kBe * kC + row];
-                f32x4 v = {0, 0, 0, 0};
-                if (col < a.dv && p0 + row < w.len) v = *reinterpret_cast<const f32x4a*>(e + row * a.dv + col);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) Elem<T>::st(Ul + row * LDV + col + j, v[j] * be);
-            }
+            TileRegs<T, 128, 256> ro, rd;
+            TileRegs<ET, 128, 256> re;
+            Walk rows = {kC, false};
+            ro.load((const T*)a.go + b * a.gos[1] + h * a.gos[2], a.gos[0], a.dv, p0, w);
+            rd.load((const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, p0, w);
+            re.load((const ET*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
+            for (int i = tid; i < kVec * kC; i += 256) vec[i] = a.vec[at * kVec * kC + i];
+            ro.store(Ol, LDV);
+            rd.store(Dl, LDV);
+            re.store(El, LDE);
         }
         __syncthreads();
-        {   // dO . O per frame: four lanes a row
-            const int row = tid >> 2, part = tid & 3, p = p0 + row;
-            float y = 0.f;
-            if (p < w.len) {
-                const int64_t o = w.frame(p) * ots + (int64_t)bh * a.dv;
-                for (int i = part * 4; i < a.dv; i += 16)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float ov = Elem<T>::ld((const T*)a.o + o + i + j);
-                        if (sizeof(T) == 2) ov += (float)a.olo[o + i + j];
-                        y += to_f(Ol[row * LDV + i + j]) * ov;
-                    }
-            }
-            y += __shfl_xor(y, 1); y += __shfl_xor(y, 2);
-            if (part == 0) ys[row] = y;
-        }
-        // states: wave = a quarter of dk
+        // states: wave = a quarter of dk; U = beta E: its factor goes with the rows
         {
             const float* s0 = a.S0 + at * a.dk * a.dv;
             const float* ds = a.dS + at * a.dk * a.dv;
@@ -916,8 +945,10 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) { cq[m][n] = f32x4{0, 0, 0, 0}; ck[m][n] = cq[m][n]; cd[m][n] = cq[m][n]; }
-            for (int kb = 0; kb * 32 < a.dv; ++kb) {
-                Frag<PT> sf[NT], df[NT];
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                if (kb * 32 >= a.dv) break;
+                Frag<OP> sf[NT], df[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const int row = (wave * NT + n) * 16 + i16, c0 = 32 * kb + 4 * g, c1 = c0 + 16;
@@ -930,25 +961,26 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
                         s_1 = *reinterpret_cast<const f32x4a*>(s0 + (int64_t)row * a.dv + c1);
                         d_1 = *reinterpret_cast<const f32x4a*>(ds + (int64_t)row * a.dv + c1);
                     }
-                    sf[n] = split<PT>(s_0, s_1);
-                    df[n] = split<PT>(d_0, d_1);
+                    sf[n] = split<OP>(s_0, s_1);
+                    df[n] = split<OP>(d_0, d_1);
                 }
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const auto of = row_frag(Ol, LDV, 16 * m, 32 * kb);
-                    const auto uf = row_frag(Ul, LDV, 16 * m, 32 * kb);
+                    const auto uf = row_frag(El, LDE, 16 * m, 32 * kb);
                     const auto vf = row_frag(Dl, LDV, 16 * m, 32 * kb);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        cq[m][n] = mma(of, sf[n], cq[m][n]);
-                        ck[m][n] = mma(uf, df[n], ck[m][n]);
-                        cd[m][n] = mma(vf, sf[n], cd[m][n]);
+                        cq[m][n] = mma<PT, OP, OP>(of, sf[n], cq[m][n]);
+                        ck[m][n] = mma<PE, OP, OP>(uf, df[n], ck[m][n]);
+                        cd[m][n] = mma<PT, OP, OP>(vf, sf[n], cd[m][n]);
                     }
                 }
             }
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const f32x4 aq = vec4(vec + kAq * kC, 16 * m), ak = vec4(vec + kAk * kC, 16 * m), kb = vec4(vec + kKb * kC, 16 * m);
+                const f32x4 aq = vec4(vec + kAq * kC, 16 * m), ak = vec4(vec + kAk * kC, 16 * m);
+                const f32x4 kb = vec4(vec + kKb * kC, 16 * m) * vec4(vec + kBe * kC, 16 * m);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     tq[m][n] += aq * cq[m][n];
@@ -956,54 +988,64 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
                 }
             }
         }
-        // M1 = dP * D * sq_i * rk_j (lower), M2 = (dN * D * rk_i * rk_j) made symmetric; wave = block column
-        for (int m = 0; m < 4; ++m) {
-            f32x4 dp = {0, 0, 0, 0}, dn = {0, 0, 0, 0};
-            if (m < wave) {
-                tile_write(M1, LDM, 16 * m, 16 * wave, dp);
-                continue;
+        // M1 = dP * D * sq_i * rk_j (lower), M2 = -dV U^T * D * rk_i * rk_j (strictly lower, made symmetric); wave = block column j
+        f32x4 dp[4], dn[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) { dp[m] = f32x4{0, 0, 0, 0}; dn[m] = dp[m]; }
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            if (kb * 32 >= a.dv) break;
+            const auto uf = row_frag(El, LDE, 16 * wave, 32 * kb);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                if (m < wave) continue;
+                dp[m] = mma<PT, PE, OP>(row_frag(Ol, LDV, 16 * m, 32 * kb), uf, dp[m]);
+                dn[m] = mma<PT, PE, OP>(row_frag(Dl, LDV, 16 * m, 32 * kb), uf, dn[m]);
             }
-            for (int kb = 0; kb * 32 < a.dv; ++kb) {
-                const auto uf = row_frag(Ul, LDV, 16 * wave, 32 * kb);
-                dp = mma(row_frag(Ol, LDV, 16 * m, 32 * kb), uf, dp);
-                dn = mma(row_frag(Dl, LDV, 16 * m, 32 * kb), uf, dn);
-            }
+        }
+        {
             const int j = 16 * wave + i16;
-            const float rkj = vec[kRk * kC + j];
+            const float rkj = vec[kRk * kC + j] * vec[kBe * kC + j];
             const double gj = G[j];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = 16 * m + 4 * g + e;
-                const float d = i >= j ? __expf((float)(G[i] - gj)) * rkj : 0.f;
-                dp[e] = i >= j ? dp[e] * d * vec[kSq * kC + i] : 0.f;
-                dn[e] = i > j ? -dn[e] * d * vec[kRk * kC + i] : 0.f;
-                if (i > j) Elem<M>::st(M2 + j * LDM + i, dn[e]);
-                if (i >= j) Elem<M>::st(M2 + i * LDM + j, dn[e]);
-            }
-            tile_write(M1, LDM, 16 * m, 16 * wave, dp);
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * m + 4 * g + e;
+                    const float d = i >= j ? __expf((float)(G[i] - gj)) * rkj : 0.f;
+                    dp[m][e] = i >= j ? dp[m][e] * d * vec[kSq * kC + i] : 0.f;
+                    dn[m][e] = i > j ? -dn[m][e] * d * vec[kRk * kC + i] : 0.f;
+                }
         }
         __syncthreads();
-        stage(Kl, LDK, (const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, DK, p0, w, tid, 256);
-        stage(Ql, LDK, (const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, DK, p0, w, tid, 256);
-        if (wave == 0) {      // dg and dbeta: lane = frame
-            float z = ys[l], be = 0.f, an = 0.f;
-            for (int s = 0; s < a.nsl; ++s) {
-                z -= a.xpart[(s * nbh * a.nc + at) * kC + l];
-                be += a.bpart[(s * nbh * a.nc + at) * kC + l];
-                an += a.apart[s * nbh * a.nc + at];
-            }
-            if (p0 + l >= w.len) z = 0.f;
+        {
+            TileRegs<T, DK, 256> rk, rq;
+            rk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, p0, w);
+            rq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, p0, w);
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) { const float u = __shfl_down(z, o); if (l + o < 64) z += u; }
-            if (p0 + l < w.len) {
-                const int64_t o = w.frame(p0 + l) * gts + bh;
-                a.gg[o] = z + an;
-                a.gbeta[o] = be;
+            for (int m = 0; m < 4; ++m) plane_write<OP>(M, 16 * m, 16 * wave, dp[m]);
+            if (wave == 0) {      // dg and dbeta: lane = frame
+                float z = 0.f, be = 0.f, an = 0.f;
+                for (int s = 0; s < a.nsl; ++s) {
+                    z += a.zpart[(s * nat + at) * kC + l];
+                    be += a.bpart[(s * nat + at) * kC + l];
+                    an += a.apart[s * nat + at];
+                }
+                if (p0 + l >= w.len) z = 0.f;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) { const float u = __shfl_down(z, o); if (l + o < 64) z += u; }
+                if (p0 + l < w.len) {
+                    const int64_t o = w.frame(p0 + l) * gts + bh;
+                    a.gg[o] = z + an;
+                    a.gbeta[o] = be;
+                }
             }
+            rk.store(Kl, LDK);
+            rq.store(Ql, LDK);
         }
         __syncthreads();
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int n0 = (wave * NT + n) * 16;
@@ -1011,12 +1053,39 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
                 const auto qf = col_frag(Ql, LDK, 32 * kb, n0);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    tq[m][n] = mma(row_frag(M1, LDM, 16 * m, 32 * kb), kf, tq[m][n]);
-                    tk[m][n] = mma(col_frag(M1, LDM, 32 * kb, 16 * m), qf, tk[m][n]);
-                    tk[m][n] = mma(row_frag(M2, LDM, 16 * m, 32 * kb), kf, tk[m][n]);
+                    if (kb <= m / 2) tq[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, 16 * m, 32 * kb), kf, tq[m][n]);
+                    if (kb >= m / 2) tk[m][n] = mma<OP, PT, OP>(plane_cols<OP>(M, 32 * kb, 16 * m), qf, tk[m][n]);
                 }
             }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if (m < wave) continue;
+            if (m > wave) plane_write<OP>(M, 16 * m, 16 * wave, dn[m]);
+            else {      // the diagonal block: its upper half is the transpose of its lower half
+                f32x4 t = dn[m];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // entry (i, j) of the upper half = lower entry (j, i): lane (j / 4 group, i), element j % 4
+                    const int i = 4 * g + e;
+                    float up = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) { const float v = __shfl(dn[m][x], (i16 >> 2) * 16 + i); if ((i16 & 3) == x) up = v; }
+                    if (i < i16) t[e] = up;
+                }
+                plane_write<OP>(M, 16 * m, 16 * wave, t);
+            }
+            if (m > wave) plane_write_t<OP>(M, 16 * m, 16 * wave, dn[m]);
         }
+        __syncthreads();
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const auto kf = col_frag(Kl, LDK, 32 * kb, (wave * NT + n) * 16);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) tk[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, 16 * m, 32 * kb), kf, tk[m][n]);
+            }
     }
     // through the normalisation: dq = tq - q |q|^-2 (q . tq)  (|.|^2 with its epsilon), dk alike
     if (a.norm) {
@@ -1077,7 +1146,7 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void gdr_recurrent_kernel(GdrArgs a) {
     __shared__ float red[2][4][8][12];
-    const int bh = blockIdx.x / a.nsl, sl = blockIdx.x % a.nsl, b = bh / a.H, h = bh % a.H, hk = h / a.r;
+    const int ns = (a.dv + 31) >> 5, bh = blockIdx.x / ns, sl = blockIdx.x % ns, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
     const int tid = threadIdx.x, wave = tid >> 6, cl = tid & 7, rg = tid >> 3;
     const int col = sl * 32 + cl * 4;
@@ -1172,34 +1241,28 @@ static int gdr_check(const char* who, int T, int B, int Hk, int H, int dk, int d
     return SP_OK;
 }
 
-static int parts_d(int dtype) { return dtype == SP_F32 ? 3 : 2; }
-
-struct GdrLayout { size_t vec, X, P, S0, E, olo, end; };
-static GdrLayout gdr_saved(int T, int B, int H, int dk, int dv, int dtype, bool train) {
+struct GdrLayout { size_t vec, X, P, S0, end; };
+static GdrLayout gdr_saved(int T, int B, int H, int dk, int dv, bool train) {
     GdrLayout s{};
     const size_t n = (size_t)B * H * ((T + kC - 1) / kC);
-    const int pd = parts_d(dtype), np = train || dtype != SP_BF16 ? pd : 1;
     size_t o = 0;
     auto put = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes, 256); return at; };
     s.vec = put(n * kVec * kC * 4);
-    s.X = put(n * pd * kC * kC * 2);
-    s.P = put(n * np * kC * kC * 2);
-    if (train) {
-        s.S0 = put(n * dk * dv * 4);
-        s.E = put(n * kC * dv * 4);
-        s.olo = put(dtype == SP_F32 ? 0 : (size_t)T * B * H * dv * 2);
-    }
+    s.X = put(n * kTri * 4);
+    s.P = put(n * kTri * 4);
+    if (train) s.S0 = put(n * dk * dv * 4);
     s.end = o;
     return s;
 }
-struct GdrBwdLayout { size_t dS, x, b, a, end; };
-static GdrBwdLayout gdr_bwd_ws(int T, int B, int H, int dk, int dv) {
+struct GdrBwdLayout { size_t dS, E, z, b, a, end; };
+static GdrBwdLayout gdr_bwd_ws(int T, int B, int H, int dk, int dv, int dtype) {
     GdrBwdLayout s{};
-    const size_t n = (size_t)B * H * ((T + kC - 1) / kC), nsl = (dv + 31) / 32;
+    const size_t n = (size_t)B * H * ((T + kC - 1) / kC), nsl = (dv + 15) / 16;
     size_t o = 0;
     auto put = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes, 256); return at; };
     s.dS = put(n * dk * dv * 4);
-    s.x = put(n * nsl * kC * 4);
+    s.E = put(n * kC * dv * (dtype == SP_BF16 ? 2 : 4));
+    s.z = put(n * nsl * kC * 4);
     s.b = put(n * nsl * kC * 4);
     s.a = put(n * nsl * 4);
     s.end = o;
@@ -1216,28 +1279,37 @@ template <typename K> static int gdr_launch(K kernel, size_t lds, int64_t blocks
     return check_launch(what);
 }
 
+// columns of dv a workgroup of the scans owns: 128 (the head's K, Q and matrices are then staged once), or 64 where that leaves CUs idle
+static bool gdr_wide(const GdrArgs& a) { return a.nsl > 4 && (int64_t)a.B * a.H >= 192; }
+
 static void gdr_fill(GdrArgs& a, const void* q, const void* k, const void* v, const float* g, const float* beta, const int32_t* lengths,
                      const int64_t* st, int T, int B, int Hk, int H, int dk, int dv, float scale, int flags) {
     a.q = q; a.k = k; a.v = v; a.g = g; a.beta = beta; a.lengths = lengths;
     for (int i = 0; i < 3; ++i) { a.qs[i] = st[i]; a.ks[i] = st[3 + i]; a.vs[i] = st[6 + i]; a.gs[i] = st[9 + i]; a.bs[i] = st[12 + i]; }
     a.T = T; a.B = B; a.Hk = Hk; a.H = H; a.r = H / Hk; a.dk = dk; a.dv = dv;
-    a.nc = (T + kC - 1) / kC; a.nsl = (dv + 31) / 32;
+    a.nc = (T + kC - 1) / kC; a.nsl = (dv + 15) / 16;
     a.scale = scale;
     a.norm = flags & SP_GDR_NORMALIZE ? 1 : 0;
     a.bidir = flags & SP_GDR_BIDIRECTIONAL ? 1 : 0;
 }
 
-template <typename T, int DK, int NP, bool TRAIN> static int gdr_forward(const GdrArgs& a, hipStream_t s) {
-    int rc = gdr_launch(gdr_prep_kernel<T, DK, NP>, PrepLds<T, DK>::bytes, (int64_t)a.B * a.H * a.nc, 256, a, s, "gdr_prep_kernel");
+template <typename T, int DK, int NW, bool TRAIN> static int gdr_scan(const GdrArgs& a, hipStream_t s) {
+    return gdr_launch(gdr_scan_kernel<T, DK, NW, TRAIN>, ScanLds<T, DK, NW>::bytes, (int64_t)a.B * a.H * ((a.nsl + NW - 1) / NW), NW * 64, a, s,
+                      "gdr_scan_kernel");
+}
+template <typename T, int DK, bool TRAIN> static int gdr_forward(const GdrArgs& a, hipStream_t s) {
+    const int rc = gdr_launch(gdr_prep_kernel<T, DK>, PrepLds<T, DK>::bytes, (int64_t)a.B * a.H * a.nc, 256, a, s, "gdr_prep_kernel");
     if (rc) return rc;
-    constexpr int NW = 4;
-    return gdr_launch(gdr_scan_kernel<T, DK, NW, NP, TRAIN>, ScanLds<T, DK, NW, NP>::bytes, (int64_t)a.B * a.H * ((a.nsl + NW - 1) / NW), NW * 64, a,
-                      s, "gdr_scan_kernel");
+    return gdr_wide(a) ? gdr_scan<T, DK, 8, TRAIN>(a, s) : gdr_scan<T, DK, 4, TRAIN>(a, s);
+}
+template <typename T, int DK, int NW> static int gdr_rscan(const GdrArgs& a, hipStream_t s) {
+    return gdr_launch(gdr_rscan_kernel<T, DK, NW>, RscanLds<T, DK, NW>::bytes, (int64_t)a.B * a.H * ((a.nsl + NW - 1) / NW), NW * 64, a, s,
+                      "gdr_rscan_kernel");
 }
 template <typename T, int DK> static int gdr_backward(const GdrArgs& a, hipStream_t s) {
-    constexpr int NW = sizeof(T) == 4 && DK == 128 ? 2 : 4;
-    int rc = gdr_launch(gdr_rscan_kernel<T, DK, NW>, RscanLds<T, DK, NW>::bytes, (int64_t)a.B * a.H * ((a.nsl + NW - 1) / NW), NW * 64, a, s,
-                        "gdr_rscan_kernel");
+    int rc;
+    if constexpr (sizeof(T) == 4 && DK == 128) rc = gdr_rscan<T, DK, 4>(a, s);      // eight waves' tiles exceed the LDS
+    else rc = gdr_wide(a) ? gdr_rscan<T, DK, 8>(a, s) : gdr_rscan<T, DK, 4>(a, s);
     if (rc) return rc;
     return gdr_launch(gdr_grads_kernel<T, DK>, GradLds<T, DK>::bytes, (int64_t)a.B * a.Hk * a.nc, 256, a, s, "gdr_grads_kernel");
 }
@@ -1248,11 +1320,11 @@ using namespace sp;
 
 extern "C" size_t sp_gdr_workspace_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype, int backward) {
     if (gdr_check("sp_gdr_workspace_bytes", T, B, Hk, H, dk, dv, 0, dtype)) return 0;
-    return backward ? gdr_bwd_ws(T, B, H, dk, dv).end : gdr_saved(T, B, H, dk, dv, dtype, false).end;
+    return backward ? gdr_bwd_ws(T, B, H, dk, dv, dtype).end : gdr_saved(T, B, H, dk, dv, false).end;
 }
 extern "C" size_t sp_gdr_saved_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype) {
     if (gdr_check("sp_gdr_saved_bytes", T, B, Hk, H, dk, dv, 0, dtype)) return 0;
-    return gdr_saved(T, B, H, dk, dv, dtype, true).end;
+    return gdr_saved(T, B, H, dk, dv, true).end;
 }
 
 extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const float* state,
@@ -1272,29 +1344,28 @@ extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const flo
     hipStream_t s = (hipStream_t)stream;
     const bool train = saved != nullptr;
     if (!train && T <= kRecurrentMax) {
-        const int64_t blocks = (int64_t)B * H * a.nsl;
+        const int64_t blocks = (int64_t)B * H * ((dv + 31) / 32);
         if (dtype == SP_F32) return gdr_launch(gdr_recurrent_kernel<float>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
         if (dtype == SP_F16) return gdr_launch(gdr_recurrent_kernel<__half>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
         return gdr_launch(gdr_recurrent_kernel<__hip_bfloat16>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
     }
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype),
                  "sp_gdr_fwd: q, k, v need 16-byte aligned rows");
-    const GdrLayout lay = gdr_saved(T, B, H, dk, dv, dtype, train);
+    const GdrLayout lay = gdr_saved(T, B, H, dk, dv, train);
     if (train ? saved_bytes < lay.end : workspace_bytes < lay.end || !workspace)
         return fail(SP_EWORKSPACE, "sp_gdr_fwd: %s %zu < %zu bytes", train ? "saved" : "workspace", train ? saved_bytes : workspace_bytes, lay.end);
     char* base = (char*)(train ? saved : workspace);
-    a.vec = (float*)(base + lay.vec); a.X = (__bf16*)(base + lay.X); a.P = (__bf16*)(base + lay.P);
-    a.S0 = (float*)(base + lay.S0); a.E = (float*)(base + lay.E); a.olo = (__bf16*)(base + lay.olo);
+    a.vec = (float*)(base + lay.vec); a.X = (float*)(base + lay.X); a.P = (float*)(base + lay.P); a.S0 = (float*)(base + lay.S0);
     const bool wide = dk > 64;
-#define SP_GDR_FWD(T_, NP_, TR_) return wide ? gdr_forward<T_, 128, NP_, TR_>(a, s) : gdr_forward<T_, 64, NP_, TR_>(a, s)
+#define SP_GDR_FWD(T_, TR_) return wide ? gdr_forward<T_, 128, TR_>(a, s) : gdr_forward<T_, 64, TR_>(a, s)
     if (train) {
-        if (dtype == SP_F32) SP_GDR_FWD(float, 3, true);
-        if (dtype == SP_F16) SP_GDR_FWD(__half, 2, true);
-        SP_GDR_FWD(__hip_bfloat16, 2, true);
+        if (dtype == SP_F32) SP_GDR_FWD(float, true);
+        if (dtype == SP_F16) SP_GDR_FWD(__half, true);
+        SP_GDR_FWD(__hip_bfloat16, true);
     }
-    if (dtype == SP_F32) SP_GDR_FWD(float, 3, false);
-    if (dtype == SP_F16) SP_GDR_FWD(__half, 2, false);
-    SP_GDR_FWD(__hip_bfloat16, 1, false);
+    if (dtype == SP_F32) SP_GDR_FWD(float, false);
+    if (dtype == SP_F16) SP_GDR_FWD(__half, false);
+    SP_GDR_FWD(__hip_bfloat16, false);
 #undef SP_GDR_FWD
 }
 
@@ -1310,19 +1381,18 @@ extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const flo
     SP_CHECK_ARG(q && k && v && g && beta && strides && o && saved && go && gq && gk && gv && gg && gbeta && workspace, "sp_gdr_bwd: null pointer");
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype) &&
                      gdr_aligned(go, strides + 15, dtype), "sp_gdr_bwd: q, k, v, go need 16-byte aligned rows");
-    const GdrLayout lay = gdr_saved(T, B, H, dk, dv, dtype, true);
-    const GdrBwdLayout ws = gdr_bwd_ws(T, B, H, dk, dv);
+    const GdrLayout lay = gdr_saved(T, B, H, dk, dv, true);
+    const GdrBwdLayout ws = gdr_bwd_ws(T, B, H, dk, dv, dtype);
     if (saved_bytes < lay.end || workspace_bytes < ws.end)
         return fail(SP_EWORKSPACE, "sp_gdr_bwd: saved %zu < %zu or workspace %zu < %zu bytes", saved_bytes, lay.end, workspace_bytes, ws.end);
     GdrArgs a{};
     gdr_fill(a, q, k, v, g, beta, lengths, strides, T, B, Hk, H, dk, dv, scale, flags);
     char* base = (char*)saved;
-    a.vec = (float*)(base + lay.vec); a.X = (__bf16*)(base + lay.X); a.P = (__bf16*)(base + lay.P);
-    a.S0 = (float*)(base + lay.S0); a.E = (float*)(base + lay.E); a.olo = (__bf16*)(base + lay.olo);
-    a.o = (void*)o; a.go = go; a.gsT = gstate_out;
+    a.vec = (float*)(base + lay.vec); a.X = (float*)(base + lay.X); a.P = (float*)(base + lay.P); a.S0 = (float*)(base + lay.S0);
+    a.go = go; a.gsT = gstate_out;
     for (int i = 0; i < 3; ++i) a.gos[i] = strides[15 + i];
     char* wb = (char*)workspace;
-    a.dS = (float*)(wb + ws.dS); a.xpart = (float*)(wb + ws.x); a.bpart = (float*)(wb + ws.b); a.apart = (float*)(wb + ws.a);
+    a.dS = (float*)(wb + ws.dS); a.E = wb + ws.E; a.zpart = (float*)(wb + ws.z); a.bpart = (float*)(wb + ws.b); a.apart = (float*)(wb + ws.a);
     a.gq = gq; a.gk = gk; a.gv = gv; a.gg = gg; a.gbeta = gbeta; a.gs0 = gstate;
     hipStream_t s = (hipStream_t)stream;
     const bool wide = dk > 64;
