@@ -80,18 +80,58 @@ template <> struct Gd<float> { static constexpr int PT = 3, OP = 3, EP = 3; usin
 
 template <int P> struct Frag { bf16x8 p[P]; };
 
+// One part is rounded to nearest.  Of several, all but the last are cut off (the upper 16 bits as they stand: one v_perm packs two, and
+// three parts of 8 bits are exactly an f32's 24); the last of two is rounded.
+__device__ __forceinline__ uint32_t cvt_pk(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
 template <int P> __device__ __forceinline__ Frag<P> split(f32x8 v) {
     Frag<P> f;
-    f.p[0] = __builtin_convertvector(v, bf16x8);
 #pragma unroll
-    for (int i = 1; i < P; ++i) {
-        v -= __builtin_convertvector(f.p[i - 1], f32x8);
-        f.p[i] = __builtin_convertvector(v, bf16x8);
+    for (int i = 0; i < P; ++i) {
+        u32x4a w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float x = v[2 * j], y = v[2 * j + 1];
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            if (i + 1 < P || P == 3) w[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            else w[j] = cvt_pk(x, y);
+            if (i + 1 < P) {
+                x -= __uint_as_float(a & 0xFFFF0000u);
+                y -= __uint_as_float(b & 0xFFFF0000u);
+                v[2 * j] = x;
+                v[2 * j + 1] = y;
+            }
+        }
+        f.p[i] = __builtin_bit_cast(bf16x8, w);
     }
     return f;
 }
 template <int P> __device__ __forceinline__ Frag<P> split(f32x4 a, f32x4 b) {
     return split<P>(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// the parts of four values, as the planes of a matrix in LDS take them
+template <int P, typename F> __device__ __forceinline__ void parts4(f32x4 v, F&& put) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        u32x2a w;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float x = v[2 * j], y = v[2 * j + 1];
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            if (i + 1 < P || P == 3) w[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            else w[j] = cvt_pk(x, y);
+            if (i + 1 < P) {
+                v[2 * j] = x - __uint_as_float(a & 0xFFFF0000u);
+                v[2 * j + 1] = y - __uint_as_float(b & 0xFFFF0000u);
+            }
+        }
+        put(i, w);
+    }
 }
 
 // acc += a b, the parts whose product matters (i + j below the larger number of parts, or below `CUT`)
@@ -226,6 +266,10 @@ struct Walk {
     int len;
     bool rev;
     __device__ __forceinline__ int64_t frame(int i) const { return rev && i < len ? len - 1 - i : i; }
+    // the lowest frame of the chunk at position p0 and, for a position p < len of that chunk, the distance from it (0 .. 63): addresses are
+    // a uniform 64-bit base and a 32-bit offset a lane (the host refuses frames that lie more than 32 MiB apart)
+    __device__ __forceinline__ int64_t low(int p0) const { return rev ? max(0, len - p0 - kC) : p0; }
+    __device__ __forceinline__ uint32_t above(int p0, int p) const { return rev ? (uint32_t)(len - 1 - p - max(0, len - p0 - kC)) : (uint32_t)(p - p0); }
 };
 __device__ __forceinline__ Walk walk_of(const GdrArgs& a, int b, int h) {
     Walk w;
@@ -234,51 +278,32 @@ __device__ __forceinline__ Walk walk_of(const GdrArgs& a, int b, int h) {
     return w;
 }
 
-// 64 frames x `ncol` columns (multiple of 8) from global rows into LDS [64][ld], columns up to `cols` and frames behind the end zero
-template <typename T>
-__device__ __forceinline__ void stage(T* dst, int ld, const T* src, int64_t ts, int ncol, int cols, int pos0, Walk w, int tid, int nt) {
-    const int vpr = cols >> 3;
-    for (int i = tid; i < kC * vpr; i += nt) {
-        const int row = i / vpr, c = (i - row * vpr) * 8, p = pos0 + row;
-        constexpr int Q = sizeof(T) / 2;       // 16-byte pieces
-        u32x4a v[Q];
-#pragma unroll
-        for (int j = 0; j < Q; ++j) v[j] = u32x4a{0, 0, 0, 0};
-        if (p < w.len && c < ncol) {
-            const u32x4a* s = reinterpret_cast<const u32x4a*>(src + w.frame(p) * ts + c);
-#pragma unroll
-            for (int j = 0; j < Q; ++j) v[j] = s[j];
-        }
-        u32x4a* d = reinterpret_cast<u32x4a*>(dst + row * ld + c);
-#pragma unroll
-        for (int j = 0; j < Q; ++j) d[j] = v[j];
-    }
-}
 // A thread's share of a tile of 64 frames x COLS columns on its way from global memory to LDS: requested a chunk ahead, in registers.
+// Loads are unconditional at clamped addresses (a branch around each would serialise them); what lies outside becomes zero on the way out.
+// Needs w.len > 0 and ncol >= 8.
 template <typename T, int COLS, int NT> struct TileRegs {
     static constexpr int Q = sizeof(T) / 2, N = (kC * COLS / 8 + NT - 1) / NT;
     u32x4a v[N][Q];
     __device__ __forceinline__ void load(const T* src, int64_t ts, int ncol, int pos0, Walk w) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8, p = pos0 + row;
-#pragma unroll
-            for (int j = 0; j < Q; ++j) v[n][j] = u32x4a{0, 0, 0, 0};
-            if (row < kC && p < w.len && c < ncol) {
-                const u32x4a* s = reinterpret_cast<const u32x4a*>(src + w.frame(p) * ts + c);
-#pragma unroll
-                for (int j = 0; j < Q; ++j) v[n][j] = s[j];
-            }
-        }
-    }
-    __device__ __forceinline__ void store(T* dst, int ld) const {
+        const char* base = reinterpret_cast<const char*>(src + w.low(pos0) * ts);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
-            if (row < kC) {
-                u32x4a* d = reinterpret_cast<u32x4a*>(dst + row * ld + c);
+            const uint32_t off = w.above(pos0, min(pos0 + row, w.len - 1)) * (uint32_t)(ts * sizeof(T)) + (uint32_t)(min(c, ncol - 8) * sizeof(T));
+            const u32x4a* s = reinterpret_cast<const u32x4a*>(base + off);
 #pragma unroll
-                for (int j = 0; j < Q; ++j) d[j] = v[n][j];
+            for (int j = 0; j < Q; ++j) v[n][j] = s[j];
+        }
+    }
+    __device__ __forceinline__ void store(T* dst, int ld, int ncol, int pos0, int len) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
+            const bool on = pos0 + row < len && c < ncol;
+            u32x4a* d = reinterpret_cast<u32x4a*>(dst + row * ld + c);
+            if (N * NT == kC * COLS / 8 || row < kC) {
+#pragma unroll
+                for (int j = 0; j < Q; ++j) d[j] = on ? v[n][j] : u32x4a{0, 0, 0, 0};
             }
         }
     }
@@ -290,8 +315,7 @@ template <int NT> struct TriRegs {
     __device__ __forceinline__ void load(const float* src) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x + n * NT;
-            if (i < kTri / 4) v[n] = reinterpret_cast<const f32x4a*>(src)[i];
+            v[n] = reinterpret_cast<const f32x4a*>(src)[min((int)threadIdx.x + n * NT, kTri / 4 - 1)];
         }
     }
     template <int P> __device__ __forceinline__ void store(__bf16* dst) const {
@@ -301,13 +325,7 @@ template <int NT> struct TriRegs {
             if (i < kTri / 4) {
                 const int bi = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, bj = blk - bi * (bi + 1) / 2;
                 __bf16* d = dst + (16 * bi + ((i >> 2) & 15)) * kLdm + 16 * bj + 4 * (i & 3);
-                f32x4 x = v[n];
-#pragma unroll
-                for (int e = 0; e < P; ++e) {
-                    const bf16x4 h = __builtin_convertvector(x, bf16x4);
-                    *reinterpret_cast<u32x2a*>(d + e * kC * kLdm) = __builtin_bit_cast(u32x2a, h);
-                    x -= __builtin_convertvector(h, f32x4);
-                }
+                parts4<P>(v[n], [&](int e, u32x2a h) { *reinterpret_cast<u32x2a*>(d + e * kC * kLdm) = h; });
             }
         }
     }
@@ -343,9 +361,10 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     const int c = blockIdx.x % a.nc, bh = blockIdx.x / a.nc, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
     if (c * kC >= w.len) return;
-    const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6;
-    stage(Kl, LDK, (const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, DK, c * kC, w, tid, 256);
-    stage(Ql, LDK, (const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, DK, c * kC, w, tid, 256);
+    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TileRegs<T, DK, 256> tk, tq;
+    tk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, c * kC, w);
+    tq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, c * kC, w);
     if (wave == 0) {
         const int p = c * kC + l;
         const bool on = p < w.len;
@@ -358,6 +377,8 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
         G[l] = s;
         vec[kBe * kC + l] = on ? a.beta[t * a.bs[0] + b * a.bs[1] + h * a.bs[2]] : 0.f;
     }
+    tk.store(Kl, LDK, a.dk, c * kC, w.len);
+    tq.store(Ql, LDK, a.dk, c * kC, w.len);
     __syncthreads();
     {   // row norms: four lanes a row
         const int row = tid >> 2, part = tid & 3;
@@ -389,7 +410,6 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
         const auto bf = row_frag(Kl, LDK, 16 * wave, 32 * kb);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            if (m < wave) continue;
             kk[m] = mma<Gd<T>::PT, Gd<T>::PT, 3>(row_frag(Kl, LDK, 16 * m, 32 * kb), bf, kk[m]);
             qk[m] = mma<Gd<T>::PT, Gd<T>::PT, 3>(row_frag(Ql, LDK, 16 * m, 32 * kb), bf, qk[m]);
         }
@@ -401,12 +421,14 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
         const double gj = G[j];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
+            const f32x4 sqi = vec4(vec + kSq * kC, 16 * m), rki = vec4(vec + kRk * kC, 16 * m);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 16 * m + 4 * (l >> 4) + e;
-                const float d = i >= j ? __expf((float)(G[i] - gj)) * rkj : 0.f;
-                kk[m][e] = i > j ? kk[m][e] * d * vec[kRk * kC + i] : 0.f;
-                qk[m][e] = i >= j ? qk[m][e] * d * vec[kSq * kC + i] : 0.f;
+                const float d = __expf((float)(G[i] - gj)) * rkj;      // above the diagonal it may be infinite: selected away
+                const float n = kk[m][e] * d * rki[e], p = qk[m][e] * d * sqi[e];
+                kk[m][e] = i > j ? n : 0.f;
+                qk[m][e] = i >= j ? p : 0.f;
             }
             tile_write(N, LDN, 16 * m, 16 * wave, kk[m]);
             tile_write(P, LDN, 16 * m, 16 * wave, qk[m]);
@@ -432,7 +454,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     __syncthreads();
     f32x4 X[4];
     {   // block column j = wave: X_ij = T_i (N_ij - sum_{j <= k < i} N_ik beta_k X_kj), on the f32 matrix instruction
-        const int j = wave, g = l >> 4, i16 = l & 15;
+        const int j = wave, i16 = l & 15;
         auto times = [&](const f32x4 av, const f32x4 bv, f32x4 acc) {   // inner index 4g + m at step m
 #pragma unroll
             for (int m = 0; m < 4; ++m) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[m], bv[m], acc, 0, 0, 0);
@@ -469,16 +491,50 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     for (int i = tid; i < kVec * kC; i += 256) vo[i] = vec[i];
 }
 
+// Nothing is scheduled across: operands of later products are not read ahead, which would cost the registers that the chunk in flight needs.
+__device__ __forceinline__ void phase_end() { __builtin_amdgcn_sched_barrier(0); }
+
+// A state's 16 columns in the accumulators' layout from / to rows [dk][dv].  One 32-bit lane offset, everything else is uniform; dk is a
+// multiple of 8, so a lane's four rows lie inside or outside together.
+template <int KT> __device__ __forceinline__ void state_load(f32x4 (&S)[KT], const float* p, int dk, int dv, int col) {
+    const int g4 = 4 * ((threadIdx.x & 63) >> 4);
+    const uint32_t off = (uint32_t)(g4 * dv + min(col, dv - 1));
+#pragma unroll
+    for (int m = 0; m < KT; ++m) {
+        // rows outside: the same lane's place in a tile that exists (dk >= 8: rows 0 .. 7 do)
+        const bool in = 16 * m + g4 < dk;
+        const uint32_t at = in ? off + 16 * m * dv : (uint32_t)min(col, dv - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = (p + e * dv)[at];
+            S[m][e] = in && col < dv ? x : 0.f;
+        }
+    }
+}
+template <int KT> __device__ __forceinline__ void state_store(const f32x4 (&S)[KT], float* p, int dk, int dv, int col) {
+    const int g4 = 4 * ((threadIdx.x & 63) >> 4);
+    const uint32_t off = (uint32_t)(g4 * dv + col);
+#pragma unroll
+    for (int m = 0; m < KT; ++m)
+        if (16 * m + g4 < dk && col < dv) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) (p + (16 * m + e) * dv)[off] = S[m][e];
+        }
+}
+
 // ---- scan -----------------------------------------------------------------------------------------------
-// rows [64][16 columns of this wave] from LDS to global rows, 16 bytes a lane
-template <typename T, typename F>
-__device__ __forceinline__ void store_rows(const T* src, int ld, int ncol, int rows, F&& dst) {
+// rows [64][16 columns of this wave] from LDS to a chunk's frames, 16 bytes a lane
+template <typename T>
+__device__ __forceinline__ void store_rows(const T* src, int ld, int ncol, T* dst, int64_t ts, int pos0, Walk w) {
     const int l = threadIdx.x & 63;
     constexpr int VE = 16 / sizeof(T), LPR = 16 / VE;       // elements a lane, lanes a row
+    char* base = reinterpret_cast<char*>(dst + w.low(pos0) * ts);
 #pragma unroll
-    for (int r = l / LPR; r < kC; r += 64 / LPR) {
-        const int c = (l % LPR) * VE;
-        if (r < rows && c < ncol) *reinterpret_cast<u32x4a*>(dst(r) + c) = *reinterpret_cast<const u32x4a*>(src + r * ld + c);
+    for (int x = 0; x < LPR; ++x) {
+        const int r = l / LPR + x * (64 / LPR), c = (l % LPR) * VE;
+        if (pos0 + r < w.len && c < ncol)
+            *reinterpret_cast<u32x4a*>(base + (w.above(pos0, pos0 + r) * (uint32_t)(ts * sizeof(T)) + (uint32_t)(c * sizeof(T)))) =
+                *reinterpret_cast<const u32x4a*>(src + r * ld + c);
     }
 }
 template <typename T>
@@ -516,18 +572,14 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
-    const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6, g = l >> 4, i16 = l & 15;
+    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = l & 15;
     const int col0 = (sg * NW + wave) * 16, col = col0 + i16;     // this wave's columns of dv
     const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv;
     f32x4 S[KT];
 #pragma unroll
-    for (int m = 0; m < KT; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * m + 4 * g + e;
-            S[m][e] = a.s0 && row < a.dk && col < a.dv ? a.s0[state + (int64_t)row * a.dv + col] : 0.f;
-        }
+    for (int m = 0; m < KT; ++m) S[m] = f32x4{0, 0, 0, 0};
+    if (a.s0) state_load(S, a.s0 + state, a.dk, a.dv, col);
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
     const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 16;
@@ -553,9 +605,9 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     for (int c = 0; c < ncl; ++c) {
         const int64_t at = (int64_t)bh * a.nc + c;
         __syncthreads();
-        rk.store(Kl, LDK);
-        rq.store(Ql, LDK);
-        rv.store(Vl, LDV);
+        rk.store(Kl, LDK, a.dk, c * kC, w.len);
+        rq.store(Ql, LDK, a.dk, c * kC, w.len);
+        rv.store(Vl, LDV, vcols, c * kC, w.len);
         rx.template store<3>(Xl);
         rp.template store<EP>(Pl);
 #pragma unroll
@@ -563,16 +615,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
         __syncthreads();
         if (c + 1 < ncl) fetch(c + 1);
         if (mycols <= 0) continue;
-        if (TRAIN) {      // for the backward
-            float* so = a.S0 + at * a.dk * a.dv;
-#pragma unroll
-            for (int m = 0; m < KT; ++m)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = 16 * m + 4 * g + e;
-                    if (row < a.dk && col < a.dv) so[(int64_t)row * a.dv + col] = S[m][e];
-                }
-        }
+        if (TRAIN) state_store(S, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col);      // for the backward
         f32x4 ks[4], qs[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) { ks[m] = f32x4{0, 0, 0, 0}; qs[m] = ks[m]; }
@@ -612,7 +655,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) tile_write(my, LDV, 16 * m, 0, qs[m]);
         lds_order();
-        store_rows(my, LDV, mycols, w.len - c * kC, [&](int r) { return op + w.frame(c * kC + r) * ots + col0; });
+        store_rows(my, LDV, mycols, op + col0, ots, c * kC, w);
         // S = e^{G_C} S + K^T (kb U)
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
         row_operands(uf, vec + kKb * kC, ks);
@@ -623,13 +666,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
             for (int kb = 0; kb < 2; ++kb) S[m] = mma(col_frag(Kl, LDK, 32 * kb, 16 * m), uf[kb], S[m]);
         }
     }
-#pragma unroll
-    for (int m = 0; m < KT; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * m + 4 * g + e;
-            if (row < a.dk && col < a.dv) a.sT[state + (int64_t)row * a.dv + col] = S[m][e];
-        }
+    state_store(S, a.sT + state, a.dk, a.dv, col);
     if (vcols > 0) zero_rows(op + sg * NW * 16, ots, vcols, w.len, a.T, tid, NT);
 }
 
@@ -657,18 +694,14 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
-    const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6, g = l >> 4, i16 = l & 15;
+    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = l & 15;
     const int slice = sg * NW + wave, col0 = slice * 16, col = col0 + i16;
     const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv, nat = (int64_t)a.B * a.H * a.nc;
     f32x4 S[KT], s0n[KT];                                   // dS; the next chunk's starting state
 #pragma unroll
-    for (int m = 0; m < KT; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * m + 4 * g + e;
-            S[m][e] = a.gsT && row < a.dk && col < a.dv ? a.gsT[state + (int64_t)row * a.dv + col] : 0.f;
-        }
+    for (int m = 0; m < KT; ++m) S[m] = f32x4{0, 0, 0, 0};
+    if (a.gsT) state_load(S, a.gsT + state, a.dk, a.dv, col);
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
     const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 16;
@@ -690,24 +723,17 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
         rp.load(a.P + at * kTri);
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
-        const float* so = a.S0 + at * a.dk * a.dv;
-#pragma unroll
-        for (int m = 0; m < KT; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * m + 4 * g + e;
-                s0n[m][e] = row < a.dk && col < a.dv ? so[(int64_t)row * a.dv + col] : 0.f;
-            }
+        state_load(s0n, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col);
     };
     clear_upper(Xl, 6, tid, NT);
     if (ncl > 0) fetch(ncl - 1);
     for (int c = ncl - 1; c >= 0; --c) {
         const int64_t at = (int64_t)bh * a.nc + c;
         __syncthreads();
-        rk.store(Kl, LDK);
-        rq.store(Ql, LDK);
-        rv.store(Vl, LDV);
-        ro.store(Ol, LDV);
+        rk.store(Kl, LDK, a.dk, c * kC, w.len);
+        rq.store(Ql, LDK, a.dk, c * kC, w.len);
+        rv.store(Vl, LDV, vcols, c * kC, w.len);
+        ro.store(Ol, LDV, vcols, c * kC, w.len);
         rx.template store<3>(Xl);
         rp.template store<3>(Pl);
 #pragma unroll
@@ -716,36 +742,31 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 #pragma unroll
         for (int m = 0; m < KT; ++m) s0[m] = s0n[m];
         __syncthreads();
-        if (c > 0) fetch(c - 1);
-        if (mycols <= 0) continue;
+        if (mycols <= 0) {
+            if (c > 0) fetch(c - 1);
+            continue;
+        }
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
         float anchor = 0.f;
         {   // dS at the chunk's end is what the gradient kernel needs; <dS, S_C> = dec <dS, S0> + sum_j dU2_j . U_j
-            float* so = a.dS + at * a.dk * a.dv;
+            state_store(S, a.dS + at * a.dk * a.dv, a.dk, a.dv, col);
+            f32x4 p = {0, 0, 0, 0};
 #pragma unroll
-            for (int m = 0; m < KT; ++m) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = 16 * m + 4 * g + e;
-                    if (row < a.dk && col < a.dv) so[(int64_t)row * a.dv + col] = S[m][e];
-                    anchor += S[m][e] * s0[m][e];
-                }
-            }
-            anchor *= dec;
+            for (int m = 0; m < KT; ++m) p += S[m] * s0[m];
+            anchor = dec * ((p[0] + p[1]) + (p[2] + p[3]));
         }
         f32x4 E[4], O[4], du[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) { E[m] = f32x4{0, 0, 0, 0}; O[m] = E[m]; du[m] = E[m]; }
 #pragma unroll
         for (int kb = 0; kb < DK / 32; ++kb) {
-            const Frag<3> sb = split<3>(s0[2 * kb], s0[2 * kb + 1]), db = split<3>(S[2 * kb], S[2 * kb + 1]);
+            const Frag<3> sb = split<3>(s0[2 * kb], s0[2 * kb + 1]);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const auto kf = row_frag(Kl, LDK, 16 * m, 32 * kb);
-                E[m] = mma(kf, sb, E[m]);
-                du[m] = mma(kf, db, du[m]);
+                E[m] = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), sb, E[m]);
                 O[m] = mma(row_frag(Ql, LDK, 16 * m, 32 * kb), sb, O[m]);
             }
+            phase_end();
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -760,6 +781,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 #pragma unroll
             for (int kb = 0; kb <= m / 2; ++kb) xs = mma(plane_rows<3>(Xl, 16 * m, 32 * kb), f[kb], xs);
             E[m] -= xs;
+            phase_end();
         }
         row_operands(f, vec + kBe * kC, E);                 // U
         f32x4 z[4];
@@ -768,6 +790,17 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 #pragma unroll
             for (int kb = 0; kb <= m / 2; ++kb) O[m] = mma(plane_rows<3>(Pl, 16 * m, 32 * kb), f[kb], O[m]);
             z[m] = O[m] * tile_read(Ol, LDV, 16 * m, wave * 16);
+            phase_end();
+        }
+#pragma unroll
+        for (int kb = 0; kb < DK / 32; ++kb) {
+            const Frag<3> db = split<3>(S[2 * kb], S[2 * kb + 1]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) du[m] = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), db, du[m]);
+            phase_end();
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
             du[m] *= vec4(vec + kKb * kC, 16 * m);
             const f32x4 p = du[m] * vec4(vec + kBe * kC, 16 * m) * E[m];
             anchor += (p[0] + p[1]) + (p[2] + p[3]);
@@ -777,6 +810,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
             const auto of = col_frag(Ol, LDV, 32 * kb, wave * 16);
 #pragma unroll
             for (int m = 0; m < 2 * kb + 2; ++m) du[m] = mma(plane_cols<3>(Pl, 32 * kb, 16 * m), of, du[m]);
+            phase_end();
         }
         row_operands(f, vec + kBe * kC, du);
         float* zo = a.zpart + (slice * nat + at) * kC;
@@ -796,6 +830,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
                 *reinterpret_cast<f32x4a*>(bo + 16 * m + 4 * g) = sb;
                 *reinterpret_cast<f32x4a*>(zo + 16 * m + 4 * g) = z[m];
             }
+            phase_end();
         }
         anchor = wave_sum(anchor);
         if (l == 0) a.apart[slice * nat + at] = anchor;
@@ -813,38 +848,30 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 #pragma unroll
         for (int m = 0; m < 4; ++m) tile_write(my, LDV, 16 * m, 0, du[m]);
         lds_order();
-        store_rows(my, LDV, mycols, w.len - c * kC, [&](int r) { return gvp + w.frame(c * kC + r) * ots + col0; });
+        store_rows(my, LDV, mycols, gvp + col0, ots, c * kC, w);
         ET* eo = (ET*)a.E + at * kC * a.dv;
         if constexpr (sizeof(ET) == sizeof(T)) {
             ET* me = reinterpret_cast<ET*>(Ol + wave * 16);
 #pragma unroll
             for (int m = 0; m < 4; ++m) tile_write(me, LDV, 16 * m, 0, E[m]);
             lds_order();
-            store_rows(me, LDV, mycols, kC, [&](int r) { return eo + (int64_t)r * a.dv + col0; });
+            store_rows(me, LDV, mycols, eo + col0, a.dv, 0, Walk{kC, false});
         } else {
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (col < a.dv) eo[(int64_t)(16 * m + 4 * g + e) * a.dv + col] = E[m][e];
+            state_store(E, eo, kC, a.dv, col);
         }
+        phase_end();
+        if (c > 0) fetch(c - 1);      // here, not earlier: the tiles in flight take 57 registers a lane, which are free only now
+        phase_end();
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
             S[m] *= dec;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 S[m] = mma(col_frag(Ql, LDK, 32 * kb, 16 * m), qf[kb], mma(col_frag(Kl, LDK, 32 * kb, 16 * m), f[kb], S[m]));
+            phase_end();
         }
     }
-    if (a.gs0) {
-#pragma unroll
-        for (int m = 0; m < KT; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * m + 4 * g + e;
-                if (row < a.dk && col < a.dv) a.gs0[state + (int64_t)row * a.dv + col] = S[m][e];
-            }
-    }
+    if (a.gs0) state_store(S, a.gs0 + state, a.dk, a.dv, col);
     if (vcols > 0) zero_rows(gvp + sg * NW * 16, ots, vcols, w.len, a.T, tid, NT);
 }
 
@@ -858,25 +885,18 @@ template <typename T, int DK> struct GradLds {
 
 template <int P> __device__ __forceinline__ void plane_write(__bf16* t, int r0, int c0, f32x4 v) {
     const int l = threadIdx.x & 63;
-    __bf16* p = t + (r0 + 4 * (l >> 4)) * kLdm + c0 + (l & 15);
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const bf16x4 h = __builtin_convertvector(v, bf16x4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[i * kC * kLdm + e * kLdm] = h[e];
-        v -= __builtin_convertvector(h, f32x4);
-    }
+    short* p = reinterpret_cast<short*>(t) + (r0 + 4 * (l >> 4)) * kLdm + c0 + (l & 15);
+    parts4<P>(v, [&](int i, u32x2a h) {
+        short* o = p + i * kC * kLdm;
+        o[0] = (short)h.x; o[kLdm] = (short)(h.x >> 16);
+        o[2 * kLdm] = (short)h.y; o[3 * kLdm] = (short)(h.y >> 16);
+    });
 }
 // the transpose of a tile: rows and columns exchanged
 template <int P> __device__ __forceinline__ void plane_write_t(__bf16* t, int r0, int c0, f32x4 v) {
     const int l = threadIdx.x & 63;
     __bf16* p = t + (c0 + (l & 15)) * kLdm + r0 + 4 * (l >> 4);
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const bf16x4 h = __builtin_convertvector(v, bf16x4);
-        *reinterpret_cast<u32x2a*>(p + i * kC * kLdm) = __builtin_bit_cast(u32x2a, h);
-        v -= __builtin_convertvector(h, f32x4);
-    }
+    parts4<P>(v, [&](int i, u32x2a h) { *reinterpret_cast<u32x2a*>(p + i * kC * kLdm) = h; });
 }
 
 // Two workgroups a CU (16-bit types): one loads while the other multiplies.
@@ -895,7 +915,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
     const double* G = reinterpret_cast<const double*>(vec + kG64 * kC);
     float* dots = vec + kVec * kC;                                        // [2][4][64]
     const int c = blockIdx.x % a.nc, bk = blockIdx.x / a.nc, b = bk / a.Hk, hk = bk % a.Hk;
-    const int tid = threadIdx.x, l = tid & 63, wave = tid >> 6, g = l >> 4, i16 = l & 15;
+    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = l & 15;
     const Walk w = walk_of(a, b, hk * a.r);
     const int64_t kts = (int64_t)a.B * a.Hk * a.dk, gts = (int64_t)a.B * a.H;
     T* gqp = (T*)a.gq + ((int64_t)b * a.Hk + hk) * a.dk;
@@ -922,6 +942,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
     for (int hh = 0; hh < a.r; ++hh) {
         const int h = hk * a.r + hh, bh = b * a.H + h;
         const int64_t at = (int64_t)bh * a.nc + c;
+        // the states' rows of one of this wave's tiles of dk, requested ahead of the barrier: lane = row, 128 columns of dv
+        f32x4 s0r[8], dsr[8];
+        auto state_rows = [&](int n) {
+            const int row = (wave * NT + n) * 16 + i16;
+            const float* s0 = a.S0 + at * a.dk * a.dv;
+            const float* ds = a.dS + at * a.dk * a.dv;
+            const uint32_t off = (uint32_t)(min(row, a.dk - 1) * a.dv);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const uint32_t at4 = off + min(16 * x + 4 * g, a.dv - 4);
+                const bool in = row < a.dk && 16 * x + 4 * g < a.dv;
+                const f32x4 u = *reinterpret_cast<const f32x4a*>(s0 + at4), v = *reinterpret_cast<const f32x4a*>(ds + at4);
+                s0r[x] = in ? u : f32x4{0, 0, 0, 0};
+                dsr[x] = in ? v : f32x4{0, 0, 0, 0};
+            }
+        };
         __syncthreads();
         {
             TileRegs<T, 128, 256> ro, rd;
@@ -931,61 +967,39 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
             rd.load((const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, p0, w);
             re.load((const ET*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
             for (int i = tid; i < kVec * kC; i += 256) vec[i] = a.vec[at * kVec * kC + i];
-            ro.store(Ol, LDV);
-            rd.store(Dl, LDV);
-            re.store(El, LDE);
+            state_rows(0);
+            ro.store(Ol, LDV, a.dv, p0, w.len);
+            rd.store(Dl, LDV, a.dv, p0, w.len);
+            re.store(El, LDE, a.dv, 0, kC);
+            phase_end();
         }
         __syncthreads();
         // states: wave = a quarter of dk; U = beta E: its factor goes with the rows
-        {
-            const float* s0 = a.S0 + at * a.dk * a.dv;
-            const float* ds = a.dS + at * a.dk * a.dv;
-            f32x4 cq[4][NT], ck[4][NT], cd[4][NT];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+        for (int n = 0; n < NT; ++n) {
+            f32x4 cq[4], ck[4], cd[4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) { cq[m][n] = f32x4{0, 0, 0, 0}; ck[m][n] = cq[m][n]; cd[m][n] = cq[m][n]; }
+            for (int m = 0; m < 4; ++m) { cq[m] = f32x4{0, 0, 0, 0}; ck[m] = cq[m]; cd[m] = cq[m]; }
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
                 if (kb * 32 >= a.dv) break;
-                Frag<OP> sf[NT], df[NT];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const int row = (wave * NT + n) * 16 + i16, c0 = 32 * kb + 4 * g, c1 = c0 + 16;
-                    f32x4 s_0 = {0, 0, 0, 0}, s_1 = s_0, d_0 = s_0, d_1 = s_0;
-                    if (row < a.dk && c0 < a.dv) {
-                        s_0 = *reinterpret_cast<const f32x4a*>(s0 + (int64_t)row * a.dv + c0);
-                        d_0 = *reinterpret_cast<const f32x4a*>(ds + (int64_t)row * a.dv + c0);
-                    }
-                    if (row < a.dk && c1 < a.dv) {
-                        s_1 = *reinterpret_cast<const f32x4a*>(s0 + (int64_t)row * a.dv + c1);
-                        d_1 = *reinterpret_cast<const f32x4a*>(ds + (int64_t)row * a.dv + c1);
-                    }
-                    sf[n] = split<OP>(s_0, s_1);
-                    df[n] = split<OP>(d_0, d_1);
-                }
+                const Frag<OP> sf = split<OP>(s0r[2 * kb], s0r[2 * kb + 1]), df = split<OP>(dsr[2 * kb], dsr[2 * kb + 1]);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    const auto of = row_frag(Ol, LDV, 16 * m, 32 * kb);
-                    const auto uf = row_frag(El, LDE, 16 * m, 32 * kb);
-                    const auto vf = row_frag(Dl, LDV, 16 * m, 32 * kb);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        cq[m][n] = mma<PT, OP, OP>(of, sf[n], cq[m][n]);
-                        ck[m][n] = mma<PE, OP, OP>(uf, df[n], ck[m][n]);
-                        cd[m][n] = mma<PT, OP, OP>(vf, sf[n], cd[m][n]);
-                    }
+                    cq[m] = mma<PT, OP, OP>(row_frag(Ol, LDV, 16 * m, 32 * kb), sf, cq[m]);
+                    ck[m] = mma<PE, OP, OP>(row_frag(El, LDE, 16 * m, 32 * kb), df, ck[m]);
+                    cd[m] = mma<PT, OP, OP>(row_frag(Dl, LDV, 16 * m, 32 * kb), sf, cd[m]);
                 }
+                phase_end();
             }
+            if (n + 1 < NT) state_rows(n + 1);
+            phase_end();
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 const f32x4 aq = vec4(vec + kAq * kC, 16 * m), ak = vec4(vec + kAk * kC, 16 * m);
                 const f32x4 kb = vec4(vec + kKb * kC, 16 * m) * vec4(vec + kBe * kC, 16 * m);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    tq[m][n] += aq * cq[m][n];
-                    tk[m][n] += kb * ck[m][n] - ak * cd[m][n];
-                }
+                tq[m][n] += aq * cq[m];
+                tk[m][n] += kb * ck[m] - ak * cd[m];
             }
         }
         // M1 = dP * D * sq_i * rk_j (lower), M2 = -dV U^T * D * rk_i * rk_j (strictly lower, made symmetric); wave = block column j
@@ -998,32 +1012,35 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
             const auto uf = row_frag(El, LDE, 16 * wave, 32 * kb);
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                if (m < wave) continue;
                 dp[m] = mma<PT, PE, OP>(row_frag(Ol, LDV, 16 * m, 32 * kb), uf, dp[m]);
                 dn[m] = mma<PT, PE, OP>(row_frag(Dl, LDV, 16 * m, 32 * kb), uf, dn[m]);
             }
+            phase_end();
         }
         {
             const int j = 16 * wave + i16;
             const float rkj = vec[kRk * kC + j] * vec[kBe * kC + j];
             const double gj = G[j];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+            for (int m = 0; m < 4; ++m) {
+                const f32x4 sqi = vec4(vec + kSq * kC, 16 * m), rki = vec4(vec + kRk * kC, 16 * m);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 16 * m + 4 * g + e;
-                    const float d = i >= j ? __expf((float)(G[i] - gj)) * rkj : 0.f;
-                    dp[m][e] = i >= j ? dp[m][e] * d * vec[kSq * kC + i] : 0.f;
-                    dn[m][e] = i > j ? -dn[m][e] * d * vec[kRk * kC + i] : 0.f;
+                    const float d = __expf((float)(G[i] - gj)) * rkj;      // above the diagonal it may be infinite: selected away
+                    const float p = dp[m][e] * d * sqi[e], n = -dn[m][e] * d * rki[e];
+                    dp[m][e] = i >= j ? p : 0.f;
+                    dn[m][e] = i > j ? n : 0.f;
                 }
+                plane_write<OP>(M, 16 * m, 16 * wave, dp[m]);
+                phase_end();
+            }
         }
         __syncthreads();
         {
             TileRegs<T, DK, 256> rk, rq;
             rk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, p0, w);
             rq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, p0, w);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) plane_write<OP>(M, 16 * m, 16 * wave, dp[m]);
             if (wave == 0) {      // dg and dbeta: lane = frame
                 float z = 0.f, be = 0.f, an = 0.f;
                 for (int s = 0; s < a.nsl; ++s) {
@@ -1040,8 +1057,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
                     a.gbeta[o] = be;
                 }
             }
-            rk.store(Kl, LDK);
-            rq.store(Ql, LDK);
+            rk.store(Kl, LDK, a.dk, c * kC, w.len);
+            rq.store(Ql, LDK, a.dk, c * kC, w.len);
         }
         __syncthreads();
 #pragma unroll
@@ -1056,6 +1073,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
                     if (kb <= m / 2) tq[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, 16 * m, 32 * kb), kf, tq[m][n]);
                     if (kb >= m / 2) tk[m][n] = mma<OP, PT, OP>(plane_cols<OP>(M, 32 * kb, 16 * m), qf, tk[m][n]);
                 }
+                phase_end();
             }
         __syncthreads();
 #pragma unroll
@@ -1085,6 +1103,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
                 const auto kf = col_frag(Kl, LDK, 32 * kb, (wave * NT + n) * 16);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) tk[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, 16 * m, 32 * kb), kf, tk[m][n]);
+                phase_end();
             }
     }
     // through the normalisation: dq = tq - q |q|^-2 (q . tq)  (|.|^2 with its epsilon), dk alike
@@ -1237,6 +1256,7 @@ static int gdr_check(const char* who, int T, int B, int Hk, int H, int dk, int d
     SP_CHECK_ARG((flags & ~(SP_GDR_NORMALIZE | SP_GDR_BIDIRECTIONAL)) == 0, "%s: unknown flags %d", who, flags);
     SP_CHECK_ARG(!(flags & SP_GDR_BIDIRECTIONAL) || Hk % 2 == 0, "%s: both directions need an even number of key heads, not %d", who, Hk);
     SP_CHECK_ARG(dtype == SP_F32 || dtype == SP_BF16 || dtype == SP_F16, "%s: dtype %d not supported (f32, bf16, f16)", who, dtype);
+    SP_CHECK_ARG((int64_t)B * H * 128 <= (1ll << 23), "%s: B=%d x H=%d exceed 65536", who, B, H);
     SP_CHECK_ARG((int64_t)B * H * ((T + kC - 1) / kC + 4) < (1ll << 22), "%s: B=%d x H=%d x %d frames exceed the grid", who, B, H, T);
     return SP_OK;
 }
@@ -1271,6 +1291,7 @@ static GdrBwdLayout gdr_bwd_ws(int T, int B, int H, int dk, int dv, int dtype) {
 
 static bool gdr_aligned(const void* p, const int64_t* st, int dtype) {
     const int64_t ve = dtype == SP_F32 ? 4 : 8;
+    if (st[0] < 0 || st[0] * 4 > (1ll << 25)) return false;
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st[0] % ve == 0 && st[1] % ve == 0 && st[2] % ve == 0;
 }
 
@@ -1350,7 +1371,7 @@ extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const flo
         return gdr_launch(gdr_recurrent_kernel<__hip_bfloat16>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
     }
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype),
-                 "sp_gdr_fwd: q, k, v need 16-byte aligned rows");
+                 "sp_gdr_fwd: q, k, v need 16-byte aligned rows and at most 2^23 elements from frame to frame");
     const GdrLayout lay = gdr_saved(T, B, H, dk, dv, train);
     if (train ? saved_bytes < lay.end : workspace_bytes < lay.end || !workspace)
         return fail(SP_EWORKSPACE, "sp_gdr_fwd: %s %zu < %zu bytes", train ? "saved" : "workspace", train ? saved_bytes : workspace_bytes, lay.end);
@@ -1380,7 +1401,7 @@ extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const flo
     SP_CHECK_ARG(T > 0, "sp_gdr_bwd: T=0 has nothing to differentiate");
     SP_CHECK_ARG(q && k && v && g && beta && strides && o && saved && go && gq && gk && gv && gg && gbeta && workspace, "sp_gdr_bwd: null pointer");
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype) &&
-                     gdr_aligned(go, strides + 15, dtype), "sp_gdr_bwd: q, k, v, go need 16-byte aligned rows");
+                     gdr_aligned(go, strides + 15, dtype), "sp_gdr_bwd: q, k, v, go need 16-byte aligned rows and at most 2^23 elements from frame to frame");
     const GdrLayout lay = gdr_saved(T, B, H, dk, dv, true);
     const GdrBwdLayout ws = gdr_bwd_ws(T, B, H, dk, dv, dtype);
     if (saved_bytes < lay.end || workspace_bytes < ws.end)
