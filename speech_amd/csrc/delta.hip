@@ -220,6 +220,28 @@ template <int P> __device__ __forceinline__ Frag<P> plane_cols(const __bf16* t, 
     return f;
 }
 
+// four row tiles' operands for one block of 32 inner indices; one column tile's for both blocks
+template <typename T, int P> __device__ __forceinline__ void row_frags(Frag<P> (&f)[4], const T* t, int ld, int c0) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m) f[m] = row_frag(t, ld, 16 * m, c0);
+}
+template <typename T, int P> __device__ __forceinline__ void col_frags(Frag<P> (&f)[2], const T* t, int ld, int m0) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) f[kb] = col_frag(t, ld, 32 * kb, m0);
+}
+// the six operands of a lower triangular 64 x 64 matrix: number x is row tile tri_m(x), block tri_k(x); of its transpose, column tile and
+// block 3 - tri_m(x), 1 - tri_k(x)
+constexpr int tri_m(int x) { return x < 2 ? x : x < 4 ? 2 : 3; }
+constexpr int tri_k(int x) { return x == 3 || x == 5; }
+template <int P, int A, int B> __device__ __forceinline__ void tri_rows(Frag<P> (&f)[6], const __bf16* t) {
+#pragma unroll
+    for (int x = A; x < B; ++x) f[x] = plane_rows<P>(t, 16 * tri_m(x), 32 * tri_k(x));
+}
+template <int P, int A, int B> __device__ __forceinline__ void tri_cols(Frag<P> (&f)[6], const __bf16* t) {
+#pragma unroll
+    for (int x = A; x < B; ++x) f[x] = plane_cols<P>(t, 32 * (1 - tri_k(x)), 16 * (3 - tri_m(x)));
+}
+
 // a 16 x 16 tile in the accumulators' layout: lane (i, g) holds rows r0 + 4g .. +3 of column c0 + i
 __device__ __forceinline__ f32x4 tile_read(const __hip_bfloat16* t, int ld, int r0, int c0) {
     const s16x4 a = tr4(t, ld, r0, c0);
@@ -260,6 +282,11 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // ---- frames ---------------------------------------------------------------------------------------------
 // position i of a head's walk -> frame: reversed heads walk an utterance's own frames backwards
 struct Walk {
@@ -286,9 +313,10 @@ template <typename T, int COLS, int NT> struct TileRegs {
     u32x4a v[N][Q];
     __device__ __forceinline__ void load(const T* src, int64_t ts, int ncol, int pos0, Walk w) {
         const char* base = reinterpret_cast<const char*>(src + w.low(pos0) * ts);
+        const int tid = opaque(threadIdx.x);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
+            const int i = tid + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
             const uint32_t off = w.above(pos0, min(pos0 + row, w.len - 1)) * (uint32_t)(ts * sizeof(T)) + (uint32_t)(min(c, ncol - 8) * sizeof(T));
             const u32x4a* s = reinterpret_cast<const u32x4a*>(base + off);
 #pragma unroll
@@ -296,14 +324,20 @@ template <typename T, int COLS, int NT> struct TileRegs {
         }
     }
     __device__ __forceinline__ void store(T* dst, int ld, int ncol, int pos0, int len) const {
+        const int tid = opaque(threadIdx.x);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int i = threadIdx.x + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
-            const bool on = pos0 + row < len && c < ncol;
+            const int i = tid + n * NT, row = i / (COLS / 8), c = i % (COLS / 8) * 8;
             u32x4a* d = reinterpret_cast<u32x4a*>(dst + row * ld + c);
             if (N * NT == kC * COLS / 8 || row < kC) {
+                if (pos0 + kC <= len && ncol == COLS) {
 #pragma unroll
-                for (int j = 0; j < Q; ++j) d[j] = on ? v[n][j] : u32x4a{0, 0, 0, 0};
+                    for (int j = 0; j < Q; ++j) d[j] = v[n][j];
+                } else {
+                    const bool on = pos0 + row < len && c < ncol;
+#pragma unroll
+                    for (int j = 0; j < Q; ++j) d[j] = on ? v[n][j] : u32x4a{0, 0, 0, 0};
+                }
             }
         }
     }
@@ -454,7 +488,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     __syncthreads();
     f32x4 X[4];
     {   // block column j = wave: X_ij = T_i (N_ij - sum_{j <= k < i} N_ik beta_k X_kj), on the f32 matrix instruction
-        const int j = wave, i16 = l & 15;
+        const int j = wave, g = l >> 4, i16 = l & 15;
         auto times = [&](const f32x4 av, const f32x4 bv, f32x4 acc) {   // inner index 4g + m at step m
 #pragma unroll
             for (int m = 0; m < 4; ++m) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(av[m], bv[m], acc, 0, 0, 0);
@@ -491,36 +525,52 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     for (int i = tid; i < kVec * kC; i += 256) vo[i] = vec[i];
 }
 
-// Nothing is scheduled across: operands of later products are not read ahead, which would cost the registers that the chunk in flight needs.
-__device__ __forceinline__ void phase_end() { __builtin_amdgcn_sched_barrier(0); }
-
-// A state's 16 columns in the accumulators' layout from / to rows [dk][dv].  One 32-bit lane offset, everything else is uniform; dk is a
-// multiple of 8, so a lane's four rows lie inside or outside together.
-template <int KT> __device__ __forceinline__ void state_load(f32x4 (&S)[KT], const float* p, int dk, int dv, int col) {
-    const int g4 = 4 * ((threadIdx.x & 63) >> 4);
-    const uint32_t off = (uint32_t)(g4 * dv + min(col, dv - 1));
+// A state's 16 columns in the accumulators' layout from / to rows [dk][dv].  One 32-bit lane offset in bytes, everything else is uniform; dk
+// is a multiple of 8, so a lane's four rows lie inside or outside together.
+template <int KT> __device__ __forceinline__ void state_load(f32x4 (&S)[KT], const float* p, int dk, int dv, int col0) {
+    const int g4 = 4 * ((threadIdx.x & 63) >> 4), col = col0 + (threadIdx.x & 15);
+    const char* base = reinterpret_cast<const char*>(p);
+    if (dk == 16 * KT && col0 + 16 <= dv) {
+        const uint32_t off = (uint32_t)(g4 * dv + col) * 4u;
 #pragma unroll
-    for (int m = 0; m < KT; ++m) {
-        // rows outside: the same lane's place in a tile that exists (dk >= 8: rows 0 .. 7 do)
-        const bool in = 16 * m + g4 < dk;
-        const uint32_t at = in ? off + 16 * m * dv : (uint32_t)min(col, dv - 1);
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float x = (p + e * dv)[at];
-            S[m][e] = in && col < dv ? x : 0.f;
+            for (int e = 0; e < 4; ++e) S[m][e] = *reinterpret_cast<const float*>(base + (uint32_t)(16 * m + e) * dv * 4u + off);
+    } else {
+#pragma unroll
+        for (int m = 0; m < KT; ++m) {
+            const bool in = 16 * m + g4 < dk && col < dv;
+            const uint32_t off = in ? (uint32_t)((16 * m + g4) * dv + col) * 4u : 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = *reinterpret_cast<const float*>(base + (uint32_t)(e * dv) * 4u + off);
+                S[m][e] = in ? x : 0.f;
+            }
         }
     }
 }
-template <int KT> __device__ __forceinline__ void state_store(const f32x4 (&S)[KT], float* p, int dk, int dv, int col) {
-    const int g4 = 4 * ((threadIdx.x & 63) >> 4);
-    const uint32_t off = (uint32_t)(g4 * dv + col);
+template <int KT> __device__ __forceinline__ void state_store(const f32x4 (&S)[KT], float* p, int dk, int dv, int col0) {
+    const int g4 = 4 * ((threadIdx.x & 63) >> 4), col = col0 + (threadIdx.x & 15);
+    char* base = reinterpret_cast<char*>(p);
+    const uint32_t off = (uint32_t)(g4 * dv + col) * 4u;
+    if (dk == 16 * KT && col0 + 16 <= dv) {
 #pragma unroll
-    for (int m = 0; m < KT; ++m)
-        if (16 * m + g4 < dk && col < dv) {
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) (p + (16 * m + e) * dv)[off] = S[m][e];
-        }
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<float*>(base + (uint32_t)(16 * m + e) * dv * 4u + off) = S[m][e];
+    } else {
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+            if (16 * m + g4 < dk && col < dv) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) *reinterpret_cast<float*>(base + (uint32_t)(16 * m + e) * dv * 4u + off) = S[m][e];
+            }
+    }
 }
+
+// Nothing is scheduled across.  Between two such lines stand the LDS reads of the next products and the matrix instructions of the present
+// ones: left alone, the compiler reads one fragment, waits for it, multiplies, and reads the next.
+__device__ __forceinline__ void phase_end() { __builtin_amdgcn_sched_barrier(0); }
 
 // ---- scan -----------------------------------------------------------------------------------------------
 // rows [64][16 columns of this wave] from LDS to a chunk's frames, 16 bytes a lane
@@ -562,7 +612,8 @@ template <typename T, int DK, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = ScanLds<T, DK, NW>;
-    constexpr int NT = NW * 64, EP = Gd<T>::EP, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    constexpr int NT = NW * 64, PT = Gd<T>::PT, EP = Gd<T>::EP, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    constexpr bool AHEAD = PT == 1;      // operands of one part fit the registers ahead of their use
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
     T* Vl = Ql + kC * LDK;
@@ -572,14 +623,14 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
-    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = l & 15;
-    const int col0 = (sg * NW + wave) * 16, col = col0 + i16;     // this wave's columns of dv
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col0 = (sg * NW + wave) * 16;                        // this wave's columns of dv
     const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv;
     f32x4 S[KT];
 #pragma unroll
     for (int m = 0; m < KT; ++m) S[m] = f32x4{0, 0, 0, 0};
-    if (a.s0) state_load(S, a.s0 + state, a.dk, a.dv, col);
+    if (a.s0) state_load(S, a.s0 + state, a.dk, a.dv, col0);
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
     const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 16;
@@ -615,40 +666,77 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
         __syncthreads();
         if (c + 1 < ncl) fetch(c + 1);
         if (mycols <= 0) continue;
-        if (TRAIN) state_store(S, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col);      // for the backward
+        if (TRAIN) state_store(S, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col0);      // for the backward
         f32x4 ks[4], qs[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) { ks[m] = f32x4{0, 0, 0, 0}; qs[m] = ks[m]; }
+        Frag<PT> kf[2][4], qf[2][4];
+        row_frags(kf[0], Kl, LDK, 0);
+        row_frags(qf[0], Ql, LDK, 0);
+        Frag<3> xf[6];
+        f32x4 vt[4];
 #pragma unroll
         for (int kb = 0; kb < DK / 32; ++kb) {
+            if (kb + 1 < DK / 32) {
+                row_frags(kf[(kb + 1) & 1], Kl, LDK, 32 * (kb + 1));
+                row_frags(qf[(kb + 1) & 1], Ql, LDK, 32 * (kb + 1));
+            } else {
+#pragma unroll
+                for (int m = 0; m < 4; ++m) vt[m] = tile_read(Vl, LDV, 16 * m, wave * 16);
+                if (AHEAD) tri_rows<3, 0, 3>(xf, Xl);
+            }
             const Frag<3> sb = split<3>(S[2 * kb], S[2 * kb + 1]);
+            if (AHEAD) phase_end();
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                ks[m] = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), sb, ks[m]);
-                qs[m] = mma<Gd<T>::PT, 3, OP>(row_frag(Ql, LDK, 16 * m, 32 * kb), sb, qs[m]);
+                ks[m] = mma(kf[kb & 1][m], sb, ks[m]);
+                qs[m] = mma<PT, 3, OP>(qf[kb & 1][m], sb, qs[m]);
             }
+            if (AHEAD) phase_end();
         }
         // Vt in ks; O's first part in qs
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            ks[m] = tile_read(Vl, LDV, 16 * m, wave * 16) - vec4(vec + kAk * kC, 16 * m) * ks[m];
+            ks[m] = vt[m] - vec4(vec + kAk * kC, 16 * m) * ks[m];
             qs[m] *= vec4(vec + kAq * kC, 16 * m);
         }
         Frag<3> uf[2];
         row_operands(uf, vec + kBe * kC, ks);
+        // E = Vt - X (beta Vt), U = beta E; X is lower triangular: row tiles 0, 1 need the first 32 columns only
+        f32x4 xs[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {      // E = Vt - X (beta Vt); X is lower triangular: row tiles 0, 1 need the first 32 columns only
-            f32x4 xs = {0, 0, 0, 0};
+        for (int m = 0; m < 4; ++m) xs[m] = f32x4{0, 0, 0, 0};
+        tri_rows<3, AHEAD ? 3 : 0, 6>(xf, Xl);
+        if (AHEAD) phase_end();
 #pragma unroll
-            for (int kb = 0; kb <= m / 2; ++kb) xs = mma(plane_rows<3>(Xl, 16 * m, 32 * kb), uf[kb], xs);
-            ks[m] = (ks[m] - xs) * vec4(vec + kBe * kC, 16 * m);      // U
-        }
+        for (int x = 0; x < 3; ++x) xs[tri_m(x)] = mma(xf[x], uf[tri_k(x)], xs[tri_m(x)]);
+        if (AHEAD) phase_end();
+        Frag<EP> pf[6];
+        tri_rows<EP, 0, 6>(pf, Pl);
+        if (AHEAD) phase_end();
+#pragma unroll
+        for (int x = 3; x < 6; ++x) xs[tri_m(x)] = mma(xf[x], uf[tri_k(x)], xs[tri_m(x)]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) ks[m] = (ks[m] - xs[m]) * vec4(vec + kBe * kC, 16 * m);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) uf[kb] = split<3>(ks[2 * kb], ks[2 * kb + 1]);
+        if (AHEAD) phase_end();
+        Frag<PT> cf[KT][2];
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < KT; ++m) col_frags(cf[m], Kl, LDK, 16 * m);
+        if (AHEAD) phase_end();
 #pragma unroll
-            for (int kb = 0; kb <= m / 2; ++kb) qs[m] = mma<EP, 3, OP>(plane_rows<EP>(Pl, 16 * m, 32 * kb), uf[kb], qs[m]);
+        for (int x = 0; x < 6; ++x) qs[tri_m(x)] = mma<EP, 3, OP>(pf[x], uf[tri_k(x)], qs[tri_m(x)]);
+        row_operands(uf, vec + kKb * kC, ks);
+        if (AHEAD) phase_end();
+        // S = e^{G_C} S + K^T (kb U)
+        const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
+#pragma unroll
+        for (int m = 0; m < KT; ++m) {
+            S[m] *= dec;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) S[m] = mma(cf[m][kb], uf[kb], S[m]);
+        }
         // O leaves through this wave's own columns of the V tile, which it has read
         lds_order();
         T* my = Vl + wave * 16;
@@ -656,17 +744,8 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
         for (int m = 0; m < 4; ++m) tile_write(my, LDV, 16 * m, 0, qs[m]);
         lds_order();
         store_rows(my, LDV, mycols, op + col0, ots, c * kC, w);
-        // S = e^{G_C} S + K^T (kb U)
-        const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
-        row_operands(uf, vec + kKb * kC, ks);
-#pragma unroll
-        for (int m = 0; m < KT; ++m) {
-            S[m] *= dec;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) S[m] = mma(col_frag(Kl, LDK, 32 * kb, 16 * m), uf[kb], S[m]);
-        }
     }
-    state_store(S, a.sT + state, a.dk, a.dv, col);
+    state_store(S, a.sT + state, a.dk, a.dv, col0);
     if (vcols > 0) zero_rows(op + sg * NW * 16, ots, vcols, w.len, a.T, tid, NT);
 }
 
@@ -683,7 +762,8 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = RscanLds<T, DK, NW>;
     using ET = typename Gd<T>::ET;
-    constexpr int NT = NW * 64, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    constexpr int NT = NW * 64, PT = Gd<T>::PT, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    constexpr bool AHEAD = PT == 1;
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
     T* Vl = Ql + kC * LDK;
@@ -694,14 +774,14 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
-    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = l & 15;
-    const int slice = sg * NW + wave, col0 = slice * 16, col = col0 + i16;
+    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = l >> 4, i16 = l & 15;
+    const int slice = sg * NW + wave, col0 = slice * 16;
     const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv, nat = (int64_t)a.B * a.H * a.nc;
     f32x4 S[KT], s0n[KT];                                   // dS; the next chunk's starting state
 #pragma unroll
     for (int m = 0; m < KT; ++m) S[m] = f32x4{0, 0, 0, 0};
-    if (a.gsT) state_load(S, a.gsT + state, a.dk, a.dv, col);
+    if (a.gsT) state_load(S, a.gsT + state, a.dk, a.dv, col0);
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
     const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2] + sg * NW * 16;
@@ -723,7 +803,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
         rp.load(a.P + at * kTri);
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
-        state_load(s0n, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col);
+        state_load(s0n, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col0);
     };
     clear_upper(Xl, 6, tid, NT);
     if (ncl > 0) fetch(ncl - 1);
@@ -749,22 +829,50 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
         float anchor = 0.f;
         {   // dS at the chunk's end is what the gradient kernel needs; <dS, S_C> = dec <dS, S0> + sum_j dU2_j . U_j
-            state_store(S, a.dS + at * a.dk * a.dv, a.dk, a.dv, col);
+            state_store(S, a.dS + at * a.dk * a.dv, a.dk, a.dv, col0);
             f32x4 p = {0, 0, 0, 0};
 #pragma unroll
             for (int m = 0; m < KT; ++m) p += S[m] * s0[m];
             anchor = dec * ((p[0] + p[1]) + (p[2] + p[3]));
         }
-        f32x4 E[4], O[4], du[4];
+        f32x4 E[4], O[4], z[4], xs[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) { E[m] = f32x4{0, 0, 0, 0}; O[m] = E[m]; du[m] = E[m]; }
+        for (int m = 0; m < 4; ++m) { E[m] = f32x4{0, 0, 0, 0}; O[m] = E[m]; }
+        Frag<PT> kf[2][4], qf[2][4];
+        Frag<3> tf[6], pf[6], f[2];
+        // six operands of a triangular matrix, each read two products ahead of its use; the last two steps read the next matrix's first two
+        auto six = [&](auto&& read, auto&& use, auto&& next) {
+            if (!AHEAD) { read(0); read(1); }
+#pragma unroll
+            for (int x = 0; x < 6; ++x) {
+                if (x < 4) read(x + 2);
+                else if (AHEAD) next(x - 4);
+                phase_end();
+                use(x);
+                phase_end();
+            }
+        };
+        auto x_rows = [&](int x) { tf[x] = plane_rows<3>(Xl, 16 * tri_m(x), 32 * tri_k(x)); };
+        auto p_rows = [&](int x) { pf[x] = plane_rows<3>(Pl, 16 * tri_m(x), 32 * tri_k(x)); };
+        auto x_cols = [&](int x) { tf[x] = plane_cols<3>(Xl, 32 * (1 - tri_k(x)), 16 * (3 - tri_m(x))); };
+        auto p_cols = [&](int x) { pf[x] = plane_cols<3>(Pl, 32 * (1 - tri_k(x)), 16 * (3 - tri_m(x))); };
+        row_frags(kf[0], Kl, LDK, 0);
+        row_frags(qf[0], Ql, LDK, 0);
 #pragma unroll
         for (int kb = 0; kb < DK / 32; ++kb) {
+            if (kb + 1 < DK / 32) {
+                row_frags(kf[(kb + 1) & 1], Kl, LDK, 32 * (kb + 1));
+                row_frags(qf[(kb + 1) & 1], Ql, LDK, 32 * (kb + 1));
+            } else if (AHEAD) {
+                x_rows(0);
+                x_rows(1);
+            }
             const Frag<3> sb = split<3>(s0[2 * kb], s0[2 * kb + 1]);
+            if (AHEAD) phase_end();
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                E[m] = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), sb, E[m]);
-                O[m] = mma(row_frag(Ql, LDK, 16 * m, 32 * kb), sb, O[m]);
+                E[m] = mma(kf[kb & 1][m], sb, E[m]);
+                O[m] = mma(qf[kb & 1][m], sb, O[m]);
             }
             phase_end();
         }
@@ -772,75 +880,77 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
         for (int m = 0; m < 4; ++m) {
             E[m] = tile_read(Vl, LDV, 16 * m, wave * 16) - vec4(vec + kAk * kC, 16 * m) * E[m];      // Vt
             O[m] *= vec4(vec + kAq * kC, 16 * m);
+            xs[m] = f32x4{0, 0, 0, 0};
         }
-        Frag<3> f[2];
         row_operands(f, vec + kBe * kC, E);
+        six(x_rows, [&](int x) { xs[tri_m(x)] = mma(tf[x], f[tri_k(x)], xs[tri_m(x)]); }, p_rows);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            f32x4 xs = {0, 0, 0, 0};
-#pragma unroll
-            for (int kb = 0; kb <= m / 2; ++kb) xs = mma(plane_rows<3>(Xl, 16 * m, 32 * kb), f[kb], xs);
-            E[m] -= xs;
-            phase_end();
-        }
+        for (int m = 0; m < 4; ++m) E[m] -= xs[m];
         row_operands(f, vec + kBe * kC, E);                 // U
-        f32x4 z[4];
+        six(p_rows, [&](int x) { O[tri_m(x)] = mma(pf[x], f[tri_k(x)], O[tri_m(x)]); },
+            [&](int x) {      // K's four row tiles
+                kf[0][2 * x] = row_frag(Kl, LDK, 32 * x, 0);
+                kf[0][2 * x + 1] = row_frag(Kl, LDK, 32 * x + 16, 0);
+            });
+        if (!AHEAD) row_frags(kf[0], Kl, LDK, 0);
+        f32x4 du[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-#pragma unroll
-            for (int kb = 0; kb <= m / 2; ++kb) O[m] = mma(plane_rows<3>(Pl, 16 * m, 32 * kb), f[kb], O[m]);
             z[m] = O[m] * tile_read(Ol, LDV, 16 * m, wave * 16);
-            phase_end();
+            du[m] = f32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int kb = 0; kb < DK / 32; ++kb) {
+            if (kb + 1 < DK / 32) row_frags(kf[(kb + 1) & 1], Kl, LDK, 32 * (kb + 1));
+            else if (AHEAD) { p_cols(0); p_cols(1); }
             const Frag<3> db = split<3>(S[2 * kb], S[2 * kb + 1]);
+            phase_end();
 #pragma unroll
-            for (int m = 0; m < 4; ++m) du[m] = mma(row_frag(Kl, LDK, 16 * m, 32 * kb), db, du[m]);
+            for (int m = 0; m < 4; ++m) du[m] = mma(kf[kb & 1][m], db, du[m]);
             phase_end();
         }
+        Frag<PT> of[2];
+        col_frags(of, Ol, LDV, wave * 16);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             du[m] *= vec4(vec + kKb * kC, 16 * m);
             const f32x4 p = du[m] * vec4(vec + kBe * kC, 16 * m) * E[m];
             anchor += (p[0] + p[1]) + (p[2] + p[3]);
         }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {      // + P^T dO: column tile m of P has rows >= 16 m
-            const auto of = col_frag(Ol, LDV, 32 * kb, wave * 16);
-#pragma unroll
-            for (int m = 0; m < 2 * kb + 2; ++m) du[m] = mma(plane_cols<3>(Pl, 32 * kb, 16 * m), of, du[m]);
-            phase_end();
-        }
+        six(p_cols, [&](int x) { du[3 - tri_m(x)] = mma(pf[x], of[1 - tri_k(x)], du[3 - tri_m(x)]); }, x_cols);      // + P^T dO
         row_operands(f, vec + kBe * kC, du);
-        float* zo = a.zpart + (slice * nat + at) * kC;
-        float* bo = a.bpart + (slice * nat + at) * kC;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {      // F = dU - X^T (beta dU), dV = beta F
-            f32x4 xs = {0, 0, 0, 0};
+        for (int m = 0; m < 4; ++m) xs[m] = f32x4{0, 0, 0, 0};
+        // F = dU - X^T (beta dU), dV = beta F
+        six(x_cols, [&](int x) { xs[3 - tri_m(x)] = mma(tf[x], f[1 - tri_k(x)], xs[3 - tri_m(x)]); }, [](int) {});
+        f32x4 sb[4];
 #pragma unroll
-            for (int kb = m / 2; kb < 2; ++kb) xs = mma(plane_cols<3>(Xl, 32 * kb, 16 * m), f[kb], xs);
-            du[m] -= xs;
-            f32x4 sb = E[m] * du[m];
+        for (int m = 0; m < 4; ++m) {
+            du[m] -= xs[m];
+            sb[m] = E[m] * du[m];
             du[m] *= vec4(vec + kBe * kC, 16 * m);
             z[m] -= du[m] * tile_read(Vl, LDV, 16 * m, wave * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { sb[e] = row16_sum(sb[e]); z[m][e] = row16_sum(z[m][e]); }
-            if (i16 == 0) {
-                *reinterpret_cast<f32x4a*>(bo + 16 * m + 4 * g) = sb;
-                *reinterpret_cast<f32x4a*>(zo + 16 * m + 4 * g) = z[m];
-            }
-            phase_end();
+            for (int e = 0; e < 4; ++e) { sb[m][e] = row16_sum(sb[m][e]); z[m][e] = row16_sum(z[m][e]); }
         }
         anchor = wave_sum(anchor);
-        if (l == 0) a.apart[slice * nat + at] = anchor;
+        if (i16 == 0) {
+            float* zo = a.zpart + (slice * nat + at) * kC + 4 * g;
+            float* bo = a.bpart + (slice * nat + at) * kC + 4 * g;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                *reinterpret_cast<f32x4a*>(bo + 16 * m) = sb[m];
+                *reinterpret_cast<f32x4a*>(zo + 16 * m) = z[m];
+            }
+            if (g == 0) a.apart[slice * nat + at] = anchor;
+        }
         // dS = dec dS + Q^T (aq dO) - K^T (ak dV)
-        Frag<3> qf[2];
+        Frag<3> of3[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             f[kb] = split<3>(-vec4(vec + kAk * kC, 32 * kb) * du[2 * kb], -vec4(vec + kAk * kC, 32 * kb + 16) * du[2 * kb + 1]);
-            qf[kb] = split<3>(vec4(vec + kAq * kC, 32 * kb) * tile_read(Ol, LDV, 32 * kb, wave * 16),
-                              vec4(vec + kAq * kC, 32 * kb + 16) * tile_read(Ol, LDV, 32 * kb + 16, wave * 16));
+            of3[kb] = split<3>(vec4(vec + kAq * kC, 32 * kb) * tile_read(Ol, LDV, 32 * kb, wave * 16),
+                               vec4(vec + kAq * kC, 32 * kb + 16) * tile_read(Ol, LDV, 32 * kb + 16, wave * 16));
         }
         // dV and E leave through this wave's own columns of the V and dO tiles, which it has read
         lds_order();
@@ -857,21 +967,28 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
             lds_order();
             store_rows(me, LDV, mycols, eo + col0, a.dv, 0, Walk{kC, false});
         } else {
-            state_store(E, eo, kC, a.dv, col);
+            state_store(E, eo, kC, a.dv, col0);
         }
         phase_end();
         if (c > 0) fetch(c - 1);      // here, not earlier: the tiles in flight take 57 registers a lane, which are free only now
         phase_end();
+        Frag<PT> ck[2][2], cq[2][2];
+        col_frags(ck[0], Kl, LDK, 0);
+        col_frags(cq[0], Ql, LDK, 0);
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
+            if (m + 1 < KT) {
+                col_frags(ck[(m + 1) & 1], Kl, LDK, 16 * (m + 1));
+                col_frags(cq[(m + 1) & 1], Ql, LDK, 16 * (m + 1));
+            }
             S[m] *= dec;
+            phase_end();
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                S[m] = mma(col_frag(Ql, LDK, 32 * kb, 16 * m), qf[kb], mma(col_frag(Kl, LDK, 32 * kb, 16 * m), f[kb], S[m]));
+            for (int kb = 0; kb < 2; ++kb) S[m] = mma(cq[m & 1][kb], of3[kb], mma(ck[m & 1][kb], f[kb], S[m]));
             phase_end();
         }
     }
-    if (a.gs0) state_store(S, a.gs0 + state, a.dk, a.dv, col);
+    if (a.gs0) state_store(S, a.gs0 + state, a.dk, a.dv, col0);
     if (vcols > 0) zero_rows(gvp + sg * NW * 16, ots, vcols, w.len, a.T, tid, NT);
 }
 
@@ -899,6 +1016,8 @@ template <int P> __device__ __forceinline__ void plane_write_t(__bf16* t, int r0
     parts4<P>(v, [&](int i, u32x2a h) { *reinterpret_cast<u32x2a*>(p + i * kC * kLdm) = h; });
 }
 
+template <typename T> struct FragOf { using type = Frag<Gd<T>::PT>; };
+
 // Two workgroups a CU (16-bit types): one loads while the other multiplies.
 template <typename T, int DK>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(GdrArgs a) {
@@ -915,7 +1034,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
     const double* G = reinterpret_cast<const double*>(vec + kG64 * kC);
     float* dots = vec + kVec * kC;                                        // [2][4][64]
     const int c = blockIdx.x % a.nc, bk = blockIdx.x / a.nc, b = bk / a.Hk, hk = bk % a.Hk;
-    const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i16 = l & 15;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Walk w = walk_of(a, b, hk * a.r);
     const int64_t kts = (int64_t)a.B * a.Hk * a.dk, gts = (int64_t)a.B * a.H;
     T* gqp = (T*)a.gq + ((int64_t)b * a.Hk + hk) * a.dk;
@@ -940,23 +1059,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
         for (int n = 0; n < NT; ++n) { tq[m][n] = f32x4{0, 0, 0, 0}; tk[m][n] = f32x4{0, 0, 0, 0}; }
     const int64_t ots = (int64_t)a.B * a.H * a.dv, nat = (int64_t)a.B * a.H * a.nc;
     for (int hh = 0; hh < a.r; ++hh) {
+        // the lane's number as the loop's own value: what follows from it (masks, addresses) is then formed where it is used, not kept in
+        // registers, and out of them in scratch memory, across the loop
+        const int l = opaque(tid & 63), g = l >> 4, i16 = l & 15;
         const int h = hk * a.r + hh, bh = b * a.H + h;
         const int64_t at = (int64_t)bh * a.nc + c;
-        // the states' rows of one of this wave's tiles of dk, requested ahead of the barrier: lane = row, 128 columns of dv
-        f32x4 s0r[8], dsr[8];
-        auto state_rows = [&](int n) {
+        // the states' rows of one of this wave's tiles of dk: lane = row, 32 columns of dv from 32 kb on
+        const float* s0 = a.S0 + at * a.dk * a.dv;
+        const float* ds = a.dS + at * a.dk * a.dv;
+        auto state_rows = [&](f32x4 (&v)[4], int n, int kb) {
             const int row = (wave * NT + n) * 16 + i16;
-            const float* s0 = a.S0 + at * a.dk * a.dv;
-            const float* ds = a.dS + at * a.dk * a.dv;
-            const uint32_t off = (uint32_t)(min(row, a.dk - 1) * a.dv);
+            const uint32_t rb = (uint32_t)(min(row, a.dk - 1) * a.dv) * 4u;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                const uint32_t at4 = off + min(16 * x + 4 * g, a.dv - 4);
-                const bool in = row < a.dk && 16 * x + 4 * g < a.dv;
-                const f32x4 u = *reinterpret_cast<const f32x4a*>(s0 + at4), v = *reinterpret_cast<const f32x4a*>(ds + at4);
-                s0r[x] = in ? u : f32x4{0, 0, 0, 0};
-                dsr[x] = in ? v : f32x4{0, 0, 0, 0};
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t off = rb + (uint32_t)min(32 * kb + 16 * x + 4 * g, a.dv - 4) * 4u;
+                v[x] = *reinterpret_cast<const f32x4a*>(reinterpret_cast<const char*>(s0) + off);
+                v[2 + x] = *reinterpret_cast<const f32x4a*>(reinterpret_cast<const char*>(ds) + off);
             }
+        };
+        auto state_cut = [&](f32x4 (&v)[4], int n, int kb) {      // what lies outside is zero
+            if ((wave * NT + n) * 16 + 16 <= a.dk && 32 * kb + 32 <= a.dv) return;
+            const int row = (wave * NT + n) * 16 + i16;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = row < a.dk && 32 * kb + 16 * (x & 1) + 4 * g < a.dv ? v[x] : f32x4{0, 0, 0, 0};
         };
         __syncthreads();
         {
@@ -967,12 +1092,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
             rd.load((const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, p0, w);
             re.load((const ET*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
             for (int i = tid; i < kVec * kC; i += 256) vec[i] = a.vec[at * kVec * kC + i];
-            state_rows(0);
             ro.store(Ol, LDV, a.dv, p0, w.len);
             rd.store(Dl, LDV, a.dv, p0, w.len);
             re.store(El, LDE, a.dv, 0, kC);
             phase_end();
         }
+        f32x4 sr[2][4];
+        state_rows(sr[0], 0, 0);
         __syncthreads();
         // states: wave = a quarter of dk; U = beta E: its factor goes with the rows
 #pragma unroll
@@ -982,17 +1108,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
             for (int m = 0; m < 4; ++m) { cq[m] = f32x4{0, 0, 0, 0}; ck[m] = cq[m]; cd[m] = cq[m]; }
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                if (kb * 32 >= a.dv) break;
-                const Frag<OP> sf = split<OP>(s0r[2 * kb], s0r[2 * kb + 1]), df = split<OP>(dsr[2 * kb], dsr[2 * kb + 1]);
+                if (kb < 3) state_rows(sr[(kb + 1) & 1], n, kb + 1);
+                else if (n + 1 < NT) state_rows(sr[0], n + 1, 0);
+                if (kb * 32 < a.dv) {
+                    state_cut(sr[kb & 1], n, kb);
+                    const Frag<OP> sf = split<OP>(sr[kb & 1][0], sr[kb & 1][1]), df = split<OP>(sr[kb & 1][2], sr[kb & 1][3]);
+                    typename FragOf<T>::type of[4], vf[4];
+                    typename FragOf<ET>::type uf[4];
+                    row_frags(of, Ol, LDV, 32 * kb);
+                    row_frags(vf, Dl, LDV, 32 * kb);
+                    row_frags(uf, El, LDE, 32 * kb);
+                    if (PT == 1) phase_end();
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    cq[m] = mma<PT, OP, OP>(row_frag(Ol, LDV, 16 * m, 32 * kb), sf, cq[m]);
-                    ck[m] = mma<PE, OP, OP>(row_frag(El, LDE, 16 * m, 32 * kb), df, ck[m]);
-                    cd[m] = mma<PT, OP, OP>(row_frag(Dl, LDV, 16 * m, 32 * kb), sf, cd[m]);
+                    for (int m = 0; m < 4; ++m) {
+                        cq[m] = mma<PT, OP, OP>(of[m], sf, cq[m]);
+                        ck[m] = mma<PE, OP, OP>(uf[m], df, ck[m]);
+                        cd[m] = mma<PT, OP, OP>(vf[m], sf, cd[m]);
+                    }
                 }
                 phase_end();
             }
-            if (n + 1 < NT) state_rows(n + 1);
             phase_end();
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
@@ -1008,12 +1143,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
         for (int m = 0; m < 4; ++m) { dp[m] = f32x4{0, 0, 0, 0}; dn[m] = dp[m]; }
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-            if (kb * 32 >= a.dv) break;
-            const auto uf = row_frag(El, LDE, 16 * wave, 32 * kb);
+            if (kb * 32 < a.dv) {
+                const auto uf = row_frag(El, LDE, 16 * wave, 32 * kb);
+                typename FragOf<T>::type of[4], vf[4];
+                row_frags(of, Ol, LDV, 32 * kb);
+                row_frags(vf, Dl, LDV, 32 * kb);
+                if (PT == 1) phase_end();
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                dp[m] = mma<PT, PE, OP>(row_frag(Ol, LDV, 16 * m, 32 * kb), uf, dp[m]);
-                dn[m] = mma<PT, PE, OP>(row_frag(Dl, LDV, 16 * m, 32 * kb), uf, dn[m]);
+                for (int m = 0; m < 4; ++m) {
+                    dp[m] = mma<PT, PE, OP>(of[m], uf, dp[m]);
+                    dn[m] = mma<PT, PE, OP>(vf[m], uf, dn[m]);
+                }
             }
             phase_end();
         }
@@ -1106,6 +1246,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
                 phase_end();
             }
     }
+    const int l = tid & 63, g = l >> 4, i16 = l & 15;
     // through the normalisation: dq = tq - q |q|^-2 (q . tq)  (|.|^2 with its epsilon), dk alike
     if (a.norm) {
 #pragma unroll
