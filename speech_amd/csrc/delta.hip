@@ -607,7 +607,8 @@ template <int P> __device__ __forceinline__ void row_operands(Frag<P> (&f)[2], c
 }
 
 // A wave owns 16 columns of dv: the state's columns, U's, O's.  Only K, Q, X, P and the vectors are shared (LDS, filled a chunk ahead
-// through registers); two barriers a chunk.
+// through registers); two barriers a chunk.  A wave whose columns lie behind dv works on zeros
+// and writes nothing.
 template <typename T, int DK, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -665,7 +666,6 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
         for (int i = 0; i < kVec * kC / NT; ++i) vec[i * NT + tid] = rvec[i];
         __syncthreads();
         if (c + 1 < ncl) fetch(c + 1);
-        if (mycols <= 0) continue;
         if (TRAIN) state_store(S, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col0);      // for the backward
         f32x4 ks[4], qs[4];
 #pragma unroll
@@ -822,10 +822,6 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 #pragma unroll
         for (int m = 0; m < KT; ++m) s0[m] = s0n[m];
         __syncthreads();
-        if (mycols <= 0) {
-            if (c > 0) fetch(c - 1);
-            continue;
-        }
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
         float anchor = 0.f;
         {   // dS at the chunk's end is what the gradient kernel needs; <dS, S_C> = dec <dS, S0> + sum_j dU2_j . U_j
@@ -934,7 +930,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
             for (int e = 0; e < 4; ++e) { sb[m][e] = row16_sum(sb[m][e]); z[m][e] = row16_sum(z[m][e]); }
         }
         anchor = wave_sum(anchor);
-        if (i16 == 0) {
+        if (i16 == 0 && mycols > 0) {
             float* zo = a.zpart + (slice * nat + at) * kC + 4 * g;
             float* bo = a.bpart + (slice * nat + at) * kC + 4 * g;
 #pragma unroll
