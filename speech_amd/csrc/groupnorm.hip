@@ -32,6 +32,10 @@ template <typename T, int VW> __device__ __forceinline__ void gn_ld(const T* p, 
 #pragma unroll
     for (int i = 0; i < VW; ++i) f[i] = Elem<T>::f(r.e[i]);
 }
+template <typename T, int VW> __device__ __forceinline__ void gn_get(const GnRaw<T, VW>& r, float (&f)[VW]) {
+#pragma unroll
+    for (int i = 0; i < VW; ++i) f[i] = Elem<T>::f(r.e[i]);
+}
 template <typename T, int VW> __device__ __forceinline__ void gn_st(T* p, const float (&f)[VW]) {
     GnRaw<T, VW> r;
 #pragma unroll
@@ -53,15 +57,42 @@ __device__ __forceinline__ float gn_act_grad(float v, int act) {
     return 1.f;
 }
 
-// Positions [lo, hi) of a sample walked by rows of threads: (f, t) advance without a division per step.
+// Positions [lo, hi) of a sample walked by rows of threads, kU positions at a time: their loads are all in flight before the first is used
+// (one position at a time moved 2.3-2.8 TB/s on the 61 MB tensors of the conv stack).  Offsets advance by additions; a tensor whose frames
+// follow each other through the bands (the usual layout) needs no correction at a band's end.
+constexpr int kU = 4, kUb = 2;      // forward; backward (three tensors and the channel sums in registers)
 struct GnWalk {
-    int f, t, df, dt;
-    __device__ __forceinline__ GnWalk(int p, int step, int T) : f(p / T), t(p % T), df(step / T), dt(step % T) {}
-    __device__ __forceinline__ void next(int T) {
-        f += df; t += dt;
-        if (t >= T) { t -= T; ++f; }
-    }
+    int p, hi, step, t, dt, T;
+    __device__ __forceinline__ GnWalk(int p_, int hi_, int step_, int T_) : p(p_), hi(hi_), step(step_), t(p_ % T_), dt(step_ % T_), T(T_) {}
+    __device__ __forceinline__ bool more() const { return p < hi; }
+    __device__ __forceinline__ bool all(int n) const { return p + (n - 1) * step < hi; }
 };
+struct GnPos {          // offsets of one tensor along a walk
+    int64_t off, inc, wrap, first;
+    __device__ __forceinline__ GnPos(GnStr s, int n, const GnWalk& w)
+        : off(n * s.n + (int64_t)(w.p / w.T) * s.f + (int64_t)w.t * s.t), inc((int64_t)(w.step / w.T) * s.f + (int64_t)w.dt * s.t), wrap(s.f - (int64_t)w.T * s.t), first(off) {}
+    // a position outside (behind the walk's end or the utterance's) is loaded from the walk's first position instead, and not used
+    __device__ __forceinline__ int64_t at(bool in) const { return in ? off : first; }
+    __device__ __forceinline__ void next(bool wrapped) { off += inc + (wrapped ? wrap : 0); }
+};
+
+template <typename... P> __device__ __forceinline__ void gn_next(GnWalk& w, P&... pos) {
+    w.p += w.step;
+    w.t += w.dt;
+    const bool wrapped = w.t >= w.T;
+    if (wrapped) w.t -= w.T;
+    (pos.next(wrapped), ...);
+}
+
+// For groups g0 .. g1: sums of part(g, lane, width) over the lanes of a wave, handed to done(g, sum) in one lane.  Waves take the groups in
+// turn: with one thread a group, the walk over 64 partial results alone took 30 us (each load waited for the one before).
+template <typename A, typename B> __device__ __forceinline__ void gn_group_sums(int g0, int g1, A&& part, B&& done) {
+    const int lane = threadIdx.x & 63;
+    for (int g = g0 + (int)(threadIdx.x >> 6); g <= g1; g += kGnThreads / 64) {
+        const float v = wave_sum(part(g, lane, 64));
+        if (lane == 0) done(g, v);
+    }
+}
 
 // ---- block route --------------------------------------------------------------------------------------
 // thread = (row, chunk of VW channels); a chunk lies inside a group or holds whole groups
@@ -84,19 +115,31 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
 #pragma unroll
         for (int i = 0; i < VW; ++i) { k[i] = 0.f; sm[i] = 0.f; sq[i] = 0.f; }
         if (on) {
-            const T* base = x + n * xs.n + chunk * VW;
-            GnWalk w(lo + row, rows, s.T);
-            for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
-                if (w.t >= len) continue;
-                float v[VW];
-                gn_ld<T, VW>(base + w.f * xs.f + w.t * xs.t, v);
-                if (cnt == 0) {
+            const T* base = x + chunk * VW;
+            GnWalk w(lo + row, hi, rows, s.T);
+            GnPos px(xs, n, w);
+            while (w.more()) {
+                GnRaw<T, VW> raw[kU];
+                bool on[kU];
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) k[i] = v[i];
+                for (int u = 0; u < kU; ++u) {
+                    on[u] = w.more() && w.t < len;
+                    raw[u] = *reinterpret_cast<const GnRaw<T, VW>*>(base + px.at(on[u]));
+                    gn_next(w, px);
                 }
-                ++cnt;
 #pragma unroll
-                for (int i = 0; i < VW; ++i) { const float d = v[i] - k[i]; sm[i] += d; sq[i] += d * d; }
+                for (int u = 0; u < kU; ++u) {
+                    if (!on[u]) continue;
+                    float v[VW];
+                    gn_get<T, VW>(raw[u], v);
+                    if (cnt == 0) {
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) k[i] = v[i];
+                    }
+                    ++cnt;
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) { const float d = v[i] - k[i]; sm[i] += d; sq[i] += d * d; }
+                }
             }
         }
         const float inv = cnt ? 1.f / (float)cnt : 0.f;
@@ -137,12 +180,12 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
         const int c0 = cb * VW, c1 = min(s.C, c0 + cpb * VW);
         const int g0 = c0 / s.Cg, g1 = (c1 - 1) / s.Cg;
         const float winv = c_all > 0.f ? 1.f / c_all : 0.f;
-        for (int g = g0 + threadIdx.x; g <= g1; g += kGnThreads) {
+        gn_group_sums(g0, g1, [&](int g, int lane, int width) {
             const int a = max(c0, g * s.Cg), b = min(c1, (g + 1) * s.Cg);
             float m = 0.f;
-            for (int c = a; c < b; ++c) m += red[c - c0];
-            gmean[g - g0] = m * winv / (float)(b - a);
-        }
+            for (int c = a + lane; c < b; c += width) m += red[c - c0];
+            return m;
+        }, [&](int g, float m) { gmean[g - g0] = m * winv / (float)(min(c1, (g + 1) * s.Cg) - max(c0, g * s.Cg)); });
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
@@ -151,16 +194,17 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
             red[threadIdx.x * VW + i] = on && cnt ? sq[i] + (float)cnt * d * d : 0.f;
         }
         tree();
-        for (int g = g0 + threadIdx.x; g <= g1; g += kGnThreads) {
+        gn_group_sums(g0, g1, [&](int g, int lane, int width) {
             const int a = max(c0, g * s.Cg), b = min(c1, (g + 1) * s.Cg);
             float m2 = 0.f;
-            for (int c = a; c < b; ++c) m2 += red[c - c0];
+            for (int c = a + lane; c < b; c += width) m2 += red[c - c0];
+            return m2;
+        }, [&](int g, float m2) {
             // slot: one per (sample, split, pass-part of the group)
-            const int sub = cb / cpb;
-            const int nsub = (nch + cpb - 1) / cpb;
+            const int sub = cb / cpb, nsub = (nch + cpb - 1) / cpb;
             float* o = part + (((int64_t)n * nsplit + split) * nsub + sub) * s.G * 3 + g * 3;
-            o[0] = c_all * (float)(b - a); o[1] = gmean[g - g0]; o[2] = m2;
-        }
+            o[0] = c_all * (float)(min(c1, (g + 1) * s.Cg) - max(c0, g * s.Cg)); o[1] = gmean[g - g0]; o[2] = m2;
+        });
         if (nch > cpb) {   // groups that this pass does not touch hold no weight
             const int sub = cb / cpb, nsub = (nch + cpb - 1) / cpb;
             for (int g = threadIdx.x; g < s.G; g += kGnThreads)
@@ -170,28 +214,36 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
     }
 }
 
-// mean and rstd of every group of sample n from the splits' triples, into LDS
+// mean and rstd of every group of sample n from the splits' triples, into LDS: a wave a group, a lane a part
 __device__ __forceinline__ void gn_merge(const float* __restrict__ part, int n, int nparts, int G, float eps, float* mean, float* rstd) {
-    for (int g = threadIdx.x; g < G; g += kGnThreads) {
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < G; g += kGnThreads / 64) {
         const float* p = part + (int64_t)n * nparts * G * 3 + g * 3;
-        float w = 0.f, m = 0.f, m2 = 0.f;
-        for (int i = 0; i < nparts; ++i) {
-            const float wi = p[(int64_t)i * G * 3];
-            if (wi > 0.f) { w += wi; m += wi * p[(int64_t)i * G * 3 + 1]; }
+        float w = 0.f, m = 0.f;
+        for (int i = lane; i < nparts; i += 64) {
+            const float wi = p[(int64_t)i * G * 3], mi = p[(int64_t)i * G * 3 + 1];
+            w += wi;
+            m += wi > 0.f ? wi * mi : 0.f;
         }
+        w = wave_sum(w);
+        m = wave_sum(m);
         const float inv = w > 0.f ? 1.f / w : 0.f;
         m *= inv;
-        for (int i = 0; i < nparts; ++i) {
-            const float wi = p[(int64_t)i * G * 3];
-            if (wi > 0.f) { const float d = p[(int64_t)i * G * 3 + 1] - m; m2 += p[(int64_t)i * G * 3 + 2] + wi * d * d; }
+        float m2 = 0.f;
+        for (int i = lane; i < nparts; i += 64) {
+            const float wi = p[(int64_t)i * G * 3], d = p[(int64_t)i * G * 3 + 1] - m, qi = p[(int64_t)i * G * 3 + 2];
+            m2 += wi > 0.f ? qi + wi * d * d : 0.f;
         }
-        mean[g] = m;
-        rstd[g] = rsqrtf(m2 * inv + eps);
+        m2 = wave_sum(m2);
+        if (lane == 0) {
+            mean[g] = m;
+            rstd[g] = rsqrtf(m2 * inv + eps);
+        }
     }
     __syncthreads();
 }
 
-template <typename T, int VW>
+template <typename T, int VW, bool RES>
 __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(const T* __restrict__ x, GnStr xs, const T* __restrict__ res, GnStr rs,
                                                               const float* __restrict__ gamma, const float* __restrict__ beta, GnShape s,
                                                               float eps, const float* __restrict__ part, int nsplit, int nparts, T* __restrict__ y,
@@ -216,33 +268,43 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(const T* __restric
             a[i] = rstd[c / s.Cg] * gamma[c];
             b[i] = beta[c];
         }
-        GnWalk w(lo + row, rows, s.T);
-        for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
-            float o[VW];
-            if (w.t < len) {
-                float v[VW];
-                gn_ld<T, VW>(x + n * xs.n + w.f * xs.f + w.t * xs.t + chunk * VW, v);
+        GnWalk w(lo + row, hi, rows, s.T);
+        GnPos px(xs, n, w), pr(rs, n, w), py(ys, n, w);
+        while (w.more()) {
+            GnRaw<T, VW> rx[kU], rr[kU];
+            int64_t at[kU];
+            bool on[kU], in[kU];
 #pragma unroll
-                for (int i = 0; i < VW; ++i) o[i] = (v[i] - mu[i]) * a[i] + b[i];
-                if (res) {
-                    gn_ld<T, VW>(res + n * rs.n + w.f * rs.f + w.t * rs.t + chunk * VW, v);
+            for (int u = 0; u < kU; ++u) {
+                on[u] = w.more();
+                in[u] = on[u] && w.t < len;
+                at[u] = py.off;
+                rx[u] = *reinterpret_cast<const GnRaw<T, VW>*>(x + px.at(in[u]) + chunk * VW);
+                if (RES) rr[u] = *reinterpret_cast<const GnRaw<T, VW>*>(res + pr.at(in[u]) + chunk * VW);
+                gn_next(w, px, pr, py);
+            }
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) o[i] += v[i];
-                }
-#pragma unroll
-                for (int i = 0; i < VW; ++i) o[i] = gn_act(o[i], s.act);
-            } else {
+            for (int u = 0; u < kU; ++u) {
+                if (!on[u]) continue;
+                float o[VW];
 #pragma unroll
                 for (int i = 0; i < VW; ++i) o[i] = 0.f;
+                if (in[u]) {
+                    float v[VW], z[VW];
+                    gn_get<T, VW>(rx[u], v);
+                    if (RES) gn_get<T, VW>(rr[u], z);
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) o[i] = gn_act((v[i] - mu[i]) * a[i] + b[i] + (RES ? z[i] : 0.f), s.act);
+                }
+                gn_st<T, VW>(y + at[u] + chunk * VW, o);
             }
-            gn_st<T, VW>(y + n * ys.n + w.f * ys.f + w.t * ys.t + chunk * VW, o);
         }
     }
 }
 
 // Backward, first pass: g = gy * act'(pre) (written as the residual's gradient), per (sample, split): channel sums of g and of g * xhat,
 // and the same weighted with gamma per group.
-template <typename T, int VW>
+template <typename T, int VW, bool RES>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __restrict__ gy, GnStr gs, const T* __restrict__ x, GnStr xs,
                                                                   const T* __restrict__ res, GnStr rs, const float* __restrict__ gamma,
                                                                   const float* __restrict__ beta, const float* __restrict__ mean,
@@ -272,25 +334,43 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __res
                 gm[i] = gamma[c];
                 bt[i] = beta[c];
             }
-            GnWalk w(lo + row, rows, s.T);
-            for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
-                float g[VW], v[VW], z[VW];
-                if (w.t < len) {
-                    gn_ld<T, VW>(gy + n * gs.n + w.f * gs.f + w.t * gs.t + chunk * VW, g);
-                    gn_ld<T, VW>(x + n * xs.n + w.f * xs.f + w.t * xs.t + chunk * VW, v);
-                    if (res) gn_ld<T, VW>(res + n * rs.n + w.f * rs.f + w.t * rs.t + chunk * VW, z);
+            GnWalk w(lo + row, hi, rows, s.T);
+            GnPos pg(gs, n, w), px(xs, n, w), pr(rs, n, w), po(grs, n, w);
+            while (w.more()) {
+                GnRaw<T, VW> rg[kUb], rx[kUb], rr[kUb];
+                int64_t at[kUb];
+                bool on[kUb], in[kUb];
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) {
-                        const float xh = (v[i] - mu[i]) * r[i];
-                        if (s.act != SP_ACT_NONE) g[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (res ? z[i] : 0.f), s.act);
-                        sb[i] += g[i];
-                        sx[i] += g[i] * xh;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) g[i] = 0.f;
+                for (int u = 0; u < kUb; ++u) {
+                    on[u] = w.more();
+                    in[u] = on[u] && w.t < len;
+                    at[u] = po.off;
+                    rg[u] = *reinterpret_cast<const GnRaw<T, VW>*>(gy + pg.at(in[u]) + chunk * VW);
+                    rx[u] = *reinterpret_cast<const GnRaw<T, VW>*>(x + px.at(in[u]) + chunk * VW);
+                    if (RES) rr[u] = *reinterpret_cast<const GnRaw<T, VW>*>(res + pr.at(in[u]) + chunk * VW);
+                    gn_next(w, pg, px, pr, po);
                 }
-                if (gres) gn_st<T, VW>(gres + n * grs.n + w.f * grs.f + w.t * grs.t + chunk * VW, g);
+#pragma unroll
+                for (int u = 0; u < kUb; ++u) {
+                    if (!on[u]) continue;
+                    float q[VW];
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) q[i] = 0.f;
+                    if (in[u]) {
+                        float v[VW], z[VW];
+                        gn_get<T, VW>(rg[u], q);
+                        gn_get<T, VW>(rx[u], v);
+                        if (RES) gn_get<T, VW>(rr[u], z);
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) {
+                            const float xh = (v[i] - mu[i]) * r[i];
+                            if (s.act != SP_ACT_NONE) q[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (RES ? z[i] : 0.f), s.act);
+                            sb[i] += q[i];
+                            sx[i] += q[i] * xh;
+                        }
+                    }
+                    if (gres) gn_st<T, VW>(gres + at[u] + chunk * VW, q);
+                }
             }
         }
         __syncthreads();
@@ -316,12 +396,14 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __res
         }
     }
     __syncthreads();   // this workgroup's own global writes are visible to it behind the barrier
-    for (int g = threadIdx.x; g < s.G; g += kGnThreads) {
-        float a = 0.f, b = 0.f;
-        for (int c = g * s.Cg; c < (g + 1) * s.Cg; ++c) { a += gamma[c] * cp[c * 2]; b += gamma[c] * cp[c * 2 + 1]; }
-        float* o = gpart + (((int64_t)n * nsplit + split) * s.G + g) * 2;
-        o[0] = a; o[1] = b;
-    }
+    float* go = gpart + ((int64_t)n * nsplit + split) * s.G * 2;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        gn_group_sums(0, s.G - 1, [&](int g, int lane, int width) {
+            float a = 0.f;
+            for (int c = g * s.Cg + lane; c < (g + 1) * s.Cg; c += width) a += gamma[c] * cp[c * 2 + q];
+            return a;
+        }, [&](int g, float a) { go[g * 2 + q] = a; });
 }
 
 // out[c] (+)= sum over parts of part[r][c][0 / 1]; a workgroup takes 32 channels, eight rows of threads walk the parts
@@ -348,7 +430,7 @@ __device__ __forceinline__ void gn_param_reduce(const float* __restrict__ cpart,
 // Backward, second pass: gx = rstd * (gamma g - mean(gamma g) - xhat mean(gamma g xhat)); the workgroups behind the N * nsplit that do so
 // add up the parameter gradients instead, 32 channels each.  g is formed again from gy, x and the residual: reading the written gres back
 // would save a read in three but carry its 16-bit rounding into gx.
-template <typename T, int VW>
+template <typename T, int VW, bool RES>
 __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(const T* __restrict__ gy, GnStr gs, const T* __restrict__ x, GnStr xs,
                                                                   const T* __restrict__ res, GnStr rs, const float* __restrict__ gamma,
                                                                   const float* __restrict__ beta, const float* __restrict__ mean,
@@ -363,14 +445,13 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(const T* __res
     }
     const int len = s.lengths ? min(max(s.lengths[n], 0), s.T) : s.T;
     const float cinv = len > 0 ? 1.f / ((float)len * (float)s.F * (float)s.Cg) : 0.f;
-    for (int g = threadIdx.x; g < s.G; g += kGnThreads) {
-        float a = 0.f, b = 0.f;
-        for (int i = 0; i < nsplit; ++i) {
-            const float* p = gpart + (((int64_t)n * nsplit + i) * s.G + g) * 2;
-            a += p[0]; b += p[1];
-        }
-        c1[g] = a * cinv; c2[g] = b * cinv;
-    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        gn_group_sums(0, s.G - 1, [&](int g, int lane, int width) {
+            float a = 0.f;
+            for (int i = lane; i < nsplit; i += width) a += gpart[(((int64_t)n * nsplit + i) * s.G + g) * 2 + q];
+            return a;
+        }, [&](int g, float a) { (q ? c2 : c1)[g] = a * cinv; });
     __syncthreads();
     const int P = s.F * s.T, nch = s.C / VW;
     const int cpb = min(nch, kGnThreads), rows = kGnThreads / cpb, row = threadIdx.x / cpb;
@@ -389,25 +470,42 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(const T* __res
             k1[i] = c1[g];
             k2[i] = c2[g];
         }
-        GnWalk w(lo + row, rows, s.T);
-        for (int p = lo + row; p < hi; p += rows, w.next(s.T)) {
-            float o[VW];
-            if (w.t < len) {
-                float g[VW], v[VW], z[VW];
-                gn_ld<T, VW>(gy + n * gs.n + w.f * gs.f + w.t * gs.t + chunk * VW, g);
-                gn_ld<T, VW>(x + n * xs.n + w.f * xs.f + w.t * xs.t + chunk * VW, v);
-                if (res) gn_ld<T, VW>(res + n * rs.n + w.f * rs.f + w.t * rs.t + chunk * VW, z);
+        GnWalk w(lo + row, hi, rows, s.T);
+        GnPos pg(gs, n, w), px(xs, n, w), pr(rs, n, w), po(gxs, n, w);
+        while (w.more()) {
+            GnRaw<T, VW> rg[kUb], rx[kUb], rr[kUb];
+            int64_t at[kUb];
+            bool on[kUb], in[kUb];
 #pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    const float xh = (v[i] - mu[i]) * r[i];
-                    if (s.act != SP_ACT_NONE) g[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (res ? z[i] : 0.f), s.act);
-                    o[i] = r[i] * (gm[i] * g[i] - k1[i] - xh * k2[i]);
-                }
-            } else {
+            for (int u = 0; u < kUb; ++u) {
+                on[u] = w.more();
+                in[u] = on[u] && w.t < len;
+                at[u] = po.off;
+                rg[u] = *reinterpret_cast<const GnRaw<T, VW>*>(gy + pg.at(in[u]) + chunk * VW);
+                rx[u] = *reinterpret_cast<const GnRaw<T, VW>*>(x + px.at(in[u]) + chunk * VW);
+                if (RES) rr[u] = *reinterpret_cast<const GnRaw<T, VW>*>(res + pr.at(in[u]) + chunk * VW);
+                gn_next(w, pg, px, pr, po);
+            }
+#pragma unroll
+            for (int u = 0; u < kUb; ++u) {
+                if (!on[u]) continue;
+                float o[VW];
 #pragma unroll
                 for (int i = 0; i < VW; ++i) o[i] = 0.f;
+                if (in[u]) {
+                    float q[VW], v[VW], z[VW];
+                    gn_get<T, VW>(rg[u], q);
+                    gn_get<T, VW>(rx[u], v);
+                    if (RES) gn_get<T, VW>(rr[u], z);
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) {
+                        const float xh = (v[i] - mu[i]) * r[i];
+                        if (s.act != SP_ACT_NONE) q[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (RES ? z[i] : 0.f), s.act);
+                        o[i] = r[i] * (gm[i] * q[i] - k1[i] - xh * k2[i]);
+                    }
+                }
+                gn_st<T, VW>(gx + at[u] + chunk * VW, o);
             }
-            gn_st<T, VW>(gx + n * gxs.n + w.f * gxs.f + w.t * gxs.t + chunk * VW, o);
         }
     }
 }
@@ -684,7 +782,7 @@ extern "C" int sp_groupnorm_fwd(const void* x, const void* residual, const float
     SP_GN_TYPES(dtype, SP_GN_VW(p.vw, {
         hipLaunchKernelGGL((gn_stats_kernel<T_, VW_>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)x, xs, s, p.splits,
                            (float*)workspace);
-        hipLaunchKernelGGL((gn_apply_kernel<T_, VW_>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)x, xs,
+        hipLaunchKernelGGL((residual ? gn_apply_kernel<T_, VW_, true> : gn_apply_kernel<T_, VW_, false>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)x, xs,
                            (const T_*)residual, rs, gamma, beta, s, eps, (const float*)workspace, p.splits, p.splits * p.nsub, (T_*)y, ys, mean, rstd); }))
     return check_launch("gn_apply_kernel");
 }
@@ -721,9 +819,9 @@ extern "C" int sp_groupnorm_bwd(const void* gy, const void* x, const void* resid
     }
     float* gpart = (float*)((char*)workspace + align_up((size_t)N * p.splits * C * 2 * sizeof(float), 256));
     SP_GN_TYPES(dtype, SP_GN_VW(p.vw, {
-        hipLaunchKernelGGL((gn_bwd_stats_kernel<T_, VW_>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)gy, gs, (const T_*)x,
+        hipLaunchKernelGGL((residual ? gn_bwd_stats_kernel<T_, VW_, true> : gn_bwd_stats_kernel<T_, VW_, false>), dim3((unsigned)N * p.splits), dim3(kGnThreads), 0, st, (const T_*)gy, gs, (const T_*)x,
                            xs, (const T_*)residual, rs, gamma, beta, mean, rstd, s, p.splits, (T_*)gres, grs, cpart, gpart);
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T_, VW_>), dim3((unsigned)N * p.splits + (C + 31) / 32), dim3(kGnThreads), 0, st,
+        hipLaunchKernelGGL((residual ? gn_bwd_apply_kernel<T_, VW_, true> : gn_bwd_apply_kernel<T_, VW_, false>), dim3((unsigned)N * p.splits + (C + 31) / 32), dim3(kGnThreads), 0, st,
                            (const T_*)gy, gs, (const T_*)x, xs, (const T_*)residual, rs, gamma, beta, mean, rstd, s, cpart, gpart, p.splits, accumulate, (T_*)gx, gxs, dgamma, dbeta); }))
     return check_launch("gn_bwd_apply_kernel");
 }
