@@ -120,6 +120,37 @@ def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+class _Here:
+    """Stands in for torch.cuda.device(d) where d is current already: entering that costs more than a small kernel's launch."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(t):
+    """Context in which t's device is the current one."""
+    import torch
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def raw_stream(t):
+    """The current stream of t's device as the integer the C ABI takes (inside on_device(t))."""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # what torch's own generated code uses: 0.1 us against 2.6
+    return get(t.get_device()) if get is not None else torch.cuda.current_stream(t.device).cuda_stream
+
+
+def addr(t):
+    """A tensor's address as the integer the C ABI takes, None for none."""
+    return None if t is None else t.data_ptr()
+
+
 def ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else None
 
@@ -127,3 +158,4 @@ def ptr(t):
 def dtype_code(t):
     import torch
     return {torch.float32: SP_F32, torch.float16: SP_F16, torch.bfloat16: SP_BF16}[t.dtype]
+

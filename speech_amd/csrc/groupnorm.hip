@@ -43,24 +43,34 @@ template <typename T, int VW> __device__ __forceinline__ void gn_st(T* p, const 
     *reinterpret_cast<GnRaw<T, VW>*>(p) = r;
 }
 
-__device__ __forceinline__ float gn_act(float v, int act) {
-    if (act == SP_ACT_RELU) return v <= 0.f ? 0.f : v;   // NaN stays NaN
-    if (act == SP_ACT_SILU) return v / (1.f + __expf(-v));
-    return v;
-}
-__device__ __forceinline__ float gn_act_grad(float v, int act) {
-    if (act == SP_ACT_RELU) return v > 0.f ? 1.f : 0.f;
-    if (act == SP_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-v));
-        return s * (1.f + v * (1.f - s));
+// v_rcp_f32 is good to one unit in the last place; the exact division costs ten instructions an element
+template <int VW> __device__ __forceinline__ void gn_act(float (&v)[VW], int act) {
+    if (act == SP_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] = v[i] <= 0.f ? 0.f : v[i];   // NaN stays NaN
+    } else if (act == SP_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] *= __builtin_amdgcn_rcpf(1.f + __expf(-v[i]));
     }
-    return 1.f;
+}
+// g *= act'(pre)
+template <int VW> __device__ __forceinline__ void gn_act_grad(float (&g)[VW], const float (&pre)[VW], int act) {
+    if (act == SP_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) g[i] = pre[i] > 0.f ? g[i] : 0.f;
+    } else if (act == SP_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-pre[i]));
+            g[i] *= s * (1.f + pre[i] * (1.f - s));
+        }
+    }
 }
 
 // Positions [lo, hi) of a sample walked by rows of threads, kU positions at a time: their loads are all in flight before the first is used
 // (one position at a time moved 2.3-2.8 TB/s on the 61 MB tensors of the conv stack).  Offsets advance by additions; a tensor whose frames
 // follow each other through the bands (the usual layout) needs no correction at a band's end.
-constexpr int kU = 4, kUb = 2;      // forward; backward (three tensors and the channel sums in registers)
+constexpr int kU = 4, kUb = 1;      // forward; backward (three tensors and the channel sums in registers)
 struct GnWalk {
     int p, hi, step, t, dt, T;
     __device__ __forceinline__ GnWalk(int p_, int hi_, int step_, int T_) : p(p_), hi(hi_), step(step_), t(p_ % T_), dt(step_ % T_), T(T_) {}
@@ -294,7 +304,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(const T* __restric
                     gn_get<T, VW>(rx[u], v);
                     if (RES) gn_get<T, VW>(rr[u], z);
 #pragma unroll
-                    for (int i = 0; i < VW; ++i) o[i] = gn_act((v[i] - mu[i]) * a[i] + b[i] + (RES ? z[i] : 0.f), s.act);
+                    for (int i = 0; i < VW; ++i) o[i] = (v[i] - mu[i]) * a[i] + b[i] + (RES ? z[i] : 0.f);
+                    gn_act<VW>(o, s.act);
                 }
                 gn_st<T, VW>(y + at[u] + chunk * VW, o);
             }
@@ -363,10 +374,14 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __res
                         if (RES) gn_get<T, VW>(rr[u], z);
 #pragma unroll
                         for (int i = 0; i < VW; ++i) {
-                            const float xh = (v[i] - mu[i]) * r[i];
-                            if (s.act != SP_ACT_NONE) q[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (RES ? z[i] : 0.f), s.act);
+                            v[i] = (v[i] - mu[i]) * r[i];
+                            z[i] = v[i] * gm[i] + bt[i] + (RES ? z[i] : 0.f);
+                        }
+                        gn_act_grad<VW>(q, z, s.act);
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) {
                             sb[i] += q[i];
-                            sx[i] += q[i] * xh;
+                            sx[i] += q[i] * v[i];
                         }
                     }
                     if (gres) gn_st<T, VW>(gres + at[u] + chunk * VW, q);
@@ -406,22 +421,21 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __res
         }, [&](int g, float a) { go[g * 2 + q] = a; });
 }
 
-// out[c] (+)= sum over parts of part[r][c][0 / 1]; a workgroup takes 32 channels, eight rows of threads walk the parts
+// out[c] (+)= sum over parts of part[r][c][0 / 1]; a workgroup takes 32 channels, its rows of 32 threads walk the parts
 __device__ __forceinline__ void gn_param_reduce(const float* __restrict__ cpart, int64_t nrows, int C, int c0, int accumulate,
                                                 float* __restrict__ dgamma, float* __restrict__ dbeta) {
-    __shared__ float red[8][32][2];
-    const int c = c0 + (threadIdx.x & 31), r0 = threadIdx.x >> 5;
+    __shared__ float red[32][32][2];
+    const int c = c0 + (threadIdx.x & 31), r0 = threadIdx.x >> 5, nr = blockDim.x >> 5;
     float a = 0.f, b = 0.f;
     if (c < C) {
 #pragma unroll 4
-        for (int64_t r = r0; r < nrows; r += 8) { a += cpart[(r * C + c) * 2]; b += cpart[(r * C + c) * 2 + 1]; }
+        for (int64_t r = r0; r < nrows; r += nr) { a += cpart[(r * C + c) * 2]; b += cpart[(r * C + c) * 2 + 1]; }
     }
     red[r0][threadIdx.x & 31][0] = a;
     red[r0][threadIdx.x & 31][1] = b;
     __syncthreads();
     if (r0 == 0 && c < C) {
-#pragma unroll
-        for (int i = 1; i < 8; ++i) { a += red[i][threadIdx.x][0]; b += red[i][threadIdx.x][1]; }
+        for (int i = 1; i < nr; ++i) { a += red[i][threadIdx.x][0]; b += red[i][threadIdx.x][1]; }
         dbeta[c] = accumulate ? dbeta[c] + a : a;
         dgamma[c] = accumulate ? dgamma[c] + b : b;
     }
@@ -499,10 +513,12 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(const T* __res
                     if (RES) gn_get<T, VW>(rr[u], z);
 #pragma unroll
                     for (int i = 0; i < VW; ++i) {
-                        const float xh = (v[i] - mu[i]) * r[i];
-                        if (s.act != SP_ACT_NONE) q[i] *= gn_act_grad((v[i] - mu[i]) * (r[i] * gm[i]) + bt[i] + (RES ? z[i] : 0.f), s.act);
-                        o[i] = r[i] * (gm[i] * q[i] - k1[i] - xh * k2[i]);
+                        v[i] = (v[i] - mu[i]) * r[i];
+                        z[i] = v[i] * gm[i] + bt[i] + (RES ? z[i] : 0.f);
                     }
+                    gn_act_grad<VW>(q, z, s.act);
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) o[i] = r[i] * (gm[i] * q[i] - k1[i] - v[i] * k2[i]);
                 }
                 gn_st<T, VW>(gx + at[u] + chunk * VW, o);
             }
@@ -511,30 +527,68 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(const T* __res
 }
 
 // ---- rows route ---------------------------------------------------------------------------------------
+// sum over `team` neighbouring lanes (a power of two), in all of them; rows of 16 lanes rotate in the vector ALU, no LDS involved
+__device__ __forceinline__ float gn_team_sum(float v, int team) {
+    if (team >= 16) {
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, false));
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x124, 0xf, 0xf, false));
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x122, 0xf, 0xf, false));
+        v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x121, 0xf, 0xf, false));
+        if (team >= 32) v += __shfl_xor(v, 16);
+        if (team == 64) v += __shfl_xor(v, 32);
+        return v;
+    }
+    for (int o = team >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
 // Unit u = (sample u / G, group u % G): Cg contiguous channels held by `team` lanes (a power of two), NCH chunks of VW each.
-template <typename T, int VW, int NCH>
+template <typename T, int VW, int NCH, bool RES>
 __global__ __launch_bounds__(kGnThreads) void gn_rows_fwd_kernel(const T* __restrict__ x, int64_t xsn, const T* __restrict__ res, int64_t rsn,
                                                                  const float* __restrict__ gamma, const float* __restrict__ beta, GnShape s,
                                                                  float eps, int team, T* __restrict__ y, int64_t ysn,
                                                                  float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    const int64_t units = (int64_t)s.N * s.G;
     const int upb = kGnThreads / team, lane = threadIdx.x & (team - 1);
     const float inv = 1.f / (float)s.Cg;
-    for (int64_t u = (int64_t)blockIdx.x * upb + threadIdx.x / team; u < units; u += (int64_t)gridDim.x * upb) {
-        const int64_t n = u / s.G;
-        const int g = (int)(u - n * s.G), c0 = g * s.Cg;
+    const uint32_t slot = blockIdx.x * upb + threadIdx.x / team;
+    const int g = (int)(slot % s.G), c0 = g * s.Cg, dn = (int)(gridDim.x * upb / s.G);
+    float gm[NCH][VW], bt[NCH][VW];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+        const int c = c0 + min((k * team + lane) * VW, s.Cg - VW);
+        gn_ld<float, VW>(gamma + c, gm[k]);
+        gn_ld<float, VW>(beta + c, bt[k]);
+    }
+    GnRaw<T, VW> nx[NCH], nr[NCH];          // the next unit's elements, requested a unit ahead
+    auto fetch = [&](int64_t n) {
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int c = c0 + min((k * team + lane) * VW, s.Cg - VW);
+            nx[k] = *reinterpret_cast<const GnRaw<T, VW>*>(x + n * xsn + c);
+            if (RES) nr[k] = *reinterpret_cast<const GnRaw<T, VW>*>(res + n * rsn + c);
+        }
+    };
+    int n = (int)(slot / s.G);
+    if (n < s.N) fetch(n);
+    for (; n < s.N; n += dn) {
         const bool dead = s.lengths && s.lengths[n] <= 0;
+        GnRaw<T, VW> cr[NCH];
         float v[NCH][VW], sm = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            gn_get<T, VW>(nx[k], v[k]);
+            cr[k] = nr[k];
+        }
+        if (n + dn < s.N) fetch(n + dn);
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
             const int c = (k * team + lane) * VW;
 #pragma unroll
-            for (int i = 0; i < VW; ++i) v[k][i] = 0.f;
-            if (c < s.Cg && !dead) gn_ld<T, VW>(x + n * xsn + c0 + c, v[k]);
+            for (int i = 0; i < VW; ++i) v[k][i] = c < s.Cg && !dead ? v[k][i] : 0.f;
 #pragma unroll
             for (int i = 0; i < VW; ++i) sm += v[k][i];
         }
-        for (int o = team >> 1; o > 0; o >>= 1) sm += __shfl_xor(sm, o);
+        sm = gn_team_sum(sm, team);
         const float mean = sm * inv;
         float q = 0.f;
 #pragma unroll
@@ -543,23 +597,21 @@ __global__ __launch_bounds__(kGnThreads) void gn_rows_fwd_kernel(const T* __rest
 #pragma unroll
                 for (int i = 0; i < VW; ++i) { v[k][i] -= mean; q += v[k][i] * v[k][i]; }
             }
-        for (int o = team >> 1; o > 0; o >>= 1) q += __shfl_xor(q, o);
+        q = gn_team_sum(q, team);
         const float rstd = rsqrtf(q * inv + eps);
-        if (lane == 0 && mean_out) { mean_out[u] = mean; rstd_out[u] = rstd; }
+        if (lane == 0 && mean_out) { mean_out[(int64_t)n * s.G + g] = mean; rstd_out[(int64_t)n * s.G + g] = rstd; }
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
             const int c = (k * team + lane) * VW;
             if (c < s.Cg) {
-                float gm[VW], bt[VW], o[VW];
-                gn_ld<float, VW>(gamma + c0 + c, gm);
-                gn_ld<float, VW>(beta + c0 + c, bt);
-                if (res && !dead) gn_ld<T, VW>(res + n * rsn + c0 + c, o);
+                float o[VW];
+                if (RES) gn_get<T, VW>(cr[k], o);
 #pragma unroll
-                for (int i = 0; i < VW; ++i) {
-                    const float pre = v[k][i] * (rstd * gm[i]) + bt[i] + (res && !dead ? o[i] : 0.f);
-                    o[i] = dead ? 0.f : gn_act(pre, s.act);
-                }
-                gn_st<T, VW>(y + n * ysn + c0 + c, o);
+                for (int i = 0; i < VW; ++i) o[i] = v[k][i] * (rstd * gm[k][i]) + bt[k][i] + (RES ? o[i] : 0.f);
+                gn_act<VW>(o, s.act);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) o[i] = dead ? 0.f : o[i];
+                gn_st<T, VW>(y + (int64_t)n * ysn + c0 + c, o);
             }
         }
     }
@@ -567,17 +619,16 @@ __global__ __launch_bounds__(kGnThreads) void gn_rows_fwd_kernel(const T* __rest
 
 // The grid steps by a multiple of G units, so a lane keeps its channels and sums its parameter gradients in registers; slot = unit slot of
 // the grid, cpart [slots / G][C][2] because slot % G is the group.
-template <typename T, int VW, int NCH>
+template <typename T, int VW, int NCH, bool RES>
 __global__ __launch_bounds__(kGnThreads) void gn_rows_bwd_kernel(const T* __restrict__ gy, int64_t gsn, const T* __restrict__ x, int64_t xsn,
                                                                  const T* __restrict__ res, int64_t rsn, const float* __restrict__ gamma,
                                                                  const float* __restrict__ beta, const float* __restrict__ mean_in,
                                                                  const float* __restrict__ rstd_in, GnShape s, int team, T* __restrict__ gx,
                                                                  int64_t gxsn, T* __restrict__ gres, int64_t grsn, float* __restrict__ cpart) {
-    const int64_t units = (int64_t)s.N * s.G;
     const int upb = kGnThreads / team, lane = threadIdx.x & (team - 1);
     const float inv = 1.f / (float)s.Cg;
-    const int64_t slot = (int64_t)blockIdx.x * upb + threadIdx.x / team;
-    const int g = (int)(slot % s.G), c0 = g * s.Cg;
+    const uint32_t slot = blockIdx.x * upb + threadIdx.x / team;
+    const int g = (int)(slot % s.G), c0 = g * s.Cg, dn = (int)(gridDim.x * upb / s.G);
     float gm[NCH][VW], bt[NCH][VW], dg[NCH][VW], db[NCH][VW];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
@@ -586,29 +637,52 @@ __global__ __launch_bounds__(kGnThreads) void gn_rows_bwd_kernel(const T* __rest
         for (int i = 0; i < VW; ++i) { gm[k][i] = bt[k][i] = dg[k][i] = db[k][i] = 0.f; }
         if (c < s.Cg) { gn_ld<float, VW>(gamma + c0 + c, gm[k]); gn_ld<float, VW>(beta + c0 + c, bt[k]); }
     }
-    for (int64_t u = slot; u < units; u += (int64_t)gridDim.x * upb) {
-        const int64_t n = u / s.G;
+    GnRaw<T, VW> ng[NCH], nx[NCH], nr[NCH];
+    float nmean = 0.f, nrstd = 0.f;
+    auto fetch = [&](int64_t n) {
+        nmean = mean_in[n * s.G + g];
+        nrstd = rstd_in[n * s.G + g];
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            const int c = c0 + min((k * team + lane) * VW, s.Cg - VW);
+            ng[k] = *reinterpret_cast<const GnRaw<T, VW>*>(gy + n * gsn + c);
+            nx[k] = *reinterpret_cast<const GnRaw<T, VW>*>(x + n * xsn + c);
+            if (RES) nr[k] = *reinterpret_cast<const GnRaw<T, VW>*>(res + n * rsn + c);
+        }
+    };
+    int n = (int)(slot / s.G);
+    if (n < s.N) fetch(n);
+    for (; n < s.N; n += dn) {
         const bool dead = s.lengths && s.lengths[n] <= 0;
-        const float mean = mean_in[u], rstd = rstd_in[u];
-        float w[NCH][VW], xh[NCH][VW], s1 = 0.f, s2 = 0.f;
+        const float mean = nmean, rstd = nrstd;
+        float w[NCH][VW], xh[NCH][VW], zr[NCH][VW], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+            gn_get<T, VW>(ng[k], w[k]);
+            gn_get<T, VW>(nx[k], xh[k]);
+            if (RES) gn_get<T, VW>(nr[k], zr[k]);
+        }
+        if (n + dn < s.N) fetch(n + dn);
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
             const int c = (k * team + lane) * VW;
             const bool on = c < s.Cg && !dead;
             float z[VW];
 #pragma unroll
-            for (int i = 0; i < VW; ++i) { w[k][i] = 0.f; xh[k][i] = 0.f; z[i] = 0.f; }
+            for (int i = 0; i < VW; ++i) {
+                w[k][i] = on ? w[k][i] : 0.f;
+                xh[k][i] = on ? xh[k][i] : 0.f;
+                z[i] = RES && on ? zr[k][i] : 0.f;
+            }
             if (on) {
-                gn_ld<T, VW>(gy + n * gsn + c0 + c, w[k]);
-                gn_ld<T, VW>(x + n * xsn + c0 + c, xh[k]);
-                if (res) gn_ld<T, VW>(res + n * rsn + c0 + c, z);
 #pragma unroll
                 for (int i = 0; i < VW; ++i) {
                     xh[k][i] = (xh[k][i] - mean) * rstd;
-                    if (s.act != SP_ACT_NONE) w[k][i] *= gn_act_grad(xh[k][i] * gm[k][i] + bt[k][i] + z[i], s.act);
+                    z[i] += xh[k][i] * gm[k][i] + bt[k][i];
                 }
+                gn_act_grad<VW>(w[k], z, s.act);
             }
-            if (gres && c < s.Cg) gn_st<T, VW>(gres + n * grsn + c0 + c, w[k]);
+            if (gres && c < s.Cg) gn_st<T, VW>(gres + (int64_t)n * grsn + c0 + c, w[k]);
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 dg[k][i] += w[k][i] * xh[k][i];
@@ -618,7 +692,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_rows_bwd_kernel(const T* __rest
                 s2 += w[k][i] * xh[k][i];
             }
         }
-        for (int o = team >> 1; o > 0; o >>= 1) { s1 += __shfl_xor(s1, o); s2 += __shfl_xor(s2, o); }
+        s1 = gn_team_sum(s1, team);
+        s2 = gn_team_sum(s2, team);
         s1 *= inv; s2 *= inv;
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
@@ -627,11 +702,11 @@ __global__ __launch_bounds__(kGnThreads) void gn_rows_bwd_kernel(const T* __rest
                 float o[VW];
 #pragma unroll
                 for (int i = 0; i < VW; ++i) o[i] = dead ? 0.f : rstd * (w[k][i] - s1 - xh[k][i] * s2);
-                gn_st<T, VW>(gx + n * gxsn + c0 + c, o);
+                gn_st<T, VW>(gx + (int64_t)n * gxsn + c0 + c, o);
             }
         }
     }
-    float* cp = cpart + (slot / s.G) * s.C * 2 + c0 * 2;
+    float* cp = cpart + (int64_t)(slot / s.G) * s.C * 2 + c0 * 2;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
         const int c = (k * team + lane) * VW;
@@ -642,7 +717,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_rows_bwd_kernel(const T* __rest
     }
 }
 
-__global__ __launch_bounds__(kGnThreads) void gn_param_kernel(const float* __restrict__ cpart, int64_t nrows, int C, int accumulate,
+__global__ __launch_bounds__(1024) void gn_param_kernel(const float* __restrict__ cpart, int64_t nrows, int C, int accumulate,
                                                               float* __restrict__ dgamma, float* __restrict__ dbeta) {
     gn_param_reduce(cpart, nrows, C, blockIdx.x * 32, accumulate, dgamma, dbeta);
 }
@@ -653,7 +728,7 @@ struct GnPlan {
     int vw;                  // channels a chunk
     int nch, team;           // rows route: chunks a lane, lanes a unit
     int splits, nsub;        // block route
-    int grid;                // rows route, backward
+    int grid, gstep;         // rows route: the backward's grid; grids are multiples of gstep, so that a lane keeps its channels
 };
 
 // `vw`: the widest vector that the tensors' addresses and strides allow
@@ -672,9 +747,10 @@ static GnPlan gn_plan(int64_t N, int F, int T, int C, int G, int vw) {
             const int upb = kGnThreads / team;
             // one persistent grid; its step is a multiple of G units, so that a lane keeps its channels
             int64_t blocks = (N * G + upb - 1) / upb;
-            if (blocks > 1024) blocks = 1024;
+            if (blocks > 768) blocks = 768;
             int step = 1;
             while ((int64_t)step * upb % G) ++step;
+            p.gstep = step;
             p.grid = (int)((blocks + step - 1) / step * step);
             return p;
         }
@@ -683,8 +759,9 @@ static GnPlan gn_plan(int64_t N, int F, int T, int C, int G, int vw) {
     p.vw = vw;
     while (p.vw > 1 && !(C % p.vw == 0 && (Cg % p.vw == 0 || p.vw % Cg == 0))) p.vw >>= 1;
     const int64_t P = (int64_t)F * T;
-    // ~2048 workgroups on the chip, at least 32 positions each
-    int64_t sp = N > 0 ? 2048 / N : 1;
+    // ~768 workgroups on the chip (each pays for its reductions: 2048 took 82 / 67 us in the backward's two passes on 61 MB, 768 49 / 43),
+    // at least 32 positions each
+    int64_t sp = N > 0 ? 768 / N : 1;
     if (sp > kGnMaxSplit) sp = kGnMaxSplit;
     if (sp > (P + 31) / 32) sp = (P + 31) / 32;
     if (sp < 1) sp = 1;
@@ -773,9 +850,10 @@ extern "C" int sp_groupnorm_fwd(const void* x, const void* residual, const float
     if (p.rows) {
         const int upb = kGnThreads / p.team;
         int64_t blocks = (N * G + upb - 1) / upb;
-        if (blocks > 65536) blocks = 65536;
+        if (blocks > 2048) blocks = 2048;      // a few units a team, the next one's loads ahead of the present one's work
+        blocks = (blocks + p.gstep - 1) / p.gstep * p.gstep;
         SP_GN_TYPES(dtype, SP_GN_VW(p.vw, SP_GN_NCH(p.nch, {
-            hipLaunchKernelGGL((gn_rows_fwd_kernel<T_, VW_, NC_>), dim3((unsigned)blocks), dim3(kGnThreads), 0, st, (const T_*)x, xs.n,
+            hipLaunchKernelGGL((residual ? gn_rows_fwd_kernel<T_, VW_, NC_, true> : gn_rows_fwd_kernel<T_, VW_, NC_, false>), dim3((unsigned)blocks), dim3(kGnThreads), 0, st, (const T_*)x, xs.n,
                                (const T_*)residual, rs.n, gamma, beta, s, eps, p.team, (T_*)y, ys.n, mean, rstd); })))
         return check_launch("gn_rows_fwd_kernel");
     }
@@ -797,7 +875,7 @@ extern "C" int sp_groupnorm_bwd(const void* gy, const void* x, const void* resid
     SP_CHECK_ARG(dgamma && dbeta, "sp_groupnorm_bwd: null pointer");
     hipStream_t st = (hipStream_t)stream;
     if (N == 0 || F == 0 || T == 0) {       // no positions: the parameter gradients are zero
-        hipLaunchKernelGGL(gn_param_kernel, dim3((C + 31) / 32), dim3(kGnThreads), 0, st, nullptr, (int64_t)0, C, accumulate, dgamma, dbeta);
+        hipLaunchKernelGGL(gn_param_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, nullptr, (int64_t)0, C, accumulate, dgamma, dbeta);
         return check_launch("gn_param_kernel");
     }
     SP_CHECK_ARG(gy && x && gamma && beta && mean && rstd && gx, "sp_groupnorm_bwd: null pointer");
@@ -811,9 +889,9 @@ extern "C" int sp_groupnorm_bwd(const void* gy, const void* x, const void* resid
     float* cpart = (float*)workspace;
     if (p.rows) {
         SP_GN_TYPES(dtype, SP_GN_VW(p.vw, SP_GN_NCH(p.nch, {
-            hipLaunchKernelGGL((gn_rows_bwd_kernel<T_, VW_, NC_>), dim3(p.grid), dim3(kGnThreads), 0, st, (const T_*)gy, gs.n, (const T_*)x,
+            hipLaunchKernelGGL((residual ? gn_rows_bwd_kernel<T_, VW_, NC_, true> : gn_rows_bwd_kernel<T_, VW_, NC_, false>), dim3(p.grid), dim3(kGnThreads), 0, st, (const T_*)gy, gs.n, (const T_*)x,
                                xs.n, (const T_*)residual, rs.n, gamma, beta, mean, rstd, s, p.team, (T_*)gx, gxs.n, (T_*)gres, grs.n, cpart); })))
-        hipLaunchKernelGGL(gn_param_kernel, dim3((C + 31) / 32), dim3(kGnThreads), 0, st, cpart, (int64_t)p.grid * (kGnThreads / p.team) / G, C,
+        hipLaunchKernelGGL(gn_param_kernel, dim3((C + 31) / 32), dim3(1024), 0, st, cpart, (int64_t)p.grid * (kGnThreads / p.team) / G, C,
                            accumulate, dgamma, dbeta);
         return check_launch("gn_rows_bwd_kernel");
     }

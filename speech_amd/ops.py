@@ -4,13 +4,14 @@ normalisations, every matrix product, recurrence, CTC, decode -- runs in the han
 kernels.  What is left to torch are dtype casts and scalings of parameter-sized tensors and the
 dropout masks' random draws."""
 import ctypes
+import functools
 import math
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_ptr
+from ._lib import addr, check, lib, on_device, ptr, raw_stream, stream_ptr
 
 HOP = 160
 N_FFT = 400
@@ -885,14 +886,30 @@ def sru_layer(x, ln_w, ln_b, weight, wc, bias, mask, d, k, C=1, eps=1e-5, pre=No
 # Group normalisation with an activation, channels last
 # ------------------------------------------------------------------------------------------
 def _same_device(x, **others):
+    dev = x.device
     for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the input on {dev}")
+
+
+def _wants_grad(*tensors):
+    """Whether autograd has to see the call; without, the kernels are called directly (a Function's apply costs a small kernel's time)."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _once(what):
+    """The backward passes here are kernels, not differentiable themselves."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is not twice differentiable: its backward cannot run under create_graph=True")
+
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_CODE = {torch.float32: _lib.SP_F32, torch.float16: _lib.SP_F16, torch.bfloat16: _lib.SP_BF16}
 
 
 def _act_tensor(t, name):
     _need_cuda(t, name)
-    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if t.dtype not in _FLOATS:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
 
 
@@ -909,39 +926,53 @@ def _gn_strides(tensors):
     return _host_i64([s for t in tensors for s in (t.stride()[:3] if t is not None else (0, 0, 0))])
 
 
-class _GroupNormFn(torch.autograd.Function):
-    """x, residual [N,F,T,C] views with unit channel stride."""
+@functools.lru_cache(maxsize=256)
+def _gn_workspace(N, F, T, C, G, backward):
+    return lib().sp_groupnorm_workspace_bytes(N, F, T, C, G, backward)
 
+
+def _gn_fwd(x, w32, b32, residual, lengths, groups, eps, act, time_major, train):
+    """-> (y, mean and rstd [2, N, G] or None); x, residual [N, F, T, C] with unit channel stride."""
+    N, F, T, C = x.shape
+    if time_major:
+        y = x.new_empty((T, N, F, C)).permute(1, 2, 0, 3)
+    else:
+        y = x.new_empty((N, F, T, C))
+    stats = w32.new_empty((2, N, groups)) if train else None
+    mean = stats.data_ptr() if train else None
+    n = _gn_workspace(N, F, T, C, groups, 0)
+    ws = x.new_empty(n, dtype=torch.uint8) if n else None
+    with on_device(x):
+        rc = lib().sp_groupnorm_fwd(x.data_ptr(), addr(residual), w32.data_ptr(), b32.data_ptr(), addr(lengths), _gn_strides((x, residual, y)),
+                                    N, F, T, C, groups, eps, act, _CODE[x.dtype], y.data_ptr(), mean,
+                                    mean + 4 * N * groups if train else None, addr(ws), n, raw_stream(x))
+    check(rc, "sp_groupnorm_fwd")
+    return y, stats
+
+
+def _f32_param(p):
+    p = p.detach()
+    return p if p.dtype == torch.float32 and p.is_contiguous() else p.float().contiguous()
+
+
+class _GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, lengths, groups, eps, act, time_major):
-        N, F, T, C = x.shape
-        w32, b32 = weight.detach().float().contiguous(), bias.detach().float().contiguous()
-        if time_major:
-            y = torch.empty((T, N, F, C), dtype=x.dtype, device=x.device).permute(1, 2, 0, 3)
-        else:
-            y = torch.empty((N, F, T, C), dtype=x.dtype, device=x.device)
-        train = any(ctx.needs_input_grad)
-        mean = torch.empty((2, N, groups), dtype=torch.float32, device=x.device) if train else None
-        with torch.cuda.device(x.device):
-            n = lib().sp_groupnorm_workspace_bytes(N, F, T, C, groups, 0)
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            check(lib().sp_groupnorm_fwd(ptr(x), ptr(residual), ptr(w32), ptr(b32), ptr(lengths), _gn_strides((x, residual, y)), N, F, T,
-                                         C, groups, eps, act, _lib.dtype_code(x), ptr(y), ptr(mean[0]) if train else None,
-                                         ptr(mean[1]) if train else None, ptr(ws), n, stream_ptr()), "sp_groupnorm_fwd")
-        if train:
-            ctx.save_for_backward(x, residual, w32, b32, mean, lengths)
+        w32, b32 = _f32_param(weight), _f32_param(bias)
+        y, stats = _gn_fwd(x, w32, b32, residual, lengths, groups, eps, act, time_major, True)
+        ctx.save_for_backward(x, residual, w32, b32, stats, lengths)
         ctx.cfg = (groups, act, weight.dtype, bias.dtype)
         ctx.params = (weight, bias)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        x, residual, w32, b32, mean, lengths = ctx.saved_tensors
+        _once("group_norm")
+        x, residual, w32, b32, stats, lengths = ctx.saved_tensors
         groups, act, wdt, bdt = ctx.cfg
         N, F, T, C = x.shape
-        gy = _unit_last(gy.to(x.dtype))
-        gx = torch.empty((N, F, T, C), dtype=x.dtype, device=x.device)
+        gy = _unit_last(gy)
+        gx = x.new_empty((N, F, T, C))
         # without an activation (and without frames to clear) the residual's gradient is gy itself
         own = ctx.needs_input_grad[3] and (act != 0 or lengths is not None)
         gres = torch.empty_like(gx) if own else None
@@ -951,19 +982,21 @@ class _GroupNormFn(torch.autograd.Function):
             dw, db = ctx.params[0].grad, ctx.params[1].grad
         else:
             dw, db = torch.empty_like(w32), torch.empty_like(b32)
-        with torch.cuda.device(x.device):
-            n = lib().sp_groupnorm_workspace_bytes(N, F, T, C, groups, 1)
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            check(lib().sp_groupnorm_bwd(ptr(gy), ptr(x), ptr(residual), ptr(w32), ptr(b32), ptr(mean[0]), ptr(mean[1]), ptr(lengths),
-                                         _gn_strides((gy, x, residual, gx, gres)), N, F, T, C, groups, act, int(direct),
-                                         _lib.dtype_code(x), ptr(gx), ptr(gres), ptr(dw), ptr(db), ptr(ws), n, stream_ptr()),
-                  "sp_groupnorm_bwd")
+        mean = stats.data_ptr()
+        n = _gn_workspace(N, F, T, C, groups, 1)
+        ws = x.new_empty(n, dtype=torch.uint8)
+        with on_device(x):
+            rc = lib().sp_groupnorm_bwd(gy.data_ptr(), x.data_ptr(), addr(residual), w32.data_ptr(), b32.data_ptr(), mean,
+                                        mean + 4 * N * groups, addr(lengths), _gn_strides((gy, x, residual, gx, gres)), N, F, T, C, groups, act,
+                                        int(direct), _CODE[x.dtype], gx.data_ptr(), addr(gres), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n,
+                                        raw_stream(x))
+        check(rc, "sp_groupnorm_bwd")
         if ctx.needs_input_grad[3] and not own:
             gres = gy
         if direct:
             sink.ready(*ctx.params)
             return gx, None, None, gres, None, None, None, None, None
-        return gx, dw.to(wdt), db.to(bdt), gres, None, None, None, None, None
+        return (gx, dw if wdt == torch.float32 else dw.to(wdt), db if bdt == torch.float32 else db.to(bdt), gres, None, None, None, None, None)
 
 
 def group_norm(x, weight, bias, groups, eps=1e-5, act="none", residual=None, lengths=None, time_major=False):
@@ -995,8 +1028,11 @@ def group_norm(x, weight, bias, groups, eps=1e-5, act="none", residual=None, len
         if tuple(lengths.shape) != (shape[0],) or lengths.is_floating_point():
             raise ValueError(f"lengths must be whole numbers [{shape[0]}]")
         lengths = lengths.to(torch.int32).contiguous()
-    y = _GroupNormFn.apply(four(_unit_last(x)), weight, bias, four(_unit_last(residual)), lengths, int(groups), float(eps),
-                           _lib.ACT_CODES[act], bool(time_major))
+    x4, r4, code = four(_unit_last(x)), four(_unit_last(residual)), _lib.ACT_CODES[act]
+    if _wants_grad(x, weight, bias, residual):
+        y = _GroupNormFn.apply(x4, weight, bias, r4, lengths, int(groups), float(eps), code, bool(time_major))
+    else:
+        y, _ = _gn_fwd(x4, _f32_param(weight), _f32_param(bias), r4, lengths, int(groups), float(eps), code, bool(time_major), False)
     return y if len(shape) == 4 else y.squeeze(1) if len(shape) == 3 else y.reshape(shape)
 
 
@@ -1005,9 +1041,10 @@ def group_norm(x, weight, bias, groups, eps=1e-5, act="none", residual=None, len
 # ------------------------------------------------------------------------------------------
 def _dropout(x, residual, rows, p, rng, site, used):
     y = torch.empty_like(x)
-    with torch.cuda.device(x.device):
-        check(lib().sp_dropout(ptr(x), ptr(residual), rows, x.numel() // max(rows, 1), p, ptr(rng), site, _lib.dtype_code(x), ptr(y),
-                               ptr(used), stream_ptr()), "sp_dropout")
+    with on_device(x):
+        rc = lib().sp_dropout(x.data_ptr(), addr(residual), rows, x.numel() // rows if rows else 0, p, rng.data_ptr(), site, _CODE[x.dtype],
+                              y.data_ptr(), addr(used), raw_stream(x))
+    check(rc, "sp_dropout")
     return y
 
 
@@ -1015,16 +1052,15 @@ class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng, site, rows):
         # the pair that this call used: `rng` may have moved on (one step further, in place) when the backward runs
-        used = torch.empty(2, dtype=torch.int64, device=x.device) if any(ctx.needs_input_grad) else None
+        used = torch.empty_like(rng)
         y = _dropout(x, residual, rows, p, rng, site, used)
-        if used is not None:
-            ctx.save_for_backward(used)
+        ctx.save_for_backward(used)
         ctx.cfg = (p, site, rows)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
+        _once("dropout")
         (used,) = ctx.saved_tensors
         p, site, rows = ctx.cfg
         gx = _dropout(gy.contiguous(), None, rows, p, used, site, None) if ctx.needs_input_grad[0] else None
@@ -1055,8 +1091,10 @@ def dropout(x, p, rng, site=0, residual=None, shared=False):
     if shared and x.dim() < 2:
         raise ValueError("shared dropout needs x [T, ...]")
     _same_device(x, rng=rng, residual=residual)
-    return _DropoutFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), float(p), rng, int(site),
-                            x.shape[0] if shared else 1)
+    xc, rc, rows = x.contiguous(), None if residual is None else residual.contiguous(), x.shape[0] if shared else 1
+    if _wants_grad(x, residual):
+        return _DropoutFn.apply(xc, rc, float(p), rng, int(site), rows)
+    return _dropout(xc, rc, rows, float(p), rng, int(site), None)
 
 
 # ------------------------------------------------------------------------------------------
@@ -1077,63 +1115,62 @@ def _gdr_strides(tensors):
     return _host_i64([s for t in tensors for s in t.stride()[:3]])
 
 
-def _gdr_fwd(q, k, v, g, beta, state, state_out, lengths, scale, flags, train):
-    T, B, Hk, dk = q.shape
-    H, dv = v.shape[2:]
-    dims = (T, B, Hk, H, dk, dv)
-    code = _lib.dtype_code(q)
-    o = torch.empty((T, B, H, dv), dtype=v.dtype, device=v.device)
-    saved = ws = None
-    ns = nw = 0
-    with torch.cuda.device(q.device):
-        if train:
-            ns = lib().sp_gdr_saved_bytes(*dims, code)
-            saved = torch.empty(ns, dtype=torch.uint8, device=q.device)
-        else:
-            nw = lib().sp_gdr_workspace_bytes(*dims, code, 0)
-            ws = torch.empty(nw, dtype=torch.uint8, device=q.device)
-        check(lib().sp_gdr_fwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(state), ptr(lengths), _gdr_strides((q, k, v, g, beta)), *dims,
-                               scale, flags, code, ptr(o), ptr(state_out), ptr(saved), ns, ptr(ws), nw, stream_ptr()), "sp_gdr_fwd")
-    return o, saved
+@functools.lru_cache(maxsize=256)
+def _gdr_bytes(T, B, Hk, H, dk, dv, code, which):
+    """which: 0 workspace of the forward, 1 of the backward, 2 what the forward keeps for the backward."""
+    if which == 2:
+        return lib().sp_gdr_saved_bytes(T, B, Hk, H, dk, dv, code)
+    return lib().sp_gdr_workspace_bytes(T, B, Hk, H, dk, dv, code, which)
+
+
+def _gdr_fwd(q, k, v, g, beta, state, state_out, lengths, dims, strides, scale, flags, train):
+    T, B, Hk, H, dk, dv = dims
+    code = _CODE[q.dtype]
+    o = v.new_empty((T, B, H, dv))
+    n = _gdr_bytes(*dims, code, 2 if train else 0)
+    buf = o.new_empty(n, dtype=torch.uint8) if n else None
+    at = addr(buf)
+    with on_device(q):
+        rc = lib().sp_gdr_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), addr(state), addr(lengths), strides, T, B,
+                              Hk, H, dk, dv, scale, flags, code, o.data_ptr(), state_out.data_ptr(), at if train else None, n if train else 0,
+                              None if train else at, 0 if train else n, raw_stream(q))
+    check(rc, "sp_gdr_fwd")
+    return o, buf
 
 
 class _GatedDeltaFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, lengths, scale, flags):
-        train = any(ctx.needs_input_grad)
-        T, B, Hk, dk = q.shape
-        H, dv = v.shape[2:]
-        final = torch.empty((B, H, dk, dv), dtype=torch.float32, device=v.device)
-        o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, scale, flags, train)
-        if train:
-            ctx.save_for_backward(q, k, v, g, beta, lengths, o, saved)
-        ctx.cfg = (scale, flags)
+    def forward(ctx, q, k, v, g, beta, state, lengths, dims, scale, flags):
+        T, B, Hk, H, dk, dv = dims
+        final = g.new_empty((B, H, dk, dv))
+        o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _gdr_strides((q, k, v, g, beta)), scale, flags, True)
+        ctx.save_for_backward(q, k, v, g, beta, lengths, o, saved)
+        ctx.cfg = (dims, scale, flags)
         ctx.set_materialize_grads(False)
         return o, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, go, gstate):
+        _once("gated_delta_rule")
         q, k, v, g, beta, lengths, o, saved = ctx.saved_tensors
-        scale, flags = ctx.cfg
-        T, B, Hk, dk = q.shape
-        H, dv = v.shape[2:]
-        dims = (T, B, Hk, H, dk, dv)
-        dev, code = q.device, _lib.dtype_code(q)
+        dims, scale, flags = ctx.cfg
+        T, B, Hk, H, dk, dv = dims
+        code = _CODE[q.dtype]
         go = _head_rows(go) if go is not None else torch.zeros_like(o)
         gstate = gstate.contiguous() if gstate is not None else None
-        gq = torch.empty((T, B, Hk, dk), dtype=q.dtype, device=dev)
-        gk = torch.empty_like(gq)
-        gv = torch.empty((T, B, H, dv), dtype=v.dtype, device=dev)
-        gg, gb = torch.empty((2, T, B, H), dtype=torch.float32, device=dev).unbind(0)
-        gs0 = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev) if ctx.needs_input_grad[5] else None
-        with torch.cuda.device(dev):
-            nw = lib().sp_gdr_workspace_bytes(*dims, code, 1)
-            ws = torch.empty(nw, dtype=torch.uint8, device=dev)
-            check(lib().sp_gdr_bwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr(lengths), _gdr_strides((q, k, v, g, beta, go)), *dims, scale,
-                                   flags, code, ptr(o), ptr(saved), saved.numel(), ptr(go), ptr(gstate), ptr(gq), ptr(gk), ptr(gv), ptr(gg),
-                                   ptr(gb), ptr(gs0), ptr(ws), nw, stream_ptr()), "sp_gdr_bwd")
-        return gq, gk, gv, gg, gb, gs0, None, None, None
+        gq, gk = q.new_empty((T, B, Hk, dk)), q.new_empty((T, B, Hk, dk))
+        gv = v.new_empty((T, B, H, dv))
+        gg, gb = g.new_empty((T, B, H)), g.new_empty((T, B, H))
+        gs0 = g.new_empty((B, H, dk, dv)) if ctx.needs_input_grad[5] else None
+        n = _gdr_bytes(*dims, code, 1)
+        ws = saved.new_empty(n)
+        with on_device(q):
+            rc = lib().sp_gdr_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), addr(lengths),
+                                  _gdr_strides((q, k, v, g, beta, go)), T, B, Hk, H, dk, dv, scale, flags, code, o.data_ptr(), saved.data_ptr(),
+                                  saved.numel(), go.data_ptr(), addr(gstate), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), gg.data_ptr(),
+                                  gb.data_ptr(), addr(gs0), ws.data_ptr(), n, raw_stream(q))
+        check(rc, "sp_gdr_bwd")
+        return gq, gk, gv, gg, gb, gs0, None, None, None, None
 
 
 def _gdr_check(q, k, v, g, beta, state, lead):
@@ -1188,7 +1225,13 @@ def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, nor
         final = torch.zeros((B, H, dk, dv), dtype=torch.float32, device=q.device) if state is None else state.clone()
         return torch.zeros_like(v), final
     flags = (_lib.GDR_NORMALIZE if normalize else 0) | (_lib.GDR_BIDIRECTIONAL if bidirectional else 0)
-    return _GatedDeltaFn.apply(_head_rows(q), _head_rows(k), _head_rows(v), g.float(), beta.float(), state, lengths, scale, flags)
+    dims = (q.shape[0], B, Hk, H, dk, dv)
+    q, k, v, g, beta = _head_rows(q), _head_rows(k), _head_rows(v), g.float(), beta.float()
+    if _wants_grad(q, k, v, g, beta, state):
+        return _GatedDeltaFn.apply(q, k, v, g, beta, state, lengths, dims, scale, flags)
+    final = g.new_empty((B, H, dk, dv))
+    o, _ = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _gdr_strides((q, k, v, g, beta)), scale, flags, False)
+    return o, final
 
 
 @torch.no_grad()
@@ -1205,7 +1248,7 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None, normalize=False):
         raise ValueError(f"scale must be finite and not zero, got {scale}")
     if B == 0:
         return torch.zeros_like(v)
-    q, k, v, g, beta = (_unit_last(t) if t.dim() == 3 else t for t in (q, k, v, g.float(), beta.float()))
-    o, _ = _gdr_fwd(q[None], k[None], v[None], g[None], beta[None], state, state, None, scale,
-                    _lib.GDR_NORMALIZE if normalize else 0, False)
+    q, k, v, g, beta = _unit_last(q), _unit_last(k), _unit_last(v), g.float(), beta.float()
+    strides = _host_i64([s for t in (q, k, v, g, beta) for s in (0, *t.stride()[:2])])       # one frame: no step from frame to frame
+    o, _ = _gdr_fwd(q, k, v, g, beta, state, state, None, (1, B, Hk, H, dk, dv), strides, scale, _lib.GDR_NORMALIZE if normalize else 0, False)
     return o[0]
