@@ -1297,92 +1297,107 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(
 }
 
 // ---- recurrent form -------------------------------------------------------------------------------------
-// Few frames: a workgroup owns 32 columns of one head's state, in registers: 8 lanes x 4 columns a row, 32 row groups of up to four rows.
-// One reduction a frame: k.S and q.S come from the state before the frame, o follows from u.
-template <typename T>
+// Few frames: a workgroup owns 32 columns of one head's state, in registers: 8 lanes x 4 columns a row, 32 row groups of four rows.  All
+// frames' keys, queries, values and gates are brought to LDS first (a frame's global loads inside the loop cost 1.7 us a frame), with the
+// three products of k and q that do not need the state.  One reduction a frame then: k.S and q.S come from the state before the frame, and
+// o follows from u.
+__device__ __forceinline__ float add_lanes_8_16_32(float v) {       // sum over the eight lanes that agree in their number mod 8
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, false));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+template <typename T, int NF>      // NF: frames that LDS holds (1 or kRecurrentMax)
 __global__ __launch_bounds__(256) void gdr_recurrent_kernel(GdrArgs a) {
-    __shared__ float red[2][4][8][12];
+    __shared__ __align__(16) float kq[2][NF][128];
+    __shared__ __align__(16) float vs[NF][32];
+    __shared__ __align__(16) float sc[NF][8];          // decay, beta, 1 / |k|, scale / |q|, qh.kh
+    __shared__ __align__(16) float red[2][4][8][8];
     const int ns = (a.dv + 31) >> 5, bh = blockIdx.x / ns, sl = blockIdx.x % ns, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
     const int tid = threadIdx.x, wave = tid >> 6, cl = tid & 7, rg = tid >> 3;
-    const int col = sl * 32 + cl * 4;
-    const bool con = col < a.dv;
-    const int64_t state = (int64_t)bh * a.dk * a.dv;
+    const int col = sl * 32 + cl * 4, row0 = rg * 4;
+    const bool con = col < a.dv && row0 < a.dk;
+    const int64_t state = (int64_t)bh * a.dk * a.dv + (int64_t)row0 * a.dv + col;
     f32x4 S[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int row = i * 32 + rg;
         S[i] = f32x4{0, 0, 0, 0};
-        if (a.s0 && con && row < a.dk) S[i] = *reinterpret_cast<const f32x4a*>(a.s0 + state + (int64_t)row * a.dv + col);
+        if (a.s0 && con) S[i] = *reinterpret_cast<const f32x4a*>(a.s0 + state + (int64_t)i * a.dv);
     }
     const T* kp = (const T*)a.k + b * a.ks[1] + hk * a.ks[2];
     const T* qp = (const T*)a.q + b * a.qs[1] + hk * a.qs[2];
     const T* vp = (const T*)a.v + b * a.vs[1] + h * a.vs[2];
-    T* op = (T*)a.o + ((int64_t)b * a.H + h) * a.dv;
-    const int64_t ots = (int64_t)a.B * a.H * a.dv;
-    for (int p = 0; p < w.len; ++p) {
+    for (int i = tid; i < w.len * 128; i += 256) {
+        const int p = i >> 7, c = i & 127;
         const int64_t t = w.frame(p);
-        float k[4], q[4], acc[11];
-        f32x4 v = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = i * 32 + rg;
-            k[i] = row < a.dk ? Elem<T>::ld(kp + t * a.ks[0] + row) : 0.f;
-            q[i] = row < a.dk ? Elem<T>::ld(qp + t * a.qs[0] + row) : 0.f;
+        kq[0][p][c] = c < a.dk ? Elem<T>::ld(kp + t * a.ks[0] + c) : 0.f;
+        kq[1][p][c] = c < a.dk ? Elem<T>::ld(qp + t * a.qs[0] + c) : 0.f;
+    }
+    for (int i = tid; i < w.len * 32; i += 256) {
+        const int p = i >> 5, c = i & 31;
+        vs[p][c] = sl * 32 + c < a.dv ? Elem<T>::ld(vp + w.frame(p) * a.vs[0] + sl * 32 + c) : 0.f;
+    }
+    __syncthreads();
+    for (int p = wave; p < w.len; p += 4) {             // a wave a frame: two entries a lane
+        const int l = tid & 63;
+        const float k0 = kq[0][p][l], k1 = kq[0][p][64 + l], q0 = kq[1][p][l], q1 = kq[1][p][64 + l];
+        const float kk = wave_sum(k0 * k0 + k1 * k1), qq = wave_sum(q0 * q0 + q1 * q1), qk = wave_sum(q0 * k0 + q1 * k1);
+        if (l == 0) {
+            const int64_t t = w.frame(p);
+            const float rk = a.norm ? 1.f / sqrtf(kk + 1e-6f) : 1.f, sq = (a.norm ? 1.f / sqrtf(qq + 1e-6f) : 1.f) * a.scale;
+            sc[p][0] = __expf(a.g[t * a.gs[0] + b * a.gs[1] + h * a.gs[2]]);
+            sc[p][1] = a.beta[t * a.bs[0] + b * a.bs[1] + h * a.bs[2]];
+            sc[p][2] = rk;
+            sc[p][3] = sq;
+            sc[p][4] = sq * rk * qk;
         }
-        if (con) {
+    }
+    __syncthreads();
+    T* op = (T*)a.o + ((int64_t)b * a.H + h) * a.dv + col;
+    const int64_t ots = (int64_t)a.B * a.H * a.dv;
+    const bool writes = rg == 0 && col < a.dv;
+    for (int p = 0; p < w.len; ++p) {
+        const f32x4 k = *reinterpret_cast<const f32x4a*>(&kq[0][p][row0]), q = *reinterpret_cast<const f32x4a*>(&kq[1][p][row0]);
+        const f32x4 v = *reinterpret_cast<const f32x4a*>(&vs[p][cl * 4]), c4 = *reinterpret_cast<const f32x4a*>(&sc[p][0]);
+        const float dec = c4[0], be = c4[1], rk = c4[2], sq = c4[3], qk = sc[p][4];
+        f32x4 ks = {0, 0, 0, 0}, qs = ks;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = Elem<T>::ld(vp + t * a.vs[0] + col + j);
-        }
-        const float gv = a.g[t * a.gs[0] + b * a.gs[1] + h * a.gs[2]], be = a.beta[t * a.bs[0] + b * a.bs[1] + h * a.bs[2]];
+        for (int i = 0; i < 4; ++i) { ks += k[i] * S[i]; qs += q[i] * S[i]; }
 #pragma unroll
-        for (int j = 0; j < 11; ++j) acc[j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { acc[j] += k[i] * S[i][j]; acc[4 + j] += q[i] * S[i][j]; }
-            acc[8] += k[i] * k[i];
-            acc[9] += q[i] * q[i];
-            acc[10] += q[i] * k[i];
-        }
-#pragma unroll
-        for (int j = 0; j < 11; ++j) {
-            acc[j] += __shfl_xor(acc[j], 8);
-            acc[j] += __shfl_xor(acc[j], 16);
-            acc[j] += __shfl_xor(acc[j], 32);
-        }
-        float(*rd)[8][12] = red[p & 1];
+        for (int j = 0; j < 4; ++j) { ks[j] = add_lanes_8_16_32(ks[j]); qs[j] = add_lanes_8_16_32(qs[j]); }
+        float(*rd)[8][8] = red[p & 1];
         if ((tid & 63) < 8) {
-#pragma unroll
-            for (int j = 0; j < 11; ++j) rd[wave][cl][j] = acc[j];
+            *reinterpret_cast<f32x4a*>(&rd[wave][cl][0]) = ks;
+            *reinterpret_cast<f32x4a*>(&rd[wave][cl][4]) = qs;
         }
         __syncthreads();
+        ks = f32x4{0, 0, 0, 0};
+        qs = ks;
 #pragma unroll
-        for (int j = 0; j < 11; ++j) acc[j] = rd[0][cl][j] + rd[1][cl][j] + rd[2][cl][j] + rd[3][cl][j];
-        const float rk = a.norm ? 1.f / sqrtf(acc[8] + 1e-6f) : 1.f, sq = (a.norm ? 1.f / sqrtf(acc[9] + 1e-6f) : 1.f) * a.scale;
-        const float dec = __expf(gv);
-        f32x4 u, o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            u[j] = be * (v[j] - dec * rk * acc[j]);
-            o[j] = sq * (dec * acc[4 + j] + rk * acc[10] * u[j]);
+        for (int x = 0; x < 4; ++x) {
+            ks += *reinterpret_cast<const f32x4a*>(&rd[x][cl][0]);
+            qs += *reinterpret_cast<const f32x4a*>(&rd[x][cl][4]);
         }
+        const f32x4 u = be * (v - (dec * rk) * ks);
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[i] = dec * S[i] + (rk * k[i]) * u;
-        if (rg == 0 && con) {
+        if (writes) {
+            const f32x4 o = (sq * dec) * qs + qk * u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) Elem<T>::st(op + t * ots + col + j, o[j]);
+            for (int j = 0; j < 4; ++j) Elem<T>::st(op + w.frame(p) * ots + j, o[j]);
         }
     }
-    if (rg == 0 && con) {
+    if (writes) {
         for (int t = w.len; t < a.T; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) Elem<T>::st(op + t * ots + col + j, 0.f);
+            for (int j = 0; j < 4; ++j) Elem<T>::st(op + t * ots + j, 0.f);
     }
+    if (con) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = i * 32 + rg;
-        if (con && row < a.dk) *reinterpret_cast<f32x4a*>(a.sT + state + (int64_t)row * a.dv + col) = S[i];
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4a*>(a.sT + state + (int64_t)i * a.dv) = S[i];
     }
 }
 
@@ -1501,11 +1516,14 @@ extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const flo
     a.s0 = state; a.sT = state_out; a.o = o;
     hipStream_t s = (hipStream_t)stream;
     const bool train = saved != nullptr;
-    if (!train && T <= kRecurrentMax) {
+    if (!train && T <= kRecurrentMax) {       // T = 0: the state is copied
         const int64_t blocks = (int64_t)B * H * ((dv + 31) / 32);
-        if (dtype == SP_F32) return gdr_launch(gdr_recurrent_kernel<float>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
-        if (dtype == SP_F16) return gdr_launch(gdr_recurrent_kernel<__half>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
-        return gdr_launch(gdr_recurrent_kernel<__hip_bfloat16>, 0, blocks, 256, a, s, "gdr_recurrent_kernel");
+#define SP_GDR_REC(T_) return T == 1 ? gdr_launch(gdr_recurrent_kernel<T_, 1>, 0, blocks, 256, a, s, "gdr_recurrent_kernel") \
+                                     : gdr_launch(gdr_recurrent_kernel<T_, kRecurrentMax>, 0, blocks, 256, a, s, "gdr_recurrent_kernel")
+        if (dtype == SP_F32) SP_GDR_REC(float);
+        if (dtype == SP_F16) SP_GDR_REC(__half);
+        SP_GDR_REC(__hip_bfloat16);
+#undef SP_GDR_REC
     }
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype),
                  "sp_gdr_fwd: q, k, v need 16-byte aligned rows and at most 2^23 elements from frame to frame");
