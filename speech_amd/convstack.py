@@ -251,3 +251,90 @@ def conv_stack(spec, cnn, blocks, training):
     bn = blocks[0].bn1
     return _ConvStackFn.apply(spec, bool(training), float(bn.momentum), float(bn.eps), cnn.weight, cnn.bias,
                               *params, *bufs)
+
+
+# ------------------------------------------------------------------------------------------
+# The stack with group normalisation (ops.group_norm) in the place of BatchNorm
+# ------------------------------------------------------------------------------------------
+class _StemFn(torch.autograd.Function):
+    """Conv2d(1, 32, 3, stride 2) on the f32 spectrogram -> bf16 [B,F,T,32]."""
+
+    @staticmethod
+    def forward(ctx, spec, w, b):
+        spec = spec.detach().float().contiguous()
+        B, _, Fin, Tin = spec.shape
+        w32, b32 = _f32(w), _f32(b)
+        with torch.cuda.device(spec.device):
+            x = torch.empty((B, (Fin - 1) // 2 + 1, (Tin - 1) // 2 + 1, C), dtype=torch.bfloat16, device=spec.device)
+            check(lib().sp_conv_stem_fwd(ptr(spec), ptr(w32), ptr(b32), B, Fin, Tin, ptr(x), stream_ptr()), "sp_conv_stem_fwd")
+        ctx.save_for_backward(spec)
+        return x
+
+    @staticmethod
+    def backward(ctx, g):
+        (spec,) = ctx.saved_tensors
+        B, _, Fin, Tin = spec.shape
+        gw = torch.zeros((32, 1, 3, 3), dtype=torch.float32, device=spec.device)
+        gb = torch.zeros(32, dtype=torch.float32, device=spec.device)
+        g = g.contiguous()
+        with torch.cuda.device(spec.device):
+            check(lib().sp_conv_stem_bwd(ptr(spec), ptr(g), B, Fin, Tin, ptr(gw), ptr(gb), stream_ptr()), "sp_conv_stem_bwd")
+        return None, gw, gb
+
+
+class _Conv3x5Fn(torch.autograd.Function):
+    """3 x 5 convolution without bias on bf16 [B,F,T,32].  The weight gradient's kernel takes dy = c[0] g + c[1] y + c[2] (BatchNorm's
+    backward folded in); here the coefficients are (1, 0, 0)."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        x = x.contiguous()
+        B, F, T, _ = x.shape
+        with torch.cuda.device(x.device):
+            pf, pb = _pack_both(_f32(w))
+            y = _conv(x, None, None, IN_ID, pf, None, None, None, EPI_NONE, B, F, T)
+        ctx.save_for_backward(x, pb)
+        ctx.wshape = w.shape
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, pb = ctx.saved_tensors
+        B, F, T, _ = x.shape
+        g = g.contiguous()
+        coef = torch.zeros(3 * C, dtype=torch.float32, device=x.device)
+        coef[:C].fill_(1.0)
+        gw = torch.zeros(ctx.wshape, dtype=torch.float32, device=x.device)
+        with torch.cuda.device(x.device):
+            gx = _conv(g, None, None, IN_ID, pb, None, None, None, EPI_NONE, B, F, T)
+            check(lib().sp_conv3x5_wgrad(ptr(x), None, IN_ID, ptr(g), ptr(g), ptr(coef), B, F, T, ptr(_wgrad_workspace(x.device)), ptr(gw),
+                                         stream_ptr()), "sp_conv3x5_wgrad")
+        return gx, gw
+
+
+def conv_stack_group(spec, cnn, blocks, f32=False):
+    """conv_stack for blocks with GroupNorm: same output layout [T', B, F*32], feature index f*32 + c.  f32: the evaluation outside
+    autocast, every convolution on sp_conv2d_f32 (no gradients)."""
+    from . import ops
+    spec = spec.detach().float().contiguous()
+    B, _, Fin, Tin = spec.shape
+    F, T = (Fin - 1) // 2 + 1, (Tin - 1) // 2 + 1
+    chl = (F * T * C, T * C, C)
+    if f32:
+        ones, zeros = torch.ones(C, dtype=torch.float32, device=spec.device), torch.zeros(C, dtype=torch.float32, device=spec.device)
+
+        def conv(x, m, stride, xs, cin, n_f, n_t, shift):
+            out = torch.empty((B, F, T, C), dtype=torch.float32, device=spec.device)
+            with torch.cuda.device(spec.device):
+                return _conv_f32(x, xs, cin, _f32(m.weight).permute(2, 3, 1, 0).contiguous(), ones, shift, None, None, False, B, n_f, n_t, stride,
+                                 out, chl)
+        x = conv(spec, cnn, 2, (Fin * Tin, Tin, 1), 1, Fin, Tin, _f32(cnn.bias))
+    else:
+        x = _StemFn.apply(spec, cnn.weight, cnn.bias)
+    for i, blk in enumerate(blocks):
+        g1, g2 = blk.bn1, blk.bn2
+        y = conv(x, blk.conv1, 1, chl, C, F, T, zeros) if f32 else _Conv3x5Fn.apply(x, blk.conv1.weight)
+        y = ops.group_norm(y, g1.weight, g1.bias, g1.num_groups, g1.eps, act="relu")
+        y = conv(y, blk.conv2, 1, chl, C, F, T, zeros) if f32 else _Conv3x5Fn.apply(y, blk.conv2.weight)
+        x = ops.group_norm(y, g2.weight, g2.bias, g2.num_groups, g2.eps, act="relu", residual=x, time_major=i == len(blocks) - 1)
+    return x.permute(2, 0, 1, 3).reshape(T, B, F * C)

@@ -14,6 +14,10 @@ activation type of the SRU stack and classifier: float32, bfloat16 (the training
 float16 (the reference trains under fp16 autocast with an fp16 recurrence, net.py:71, and evaluates
 with model.half(), scripts/eval_dataset.py).  ResidualBlock.forward below is the plain
 torch statement of one block and is used only by tests as the reference of the kernels.
+
+Two variants without a counterpart in the reference: ``norm="group"`` normalises the blocks over groups of channels of each utterance
+instead of over the batch (no coupling between utterances or data-parallel ranks, one form for training and evaluation), and
+``rnn="delta"`` replaces the SRU stack by gated delta rule layers (GatedDeltaLayer).
 """
 import math
 
@@ -25,16 +29,17 @@ from . import convstack, ops
 
 
 class ResidualBlock(nn.Module):
-    """net.py:6-42: conv(3 x t) -> BN -> ReLU -> conv -> BN -> += residual -> ReLU."""
+    """net.py:6-42: conv(3 x t) -> BN -> ReLU -> conv -> BN -> += residual -> ReLU.  groups > 0: group normalisation in the place
+    of BatchNorm; the convolutions then have no bias (the normalisation's own one follows)."""
 
-    def __init__(self, in_channels, out_channels, t_kernel_s):
+    def __init__(self, in_channels, out_channels, t_kernel_s, groups=0):
         super().__init__()
         pad = (3 // 2, t_kernel_s // 2)
-        self.conv1 = nn.Conv2d(in_channels, out_channels, (3, t_kernel_s), 1, padding=pad)
-        self.conv2 = nn.Conv2d(out_channels, out_channels, (3, t_kernel_s), 1, padding=pad)
+        self.conv1 = nn.Conv2d(in_channels, out_channels, (3, t_kernel_s), 1, padding=pad, bias=not groups)
+        self.conv2 = nn.Conv2d(out_channels, out_channels, (3, t_kernel_s), 1, padding=pad, bias=not groups)
         self.relu = nn.ReLU(inplace=True)
-        self.bn1 = nn.BatchNorm2d(out_channels)
-        self.bn2 = nn.BatchNorm2d(out_channels)
+        self.bn1 = nn.GroupNorm(groups, out_channels) if groups else nn.BatchNorm2d(out_channels)
+        self.bn2 = nn.GroupNorm(groups, out_channels) if groups else nn.BatchNorm2d(out_channels)
         for conv in (self.conv1, self.conv2):
             nn.init.kaiming_normal_(conv.weight, mode="fan_out", nonlinearity="relu")
         nn.init.ones_(self.bn1.weight)
@@ -179,15 +184,116 @@ class SRU(nn.Module):
         return x, None
 
 
-class SRModel(nn.Module):
-    def __init__(self, n_rnn_layers, rnn_dim, n_vocab, n_feats, dropout, projection_size=0,
-                 compute_dtype=torch.float32):
+class GatedDeltaLayer(nn.Module):
+    """One gated delta rule layer over time-major activations [T, B, n_in] -> [T, B, n_out]:
+
+        q, k, v, a, b = LayerNorm(x) W_in            per head: dk, dk, dv = n_out / heads, 1, 1
+        o = gated_delta_rule(q, k, v, g = -exp(A) softplus(a + a0), beta = sigmoid(b))      q, k normalised
+        y = dropout(SiLU(GroupNorm(o, one group a head)) W_out) (+ x where the widths agree)
+
+    bidirectional: the second half of the heads walks backwards.  step() is the streaming form of the unidirectional layer."""
+
+    GROUP_EPS = 1e-5
+
+    def __init__(self, n_in, n_out, heads=8, dk=64, dropout=0.0, bidirectional=True, site=0):
         super().__init__()
+        if n_out % (8 * heads) or dk % 8 or (bidirectional and heads % 2):
+            raise ValueError(f"{n_out} outputs do not make {heads} heads of a multiple of 8 (an even number of heads for both directions)")
+        self.heads, self.dk, self.dv = heads, dk, n_out // heads
+        self.dropout, self.bidirectional, self.site = dropout, bidirectional, site
+        self.residual = n_in == n_out
+        self.layer_norm = nn.LayerNorm(n_in)
+        width = heads * (2 * dk + self.dv) + 2 * heads
+        self.w_in = nn.Parameter(torch.empty(n_in, width + -width % 8))        # rows of whole 16-byte pieces
+        self.w_out = nn.Parameter(torch.empty(n_out, n_out))
+        self.group_norm = nn.GroupNorm(heads, n_out, eps=self.GROUP_EPS)
+        self.a_log = nn.Parameter(torch.empty(heads))
+        self.a_bias = nn.Parameter(torch.empty(heads))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        """Decay rates spread over the heads from a few to a few hundred frames."""
+        with torch.no_grad():
+            self.w_in.normal_(std=self.w_in.shape[0] ** -0.5)
+            self.w_out.normal_(std=self.w_out.shape[0] ** -0.5)
+            self.a_log.uniform_(math.log(0.01), math.log(1.0))
+            self.a_bias.zero_()
+
+    def _split(self, x):
+        """x [..., n_in] -> q, k [..., H, dk], v [..., H, dv], g, beta f32 [..., H]: views into one projection."""
+        lead, H = x.shape[:-1], self.heads
+        ln = self.layer_norm
+        xn = ops.layer_norm(x, ln.weight, ln.bias, ln.eps)
+        u = ops.matmul(xn.reshape(-1, xn.shape[-1]), self.w_in).view(*lead, -1)
+        nq, nv = H * self.dk, H * self.dv
+        q, k = u[..., :nq].unflatten(-1, (H, self.dk)), u[..., nq:2 * nq].unflatten(-1, (H, self.dk))
+        v = u[..., 2 * nq:2 * nq + nv].unflatten(-1, (H, self.dv))
+        a, b = u[..., 2 * nq + nv:2 * nq + nv + H], u[..., 2 * nq + nv + H:2 * nq + nv + 2 * H]
+        g = -torch.exp(self.a_log.float()) * F.softplus(a.float() + self.a_bias.float())
+        return q, k, v, g, torch.sigmoid(b.float())
+
+    def _out(self, o, x, rng):
+        gn = self.group_norm
+        o = o.reshape(-1, self.heads * self.dv)
+        y = ops.matmul(ops.group_norm(o, gn.weight, gn.bias, self.heads, gn.eps, act="silu"), self.w_out).view(*x.shape[:-1], -1)
+        res = x if self.residual else None
+        if self.training and self.dropout > 0:
+            return ops.dropout(y, self.dropout, rng, self.site, residual=res)
+        return y if res is None else y + res
+
+    def forward(self, x, rng=None, lengths=None, state=None):
+        """rng: ops.dropout_rng's pair (training with dropout only) -> (y, final state)."""
+        q, k, v, g, beta = self._split(x)
+        o, final = ops.gated_delta_rule(q, k, v, g, beta, state, lengths, normalize=True, bidirectional=self.bidirectional)
+        return self._out(o, x, rng), final
+
+    @torch.no_grad()
+    def step(self, x, state):
+        """One frame x [B, n_in] of every session; `state` f32 [B, heads, dk, dv] is updated in place.  Evaluation only."""
+        if self.bidirectional:
+            raise RuntimeError("a bidirectional layer cannot run frame by frame")
+        return self._out(ops.gated_delta_step(*self._split(x), state, normalize=True), x, None)
+
+
+class GatedDelta(nn.Module):
+    """A stack of GatedDeltaLayers with the dropouts' generator state: (seed, step), one step further after every training pass."""
+
+    def __init__(self, n_in, n_out, n_layers, dropout=0.0, heads=8, dk=64, bidirectional=True):
+        super().__init__()
+        self.layers = nn.ModuleList(
+            GatedDeltaLayer(n_in if i == 0 else n_out, n_out, heads, dk, dropout if i + 1 != n_layers else 0.0, bidirectional, site=i)
+            for i in range(n_layers))
+        # the seed torch was seeded with: data-parallel ranks seed apart (train.main)
+        self.register_buffer("dropout_state", torch.tensor([torch.initial_seed() % (1 << 62), 0], dtype=torch.int64))
+
+    def forward(self, x, lengths=None):
+        for layer in self.layers:
+            x, _ = layer(x, self.dropout_state, lengths)
+        if self.training:
+            self.dropout_state[1] += 1
+        return x, None
+
+
+class SRModel(nn.Module):
+    NORM_GROUPS = 8
+
+    def __init__(self, n_rnn_layers, rnn_dim, n_vocab, n_feats, dropout, projection_size=0,
+                 compute_dtype=torch.float32, norm="batch", rnn="sru"):
+        super().__init__()
+        if norm not in ("batch", "group") or rnn not in ("sru", "delta"):
+            raise ValueError(f"norm must be 'batch' or 'group' and rnn 'sru' or 'delta', got {norm!r} and {rnn!r}")
+        if rnn == "delta" and projection_size:
+            raise ValueError("projection_size belongs to the SRU stack")
+        self.norm, self.rnn = norm, rnn
         self.cnn = nn.Conv2d(1, 32, 3, stride=2, padding=3 // 2)
-        self.resnet_layers = nn.Sequential(*[ResidualBlock(32, 32, t_kernel_s=5) for _ in range(3)])
+        groups = self.NORM_GROUPS if norm == "group" else 0
+        self.resnet_layers = nn.Sequential(*[ResidualBlock(32, 32, t_kernel_s=5, groups=groups) for _ in range(3)])
         n_features = 32 * n_feats // 2
-        self.sru_layers = SRU(n_features, rnn_dim, n_rnn_layers, dropout=dropout,
-                              projection_size=projection_size, in_layout=(32, n_feats // 2))
+        if rnn == "delta":
+            self.delta_layers = GatedDelta(n_features, 2 * rnn_dim, n_rnn_layers, dropout)
+        else:
+            self.sru_layers = SRU(n_features, rnn_dim, n_rnn_layers, dropout=dropout,
+                                  projection_size=projection_size, in_layout=(32, n_feats // 2))
         self.classifier = nn.Sequential(nn.LayerNorm(2 * rnn_dim),
                                         nn.Linear(2 * rnn_dim, n_vocab + 1, bias=False))
         self.compute_dtype = compute_dtype
@@ -195,13 +301,16 @@ class SRModel(nn.Module):
     def encode(self, x):
         """[B, 1, F, T] f32 spectrogram -> layer-normed encoder output, time-major [T', B, 2*rnn_dim]."""
         cd = self.compute_dtype
-        if cd == torch.float32 and not self.training and not torch.is_grad_enabled():
+        if self.norm == "group":
+            f32 = cd == torch.float32 and not self.training and not torch.is_grad_enabled()
+            x = convstack.conv_stack_group(x, self.cnn, list(self.resnet_layers), f32)
+        elif cd == torch.float32 and not self.training and not torch.is_grad_enabled():
             # fp32 evaluation (train.py:162-168, outside autocast): the conv stack in f32 as well
             x = convstack.conv_stack_eval_f32(x, self.cnn, list(self.resnet_layers))
         else:
             # conv stack on the channel-last bf16 kernels -> [T', B, (F/2)*32], feature = f*32 + c
             x = convstack.conv_stack(x, self.cnn, list(self.resnet_layers), self.training)
-        x, _ = self.sru_layers(x.to(cd))
+        x, _ = (self.delta_layers if self.rnn == "delta" else self.sru_layers)(x.to(cd))
         ln = self.classifier[0]
         return ops.layer_norm(x, ln.weight, ln.bias, ln.eps)
 

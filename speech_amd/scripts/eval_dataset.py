@@ -109,6 +109,8 @@ def parse_args(argv=None):
     p.add_argument("--n_rnn_layers", type=int, default=10)
     p.add_argument("--rnn_dim", type=int, default=512)
     p.add_argument("--projection_size", type=int, default=0)
+    p.add_argument("--norm", choices=["batch", "group"], default="batch")
+    p.add_argument("--rnn", choices=["sru", "delta"], default="sru")
     a = p.parse_args(argv)
     if a.beam_decode not in ("True", "False"):
         p.error("beam_decode must be True or False")
@@ -123,7 +125,7 @@ def main(argv=None, log=print):
                "n_vocab": 28, "n_feats": data.N_MELS, "projection_size": a.projection_size}      # eval_dataset.py:74-84
     dtype = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}[a.dtype]
     model = net.SRModel(hparams["n_rnn_layers"], hparams["rnn_dim"], hparams["n_vocab"], hparams["n_feats"],
-                        hparams["dropout"], hparams["projection_size"], compute_dtype=dtype).cuda()
+                        hparams["dropout"], hparams["projection_size"], compute_dtype=dtype, norm=a.norm, rnn=a.rnn).cuda()
     dataset, loader_bs = build_dataset(a.dataset_type, hparams["batch_size"], a.manifest_root, a.root_map, a.ibm_root)
     if a.model_file:
         model.load_checkpoint(torch.load(a.model_file, map_location="cpu", weights_only=True))

@@ -523,7 +523,8 @@ def main(hparams):
     log = print if rank == 0 else (lambda *a, **k: None)
     dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}[hparams["dtype"]]
     model = net.SRModel(hparams["n_rnn_layers"], hparams["rnn_dim"], hparams["n_vocab"], hparams["n_feats"],
-                        hparams["dropout"], hparams["projection_size"], compute_dtype=dtype).cuda()
+                        hparams["dropout"], hparams["projection_size"], compute_dtype=dtype,
+                        norm=hparams.get("norm", "batch"), rnn=hparams.get("rnn", "sru")).cuda()
     log("Num Model Parameters", sum(p.nelement() for p in model.parameters()))
     optimizer = FlatAdam(model.parameters(), lr=hparams["learning_rate"], weight_decay=hparams["weight_decay"],
                          state_bits=hparams.get("optim_bits", 32))
@@ -588,6 +589,8 @@ def parse_args(argv=None):
     p.add_argument("--num_workers", type=int, default=6)
     p.add_argument("--optim_bits", type=int, choices=[32, 8], default=32,
                    help="optimizer state: 32 = fp32 moments, 8 = block-wise 8-bit moments as bitsandbytes Adam8bit (train.py:254)")
+    p.add_argument("--norm", choices=["batch", "group"], default="batch", help="normalisation of the conv blocks (group: per utterance)")
+    p.add_argument("--rnn", choices=["sru", "delta"], default="sru", help="recurrent layers: the reference's SRU or the gated delta rule")
     a = p.parse_args(argv)
     return {
         "datasets": a.datasets, "multiplier": a.multiplier, "batch_size": 32 * a.multiplier,
@@ -596,7 +599,7 @@ def parse_args(argv=None):
         "clip_grad_norm": a.clip_grad_norm, "one_iter": a.one_iter, "projection_size": a.projection_size,
         "synthetic": a.synthetic, "synthetic_clips": a.synthetic_clips, "steps": a.steps,
         "dtype": a.dtype, "checkpoint": a.checkpoint, "resume": a.resume, "eval_dtype": a.eval_dtype,
-        "optim_bits": a.optim_bits, "device": a.device, "manifest_root": a.manifest_root, "ibm_root": a.ibm_root, "num_workers": a.num_workers,
+        "norm": a.norm, "rnn": a.rnn, "optim_bits": a.optim_bits, "device": a.device, "manifest_root": a.manifest_root, "ibm_root": a.ibm_root, "num_workers": a.num_workers,
         "root_map": tuple(tuple(kv.split("=", 1)) for kv in a.root_map.split(",") if kv) or None,
     }
 
