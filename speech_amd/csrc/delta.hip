@@ -28,7 +28,10 @@
 namespace sp {
 
 constexpr int kC = 64;              // frames a chunk
-constexpr int kRecurrentMax = 32;   // frames up to which the recurrent kernel runs (inference)
+// Frames up to which the recurrent kernel runs (inference).  It costs 3 us + 0.95 us a frame for few heads, the two chunked kernels 17 to
+// 20 us for any number up to 64, and their second launch: at 12 frames 14.7 us against 16.6 (8 heads, bf16, dk 64), 14.8 against 20 (dk 128),
+// at 16 frames 18.2 against 17; at 12 frames of 256 heads 24.9 against 21.1, of 512 at dk 128 43 against 38, at 8 frames 31 against 39.
+constexpr int kRecurrentMax = 12;
 constexpr int kLdm = 72;            // row pitch (elements) of a 64 x 64 matrix plane in LDS: 16 rows of 8 bytes fall on distinct banks
 constexpr int kVec = 8;             // per-chunk vectors of 64 floats: aq, ak, kb, beta, rk, sq, G (as 64 doubles)
 constexpr int kTri = 10 * 256;      // a lower triangular 64 x 64 matrix: ten 16 x 16 blocks (row block major), f32
@@ -1016,7 +1019,7 @@ template <typename T> struct FragOf { using type = Frag<Gd<T>::PT>; };
 
 // Two workgroups a CU (16-bit types): one loads while the other multiplies.
 template <typename T, int DK>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void gdr_grads_kernel(GdrArgs a) {
+__global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_grads_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = GradLds<T, DK>;
     using ET = typename Gd<T>::ET;
@@ -1452,8 +1455,13 @@ template <typename K> static int gdr_launch(K kernel, size_t lds, int64_t blocks
     return check_launch(what);
 }
 
-// columns of dv a workgroup of the scans owns: 128 (the head's K, Q and matrices are then staged once), or 64 where that leaves CUs idle
-static bool gdr_wide(const GdrArgs& a) { return a.nsl > 4 && (int64_t)a.B * a.H >= 192; }
+// Columns of dv a workgroup of the scans owns: 128 in eight waves (a head's K, Q and matrices are then staged once), or 64 in four where the
+// eight would leave CUs idle that the four fill: up to 128 heads.  T = 751, bf16, dk 64, dv 128, wide against narrow: 160 heads scan 84 us
+// against 126, reverse scan 182 against 245; 256 heads 98 against 141 and 215 against 264; 64 heads 70 against 59 and 147 against 117.
+// Eight waves have 256 registers each.  Where the tiles do not fit those, the narrow form is the faster one at 256 heads as well: the
+// reverse scan of dk 128 (bf16 400 us against 358, f16 700 against 525) and of f32 (dk 64: 488 against 420; dk 128 exceeds the LDS), the
+// scan of f32 at dk 128 (373 against 358).
+static bool gdr_wide(const GdrArgs& a) { return a.nsl > 4 && (int64_t)a.B * a.H > 128; }
 
 static void gdr_fill(GdrArgs& a, const void* q, const void* k, const void* v, const float* g, const float* beta, const int32_t* lengths,
                      const int64_t* st, int T, int B, int Hk, int H, int dk, int dv, float scale, int flags) {
@@ -1473,17 +1481,21 @@ template <typename T, int DK, int NW, bool TRAIN> static int gdr_scan(const GdrA
 template <typename T, int DK, bool TRAIN> static int gdr_forward(const GdrArgs& a, hipStream_t s) {
     const int rc = gdr_launch(gdr_prep_kernel<T, DK>, PrepLds<T, DK>::bytes, (int64_t)a.B * a.H * a.nc, 256, a, s, "gdr_prep_kernel");
     if (rc) return rc;
-    return gdr_wide(a) ? gdr_scan<T, DK, 8, TRAIN>(a, s) : gdr_scan<T, DK, 4, TRAIN>(a, s);
+    if constexpr (sizeof(T) == 2 || DK == 64)
+        if (gdr_wide(a)) return gdr_scan<T, DK, 8, TRAIN>(a, s);
+    return gdr_scan<T, DK, 4, TRAIN>(a, s);
 }
 template <typename T, int DK, int NW> static int gdr_rscan(const GdrArgs& a, hipStream_t s) {
     return gdr_launch(gdr_rscan_kernel<T, DK, NW>, RscanLds<T, DK, NW>::bytes, (int64_t)a.B * a.H * ((a.nsl + NW - 1) / NW), NW * 64, a, s,
                       "gdr_rscan_kernel");
 }
 template <typename T, int DK> static int gdr_backward(const GdrArgs& a, hipStream_t s) {
-    int rc;
-    if constexpr (sizeof(T) == 4 && DK == 128) rc = gdr_rscan<T, DK, 4>(a, s);      // eight waves' tiles exceed the LDS
-    else rc = gdr_wide(a) ? gdr_rscan<T, DK, 8>(a, s) : gdr_rscan<T, DK, 4>(a, s);
-    if (rc) return rc;
+    const auto walk = [&] {
+        if constexpr (sizeof(T) == 2 && DK == 64)
+            if (gdr_wide(a)) return gdr_rscan<T, DK, 8>(a, s);
+        return gdr_rscan<T, DK, 4>(a, s);
+    };
+    if (const int rc = walk()) return rc;
     return gdr_launch(gdr_grads_kernel<T, DK>, GradLds<T, DK>::bytes, (int64_t)a.B * a.Hk * a.nc, 256, a, s, "gdr_grads_kernel");
 }
 

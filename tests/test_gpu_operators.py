@@ -436,9 +436,9 @@ def test_delta_ragged_shared_heads(cuda, dtype, normalize, bidirectional, state)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("T", [1, 7, 32, 33, 100])
+@pytest.mark.parametrize("T", [1, 7, 12, 13, 32, 33, 100])
 def test_delta_inference_forms_agree(cuda, T, dtype):
-    """Up to 32 frames run the recurrent kernel, more the chunked one; ragged, both directions."""
+    """Up to 12 frames run the recurrent kernel, more the chunked one; ragged, both directions."""
     args, go, gs = delta_inputs(T, 4, 2, 2, 40, 56, dtype, T)
     delta_check(cuda, args, go, gs, [T, 0, T // 2, 1], normalize=True, bidirectional=True, train=False)
 
