@@ -379,9 +379,17 @@ __device__ __forceinline__ void clear_upper(__bf16* t, int planes, int tid, int 
 // ---- prep -----------------------------------------------------------------------------------------------
 template <typename T, int DK> struct PrepLds {
     static constexpr int LDK = DK + 8, LDN = kC + 4;
-    static constexpr size_t in = (size_t)2 * kC * LDK * sizeof(T), mat = (size_t)2 * kC * LDN * 4;
+    static constexpr size_t in = (size_t)2 * kC * LDK * sizeof(T), mat = (size_t)kC * LDN * 4;
     static constexpr size_t bytes = (in > mat ? in : mat) + 4 * 16 * 20 * 4 + kVec * kC * 4;
 };
+
+// block (i, j) of a lower triangular matrix, from the accumulators' layout
+__device__ __forceinline__ void block_store(float* t, int i, int j, f32x4 v) {
+    const int l = threadIdx.x & 63;
+    float* p = t + (i * (i + 1) / 2 + j) * 256 + 64 * (l >> 4) + (l & 15);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[16 * e] = v[e];
+}
 
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
@@ -391,13 +399,13 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
     float* N = reinterpret_cast<float*>(smem);    // over K and Q once their products are done
-    float* P = N + kC * LDN;
     float* Tb = reinterpret_cast<float*>(smem + (L::in > L::mat ? L::in : L::mat));   // [4][16][20]
     float* vec = Tb + 4 * 16 * 20;
     double* G = reinterpret_cast<double*>(vec + kG64 * kC);
     const int c = blockIdx.x % a.nc, bh = blockIdx.x / a.nc, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
     if (c * kC >= w.len) return;
+    const int64_t at = (int64_t)bh * a.nc + c;
     const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TileRegs<T, DK, 256> tk, tq;
     tk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, c * kC, w);
@@ -420,11 +428,16 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     {   // row norms: four lanes a row
         const int row = tid >> 2, part = tid & 3;
         float sk = 0.f, sq = 0.f;
-        if (a.norm)
-            for (int i = part; i < DK; i += 4) {
-                const float kv = to_f(Kl[row * LDK + i]), qv = to_f(Ql[row * LDK + i]);
-                sk += kv * kv; sq += qv * qv;
+        if (a.norm) {
+#pragma unroll
+            for (int i = 0; i < DK / 32; ++i) {
+                T x[8], y[8];
+                __builtin_memcpy(x, __builtin_assume_aligned(Kl + row * LDK + 32 * i + 8 * part, 16), sizeof(x));
+                __builtin_memcpy(y, __builtin_assume_aligned(Ql + row * LDK + 32 * i + 8 * part, 16), sizeof(y));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { sk += to_f(x[e]) * to_f(x[e]); sq += to_f(y[e]) * to_f(y[e]); }
             }
+        }
         sk += __shfl_xor(sk, 1); sk += __shfl_xor(sk, 2);
         sq += __shfl_xor(sq, 1); sq += __shfl_xor(sq, 2);
         if (part == 0) {
@@ -468,7 +481,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
                 qk[m][e] = i >= j ? p : 0.f;
             }
             tile_write(N, LDN, 16 * m, 16 * wave, kk[m]);
-            tile_write(P, LDN, 16 * m, 16 * wave, qk[m]);
+            if (m >= wave) block_store(a.P + at * kTri, m, wave, qk[m]);
         }
     }
     __syncthreads();
@@ -511,18 +524,8 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
             }
             const f32x4 rhs = tile_read(N, LDN, 16 * i, 16 * j) - s;
             X[i] = times(*reinterpret_cast<const f32x4a*>(Tb + i * 16 * 20 + i16 * 20 + 4 * g), rhs, f32x4{0, 0, 0, 0});
+            block_store(a.X + at * kTri, i, j, X[i]);
         }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tile_write(N, LDN, 16 * i, 16 * wave, X[i]);
-    __syncthreads();
-    const int64_t at = (int64_t)bh * a.nc + c;
-    for (int i = tid; i < kTri / 4; i += 256) {
-        const int blk = i >> 6, bi = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, bj = blk - bi * (bi + 1) / 2;
-        const int src = (16 * bi + ((i >> 2) & 15)) * LDN + 16 * bj + 4 * (i & 3);
-        reinterpret_cast<f32x4a*>(a.X + at * kTri)[i] = *reinterpret_cast<const f32x4a*>(N + src);
-        reinterpret_cast<f32x4a*>(a.P + at * kTri)[i] = *reinterpret_cast<const f32x4a*>(P + src);
     }
     float* vo = a.vec + at * kVec * kC;
     for (int i = tid; i < kVec * kC; i += 256) vo[i] = vec[i];
@@ -798,6 +801,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     float rvec[kVec * kC / NT];
     auto fetch = [&](int c) {
         const int64_t at = (int64_t)bh * a.nc + c;
+        state_load(s0n, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col0);
         rk.load(kp, a.ks[0], a.dk, c * kC, w);
         rq.load(qp, a.qs[0], a.dk, c * kC, w);
         rv.load(vp, a.vs[0], vcols, c * kC, w);
@@ -806,7 +810,6 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
         rp.load(a.P + at * kTri);
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
-        state_load(s0n, a.S0 + at * a.dk * a.dv, a.dk, a.dv, col0);
     };
     clear_upper(Xl, 6, tid, NT);
     if (ncl > 0) fetch(ncl - 1);
@@ -1024,7 +1027,10 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
     using L = GradLds<T, DK>;
     using ET = typename Gd<T>::ET;
     constexpr int PT = Gd<T>::PT, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, LDE = L::LDE, NT = DK / 64;
-    constexpr int PE = sizeof(ET) == 2 ? 1 : 3;
+    constexpr int PE = sizeof(ET) == 2 ? 1 : 3, AHEAD = 3;          // pieces of the states in flight or in use
+    // one workgroup a CU: the second half's operands are asked for before the first half's last products (dk 128: 299 us against 319); two
+    // hide that wait for each other, and the registers count (dk 64: 172 against 180)
+    constexpr bool EARLY = PT > 1 || DK > 64;
     T *Ol = reinterpret_cast<T*>(smem), *Dl = Ol + kC * LDV;              // dO, dV
     ET* El = reinterpret_cast<ET*>(Dl + kC * LDV);
     T *Kl = reinterpret_cast<T*>(smem), *Ql = Kl + kC * LDK;              // later
@@ -1082,6 +1088,7 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] = row < a.dk && 32 * kb + 16 * (x & 1) + 4 * g < a.dv ? v[x] : f32x4{0, 0, 0, 0};
         };
+        f32x4 sr[AHEAD][4];
         __syncthreads();
         {
             TileRegs<T, 128, 256> ro, rd;
@@ -1091,13 +1098,14 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
             rd.load((const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, p0, w);
             re.load((const ET*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
             for (int i = tid; i < kVec * kC; i += 256) vec[i] = a.vec[at * kVec * kC + i];
+#pragma unroll
+            for (int i = 0; i + 1 < AHEAD; ++i) state_rows(sr[i], i / 4, i % 4);
+            phase_end();
             ro.store(Ol, LDV, a.dv, p0, w.len);
             rd.store(Dl, LDV, a.dv, p0, w.len);
             re.store(El, LDE, a.dv, 0, kC);
             phase_end();
         }
-        f32x4 sr[2][4];
-        state_rows(sr[0], 0, 0);
         __syncthreads();
         // states: wave = a quarter of dk; U = beta E: its factor goes with the rows
 #pragma unroll
@@ -1107,11 +1115,12 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
             for (int m = 0; m < 4; ++m) { cq[m] = f32x4{0, 0, 0, 0}; ck[m] = cq[m]; cd[m] = cq[m]; }
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                if (kb < 3) state_rows(sr[(kb + 1) & 1], n, kb + 1);
-                else if (n + 1 < NT) state_rows(sr[0], n + 1, 0);
+                const int nx = 4 * n + kb + AHEAD - 1;
+                if (nx < 4 * NT) state_rows(sr[nx % AHEAD], nx / 4, nx % 4);
+                f32x4 (&cur)[4] = sr[(4 * n + kb) % AHEAD];
                 if (kb * 32 < a.dv) {
-                    state_cut(sr[kb & 1], n, kb);
-                    const Frag<OP> sf = split<OP>(sr[kb & 1][0], sr[kb & 1][1]), df = split<OP>(sr[kb & 1][2], sr[kb & 1][3]);
+                    state_cut(cur, n, kb);
+                    const Frag<OP> sf = split<OP>(cur[0], cur[1]), df = split<OP>(cur[2], cur[3]);
                     typename FragOf<T>::type of[4], vf[4];
                     typename FragOf<ET>::type uf[4];
                     row_frags(of, Ol, LDV, 32 * kb);
@@ -1136,6 +1145,16 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
                 tk[m][n] += kb * ck[m] - ak * cd[m];
             }
         }
+        TileRegs<T, DK, 256> rk, rq;
+        float part[8], anchor;                                // the slices' partial sums, all at once: a loop over them waited for each
+        auto load_rest = [&] {
+            rk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, p0, w);
+            rq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, p0, w);
+            const float* parts = wave == 0 ? a.zpart : a.bpart;      // the other waves load along
+#pragma unroll
+            for (int s = 0; s < 8; ++s) part[s] = parts[(min(s, a.nsl - 1) * nat + at) * kC + l];
+            anchor = a.apart[min(l & 7, a.nsl - 1) * nat + at];
+        };
         // M1 = dP * D * sq_i * rk_j (lower), M2 = -dV U^T * D * rk_i * rk_j (strictly lower, made symmetric); wave = block column j
         f32x4 dp[4], dn[4];
 #pragma unroll
@@ -1156,6 +1175,7 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
             }
             phase_end();
         }
+        if (EARLY) { load_rest(); phase_end(); }
         {
             const int j = 16 * wave + i16;
             const float rkj = vec[kRk * kC + j] * vec[kBe * kC + j];
@@ -1177,24 +1197,28 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
         }
         __syncthreads();
         {
-            TileRegs<T, DK, 256> rk, rq;
-            rk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, p0, w);
-            rq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, p0, w);
-            if (wave == 0) {      // dg and dbeta: lane = frame
-                float z = 0.f, be = 0.f, an = 0.f;
-                for (int s = 0; s < a.nsl; ++s) {
-                    z += a.zpart[(s * nat + at) * kC + l];
-                    be += a.bpart[(s * nat + at) * kC + l];
-                    an += a.apart[s * nat + at];
-                }
+            if (!EARLY) load_rest();
+            if (wave == 0) {      // dg: lane = frame
+                float z = 0.f;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) z += s < a.nsl ? part[s] : 0.f;
+                float an = (l & 7) < a.nsl ? anchor : 0.f;
+                an += __shfl_xor(an, 1);
+                an += __shfl_xor(an, 2);
+                an += __shfl_xor(an, 4);
                 if (p0 + l >= w.len) z = 0.f;
 #pragma unroll
                 for (int o = 1; o < 64; o <<= 1) { const float u = __shfl_down(z, o); if (l + o < 64) z += u; }
                 if (p0 + l < w.len) {
                     const int64_t o = w.frame(p0 + l) * gts + bh;
                     a.gg[o] = z + an;
-                    a.gbeta[o] = be;
                 }
+            }
+            if (wave == 1) {      // dbeta
+                float be = 0.f;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) be += s < a.nsl ? part[s] : 0.f;
+                if (p0 + l < w.len) a.gbeta[w.frame(p0 + l) * gts + bh] = be;
             }
             rk.store(Kl, LDK, a.dk, c * kC, w.len);
             rq.store(Ql, LDK, a.dk, c * kC, w.len);
