@@ -96,12 +96,48 @@ template <typename... P> __device__ __forceinline__ void gn_next(GnWalk& w, P&..
 
 // For groups g0 .. g1: sums of part(g, lane, width) over the lanes of a wave, handed to done(g, sum) in one lane.  Waves take the groups in
 // turn: with one thread a group, the walk over 64 partial results alone took 30 us (each load waited for the one before).
+__device__ __forceinline__ float gn_wave_sum(float v) {      // sums over 16 lanes by rotations inside the register, then over the four rows
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x124, 0xf, 0xf, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x122, 0xf, 0xf, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x121, 0xf, 0xf, false));
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
 template <typename A, typename B> __device__ __forceinline__ void gn_group_sums(int g0, int g1, A&& part, B&& done) {
     const int lane = threadIdx.x & 63;
     for (int g = g0 + (int)(threadIdx.x >> 6); g <= g1; g += kGnThreads / 64) {
-        const float v = wave_sum(part(g, lane, 64));
+        const float v = gn_wave_sum(part(g, lane, 64));
         if (lane == 0) done(g, v);
     }
+}
+
+// Sums of every thread's NV values over the rows (threads cpb apart) that hold the same chunk.  They end in red[w * cpb * NV + chunk * NV + i],
+// to be added over the w < (the result) that is returned: one per wave where a wave holds whole rows (sums by lane exchange, one barrier;
+// the tree through LDS that other widths take has eight), one otherwise.
+template <int NV> __device__ __forceinline__ int gn_row_sums(float (&v)[NV], float* red, int cpb, int row, int rows) {
+    if (cpb <= 64 && (cpb & (cpb - 1)) == 0) {
+        for (int o = cpb; o < 64; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o);
+        const int lane = threadIdx.x & 63;
+        if (lane < cpb)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) red[((threadIdx.x >> 6) * cpb + lane) * NV + i] = v[i];
+        __syncthreads();
+        return kGnThreads / 64;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) red[threadIdx.x * NV + i] = v[i];
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if (row < o && row + o < rows) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) red[threadIdx.x * NV + i] += red[(threadIdx.x + o * cpb) * NV + i];
+        }
+        __syncthreads();
+    }
+    return 1;
 }
 
 // ---- block route --------------------------------------------------------------------------------------
@@ -153,39 +189,19 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
             }
         }
         const float inv = cnt ? 1.f / (float)cnt : 0.f;
-        float c_all;
-        if (s.lengths) {
-            __syncthreads();
-            red[threadIdx.x] = (threadIdx.x % cpb == 0 && row < rows) ? (float)cnt : 0.f;
-            __syncthreads();
-            for (int o = kGnThreads / 2; o > 0; o >>= 1) {
-                if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-                __syncthreads();
-            }
-            c_all = red[0];
-        } else {
-            c_all = (float)max(0, hi - lo);
-        }
-        __syncthreads();
-        float mean[VW];
+        // positions below p that are counted: whole bands of len frames and the last one's
+        const auto counted = [&](int p) { return p / s.T * len + min(p % s.T, len); };
+        const float c_all = hi > lo ? (float)(counted(hi) - counted(lo)) : 0.f;
+        float mean[VW], sum[VW];
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
             mean[i] = k[i] + sm[i] * inv;
-            red[threadIdx.x * VW + i] = (float)cnt * mean[i];
+            sum[i] = (float)cnt * mean[i];
             sq[i] -= sm[i] * sm[i] * inv;
             if (sq[i] < 0.f) sq[i] = 0.f;
         }
-        auto tree = [&]() {                                    // sums over the rows, left in row 0's slots
-            __syncthreads();
-            for (int o = 128; o > 0; o >>= 1) {
-                if (row < o && row + o < rows) {
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) red[threadIdx.x * VW + i] += red[(threadIdx.x + o * cpb) * VW + i];
-                }
-                __syncthreads();
-            }
-        };
-        tree();
+        __syncthreads();                                       // the pass before has read its sums
+        const int nw = gn_row_sums<VW>(sum, red, cpb, row, rows);
         // channels of this pass: [cb * VW, cb * VW + cpb * VW); a group may span passes only when VW == 1 (C > 256): see below
         const int c0 = cb * VW, c1 = min(s.C, c0 + cpb * VW);
         const int g0 = c0 / s.Cg, g1 = (c1 - 1) / s.Cg;
@@ -193,7 +209,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
         gn_group_sums(g0, g1, [&](int g, int lane, int width) {
             const int a = max(c0, g * s.Cg), b = min(c1, (g + 1) * s.Cg);
             float m = 0.f;
-            for (int c = a + lane; c < b; c += width) m += red[c - c0];
+            for (int c = a + lane; c < b; c += width)
+                for (int w = 0; w < nw; ++w) m += red[w * cpb * VW + c - c0];
             return m;
         }, [&](int g, float m) { gmean[g - g0] = m * winv / (float)(min(c1, (g + 1) * s.Cg) - max(c0, g * s.Cg)); });
         __syncthreads();
@@ -201,13 +218,14 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
         for (int i = 0; i < VW; ++i) {
             const int c = chunk * VW + i;
             const float d = on ? mean[i] - gmean[c / s.Cg - g0] : 0.f;
-            red[threadIdx.x * VW + i] = on && cnt ? sq[i] + (float)cnt * d * d : 0.f;
+            sum[i] = on && cnt ? sq[i] + (float)cnt * d * d : 0.f;
         }
-        tree();
+        gn_row_sums<VW>(sum, red, cpb, row, rows);
         gn_group_sums(g0, g1, [&](int g, int lane, int width) {
             const int a = max(c0, g * s.Cg), b = min(c1, (g + 1) * s.Cg);
             float m2 = 0.f;
-            for (int c = a + lane; c < b; c += width) m2 += red[c - c0];
+            for (int c = a + lane; c < b; c += width)
+                for (int w = 0; w < nw; ++w) m2 += red[w * cpb * VW + c - c0];
             return m2;
         }, [&](int g, float m2) {
             // slot: one per (sample, split, pass-part of the group)
@@ -235,8 +253,8 @@ __device__ __forceinline__ void gn_merge(const float* __restrict__ part, int n, 
             w += wi;
             m += wi > 0.f ? wi * mi : 0.f;
         }
-        w = wave_sum(w);
-        m = wave_sum(m);
+        w = gn_wave_sum(w);
+        m = gn_wave_sum(m);
         const float inv = w > 0.f ? 1.f / w : 0.f;
         m *= inv;
         float m2 = 0.f;
@@ -244,7 +262,7 @@ __device__ __forceinline__ void gn_merge(const float* __restrict__ part, int n, 
             const float wi = p[(int64_t)i * G * 3], d = p[(int64_t)i * G * 3 + 1] - m, qi = p[(int64_t)i * G * 3 + 2];
             m2 += wi > 0.f ? qi + wi * d * d : 0.f;
         }
-        m2 = wave_sum(m2);
+        m2 = gn_wave_sum(m2);
         if (lane == 0) {
             mean[g] = m;
             rstd[g] = rsqrtf(m2 * inv + eps);
@@ -388,35 +406,30 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(const T* __res
                 }
             }
         }
+        float sums[2 * VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) { sums[i] = sb[i]; sums[VW + i] = sx[i]; }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < VW; ++i) {
-            red[threadIdx.x * VW * 2 + i] = sb[i];
-            red[threadIdx.x * VW * 2 + VW + i] = sx[i];
+        const int nw = gn_row_sums<2 * VW>(sums, red, cpb, row, rows);
+        // the total of a channel's sum q, into the first wave's place
+        for (int c = threadIdx.x; c < cpb * VW * 2; c += kGnThreads) {
+            float t = red[c];
+            for (int w = 1; w < nw; ++w) t += red[w * cpb * VW * 2 + c];
+            red[c] = t;
+            const int ch = cb + c / (2 * VW), q = c / VW & 1;
+            if (ch < nch) cp[(ch * VW + c % VW) * 2 + q] = t;
         }
         __syncthreads();
-        for (int o = 128; o > 0; o >>= 1) {
-            if (row < o && row + o < rows) {
-#pragma unroll
-                for (int i = 0; i < 2 * VW; ++i) red[threadIdx.x * VW * 2 + i] += red[(threadIdx.x + o * cpb) * VW * 2 + i];
-            }
-            __syncthreads();
-        }
-        if (on && row == 0) {
-#pragma unroll
-            for (int i = 0; i < VW; ++i) {
-                cp[(chunk * VW + i) * 2] = red[threadIdx.x * VW * 2 + i];
-                cp[(chunk * VW + i) * 2 + 1] = red[threadIdx.x * VW * 2 + VW + i];
-            }
-        }
     }
-    __syncthreads();   // this workgroup's own global writes are visible to it behind the barrier
+    // per group, weighted with gamma: from LDS where one pass held all channels, else from what the passes wrote (this workgroup's own
+    // global writes, visible to it behind the barrier)
     float* go = gpart + ((int64_t)n * nsplit + split) * s.G * 2;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
         gn_group_sums(0, s.G - 1, [&](int g, int lane, int width) {
             float a = 0.f;
-            for (int c = g * s.Cg + lane; c < (g + 1) * s.Cg; c += width) a += gamma[c] * cp[c * 2 + q];
+            for (int c = g * s.Cg + lane; c < (g + 1) * s.Cg; c += width)
+                a += gamma[c] * (nch <= kGnThreads ? red[(c / VW * 2 + q) * VW + c % VW] : cp[c * 2 + q]);
             return a;
         }, [&](int g, float a) { go[g * 2 + q] = a; });
 }
