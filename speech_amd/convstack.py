@@ -272,6 +272,8 @@ class _StemFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        from .ops import _once
+        _once("the conv stack")
         (spec,) = ctx.saved_tensors
         B, _, Fin, Tin = spec.shape
         gw = torch.zeros((32, 1, 3, 3), dtype=torch.float32, device=spec.device)
@@ -299,15 +301,18 @@ class _Conv3x5Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        from .ops import _once
+        _once("the conv stack")
         x, pb = ctx.saved_tensors
         B, F, T, _ = x.shape
         g = g.contiguous()
         coef = torch.zeros(3 * C, dtype=torch.float32, device=x.device)
         coef[:C].fill_(1.0)
         gw = torch.zeros(ctx.wshape, dtype=torch.float32, device=x.device)
+        ws = torch.empty(CONV_WGRAD_WS_WORDS, dtype=torch.float32, device=x.device)      # its own: captured graphs may run side by side
         with torch.cuda.device(x.device):
             gx = _conv(g, None, None, IN_ID, pb, None, None, None, EPI_NONE, B, F, T)
-            check(lib().sp_conv3x5_wgrad(ptr(x), None, IN_ID, ptr(g), ptr(g), ptr(coef), B, F, T, ptr(_wgrad_workspace(x.device)), ptr(gw),
+            check(lib().sp_conv3x5_wgrad(ptr(x), None, IN_ID, ptr(g), ptr(g), ptr(coef), B, F, T, ptr(ws), ptr(gw),
                                          stream_ptr()), "sp_conv3x5_wgrad")
         return gx, gw
 

@@ -772,8 +772,8 @@ static GnPlan gn_plan(int64_t N, int F, int T, int C, int G, int vw) {
     p.vw = vw;
     while (p.vw > 1 && !(C % p.vw == 0 && (Cg % p.vw == 0 || p.vw % Cg == 0))) p.vw >>= 1;
     const int64_t P = (int64_t)F * T;
-    // ~768 workgroups on the chip (each pays for its reductions: 2048 took 82 / 67 us in the backward's two passes on 61 MB, 768 49 / 43),
-    // at least 32 positions each
+    // ~768 workgroups on the chip, at least 32 positions each.  Each pays for its reductions; the backward's two passes on 61 MB tensors took
+    // 48 + 42 us with 512, 44 + 43 with 768, 46 + 49 with 1024, 49 + 55 with 1536
     int64_t sp = N > 0 ? 768 / N : 1;
     if (sp > kGnMaxSplit) sp = kGnMaxSplit;
     if (sp > (P + 31) / 32) sp = (P + 31) / 32;

@@ -199,6 +199,8 @@ class GatedDeltaLayer(nn.Module):
         super().__init__()
         if n_out % (8 * heads) or dk % 8 or (bidirectional and heads % 2):
             raise ValueError(f"{n_out} outputs do not make {heads} heads of a multiple of 8 (an even number of heads for both directions)")
+        if n_out > 128 * heads or dk > 128:
+            raise ValueError(f"heads are at most 128 wide, got {n_out // heads} (and dk = {dk})")
         self.heads, self.dk, self.dv = heads, dk, n_out // heads
         self.dropout, self.bidirectional, self.site = dropout, bidirectional, site
         self.residual = n_in == n_out
@@ -266,6 +268,10 @@ class GatedDelta(nn.Module):
         # the seed torch was seeded with: data-parallel ranks seed apart (train.main)
         self.register_buffer("dropout_state", torch.tensor([torch.initial_seed() % (1 << 62), 0], dtype=torch.int64))
 
+    def reseed(self, seed):
+        """Data-parallel ranks that load one checkpoint draw different masks again (the step is kept)."""
+        self.dropout_state[0] = seed % (1 << 62)
+
     def forward(self, x, lengths=None):
         for layer in self.layers:
             x, _ = layer(x, self.dropout_state, lengths)
@@ -290,7 +296,8 @@ class SRModel(nn.Module):
         self.resnet_layers = nn.Sequential(*[ResidualBlock(32, 32, t_kernel_s=5, groups=groups) for _ in range(3)])
         n_features = 32 * n_feats // 2
         if rnn == "delta":
-            self.delta_layers = GatedDelta(n_features, 2 * rnn_dim, n_rnn_layers, dropout)
+            heads = 8 * max(1, -(-2 * rnn_dim // 1024))          # eight, or as many times eight as keep them 128 wide
+            self.delta_layers = GatedDelta(n_features, 2 * rnn_dim, n_rnn_layers, dropout, heads)
         else:
             self.sru_layers = SRU(n_features, rnn_dim, n_rnn_layers, dropout=dropout,
                                   projection_size=projection_size, in_layout=(32, n_feats // 2))

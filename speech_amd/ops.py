@@ -922,8 +922,20 @@ def _host_i64(values):
     return (ctypes.c_int64 * len(values))(*values)
 
 
+def _steps(t):
+    """The first three strides; a dimension of size one has none worth keeping (torch leaves any number there, aligned or not)."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())]
+
+
+def _lengths(lengths, n):
+    """int32 [n] on the device, or ValueError."""
+    if tuple(lengths.shape) != (n,) or lengths.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+        raise ValueError(f"lengths must be whole numbers [{n}]")
+    return lengths.to(torch.int32).contiguous()
+
+
 def _gn_strides(tensors):
-    return _host_i64([s for t in tensors for s in (t.stride()[:3] if t is not None else (0, 0, 0))])
+    return _host_i64([s for t in tensors for s in (_steps(t) if t is not None else (0, 0, 0))])
 
 
 @functools.lru_cache(maxsize=256)
@@ -1025,9 +1037,7 @@ def group_norm(x, weight, bias, groups, eps=1e-5, act="none", residual=None, len
     def four(t):
         return None if t is None else t.view(t.shape[0], 1, 1, C) if t.dim() == 2 else t.unsqueeze(1) if t.dim() == 3 else t
     if lengths is not None:
-        if tuple(lengths.shape) != (shape[0],) or lengths.is_floating_point():
-            raise ValueError(f"lengths must be whole numbers [{shape[0]}]")
-        lengths = lengths.to(torch.int32).contiguous()
+        lengths = _lengths(lengths, shape[0])
     x4, r4, code = four(_unit_last(x)), four(_unit_last(residual)), _lib.ACT_CODES[act]
     if _wants_grad(x, weight, bias, residual):
         y = _GroupNormFn.apply(x4, weight, bias, r4, lengths, int(groups), float(eps), code, bool(time_major))
@@ -1100,19 +1110,19 @@ def dropout(x, p, rng, site=0, residual=None, shared=False):
 # ------------------------------------------------------------------------------------------
 # Gated delta rule
 # ------------------------------------------------------------------------------------------
-def _head_rows(t, gates=False):
-    """t as the kernels take it: unit stride inside a head, 16-byte aligned rows (gates: any strides); a copy where it is not."""
-    if gates:
-        return t
+def _head_rows(t):
+    """t as the chunked kernels take it: unit stride inside a head, 16-byte aligned rows, frames at most 2^23 elements apart; a copy where
+    it is not."""
     ve = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % ve == 0 for s in t.stride()[:-1]):
+    st = _steps(t)
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and st[0] <= 1 << 23 and not any(s % ve for s in st):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _gdr_strides(tensors):
-    return _host_i64([s for t in tensors for s in t.stride()[:3]])
+    return _host_i64([s for t in tensors for s in _steps(t)])
 
 
 @functools.lru_cache(maxsize=256)
@@ -1211,9 +1221,7 @@ def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, nor
         raise ValueError(f"both directions need an even number of key heads, not {Hk}")
     if lengths is not None:
         _same_device(q, lengths=lengths)
-        if tuple(lengths.shape) != (B,) or lengths.is_floating_point():
-            raise ValueError(f"lengths must be whole numbers [{B}]")
-        lengths = lengths.to(torch.int32).contiguous()
+        lengths = _lengths(lengths, B)
     scale = dk ** -0.5 if scale is None else float(scale)
     if scale == 0.0 or not math.isfinite(scale):
         raise ValueError(f"scale must be finite and not zero, got {scale}")

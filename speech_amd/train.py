@@ -531,6 +531,8 @@ def main(hparams):
     start_epoch = start_iter = 0
     if hparams.get("resume"):      # weights, and with a full checkpoint the optimizer state, epoch and step count
         start_epoch, start_iter = resume_from(hparams["resume"], model, optimizer)
+        if hparams.get("rnn") == "delta":
+            model.delta_layers.reseed(torch.initial_seed())
     dp = BucketedAllReduce(optimizer) if world > 1 else None
 
     train_loader, sampler, evals = build_loaders(hparams, rank, world)

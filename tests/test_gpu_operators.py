@@ -222,7 +222,7 @@ def test_group_norm_refuses(cuda):
     x, w = torch.zeros(2, 3, 8, device=cuda), torch.ones(8, device=cuda)
     for kw, text in [(dict(groups=3), "groups"), (dict(act="gelu"), "act"), (dict(residual=x[:1]), "residual"), (dict(residual=x.half()), "residual"),
                      (dict(lengths=torch.ones(3, dtype=torch.int64, device=cuda)), "lengths"), (dict(lengths=torch.ones(2, device=cuda)), "lengths"),
-                     (dict(lengths=torch.ones(2, dtype=torch.int64)), "lengths is on"), (dict(weight=w[:4]), "weight"), (dict(x=x.int()), "float"),
+                     (dict(lengths=torch.ones(2, dtype=torch.bool, device=cuda)), "lengths"), (dict(lengths=torch.ones(2, dtype=torch.int64)), "lengths is on"), (dict(weight=w[:4]), "weight"), (dict(x=x.int()), "float"),
                      (dict(x=x[0, 0]), "must be"), (dict(bias=w.cpu()), "bias is on")]:
         a = dict(x=x, weight=w, bias=w, groups=2)
         a.update(kw)
@@ -559,6 +559,7 @@ def test_delta_refuses(cuda):
                      (dict(beta=g.long()), "g and beta"), (dict(state=s.half()), "state"), (dict(state=s[:1]), "state"), (dict(scale=0.0), "scale"),
                      (dict(scale=float("nan")), "scale"), (dict(lengths=torch.ones(3, dtype=torch.int32, device=cuda)), "lengths"),
                      (dict(lengths=torch.ones(2, device=cuda)), "lengths"), (dict(lengths=torch.ones(2, dtype=torch.int32)), "lengths is on"),
+                     (dict(lengths=torch.ones(2, dtype=torch.bool, device=cuda)), "lengths"),
                      (dict(q=torch.zeros(4, 2, 2, 12, device=cuda), k=torch.zeros(4, 2, 2, 12, device=cuda)), "multiples of 8"),
                      (dict(q=q[:, :, :1], k=q[:, :, :1], bidirectional=True), "even"), (dict(state=s.cpu()), "state is on")]:
         a = dict(q=q, k=q, v=v, g=g, beta=g)
@@ -588,6 +589,41 @@ def test_delta_repeats_bit_for_bit(cuda):
         out = [o.detach(), f.detach(), *torch.autograd.grad([o, f], xs, [go.to(cuda), gs.to(cuda)])]
         first = first or out
         assert all(torch.equal(u, v) for u, v in zip(out, first))
+
+
+def test_delta_strides_of_size_one_and_far_frames(cuda):
+    """A dimension of size one may carry any stride; frames may lie far apart: the same numbers as from dense tensors."""
+    from speech_amd import ops
+    base = torch.randn(4000, device=cuda)
+    q, k = (base.as_strided((1, 1, 2, 16), (33, 35, 16, 1), o) for o in (0, 40))
+    v = base.as_strided((1, 1, 2, 24), (7, 5, 24, 1), 100)
+    g, beta = -torch.rand(1, 1, 2, device=cuda), torch.rand(1, 1, 2, device=cuda)
+    for train in (False, True):
+        a = [t.detach().requires_grad_(train) for t in (q, k, v, g, beta)]
+        b = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_(train) for t in (q, k, v, g, beta)]
+        (o, f), (p, e) = ops.gated_delta_rule(*a, normalize=True), ops.gated_delta_rule(*b, normalize=True)
+        assert torch.equal(o, p) and torch.equal(f, e)
+        if train:
+            assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(o.sum(), a), torch.autograd.grad(p.sum(), b)))
+    far = torch.zeros(20, (1 << 23) + 8, device=cuda)
+    q = far[:, :32].view(20, 1, 2, 16)
+    q.copy_(torch.randn(20, 1, 2, 16, device=cuda))
+    v, g, beta = torch.randn(20, 1, 2, 24, device=cuda), -torch.rand(20, 1, 2, device=cuda), torch.rand(20, 1, 2, device=cuda)
+    for n in (20, 5):
+        x = ops.gated_delta_rule(q[:n], q[:n], v[:n], g[:n], beta[:n], normalize=True)
+        y = ops.gated_delta_rule(q[:n].clone(), q[:n].clone(), v[:n], g[:n], beta[:n], normalize=True)
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+
+
+def test_group_norm_without_frames(cuda):
+    from speech_amd import ops
+    x = torch.zeros(2, 0, 8, device=cuda, requires_grad=True)
+    w, b = torch.ones(8, device=cuda, requires_grad=True), torch.zeros(8, device=cuda, requires_grad=True)
+    y = ops.group_norm(x, w, b, 2, act="silu")
+    gx, gw, gb = torch.autograd.grad(y.sum(), [x, w, b])
+    assert y.shape == x.shape == gx.shape and not gw.any() and not gb.any()
+    one = torch.randn(3, 1, 1, 8, device=cuda).as_strided((3, 1, 1, 8), (8, 3, 5, 1))
+    assert torch.equal(ops.group_norm(one, w, b, 2), ops.group_norm(one.clone(memory_format=torch.contiguous_format), w, b, 2))
 
 
 # ------------------------------------------------------------------------------------------ streams, graphs, the operators together
@@ -649,6 +685,15 @@ def test_layer_against_plain_torch(cuda):
     for name, u_, w_ in [("y", y, ref), ("final", final, rf)] + list(zip(("x", *names), got, want)):
         e = float((u_.detach().double().cpu() - w_.detach()).norm() / w_.detach().norm())
         assert e <= 2048 * 2.0 ** -24, (name, e)
+
+
+def test_stack_is_not_twice_differentiable(cuda):
+    from speech_amd import net
+    m = net.SRModel(1, 64, 28, 80, 0.0, norm="group", rnn="delta").to(cuda).train()
+    loss = m(torch.rand(1, 1, 80, 20, device=cuda)).sum()
+    for p in (m.cnn.weight, m.resnet_layers[0].conv1.weight):
+        with pytest.raises(RuntimeError, match="twice"):
+            torch.autograd.grad(loss, p, create_graph=True)
 
 
 def test_graph_capture(cuda):

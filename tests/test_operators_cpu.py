@@ -125,6 +125,20 @@ def test_model_variants_check_their_arguments():
     assert not any(k.startswith("delta") for k in net.SRModel(2, 64, 28, 80, 0.1).state_dict())
 
 
+def test_delta_layers_refuse_wide_heads_and_reseed():
+    from speech_amd import net
+    with pytest.raises(ValueError, match="at most 128 wide"):
+        net.GatedDeltaLayer(64, 2048, heads=8)
+    with pytest.raises(ValueError, match="at most 128 wide"):
+        net.GatedDeltaLayer(64, 1024, heads=8, dk=136)
+    assert net.SRModel(1, 1024, 28, 80, 0.0, rnn="delta").delta_layers.layers[0].heads == 16
+    m = net.GatedDelta(64, 64, 1, 0.1)
+    m.dropout_state[1] = 7
+    m.load_state_dict(net.GatedDelta(64, 64, 1, 0.1).state_dict())          # another rank's seed and step
+    m.reseed(12345)
+    assert m.dropout_state.tolist() == [12345, 0]
+
+
 def test_train_flags():
     from speech_amd import train
     hp = train.parse_args(["--synthetic", "--norm", "group", "--rnn", "delta"])
