@@ -130,13 +130,13 @@ class _Here:
         return False
 
 
-_HERE = _Here()
+_CURRENT = _Here()
 
 
 def on_device(t):
     """Context in which t's device is the current one."""
     import torch
-    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _CURRENT if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def raw_stream(t):
@@ -158,4 +158,3 @@ def ptr(t):
 def dtype_code(t):
     import torch
     return {torch.float32: SP_F32, torch.float16: SP_F16, torch.bfloat16: SP_BF16}[t.dtype]
-
