@@ -376,7 +376,14 @@ __device__ __forceinline__ void clear_upper(__bf16* t, int planes, int tid, int 
     }
 }
 
+// Measured below at T = 751, 256 heads (32 x 8), dk 64, dv 128, bf16, normalised, both directions, unless another shape is named.
+
 // ---- prep -----------------------------------------------------------------------------------------------
+// A workgroup forms N, P, the inverse's X and the chunk's vectors for one (head, chunk): 3072 workgroups, 44 us (94 MB: 2.1 TB/s).  Bound by
+// its chain of dependent steps (loads, prefix sum, norms, products, substitution), not by bytes or rate: so little LDS (26 KB) and few
+// registers (92) that five workgroups share a CU and fill each other's waits; with N and P both kept in LDS it was three, and 53 us.
+// X by blocks of 16: the four diagonal blocks of (I + N diag(beta))^-1 by substitution, one a wave, the blocks below them by products on the
+// f32 matrix instruction: the inverse multiplies everything behind it, and bf16 parts would have to be formed of each intermediate block.
 template <typename T, int DK> struct PrepLds {
     static constexpr int LDK = DK + 8, LDN = kC + 4;
     static constexpr size_t in = (size_t)2 * kC * LDK * sizeof(T), mat = (size_t)kC * LDN * 4;
@@ -613,8 +620,11 @@ template <int P> __device__ __forceinline__ void row_operands(Frag<P> (&f)[2], c
 }
 
 // A wave owns 16 columns of dv: the state's columns, U's, O's.  Only K, Q, X, P and the vectors are shared (LDS, filled a chunk ahead
-// through registers); two barriers a chunk.  A wave whose columns lie behind dv works on zeros
-// and writes nothing.
+// through registers); two barriers a chunk.  A wave whose columns lie behind dv works on zeros and writes nothing: as many steps as the
+// others, and no branch around the matrix instructions.
+// 98 us, 12 chunks in turn: 8 us a chunk, of which the matrix pipes are busy 18 %.  Bound by the chain of four dependent products a chunk
+// (K S, X, P, K^T U) at two waves a SIMD; the states are the only thing that could be split further, and every split loads K, Q, X and P
+// again.  Inference at dk 128 (T = 1501, 128 heads, one wave a SIMD): 132 us, 24 chunks.
 template <typename T, int DK, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -763,6 +773,10 @@ template <typename T, int DK, int NW> struct RscanLds {
 
 // E and O are formed again from the state at the chunk's start: 36 + 84 more matrix instructions a wave and chunk instead of 100 KB more
 // traffic a chunk (E in f32 and the rest of O that its rounding dropped, written by the forward and read back).
+// 211 us, 17.5 us a chunk (f32 at 30 heads, dk 40, dv 72, 301 frames: 76 us): 246 matrix instructions a wave and chunk keep the pipes busy 18 %
+// of the time, the waves issue in 29 % of their cycles, 400 MB move.  Bound by latency at two waves a SIMD, which 256 registers a lane allow: without
+// the next chunk's loads 157 us (they find registers only at the chunk's end), without the stores 211.
+// Measured and not kept: those loads earlier (they spill), their lines touched into the L2 cache a chunk ahead (230 us).
 template <typename T, int DK, int NW>
 __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -1020,7 +1034,11 @@ template <int P> __device__ __forceinline__ void plane_write_t(__bf16* t, int r0
 
 template <typename T> struct FragOf { using type = Frag<Gd<T>::PT>; };
 
-// Two workgroups a CU (16-bit types): one loads while the other multiplies.
+// One workgroup a (key head, chunk), its value heads in turn: shared heads' gradients are sums in registers, in a fixed order.  A wave owns a
+// quarter of dk in the products with the states and 16 columns j of the 64 x 64 products.  172 us: 317 MB at 1.8 TB/s, matrix pipes busy 8 %:
+// bound by the waits between its six phases.  Two workgroups a CU for bf16 at dk 64 (one: 287 us against 203 when this was measured); elsewhere
+// 256 registers do not hold the tiles and one workgroup with 512 is faster (then bf16, dk 128: 387 us against 405; f16 dk 64 377 / 401, dk 128
+// 522 / 628).
 template <typename T, int DK>
 __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_grads_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -1324,6 +1342,8 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
 }
 
 // ---- recurrent form -------------------------------------------------------------------------------------
+// One frame of 512 heads of 128 x 128: 14.6 us, 67 MB of state read and written at 4.6 TB/s, HBM-bound.  One frame of 8 heads: 4.9 us, of
+// which an empty launch is 3.5; each further frame 0.95 us, one reduction over LDS.
 // Few frames: a workgroup owns 32 columns of one head's state, in registers: 8 lanes x 4 columns a row, 32 row groups of four rows.  All
 // frames' keys, queries, values and gates are brought to LDS first (a frame's global loads inside the loop cost 1.7 us a frame), with the
 // three products of k and q that do not need the state.  One reduction a frame then: k.S and q.S come from the state before the frame, and

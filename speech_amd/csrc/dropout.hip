@@ -7,6 +7,8 @@
 // share beyond what the memory time hides; the rate is then honoured to 2^-17 (documented, the scale follows the honoured rate).
 // A thread owns one counter (eight elements, 16 or 32 bytes) and, in the shared form, walks that counter's elements down the rows: the
 // generator runs once for all of them.
+// Measured at 24032 x 1024 bf16: with a residual 23.4 us (147 MB at 6.3 TB/s), without (the backward) 20.3 us (98 MB at 4.8 TB/s: here the
+// products show).
 #include "common.h"
 
 namespace sp {

@@ -5,7 +5,10 @@
 // the conv stack's blocks (the reference normalises those over the batch, net.py:24-25) and of a recurrent layer's output.
 //
 // HBM-bound: forward reads x (and the residual) and writes y; the statistics need x before the first output, so x is read twice -- the
-// second time from the Infinity Cache at the conv stack's size (61 MB).  Two routes, chosen by the shape alone:
+// second time from the Infinity Cache at the conv stack's size (61 MB).  The backward reads gy, x and the residual twice for the same reason.
+// Measured at [32][40][751][32] bf16 with SiLU and residual: statistics 17 us, apply 32 (5.8 TB/s), backward statistics 44 (5.6), backward
+// apply 43 (5.7); rows, 24032 x 1024 bf16, 8 groups: forward 22 us (4.5 TB/s), backward 36 (4.1) + 7.4 for the parameters' gradients.
+// Two routes, chosen by the shape alone:
 //   rows    one position a sample (F * T == 1): a (sample, group) is a contiguous segment that a team of lanes holds in registers; one
 //           read, one write, two-pass statistics.
 //   blocks  everything else: a statistics kernel over (sample, split) and an apply kernel that merges the splits' partials itself.

@@ -934,8 +934,19 @@ def _lengths(lengths, n):
     return lengths.to(torch.int32).contiguous()
 
 
-def _gn_strides(tensors):
-    return _host_i64([s for t in tensors for s in (_steps(t) if t is not None else (0, 0, 0))])
+@functools.lru_cache(maxsize=1024)
+def _stride_block(*layout):
+    """The kernels' stride table of tensors given as (shape, stride, shape, stride, ...); (None, None) for one that is not there.  Kept:
+    building it costs more than a small kernel's launch."""
+    return _host_i64([s for shape, st in zip(layout[::2], layout[1::2])
+                      for s in ((0, 0, 0) if shape is None else [a if n > 1 else 0 for n, a in zip(shape[:3], st)])])
+
+
+def _strides(*tensors):
+    layout = []
+    for t in tensors:
+        layout += (None, None) if t is None else (t.shape, t.stride())
+    return _stride_block(*layout)
 
 
 @functools.lru_cache(maxsize=256)
@@ -955,7 +966,7 @@ def _gn_fwd(x, w32, b32, residual, lengths, groups, eps, act, time_major, train)
     n = _gn_workspace(N, F, T, C, groups, 0)
     ws = x.new_empty(n, dtype=torch.uint8) if n else None
     with on_device(x):
-        rc = lib().sp_groupnorm_fwd(x.data_ptr(), addr(residual), w32.data_ptr(), b32.data_ptr(), addr(lengths), _gn_strides((x, residual, y)),
+        rc = lib().sp_groupnorm_fwd(x.data_ptr(), addr(residual), w32.data_ptr(), b32.data_ptr(), addr(lengths), _strides(x, residual, y),
                                     N, F, T, C, groups, eps, act, _CODE[x.dtype], y.data_ptr(), mean,
                                     mean + 4 * N * groups if train else None, addr(ws), n, raw_stream(x))
     check(rc, "sp_groupnorm_fwd")
@@ -999,7 +1010,7 @@ class _GroupNormFn(torch.autograd.Function):
         ws = x.new_empty(n, dtype=torch.uint8)
         with on_device(x):
             rc = lib().sp_groupnorm_bwd(gy.data_ptr(), x.data_ptr(), addr(residual), w32.data_ptr(), b32.data_ptr(), mean,
-                                        mean + 4 * N * groups, addr(lengths), _gn_strides((gy, x, residual, gx, gres)), N, F, T, C, groups, act,
+                                        mean + 4 * N * groups, addr(lengths), _strides(gy, x, residual, gx, gres), N, F, T, C, groups, act,
                                         int(direct), _CODE[x.dtype], gx.data_ptr(), addr(gres), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), n,
                                         raw_stream(x))
         check(rc, "sp_groupnorm_bwd")
@@ -1121,10 +1132,6 @@ def _head_rows(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _gdr_strides(tensors):
-    return _host_i64([s for t in tensors for s in _steps(t)])
-
-
 @functools.lru_cache(maxsize=256)
 def _gdr_bytes(T, B, Hk, H, dk, dv, code, which):
     """which: 0 workspace of the forward, 1 of the backward, 2 what the forward keeps for the backward."""
@@ -1153,7 +1160,7 @@ class _GatedDeltaFn(torch.autograd.Function):
     def forward(ctx, q, k, v, g, beta, state, lengths, dims, scale, flags):
         T, B, Hk, H, dk, dv = dims
         final = g.new_empty((B, H, dk, dv))
-        o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _gdr_strides((q, k, v, g, beta)), scale, flags, True)
+        o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _strides(q, k, v, g, beta), scale, flags, True)
         ctx.save_for_backward(q, k, v, g, beta, lengths, o, saved)
         ctx.cfg = (dims, scale, flags)
         ctx.set_materialize_grads(False)
@@ -1176,7 +1183,7 @@ class _GatedDeltaFn(torch.autograd.Function):
         ws = saved.new_empty(n)
         with on_device(q):
             rc = lib().sp_gdr_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), addr(lengths),
-                                  _gdr_strides((q, k, v, g, beta, go)), T, B, Hk, H, dk, dv, scale, flags, code, o.data_ptr(), saved.data_ptr(),
+                                  _strides(q, k, v, g, beta, go), T, B, Hk, H, dk, dv, scale, flags, code, o.data_ptr(), saved.data_ptr(),
                                   saved.numel(), go.data_ptr(), addr(gstate), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), gg.data_ptr(),
                                   gb.data_ptr(), addr(gs0), ws.data_ptr(), n, raw_stream(q))
         check(rc, "sp_gdr_bwd")
@@ -1238,7 +1245,7 @@ def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, nor
     if _wants_grad(q, k, v, g, beta, state):
         return _GatedDeltaFn.apply(q, k, v, g, beta, state, lengths, dims, scale, flags)
     final = g.new_empty((B, H, dk, dv))
-    o, _ = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _gdr_strides((q, k, v, g, beta)), scale, flags, False)
+    o, _ = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _strides(q, k, v, g, beta), scale, flags, False)
     return o, final
 
 
