@@ -379,7 +379,7 @@ __device__ __forceinline__ void clear_upper(__bf16* t, int planes, int tid, int 
 // Measured below at T = 751, 256 heads (32 x 8), dk 64, dv 128, bf16, normalised, both directions, unless another shape is named.
 
 // ---- prep -----------------------------------------------------------------------------------------------
-// A workgroup forms N, P, the inverse's X and the chunk's vectors for one (head, chunk): 3072 workgroups, 44 us (94 MB: 2.1 TB/s).  Bound by
+// A workgroup forms N, P, the inverse's X and the chunk's vectors for one (head, chunk): 44 us (94 MB: 2.1 TB/s).  Bound by
 // its chain of dependent steps (loads, prefix sum, norms, products, substitution), not by bytes or rate: so little LDS (26 KB) and few
 // registers (92) that five workgroups share a CU and fill each other's waits; with N and P both kept in LDS it was three, and 53 us.
 // X by blocks of 16: the four diagonal blocks of (I + N diag(beta))^-1 by substitution, one a wave, the blocks below them by products on the
