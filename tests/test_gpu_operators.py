@@ -901,3 +901,59 @@ def test_conv_functions_of_the_group_stack(cuda):
     close(y, ref, float(ref.detach().abs().max()), 16)
     for u, v in zip(torch.autograd.grad(y, leaves, gy.to(cuda)), torch.autograd.grad(ref, r, gy.double())):
         close(u, v, float(v.abs().max()), 836, torch.float32)
+
+
+def test_concurrent_streams(cuda):
+    """Two streams run training passes of the layer at the same time: no workspace is shared, each gets the results of a run alone."""
+    from speech_amd import ops
+    layer, x = _layer(cuda)
+    gy = torch.randn_like(x)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    inputs = [x, torch.randn_like(x)]
+
+    def run(xv, seed):
+        xl = xv.clone().requires_grad_(True)
+        y, f = layer(xl, ops.dropout_rng(seed, cuda))
+        return [y.detach(), f.detach(), torch.autograd.grad(y, xl, gy)[0]]
+    want = [run(v, i) for i, v in enumerate(inputs)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(inputs[i], i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for g in got[i]:
+            assert all(torch.equal(u, w) for u, w in zip(g, want[i]))
+
+
+def test_variant_trains_resumes_and_evaluates_from_the_commands(cuda, tmp_path, monkeypatch):
+    """`--norm group --rnn delta` through train.main (synthetic clips), its checkpoint through --resume and through
+    scripts/eval_dataset's model construction."""
+    import wave
+    from speech_amd import train
+    from speech_amd.scripts import eval_dataset as ev
+    monkeypatch.delenv("WORLD_SIZE", raising=False)
+    ckpt = tmp_path / "variant.pth"
+    args = ["--one_iter", "--synthetic", "--synthetic_clips", "16", "--steps", "2", "--multiplier", "1", "--num_workers", "0", "--norm", "group",
+            "--rnn", "delta", "--dtype", "bf16", "--checkpoint", str(ckpt)]
+    hp = train.parse_args(args)
+    hp.update(batch_size=4, n_rnn_layers=2, rnn_dim=64)
+    assert np.isfinite(train.main(hp))
+    hp = train.parse_args(args + ["--resume", str(ckpt)])
+    hp.update(batch_size=4, n_rnn_layers=2, rnn_dim=64, epochs=2, one_iter=False)
+    assert torch.load(ckpt, weights_only=True)["model_state_dict"]["delta_layers.dropout_state"].tolist() == [7, 2]
+    assert np.isfinite(train.main(hp))
+    ibm = tmp_path / "ibm"
+    ibm.mkdir()
+    rs = np.random.RandomState(4)
+    for k in range(3):
+        with wave.open(str(ibm / f"i{k}.wav"), "wb") as f:
+            f.setnchannels(1); f.setsampwidth(2); f.setframerate(16000)
+            f.writeframes((rs.randn(6000 + 300 * k) * 2500).clip(-32768, 32767).astype("<i2").tobytes())
+        (ibm / f"i{k}.txt").write_text("ibm line")
+    for dtype in ("fp16", "fp32"):
+        cer, _ = ev.main(["False", "ibm", str(ckpt), "--ibm_root", str(ibm), "--n_rnn_layers", "2", "--rnn_dim", "64", "--batch_size", "2",
+                          "--num_workers", "0", "--norm", "group", "--rnn", "delta", "--dtype", dtype], log=lambda *a: None)
+        assert np.isfinite(cer)
