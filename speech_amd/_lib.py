@@ -120,32 +120,6 @@ def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-class _Here:
-    """Stands in for torch.cuda.device(d) where d is current already: entering that costs more than a small kernel's launch."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_CURRENT = _Here()
-
-
-def on_device(t):
-    """Context in which t's device is the current one."""
-    import torch
-    return _CURRENT if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def raw_stream(t):
-    """The current stream of t's device as the integer the C ABI takes (inside on_device(t))."""
-    import torch
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # what torch's own generated code uses: 0.1 us against 2.6
-    return get(t.get_device()) if get is not None else torch.cuda.current_stream(t.device).cuda_stream
-
-
 def addr(t):
     """A tensor's address as the integer the C ABI takes, None for none."""
     return None if t is None else t.data_ptr()

@@ -11,7 +11,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import addr, check, lib, on_device, ptr, raw_stream, stream_ptr
+from ._lib import addr, check, lib, ptr, stream_ptr
 
 HOP = 160
 N_FFT = 400
@@ -885,6 +885,30 @@ def sru_layer(x, ln_w, ln_b, weight, wc, bias, mask, d, k, C=1, eps=1e-5, pre=No
 # ------------------------------------------------------------------------------------------
 # Group normalisation with an activation, channels last
 # ------------------------------------------------------------------------------------------
+class _Here:
+    """Stands in for torch.cuda.device(d) where d is current already: entering that costs more than a small kernel's launch."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_CURRENT = _Here()
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # what torch's own generated code uses: 0.1 us against 2.6
+
+
+def on_device(t):
+    """Context in which t's device is the current one."""
+    return _CURRENT if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def raw_stream(t):
+    """The current stream of t's device as the integer the C ABI takes (inside on_device(t))."""
+    return _RAW_STREAM(t.get_device()) if _RAW_STREAM is not None else torch.cuda.current_stream(t.device).cuda_stream
+
+
 def _same_device(x, **others):
     dev = x.device
     for name, t in others.items():
@@ -974,8 +998,7 @@ def _gn_fwd(x, w32, b32, residual, lengths, groups, eps, act, time_major, train)
 
 
 def _f32_param(p):
-    p = p.detach()
-    return p if p.dtype == torch.float32 and p.is_contiguous() else p.float().contiguous()
+    return p if p.dtype == torch.float32 and p.is_contiguous() else p.detach().float().contiguous()
 
 
 class _GroupNormFn(torch.autograd.Function):
@@ -1190,26 +1213,36 @@ class _GatedDeltaFn(torch.autograd.Function):
         return gq, gk, gv, gg, gb, gs0, None, None, None, None
 
 
-def _gdr_check(q, k, v, g, beta, state, lead):
-    _act_tensor(q, "q")
-    if q.dim() != len(lead) + 2 or k.shape != q.shape or v.dim() != q.dim() or v.shape[:-2] != q.shape[:-2]:
-        raise ValueError(f"q and k must be [{', '.join(lead)}, Hk, dk] and v [{', '.join(lead)}, H, dv], got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError("q, k and v must have one dtype")
-    Hk, dk = q.shape[-2:]
-    H, dv = v.shape[-2:]
+@functools.lru_cache(maxsize=1024)
+def _gdr_dims(lead, q, k, v, g, beta, state):
+    """The shapes' check, kept by shape (a call that raises is not): a single token's call is shorter than it."""
+    if len(q) != len(lead) + 2 or k != q or len(v) != len(q) or v[:-2] != q[:-2]:
+        raise ValueError(f"q and k must be [{', '.join(lead)}, Hk, dk] and v [{', '.join(lead)}, H, dv], got {tuple(q)}, {tuple(k)} and {tuple(v)}")
+    Hk, dk = q[-2:]
+    H, dv = v[-2:]
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{H} value heads do not share {Hk} key heads evenly")
     if not (8 <= dk <= 128 and dk % 8 == 0 and 8 <= dv <= 128 and dv % 8 == 0):
         raise ValueError(f"head widths must be multiples of 8 up to 128, got dk={dk}, dv={dv}")
-    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1] or not g.is_floating_point() or not beta.is_floating_point():
+    if g != v[:-1] or beta != v[:-1]:
         raise ValueError(f"g and beta must be floating point [{', '.join(lead)}, H]")
-    B = q.shape[-3]
-    if state is not None and (tuple(state.shape) != (B, H, dk, dv) or state.dtype != torch.float32):
+    B = q[-3]
+    if state is not None and state != (B, H, dk, dv):
         raise ValueError(f"state must be float32 {(B, H, dk, dv)}")
-    _same_device(q, k=k, v=v, g=g, beta=beta, state=state)
     return B, Hk, dk, H, dv
+
+
+def _gdr_check(q, k, v, g, beta, state, lead):
+    _act_tensor(q, "q")
+    dims = _gdr_dims(lead, q.shape, k.shape, v.shape, g.shape, beta.shape, None if state is None else state.shape)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one dtype")
+    if not g.is_floating_point() or not beta.is_floating_point():
+        raise ValueError(f"g and beta must be floating point [{', '.join(lead)}, H]")
+    if state is not None and state.dtype != torch.float32:
+        raise ValueError(f"state must be float32 {tuple(state.shape)}")
+    _same_device(q, k=k, v=v, g=g, beta=beta, state=state)
+    return dims
 
 
 def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, normalize=False, bidirectional=False):
@@ -1249,7 +1282,12 @@ def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, nor
     return o, final
 
 
-@torch.no_grad()
+@functools.lru_cache(maxsize=1024)
+def _step_strides(*strides):
+    """One frame: no step from frame to frame."""
+    return _host_i64([s for st in strides for s in (0, *st[:2])])
+
+
 def gated_delta_step(q, k, v, g, beta, state, scale=None, normalize=False):
     """One frame of gated_delta_rule for serving: q, k [B, Hk, dk], v [B, H, dv], g, beta [B, H] -> o [B, H, dv]; `state` (float32,
     contiguous [B, H, dk, dv]) is updated in place.  Not differentiable."""
@@ -1264,6 +1302,13 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None, normalize=False):
     if B == 0:
         return torch.zeros_like(v)
     q, k, v, g, beta = _unit_last(q), _unit_last(k), _unit_last(v), g.float(), beta.float()
-    strides = _host_i64([s for t in (q, k, v, g, beta) for s in (0, *t.stride()[:2])])       # one frame: no step from frame to frame
-    o, _ = _gdr_fwd(q, k, v, g, beta, state, state, None, (1, B, Hk, H, dk, dv), strides, scale, _lib.GDR_NORMALIZE if normalize else 0, False)
-    return o[0]
+    strides = _step_strides(q.stride(), k.stride(), v.stride(), g.stride(), beta.stride())
+    o = v.new_empty((B, H, dv))
+    with on_device(q):
+        rc = lib().sp_gdr_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(), None, strides, 1, B, Hk, H,
+                              dk, dv, scale, _lib.GDR_NORMALIZE if normalize else 0, _CODE[q.dtype], o.data_ptr(), state.data_ptr(), None, 0, None,
+                              0, raw_stream(q))
+    check(rc, "sp_gdr_fwd")
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)       # whoever saved the state for a backward pass is told
+    return o

@@ -551,6 +551,24 @@ def test_delta_step(cuda, dtype, B, Hk, r, dk, dv):
     close(out, ro, float(ro.abs().max()), 64 * 6)
 
 
+def test_delta_step_tells_autograd_of_the_new_state(cuda):
+    from speech_amd import ops
+    args, _, _ = delta_inputs(1, 2, 2, 1, 16, 16, torch.float32, 7)
+    q, k, v, g, beta, state = (t.to(cuda) for t in args)
+    w = torch.ones_like(state, requires_grad=True)
+    loss = (w * state).sum()                                 # saves the state
+    ops.gated_delta_step(q[0], k[0], v[0], g[0], beta[0], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        s = state.clone()
+        a = ops.gated_delta_step(q[0], k[0], v[0], g[0], beta[0], s)
+    b = ops.gated_delta_step(q[0], k[0], v[0], g[0], beta[0], state)
+    assert torch.equal(a, b) and torch.equal(s, state)
+    o = ops.gated_delta_step(q[0].requires_grad_(True), k[0], v[0], g[0].requires_grad_(True), beta[0], state)
+    assert not o.requires_grad and not state.requires_grad
+
+
 def test_delta_refuses(cuda):
     from speech_amd import ops
     q, v, g = torch.zeros(4, 2, 2, 16, device=cuda), torch.zeros(4, 2, 4, 24, device=cuda), torch.zeros(4, 2, 4, device=cuda)
