@@ -240,10 +240,6 @@ template <int P, int A, int B> __device__ __forceinline__ void tri_rows(Frag<P> 
 #pragma unroll
     for (int x = A; x < B; ++x) f[x] = plane_rows<P>(t, 16 * tri_m(x), 32 * tri_k(x));
 }
-template <int P, int A, int B> __device__ __forceinline__ void tri_cols(Frag<P> (&f)[6], const __bf16* t) {
-#pragma unroll
-    for (int x = A; x < B; ++x) f[x] = plane_cols<P>(t, 32 * (1 - tri_k(x)), 16 * (3 - tri_m(x)));
-}
 
 // a 16 x 16 tile in the accumulators' layout: lane (i, g) holds rows r0 + 4g .. +3 of column c0 + i
 __device__ __forceinline__ f32x4 tile_read(const __hip_bfloat16* t, int ld, int r0, int c0) {

@@ -78,7 +78,6 @@ struct GnWalk {
     int p, hi, step, t, dt, T;
     __device__ __forceinline__ GnWalk(int p_, int hi_, int step_, int T_) : p(p_), hi(hi_), step(step_), t(p_ % T_), dt(step_ % T_), T(T_) {}
     __device__ __forceinline__ bool more() const { return p < hi; }
-    __device__ __forceinline__ bool all(int n) const { return p + (n - 1) * step < hi; }
 };
 struct GnPos {          // offsets of one tensor along a walk
     int64_t off, inc, wrap, first;
