@@ -401,7 +401,8 @@ int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period
  * [0, T] are clamped): frames behind an utterance's end are not read, leave the state alone and come out as zeros.  SP_GDR_BIDIRECTIONAL:
  * value heads h >= H / 2 walk each utterance's own frames backwards (Hk even).  o: [T][B][H][dv] dense.
  * strides: HOST array of element strides (t, b, h): fwd q, k, v, g, beta (15); bwd the same and go's (18).  q, k, v, go: unit stride inside
- * a head, addresses and strides aligned to 16 bytes (a forward of up to 32 frames without `saved` takes any).
+ * a head, addresses and strides aligned to 16 bytes, frames at most 2^23 elements apart (a forward of up to 12 frames without `saved` takes
+ * any); state, state_out, o aligned to 16 bytes.  B * H <= 65536.
  * saved: NULL (inference), or sp_gdr_saved_bytes() device bytes that the forward fills and the backward reads; workspace:
  * sp_gdr_workspace_bytes(.., backward), for an inference forward and for the backward (a forward with `saved` needs none).
  * Backward: go = d loss / d o, gstate_out = d loss / d state_out or NULL; writes gq, gk [T][B][Hk][dk], gv [T][B][H][dv] (dense, dtype), gg,

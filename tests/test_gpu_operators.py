@@ -644,6 +644,47 @@ def test_group_norm_without_frames(cuda):
     assert torch.equal(ops.group_norm(one, w, b, 2), ops.group_norm(one.clone(memory_format=torch.contiguous_format), w, b, 2))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_delta_step_takes_any_view(cuda, dtype):
+    """Odd first elements, odd strides, gates with gaps: the numbers of dense tensors."""
+    from speech_amd import ops
+    base = torch.randn(9000, device=cuda).to(dtype)
+    q, k = (base.as_strided((3, 2, 24), (1001, 31, 1), o) for o in (1, 501))
+    v = base.as_strided((3, 4, 40), (2003, 83, 1), 4003)
+    g, beta = -torch.rand(3, 9, device=cuda)[:, 1::2], torch.rand(4, 3, device=cuda).t()
+    state = torch.randn(3, 4, 24, 40, device=cuda)
+    other = state.clone()
+    o = ops.gated_delta_step(q, k, v, g, beta, state, normalize=True)
+    dense = [t.clone(memory_format=torch.contiguous_format) for t in (q, k, v, g, beta)]
+    assert torch.equal(o, ops.gated_delta_step(*dense, other, normalize=True)) and torch.equal(state, other)
+    rule = ops.gated_delta_rule(*(t[None] for t in (q, k, v, g, beta)), state=torch.randn(3, 4, 24, 40, device=cuda) * 0 + other, normalize=True)
+    assert torch.equal(rule[0][0], ops.gated_delta_step(*dense, other, normalize=True)) and torch.equal(rule[1], other)
+
+
+@pytest.mark.parametrize("T", [7, 100])
+def test_in_place_entry_points(cuda, T):
+    """The C ABI's in-place forms: state_out = state of both forward forms, y = x and y = residual of the dropout."""
+    from speech_amd import _lib, ops
+    h = _lib.lib()
+    args, _, _ = delta_inputs(T, 2, 2, 2, 16, 40, torch.bfloat16, 3)
+    q, k, v, g, beta, state = (t.to(cuda) for t in args)
+    o, final = ops.gated_delta_rule(q, k, v, g, beta, state=state)
+    o2 = torch.empty_like(o)
+    n = h.sp_gdr_workspace_bytes(T, 2, 2, 4, 16, 40, _lib.SP_BF16, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=cuda)
+    strides = ops._strides(q, k, v, g, beta)
+    _lib.check(h.sp_gdr_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(), None, strides, T, 2, 2, 4, 16, 40,
+                            16 ** -0.5, 0, _lib.SP_BF16, o2.data_ptr(), state.data_ptr(), None, 0, ws.data_ptr(), n, ops.raw_stream(q)))
+    assert torch.equal(o, o2) and torch.equal(final, state)
+    x, r = torch.randn(1003, device=cuda), torch.randn(1003, device=cuda)
+    rng = ops.dropout_rng(4, cuda)
+    want = ops.dropout(x, 0.3, rng, 1, residual=r)
+    for y in (x.clone(), r.clone()):
+        a, b = (y, r) if torch.equal(y, x) else (x, y)
+        _lib.check(h.sp_dropout(a.data_ptr(), b.data_ptr(), 1, 1003, 0.3, rng.data_ptr(), 1, _lib.SP_F32, y.data_ptr(), None, ops.raw_stream(x)))
+        assert torch.equal(y, want)
+
+
 # ------------------------------------------------------------------------------------------ streams, graphs, the operators together
 def _layer(cuda, dtype=torch.bfloat16):
     from speech_amd import net
