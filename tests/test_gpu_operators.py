@@ -685,6 +685,39 @@ def test_in_place_entry_points(cuda, T):
         assert torch.equal(y, want)
 
 
+def test_offsets_beyond_32_bits(cuda):
+    """Samples, utterances and elements that lie more than 2^32 bytes and 2^31 elements into a tensor."""
+    from speech_amd import ops
+    far = (1 << 31) + 4096
+    base = torch.empty(far + (1 << 16), dtype=torch.bfloat16, device=cuda)
+    x = base.as_strided((2, 3, 10, 32), (far, 320, 32, 1))
+    x.copy_(torch.randn(2, 3, 10, 32, device=cuda))
+    w, b = torch.rand(32, device=cuda), torch.rand(32, device=cuda)
+    dense = x.clone(memory_format=torch.contiguous_format)
+    assert torch.equal(ops.group_norm(x, w, b, 4, act="silu", residual=x), ops.group_norm(dense, w, b, 4, act="silu", residual=dense))
+    xg, dg = x.detach().requires_grad_(True), dense.requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(ops.group_norm(xg, w, b, 4).float().square().sum(), xg)[0],
+                       torch.autograd.grad(ops.group_norm(dg, w, b, 4).float().square().sum(), dg)[0])
+    for T in (3, 70):
+        q = base.as_strided((T, 2, 2, 16), (32, far, 16, 1))
+        q.copy_(torch.randn(T, 2, 2, 16, device=cuda))
+        g = -torch.rand(T, 2, 2, device=cuda)
+        a = ops.gated_delta_rule(q, q, q, g, -g, normalize=True)
+        d = q.clone(memory_format=torch.contiguous_format)
+        c = ops.gated_delta_rule(d, d, d, g, -g, normalize=True)
+        assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+    base.fill_(1.0)
+    y = ops.dropout(base, 0.5, ops.dropout_rng(6, cuda, 2), 1)
+    u = np.uint64
+    at = np.arange((base.numel() - 4096) // 8, base.numel() // 8, dtype=u)
+    c = [at & u(0xFFFFFFFF), at >> u(32), np.full_like(at, 2), np.full_like(at, 1)]
+    for r in range(10):
+        p0, p1 = u(0xD2511F53) * c[0], u(0xCD9E8D57) * c[2]
+        c = [(p1 >> u(32)) ^ c[1] ^ u((6 + r * 0x9E3779B9) & 0xFFFFFFFF), p1 & u(0xFFFFFFFF), (p0 >> u(32)) ^ c[3] ^ u((r * 0xBB67AE85) & 0xFFFFFFFF), p0 & u(0xFFFFFFFF)]
+    keep = np.stack(c, -1).astype("<u4").view("<u2").reshape(-1) >= 32768
+    assert torch.equal(y[-4096:].cpu() != 0, torch.from_numpy(keep))
+
+
 # ------------------------------------------------------------------------------------------ streams, graphs, the operators together
 def _layer(cuda, dtype=torch.bfloat16):
     from speech_amd import net
