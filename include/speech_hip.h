@@ -407,9 +407,12 @@ int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period
  * sp_gdr_workspace_bytes(.., backward), for an inference forward and for the backward (a forward with `saved` needs none).
  * Backward: go = d loss / d o, gstate_out = d loss / d state_out or NULL; writes gq, gk [T][B][Hk][dk], gv [T][B][H][dv] (dense, dtype), gg,
  * gbeta f32 [T][B][H] dense, gstate f32 or NULL; frames behind an utterance's end get zeros.  T >= 1.  Results are bit-reproducible.
+ * SP_GDR_NO_STATE (backward): the forward had state = NULL; the decay of every walk's first frame then met nothing, and its gradient is
+ * written as the exact 0 that it is instead of the rounding of two sums that cancel.
  * --------------------------------------------------------------------------------------- */
 #define SP_GDR_NORMALIZE 1
 #define SP_GDR_BIDIRECTIONAL 2
+#define SP_GDR_NO_STATE 4
 size_t sp_gdr_workspace_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype, int backward);
 size_t sp_gdr_saved_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype);
 int sp_gdr_fwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const float* state,

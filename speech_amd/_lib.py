@@ -11,7 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libspeech_hip.so")
 
 SP_F32, SP_F16, SP_BF16 = 0, 1, 2
 ACT_CODES = {"none": 0, "relu": 1, "silu": 2}   # SP_ACT_*
-GDR_NORMALIZE, GDR_BIDIRECTIONAL = 1, 2         # SP_GDR_*
+GDR_NORMALIZE, GDR_BIDIRECTIONAL, GDR_NO_STATE = 1, 2, 4         # SP_GDR_*
 SUMSQ_WORDS = 1025   # SP_SUMSQ_WORDS of include/speech_hip.h
 ADAM8_BLOCK = 2048   # SP_ADAM8_BLOCK
 CONV_WGRAD_WS_WORDS = 512 * 15 * 32 * 32   # SP_CONV_WGRAD_WS_WORDS: one slab per persistent workgroup

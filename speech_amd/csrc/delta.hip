@@ -55,7 +55,7 @@ struct GdrArgs {
     int64_t qs[3], ks[3], vs[3], gs[3], bs[3];       // element strides (t, b, h)
     int T, B, Hk, H, r, dk, dv, nc, nsl;             // nsl: slices of 16 columns of dv
     float scale;
-    int norm, bidir;
+    int norm, bidir, fresh;                          // fresh: the walk began without a state
     void* o;
     float* sT;
     // kept between the kernels (and, in training, for the backward)
@@ -531,7 +531,8 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
         }
     }
     float* vo = a.vec + at * kVec * kC;
-    for (int i = tid; i < kVec * kC; i += 256) vo[i] = vec[i];
+#pragma unroll
+    for (int x = 0; x < kVec * kC / 256; ++x) vo[x * 256 + tid] = vec[x * 256 + tid];
 }
 
 // A state's 16 columns in the accumulators' layout from / to rows [dk][dv].  One 32-bit lane offset in bytes, everything else is uniform; dk
@@ -1111,7 +1112,11 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
             ro.load((const T*)a.go + b * a.gos[1] + h * a.gos[2], a.gos[0], a.dv, p0, w);
             rd.load((const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, p0, w);
             re.load((const ET*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
-            for (int i = tid; i < kVec * kC; i += 256) vec[i] = a.vec[at * kVec * kC + i];
+            // a loop over i = tid, tid + 256, ... would end lane by lane, and at such an exit the compiler has put a copy of a register that
+            // lives on (to an accumulation register, where 256 do not suffice) in front of the instruction that turns the lanes on again:
+            // the copy wrote nothing.  No loop in this kernel ends lane by lane while the tiles are live.
+#pragma unroll
+            for (int x = 0; x < kVec * kC / 256; ++x) vec[x * 256 + tid] = a.vec[at * kVec * kC + x * 256 + tid];
 #pragma unroll
             for (int i = 0; i + 1 < AHEAD; ++i) state_rows(sr[i], i / 4, i % 4);
             phase_end();
@@ -1225,7 +1230,7 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
                 for (int o = 1; o < 64; o <<= 1) { const float u = __shfl_down(z, o); if (l + o < 64) z += u; }
                 if (p0 + l < w.len) {
                     const int64_t o = w.frame(p0 + l) * gts + bh;
-                    a.gg[o] = z + an;
+                    a.gg[o] = a.fresh && p0 + l == 0 ? 0.f : z + an;
                 }
             }
             if (wave == 1) {      // dbeta
@@ -1512,6 +1517,7 @@ static void gdr_fill(GdrArgs& a, const void* q, const void* k, const void* v, co
     a.scale = scale;
     a.norm = flags & SP_GDR_NORMALIZE ? 1 : 0;
     a.bidir = flags & SP_GDR_BIDIRECTIONAL ? 1 : 0;
+    a.fresh = flags & SP_GDR_NO_STATE ? 1 : 0;
 }
 
 template <typename T, int DK, int NW, bool TRAIN> static int gdr_scan(const GdrArgs& a, hipStream_t s) {
@@ -1601,7 +1607,7 @@ extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const flo
                           const int64_t* strides, int T, int B, int Hk, int H, int dk, int dv, float scale, int flags, int dtype,
                           const void* o, const void* saved, size_t saved_bytes, const void* go, const float* gstate_out, void* gq, void* gk,
                           void* gv, float* gg, float* gbeta, float* gstate, void* workspace, size_t workspace_bytes, void* stream) {
-    int rc = gdr_check("sp_gdr_bwd", T, B, Hk, H, dk, dv, flags, dtype);
+    int rc = gdr_check("sp_gdr_bwd", T, B, Hk, H, dk, dv, flags & ~SP_GDR_NO_STATE, dtype);
     if (rc) return rc;
     if (B == 0) return SP_OK;
     SP_CHECK_ARG(scale != 0.f, "sp_gdr_bwd: scale is zero");

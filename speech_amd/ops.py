@@ -1185,7 +1185,7 @@ class _GatedDeltaFn(torch.autograd.Function):
         final = g.new_empty((B, H, dk, dv))
         o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _strides(q, k, v, g, beta), scale, flags, True)
         ctx.save_for_backward(q, k, v, g, beta, lengths, o, saved)
-        ctx.cfg = (dims, scale, flags)
+        ctx.cfg = (dims, scale, flags | (_lib.GDR_NO_STATE if state is None else 0))
         ctx.set_materialize_grads(False)
         return o, final
 

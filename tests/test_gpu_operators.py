@@ -468,6 +468,22 @@ def test_delta_gates(cuda, T):
     delta_check(cuda, ref, go, gs, dirty=args, train=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_delta_first_decay_without_a_state(cuda, dtype):
+    """The first frame of every walk meets no state: its decay's gradient is exactly zero, in both directions and for every length."""
+    from speech_amd import ops
+    lengths = [1, 70, 64, 0]
+    args, go, gs = delta_inputs(70, 4, 2, 2, 24, 40, dtype, 4, state=False)
+    xs = [t.to(cuda).requires_grad_(True) for t in args[:5]]
+    o, f = ops.gated_delta_rule(*xs, lengths=torch.tensor(lengths, device=cuda), bidirectional=True)
+    gg = torch.autograd.grad([o, f], xs, [go.to(cuda), gs.to(cuda)])[3]
+    for b, n in enumerate(lengths):
+        if n:
+            assert not gg[0, b, :2].any() and not gg[n - 1, b, 2:].any()
+        if n > 1:
+            assert gg[1:n, b, :2].all() and gg[:n - 1, b, 2:].all()
+
+
 def test_delta_zero_rows_and_scale(cuda):
     args, go, gs = delta_inputs(70, 2, 2, 1, 16, 16, torch.float32, 5)
     args[0][::5] = 0
