@@ -1032,7 +1032,7 @@ template <int P> __device__ __forceinline__ void plane_write_t(__bf16* t, int r0
 template <typename T> struct FragOf { using type = Frag<Gd<T>::PT>; };
 
 // One workgroup a (key head, chunk), its value heads in turn: shared heads' gradients are sums in registers, in a fixed order.  A wave owns a
-// quarter of dk in the products with the states and 16 columns j of the 64 x 64 products.  172 us: 317 MB at 1.8 TB/s, matrix pipes busy 8 %:
+// quarter of dk in the products with the states and 16 columns j of the 64 x 64 products.  176 us: 317 MB at 1.8 TB/s, matrix pipes busy 8 %:
 // bound by the waits between its six phases.  Two workgroups a CU for bf16 at dk 64 (one: 287 us against 203 when this was measured); elsewhere
 // 256 registers do not hold the tiles and one workgroup with 512 is faster (then bf16, dk 128: 387 us against 405; f16 dk 64 377 / 401, dk 128
 // 522 / 628).
