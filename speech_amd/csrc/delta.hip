@@ -75,11 +75,12 @@ struct GdrArgs {
 };
 
 // ---- operand fragments --------------------------------------------------------------------------------
-// PT: parts of an input; OP: parts that reach a 16-bit output; EP: parts of P in o's product; ET: type that E is kept in for dq and dk
+// PT: parts of an input; OP: parts of what is derived, where it reaches a 16-bit output only (S, U, P in o's product); ET: type that E is kept
+// in for dq and dk
 template <typename T> struct Gd;
-template <> struct Gd<__hip_bfloat16> { static constexpr int PT = 1, OP = 2, EP = 1; using ET = __hip_bfloat16; };
-template <> struct Gd<__half> { static constexpr int PT = 2, OP = 2, EP = 2; using ET = float; };
-template <> struct Gd<float> { static constexpr int PT = 3, OP = 3, EP = 3; using ET = float; };
+template <> struct Gd<__hip_bfloat16> { static constexpr int PT = 1, OP = 2; using ET = __hip_bfloat16; };
+template <> struct Gd<__half> { static constexpr int PT = 2, OP = 2; using ET = float; };
+template <> struct Gd<float> { static constexpr int PT = 3, OP = 3; using ET = float; };
 
 template <int P> struct Frag { bf16x8 p[P]; };
 
@@ -607,7 +608,7 @@ __device__ __forceinline__ void zero_rows(T* dst, int64_t ts, int ncol, int from
 
 template <typename T, int DK, int NW> struct ScanLds {
     static constexpr int LDK = DK + 8, LDV = NW * 16 + 8;
-    static constexpr size_t bytes = (size_t)kC * (2 * LDK + LDV) * sizeof(T) + (size_t)(3 + Gd<T>::EP) * kC * kLdm * 2 + kVec * kC * 4;
+    static constexpr size_t bytes = (size_t)kC * (2 * LDK + LDV) * sizeof(T) + (size_t)(3 + Gd<T>::OP) * kC * kLdm * 2 + kVec * kC * 4;
 };
 
 // B operands (inner index = rows of the accumulators) of 64 frames: row tiles 2 kb and 2 kb + 1, each scaled by a vector
@@ -619,21 +620,22 @@ template <int P> __device__ __forceinline__ void row_operands(Frag<P> (&f)[2], c
 // A wave owns 16 columns of dv: the state's columns, U's, O's.  Only K, Q, X, P and the vectors are shared (LDS, filled a chunk ahead
 // through registers); two barriers a chunk.  A wave whose columns lie behind dv works on zeros and writes nothing: as many steps as the
 // others, and no branch around the matrix instructions.
-// 98 us, 12 chunks in turn: 8 us a chunk, of which the matrix pipes are busy 18 %.  Bound by the chain of four dependent products a chunk
+// 101 us, 12 chunks in turn: 8.4 us a chunk, of which the matrix pipes are busy 18 %.  P takes two parts: with one, o was off by 1.34 times its own
+// rounding (bf16: 2.2e-3 of the two-norm instead of 1.66e-3) for 2.5 us less.  Bound by the chain of four dependent products a chunk
 // (K S, X, P, K^T U) at two waves a SIMD; the states are the only thing that could be split further, and every split loads K, Q, X and P
-// again.  Inference at dk 128 (T = 1501, 128 heads, one wave a SIMD): 132 us, 24 chunks.
+// again.  Inference at dk 128 (T = 1501, 128 heads, one wave a SIMD): 139 us, 24 chunks (132 with one part of P).
 template <typename T, int DK, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = ScanLds<T, DK, NW>;
-    constexpr int NT = NW * 64, PT = Gd<T>::PT, EP = Gd<T>::EP, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
+    constexpr int NT = NW * 64, PT = Gd<T>::PT, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
     constexpr bool AHEAD = PT == 1;      // operands of one part fit the registers ahead of their use
     T* Kl = reinterpret_cast<T*>(smem);
     T* Ql = Kl + kC * LDK;
     T* Vl = Ql + kC * LDK;
     __bf16* Xl = reinterpret_cast<__bf16*>(Vl + kC * LDV);
     __bf16* Pl = Xl + 3 * kC * kLdm;
-    float* vec = reinterpret_cast<float*>(Pl + EP * kC * kLdm);
+    float* vec = reinterpret_cast<float*>(Pl + OP * kC * kLdm);
     const int groups = (a.nsl + NW - 1) / NW;
     const int bh = blockIdx.x / groups, sg = blockIdx.x % groups, b = bh / a.H, h = bh % a.H, hk = h / a.r;
     const Walk w = walk_of(a, b, h);
@@ -665,7 +667,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
     };
-    clear_upper(Xl, 3 + EP, tid, NT);
+    clear_upper(Xl, 3 + OP, tid, NT);
     if (ncl > 0) fetch(0);
     for (int c = 0; c < ncl; ++c) {
         const int64_t at = (int64_t)bh * a.nc + c;
@@ -674,7 +676,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
         rq.store(Ql, LDK, a.dk, c * kC, w.len);
         rv.store(Vl, LDV, vcols, c * kC, w.len);
         rx.template store<3>(Xl);
-        rp.template store<EP>(Pl);
+        rp.template store<OP>(Pl);
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) vec[i * NT + tid] = rvec[i];
         __syncthreads();
@@ -724,8 +726,8 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
 #pragma unroll
         for (int x = 0; x < 3; ++x) xs[tri_m(x)] = mma(xf[x], uf[tri_k(x)], xs[tri_m(x)]);
         if (AHEAD) phase_end();
-        Frag<EP> pf[6];
-        tri_rows<EP, 0, 6>(pf, Pl);
+        Frag<OP> pf[6];
+        tri_rows<OP, 0, 3>(pf, Pl);
         if (AHEAD) phase_end();
 #pragma unroll
         for (int x = 3; x < 6; ++x) xs[tri_m(x)] = mma(xf[x], uf[tri_k(x)], xs[tri_m(x)]);
@@ -734,18 +736,22 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) uf[kb] = split<3>(ks[2 * kb], ks[2 * kb + 1]);
         if (AHEAD) phase_end();
+        tri_rows<OP, 3, 6>(pf, Pl);
+        constexpr int FIRST = AHEAD && KT > 4 ? 2 : KT;      // of eight tiles of K's operands the registers hold two ahead of their use
         Frag<PT> cf[KT][2];
 #pragma unroll
-        for (int m = 0; m < KT; ++m) col_frags(cf[m], Kl, LDK, 16 * m);
+        for (int m = 0; m < FIRST; ++m) col_frags(cf[m], Kl, LDK, 16 * m);
         if (AHEAD) phase_end();
 #pragma unroll
-        for (int x = 0; x < 6; ++x) qs[tri_m(x)] = mma<EP, 3, OP>(pf[x], uf[tri_k(x)], qs[tri_m(x)]);
+        for (int x = 0; x < 6; ++x) qs[tri_m(x)] = mma<OP, 3, OP>(pf[x], uf[tri_k(x)], qs[tri_m(x)]);
         row_operands(uf, vec + kKb * kC, ks);
         if (AHEAD) phase_end();
         // S = e^{G_C} S + K^T (kb U)
         const float dec = __expf((float)reinterpret_cast<const double*>(vec + kG64 * kC)[kC - 1]);
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
+            if (m + FIRST < KT) col_frags(cf[m + FIRST], Kl, LDK, 16 * (m + FIRST));
+            if (FIRST < KT) phase_end();
             S[m] *= dec;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) S[m] = mma(cf[m][kb], uf[kb], S[m]);

@@ -1,0 +1,31 @@
+"""Group normalisation, dropout and the gated delta rule at their edges: precision of 16-bit results, long walks of a thread, the scans' wide
+form, padding that must have no influence, calls that must be refused.  References are stated in 64 bits on the CPU."""
+import pytest
+import torch
+
+from test_gpu_operators import DTYPES, delta_inputs, delta_reference, ids
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------ precision of 16-bit results
+def rounded_once(u, w, what):
+    """||u - w|| <= (r + 2^-12) ||w||, r ||w|| the two-norm of w's own rounding to u's type (bf16: r = 2^-9.2).  What is rounded comes from products
+    whose operands have at least 16 bits: each factor is off by at most 2^-16 of itself, a product by 3 * 2^-16 with the part of it that is
+    left out.  The errors of a sum's terms have either sign and grow as the terms' two-norm, which is at most four times the result's for
+    the inputs here: 3 * 4 * 2^-16 < 2^-12."""
+    dtype, u, w = u.dtype, u.detach().double().cpu(), w.detach().double()
+    once, err = float((w.to(dtype).double() - w).norm() / w.norm()), float((u - w).norm() / w.norm())
+    assert err <= once + 2.0 ** -12, (what, err, once)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=ids)
+@pytest.mark.parametrize("T,B,Hk,r,dk,dv", [(40, 2, 2, 1, 64, 128), (200, 1, 1, 2, 128, 72), (70, 9, 16, 1, 16, 72)], ids=str)
+@pytest.mark.parametrize("train", [False, True])
+def test_delta_output_is_rounded_once(cuda, dtype, T, B, Hk, r, dk, dv, train):
+    from speech_amd import ops
+    args, _, _ = delta_inputs(T, B, Hk, r, dk, dv, dtype, 11)
+    dev = [t.to(cuda).requires_grad_(train) for t in args]
+    o, _ = ops.gated_delta_rule(*dev[:5], state=dev[5], normalize=True)
+    ro, _ = delta_reference(*(t.double() for t in args), None, dk ** -0.5, True, False)
+    rounded_once(o, ro, "o")
