@@ -25,6 +25,8 @@
 // reverse with dS) -> grads (dq, dk, dg, dbeta of a chunk; all chunks at once).  Few frames (streaming, single tokens): one recurrent kernel.
 #include "common.h"
 
+#include <type_traits>
+
 namespace sp {
 
 constexpr int kC = 64;              // frames a chunk
@@ -66,7 +68,7 @@ struct GdrArgs {
     const void* go;
     const float* gsT;
     float* dS;               // [bh][nc][dk][dv]: the state's gradient at the chunk's end
-    void* E;                 // [bh][nc][64][dv] (bf16 for bf16 inputs, else f32)
+    uint32_t* E;             // [bh][nc][64][dv]: f32; for 16-bit types words of pack_ev
     float *zpart, *bpart;    // [nsl][bh][nc][64]: dO.O - dV.V and E.F over 16 columns
     float* apart;            // [nsl][bh][nc]
     void *gq, *gk, *gv;
@@ -75,12 +77,11 @@ struct GdrArgs {
 };
 
 // ---- operand fragments --------------------------------------------------------------------------------
-// PT: parts of an input; OP: parts of what is derived, where it reaches a 16-bit output only (S, U, P in o's product); ET: type that E is kept
-// in for dq and dk
+// PT: parts of an input; OP: parts of what is derived, where it reaches a 16-bit output only (S, U, P in o's product)
 template <typename T> struct Gd;
-template <> struct Gd<__hip_bfloat16> { static constexpr int PT = 1, OP = 2; using ET = __hip_bfloat16; };
-template <> struct Gd<__half> { static constexpr int PT = 2, OP = 2; using ET = float; };
-template <> struct Gd<float> { static constexpr int PT = 3, OP = 3; using ET = float; };
+template <> struct Gd<__hip_bfloat16> { static constexpr int PT = 1, OP = 2; };
+template <> struct Gd<__half> { static constexpr int PT = 2, OP = 2; };
+template <> struct Gd<float> { static constexpr int PT = 3, OP = 3; };
 
 template <int P> struct Frag { bf16x8 p[P]; };
 
@@ -774,17 +775,35 @@ template <typename T, int DK, int NW> struct RscanLds {
     static constexpr size_t bytes = (size_t)kC * (2 * LDK + 2 * LDV) * sizeof(T) + (size_t)6 * kC * kLdm * 2 + kVec * kC * 4;
 };
 
+// What the gradients of q and k take of E and dV.  Of 16-bit types two parts of each (with E in one bf16 part dq and dk were off by 1.34 and 1.47 times
+// their own rounding, with dV as it is written, in gv, dk by 1.1 times).  One word holds the upper 24 bits of E, which are its two parts, and the
+// eight bits that follow dV's rounded mantissa, as a signed number: four bytes an element as for f32, and no third tensor (one more
+// took the reverse scan from 217 to 230 us).
+template <typename T> struct BehindT;
+template <> struct BehindT<__hip_bfloat16> { static constexpr int SHIFT = 8; };       // f32 bits behind the type's mantissa: 16 and 13, eight of them kept
+template <> struct BehindT<__half> { static constexpr int SHIFT = 5; };
+template <typename T> __device__ __forceinline__ uint32_t pack_ev(float e, float v) {
+    constexpr int S = BehindT<T>::SHIFT;
+    T t;
+    Elem<T>::st(&t, v);
+    const int d = (int)(__float_as_uint(v) - __float_as_uint(to_f(t))) + (1 << (S - 1));
+    return (__float_as_uint(e) & 0xFFFFFF00u) | ((uint32_t)max(min(d >> S, 127), -128) & 0xFFu);
+}
+// what dV's rounded value lacks, exactly (eight bits)
+template <typename T> __device__ __forceinline__ float behind(float v, uint32_t word) {
+    return __uint_as_float(__float_as_uint(v) + ((uint32_t)((int)(word << 24) >> 24) << BehindT<T>::SHIFT)) - v;
+}
+
 // E and O are formed again from the state at the chunk's start: 36 + 84 more matrix instructions a wave and chunk instead of 100 KB more
 // traffic a chunk (E in f32 and the rest of O that its rounding dropped, written by the forward and read back).
-// 211 us, 17.5 us a chunk (f32 at 30 heads, dk 40, dv 72, 301 frames: 76 us): 246 matrix instructions a wave and chunk keep the pipes busy 18 %
-// of the time, the waves issue in 29 % of their cycles, 400 MB move.  Bound by latency at two waves a SIMD, which 256 registers a lane allow: without
-// the next chunk's loads 157 us (they find registers only at the chunk's end), without the stores 211.
-// Measured and not kept: those loads earlier (they spill), their lines touched into the L2 cache a chunk ahead (230 us).
+// 223 us, 18.6 us a chunk (f32 at 30 heads, dk 40, dv 72, 301 frames: 76 us): 246 matrix instructions a wave and chunk keep the pipes busy 17 %
+// of the time, 425 MB move.  Bound by latency at two waves a SIMD, which 256 registers a lane allow: without the next chunk's loads it took three
+// quarters of the time (they find registers only at the chunk's end).
+// Measured and not kept: those loads earlier (they spill), their lines touched into the L2 cache a chunk ahead (7 % more).
 template <typename T, int DK, int NW>
 __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = RscanLds<T, DK, NW>;
-    using ET = typename Gd<T>::ET;
     constexpr int NT = NW * 64, PT = Gd<T>::PT, LDK = L::LDK, LDV = L::LDV, KT = DK / 16;
     constexpr bool AHEAD = PT == 1;
     T* Kl = reinterpret_cast<T*>(smem);
@@ -971,21 +990,25 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
             of3[kb] = split<3>(vec4(vec + kAq * kC, 32 * kb) * tile_read(Ol, LDV, 32 * kb, wave * 16),
                                vec4(vec + kAq * kC, 32 * kb + 16) * tile_read(Ol, LDV, 32 * kb + 16, wave * 16));
         }
-        // dV and E leave through this wave's own columns of the V and dO tiles, which it has read
+        // dV leaves through this wave's own columns of the V tile, which it has read; E (f32) through those of the dO tile
         lds_order();
         T* my = Vl + wave * 16;
 #pragma unroll
         for (int m = 0; m < 4; ++m) tile_write(my, LDV, 16 * m, 0, du[m]);
         lds_order();
         store_rows(my, LDV, mycols, gvp + col0, ots, c * kC, w);
-        ET* eo = (ET*)a.E + at * kC * a.dv;
-        if constexpr (sizeof(ET) == sizeof(T)) {
-            ET* me = reinterpret_cast<ET*>(Ol + wave * 16);
+        float* eo = (float*)a.E + at * kC * a.dv;
+        if constexpr (sizeof(T) == 4) {
+            T* me = Ol + wave * 16;
 #pragma unroll
             for (int m = 0; m < 4; ++m) tile_write(me, LDV, 16 * m, 0, E[m]);
             lds_order();
             store_rows(me, LDV, mycols, eo + col0, a.dv, 0, Walk{kC, false});
         } else {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) E[m][e] = __uint_as_float(pack_ev<T>(E[m][e], du[m][e]));
             state_store(E, eo, kC, a.dv, col0);
         }
         phase_end();
@@ -1013,10 +1036,12 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 
 // ---- gradients of a chunk ---------------------------------------------------------------------------------
 template <typename T, int DK> struct GradLds {
-    static constexpr int LDK = DK + 8, LDV = sizeof(T) == 4 ? 132 : 136, LDE = sizeof(typename Gd<T>::ET) == 4 ? 132 : 136;
-    static constexpr size_t one = (size_t)2 * kC * LDV * sizeof(T) + (size_t)kC * LDE * sizeof(typename Gd<T>::ET), two = (size_t)2 * kC * LDK * sizeof(T);
-    static constexpr size_t tiles = one > two ? one : two, mat = (size_t)Gd<T>::OP * kC * kLdm * 2;
-    static constexpr size_t bytes = tiles + mat + (kVec + 8) * kC * 4;
+    static constexpr int LDK = DK + 8, LDV = sizeof(T) == 4 ? 132 : 136;
+    static constexpr size_t values = (size_t)(sizeof(T) == 4 ? 3 : 5) * kC * LDV * sizeof(T);      // dO, dV, E; 16-bit types: dV's rest, two parts of E
+    static constexpr size_t keys = (size_t)2 * kC * LDK * sizeof(T), mat = (size_t)Gd<T>::OP * kC * kLdm * 2, vecs = (kVec + 8) * kC * 4;
+    static constexpr bool ROOM = values + keys + mat + vecs <= 160 * 1024;      // K, Q and the matrix stand beside the values, else in their place
+    static constexpr size_t at_keys = ROOM ? values : 0, at_mat = at_keys + keys, at_vec = at_mat + mat > values ? at_mat + mat : values;
+    static constexpr size_t bytes = at_vec + vecs;
 };
 
 template <int P> __device__ __forceinline__ void plane_write(__bf16* t, int r0, int c0, f32x4 v) {
@@ -1035,32 +1060,53 @@ template <int P> __device__ __forceinline__ void plane_write_t(__bf16* t, int r0
     parts4<P>(v, [&](int i, u32x2a h) { *reinterpret_cast<u32x2a*>(p + i * kC * kLdm) = h; });
 }
 
-template <typename T> struct FragOf { using type = Frag<Gd<T>::PT>; };
+// words of pack_ev and dV's values on their way to LDS: three planes of bf16, E's upper and lower part and dV's rest
+template <typename T>
+__device__ __forceinline__ void store_ev(const TileRegs<T, 128, 512>& v, const TileRegs<float, 128, 512>& e, __hip_bfloat16* dst, int ld, int ncol) {
+    const int tid = opaque(threadIdx.x);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int i = tid + n * 512, row = i / 16, c = i % 16 * 8;
+        T t[8];
+        __builtin_memcpy(t, &v.v[n][0], sizeof(t));
+        f32x8 x, r;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t word = e.v[n][k >> 2][k & 3];
+            x[k] = __uint_as_float(word & 0xFFFFFF00u);
+            r[k] = behind<T>(to_f(t[k]), word);
+        }
+        const Frag<2> f = split<2>(x);
+        const bf16x8 planes[3] = {f.p[0], f.p[1], split<1>(r).p[0]};
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            *reinterpret_cast<u32x4a*>(dst + (p * kC + row) * ld + c) = c < ncol ? __builtin_bit_cast(u32x4a, planes[p]) : u32x4a{0, 0, 0, 0};
+    }
+}
 
-// One workgroup a (key head, chunk), its value heads in turn: shared heads' gradients are sums in registers, in a fixed order.  A wave owns a
-// quarter of dk in the products with the states and 16 columns j of the 64 x 64 products.  176 us: 317 MB at 1.8 TB/s, matrix pipes busy 8 %:
-// bound by the waits between its six phases.  Two workgroups a CU for bf16 at dk 64 (one: 287 us against 203 when this was measured); elsewhere
-// 256 registers do not hold the tiles and one workgroup with 512 is faster (then bf16, dk 128: 387 us against 405; f16 dk 64 377 / 401, dk 128
-// 522 / 628).
+// One workgroup a (key head, chunk), its value heads in turn: shared heads' gradients are sums in registers, in a fixed order.  Eight waves: a
+// wave owns a quarter of dk in the products with the states and 16 columns j of the 64 x 64 products, and half of the rows of both.  219 us (one
+// value head a key head; four: 160): 342 MB at 1.5 TB/s, bound by the waits between its phases.  Two parts of E and of dV take 128 KB of LDS, so one
+// workgroup a CU; four waves a workgroup, two of them a CU, held one part of each: 173 us, dq off by 1.34 times its own rounding, dk by 1.47.
+// Other shapes of the same size, eight waves against four: f32 dk 64 302 us / 363, dk 128 451 / 608, f16 dk 64 245 / 272, dk 128 337 / 415,
+// bf16 dk 128 313 / 289 (one part).
 template <typename T, int DK>
-__global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_grads_kernel(GdrArgs a) {
+__global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
     using L = GradLds<T, DK>;
-    using ET = typename Gd<T>::ET;
-    constexpr int PT = Gd<T>::PT, OP = Gd<T>::OP, LDK = L::LDK, LDV = L::LDV, LDE = L::LDE, NT = DK / 64;
-    constexpr int PE = sizeof(ET) == 2 ? 1 : 3, AHEAD = 3;          // pieces of the states in flight or in use
-    // one workgroup a CU: the second half's operands are asked for before the first half's last products (dk 128: 299 us against 319); two
-    // hide that wait for each other, and the registers count (dk 64: 172 against 180)
-    constexpr bool EARLY = PT > 1 || DK > 64;
+    constexpr bool HALF = sizeof(T) == 2;
+    using ET = std::conditional_t<HALF, __hip_bfloat16, float>;
+    constexpr int PT = Gd<T>::PT, OP = Gd<T>::OP, PE = HALF ? 2 : 3, LDK = L::LDK, LDV = L::LDV, NT = DK / 64;
+    constexpr int NTH = 512, AHEAD = 2;                                   // pieces of the states in flight or in use (3: 0 to 4 % slower, 5: 9 %)
     T *Ol = reinterpret_cast<T*>(smem), *Dl = Ol + kC * LDV;              // dO, dV
-    ET* El = reinterpret_cast<ET*>(Dl + kC * LDV);
-    T *Kl = reinterpret_cast<T*>(smem), *Ql = Kl + kC * LDK;              // later
-    __bf16* M = reinterpret_cast<__bf16*>(smem + L::tiles);
-    float* vec = reinterpret_cast<float*>(smem + L::tiles + L::mat);
+    ET *El = reinterpret_cast<ET*>(Dl + kC * LDV), *Rl = El + 2 * kC * LDV;      // E (16-bit types: two planes), dV's rest
+    T *Kl = reinterpret_cast<T*>(smem + L::at_keys), *Ql = Kl + kC * LDK;
+    __bf16* M = reinterpret_cast<__bf16*>(smem + L::at_mat);
+    float* vec = reinterpret_cast<float*>(smem + L::at_vec);
     const double* G = reinterpret_cast<const double*>(vec + kG64 * kC);
     float* dots = vec + kVec * kC;                                        // [2][4][64]
     const int c = blockIdx.x % a.nc, bk = blockIdx.x / a.nc, b = bk / a.Hk, hk = bk % a.Hk;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 2, wc = wave & 3;
     const Walk w = walk_of(a, b, hk * a.r);
     const int64_t kts = (int64_t)a.B * a.Hk * a.dk, gts = (int64_t)a.B * a.H;
     T* gqp = (T*)a.gq + ((int64_t)b * a.Hk + hk) * a.dk;
@@ -1069,21 +1115,22 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
     // frames of this chunk behind the utterance's end: zero gradients
     const int z0 = max(p0, w.len), z1 = min(p0 + kC, a.T);
     if (z0 < z1) {
-        zero_rows(gqp, kts, a.dk, z0, z1, tid, 256);
-        zero_rows(gkp, kts, a.dk, z0, z1, tid, 256);
-        for (int i = tid; i < (z1 - z0) * a.r; i += 256) {
+        zero_rows(gqp, kts, a.dk, z0, z1, tid, NTH);
+        zero_rows(gkp, kts, a.dk, z0, z1, tid, NTH);
+        for (int i = tid; i < (z1 - z0) * a.r; i += NTH) {
             const int64_t o = (int64_t)(z0 + i / a.r) * gts + (int64_t)b * a.H + hk * a.r + i % a.r;
             a.gg[o] = 0.f;
             a.gbeta[o] = 0.f;
         }
     }
     if (p0 >= w.len) return;
-    f32x4 tq[4][NT], tk[4][NT];
+    f32x4 tq[2][NT], tk[2][NT];                               // rows 32 wr + 16 m + ..
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) { tq[m][n] = f32x4{0, 0, 0, 0}; tk[m][n] = f32x4{0, 0, 0, 0}; }
     const int64_t ots = (int64_t)a.B * a.H * a.dv, nat = (int64_t)a.B * a.H * a.nc;
+    const int r0 = 32 * wr;
     for (int hh = 0; hh < a.r; ++hh) {
         // the lane's number as the loop's own value: what follows from it (masks, addresses) is then formed where it is used, not kept in
         // registers, and out of them in scratch memory, across the loop
@@ -1094,7 +1141,7 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
         const float* s0 = a.S0 + at * a.dk * a.dv;
         const float* ds = a.dS + at * a.dk * a.dv;
         auto state_rows = [&](f32x4 (&v)[4], int n, int kb) {
-            const int row = (wave * NT + n) * 16 + i16;
+            const int row = (wc * NT + n) * 16 + i16;
             const uint32_t rb = (uint32_t)(min(row, a.dk - 1) * a.dv) * 4u;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -1104,40 +1151,61 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
             }
         };
         auto state_cut = [&](f32x4 (&v)[4], int n, int kb) {      // what lies outside is zero
-            if ((wave * NT + n) * 16 + 16 <= a.dk && 32 * kb + 32 <= a.dv) return;
-            const int row = (wave * NT + n) * 16 + i16;
+            if ((wc * NT + n) * 16 + 16 <= a.dk && 32 * kb + 32 <= a.dv) return;
+            const int row = (wc * NT + n) * 16 + i16;
 #pragma unroll
             for (int x = 0; x < 4; ++x) v[x] = row < a.dk && 32 * kb + 16 * (x & 1) + 4 * g < a.dv ? v[x] : f32x4{0, 0, 0, 0};
         };
+        // operands from rows of E (its parts) and of dV
+        auto e_frag = [&](int row, int kb) {
+            if constexpr (HALF) {
+                Frag<2> f;
+                f.p[0] = row_frag(El, LDV, row, 32 * kb).p[0];
+                f.p[1] = row_frag(El + kC * LDV, LDV, row, 32 * kb).p[0];
+                return f;
+            } else return row_frag(El, LDV, row, 32 * kb);
+        };
         f32x4 sr[AHEAD][4];
+        TileRegs<T, DK, NTH> rk, rq;
+        auto load_keys = [&] {
+            rk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, p0, w);
+            rq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, p0, w);
+        };
+        auto store_keys = [&] {
+            rk.store(Kl, LDK, a.dk, c * kC, w.len);
+            rq.store(Ql, LDK, a.dk, c * kC, w.len);
+        };
         __syncthreads();
         {
-            TileRegs<T, 128, 256> ro, rd;
-            TileRegs<ET, 128, 256> re;
-            Walk rows = {kC, false};
+            TileRegs<T, 128, NTH> ro, rd;
+            TileRegs<float, 128, NTH> re;
+            const Walk rows = {kC, false};
             ro.load((const T*)a.go + b * a.gos[1] + h * a.gos[2], a.gos[0], a.dv, p0, w);
             rd.load((const T*)a.gv + (int64_t)bh * a.dv, ots, a.dv, p0, w);
-            re.load((const ET*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
-            // a loop over i = tid, tid + 256, ... would end lane by lane, and at such an exit the compiler has put a copy of a register that
+            re.load((const float*)a.E + at * kC * a.dv, a.dv, a.dv, 0, rows);
+            if (L::ROOM) load_keys();
+            // a loop over i = tid, tid + 512, ... would end lane by lane, and at such an exit the compiler has put a copy of a register that
             // lives on (to an accumulation register, where 256 do not suffice) in front of the instruction that turns the lanes on again:
             // the copy wrote nothing.  No loop in this kernel ends lane by lane while the tiles are live.
-#pragma unroll
-            for (int x = 0; x < kVec * kC / 256; ++x) vec[x * 256 + tid] = a.vec[at * kVec * kC + x * 256 + tid];
+            static_assert(kVec * kC == NTH, "one entry a thread");
+            vec[tid] = a.vec[at * kVec * kC + tid];
 #pragma unroll
             for (int i = 0; i + 1 < AHEAD; ++i) state_rows(sr[i], i / 4, i % 4);
             phase_end();
             ro.store(Ol, LDV, a.dv, p0, w.len);
             rd.store(Dl, LDV, a.dv, p0, w.len);
-            re.store(El, LDE, a.dv, 0, kC);
+            if constexpr (HALF) store_ev<T>(rd, re, El, LDV, a.dv);
+            else re.store(El, LDV, a.dv, 0, kC);
+            if (L::ROOM) store_keys();
             phase_end();
         }
         __syncthreads();
         // states: wave = a quarter of dk; U = beta E: its factor goes with the rows
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            f32x4 cq[4], ck[4], cd[4];
+            f32x4 cq[2], ck[2], cd[2];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) { cq[m] = f32x4{0, 0, 0, 0}; ck[m] = cq[m]; cd[m] = cq[m]; }
+            for (int m = 0; m < 2; ++m) { cq[m] = f32x4{0, 0, 0, 0}; ck[m] = cq[m]; cd[m] = cq[m]; }
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
                 const int nx = 4 * n + kb + AHEAD - 1;
@@ -1146,128 +1214,137 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
                 if (kb * 32 < a.dv) {
                     state_cut(cur, n, kb);
                     const Frag<OP> sf = split<OP>(cur[0], cur[1]), df = split<OP>(cur[2], cur[3]);
-                    typename FragOf<T>::type of[4], vf[4];
-                    typename FragOf<ET>::type uf[4];
-                    row_frags(of, Ol, LDV, 32 * kb);
-                    row_frags(vf, Dl, LDV, 32 * kb);
-                    row_frags(uf, El, LDE, 32 * kb);
+                    Frag<PT> of[2], vf[2];
+                    Frag<PE> uf[2];
+                    Frag<1> lf[2], s1;
+                    s1.p[0] = sf.p[0];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        of[m] = row_frag(Ol, LDV, r0 + 16 * m, 32 * kb);
+                        vf[m] = row_frag(Dl, LDV, r0 + 16 * m, 32 * kb);
+                        uf[m] = e_frag(r0 + 16 * m, kb);
+                        if constexpr (HALF) lf[m] = row_frag(Rl, LDV, r0 + 16 * m, 32 * kb);
+                    }
                     if (PT == 1) phase_end();
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
+                    for (int m = 0; m < 2; ++m) {
                         cq[m] = mma<PT, OP, OP>(of[m], sf, cq[m]);
                         ck[m] = mma<PE, OP, OP>(uf[m], df, ck[m]);
                         cd[m] = mma<PT, OP, OP>(vf[m], sf, cd[m]);
+                        if constexpr (HALF) cd[m] = mma(lf[m], s1, cd[m]);
                     }
                 }
                 phase_end();
             }
             phase_end();
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const f32x4 aq = vec4(vec + kAq * kC, 16 * m), ak = vec4(vec + kAk * kC, 16 * m);
-                const f32x4 kb = vec4(vec + kKb * kC, 16 * m) * vec4(vec + kBe * kC, 16 * m);
+            for (int m = 0; m < 2; ++m) {
+                const f32x4 aq = vec4(vec + kAq * kC, r0 + 16 * m), ak = vec4(vec + kAk * kC, r0 + 16 * m);
+                const f32x4 kb = vec4(vec + kKb * kC, r0 + 16 * m) * vec4(vec + kBe * kC, r0 + 16 * m);
                 tq[m][n] += aq * cq[m];
                 tk[m][n] += kb * ck[m] - ak * cd[m];
             }
         }
-        TileRegs<T, DK, 256> rk, rq;
-        float part[8], anchor;                                // the slices' partial sums, all at once: a loop over them waited for each
-        auto load_rest = [&] {
-            rk.load((const T*)a.k + b * a.ks[1] + hk * a.ks[2], a.ks[0], a.dk, p0, w);
-            rq.load((const T*)a.q + b * a.qs[1] + hk * a.qs[2], a.qs[0], a.dk, p0, w);
-            const float* parts = wave == 0 ? a.zpart : a.bpart;      // the other waves load along
+        // M1 = dP * D * sq_i * rk_j (lower), M2 = -dV U^T * D * rk_i * rk_j (strictly lower, made symmetric); wc = block column j
+        f32x4 dp[2], dn[2];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) part[s] = parts[(min(s, a.nsl - 1) * nat + at) * kC + l];
-            anchor = a.apart[min(l & 7, a.nsl - 1) * nat + at];
-        };
-        // M1 = dP * D * sq_i * rk_j (lower), M2 = -dV U^T * D * rk_i * rk_j (strictly lower, made symmetric); wave = block column j
-        f32x4 dp[4], dn[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) { dp[m] = f32x4{0, 0, 0, 0}; dn[m] = dp[m]; }
+        for (int m = 0; m < 2; ++m) { dp[m] = f32x4{0, 0, 0, 0}; dn[m] = dp[m]; }
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
             if (kb * 32 < a.dv) {
-                const auto uf = row_frag(El, LDE, 16 * wave, 32 * kb);
-                typename FragOf<T>::type of[4], vf[4];
-                row_frags(of, Ol, LDV, 32 * kb);
-                row_frags(vf, Dl, LDV, 32 * kb);
+                const Frag<PE> uf = e_frag(16 * wc, kb);
+                Frag<PT> of[2], vf[2];
+                Frag<1> lf[2], u1;
+                u1.p[0] = uf.p[0];
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    of[m] = row_frag(Ol, LDV, r0 + 16 * m, 32 * kb);
+                    vf[m] = row_frag(Dl, LDV, r0 + 16 * m, 32 * kb);
+                    if constexpr (HALF) lf[m] = row_frag(Rl, LDV, r0 + 16 * m, 32 * kb);
+                }
                 if (PT == 1) phase_end();
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
+                for (int m = 0; m < 2; ++m) {
                     dp[m] = mma<PT, PE, OP>(of[m], uf, dp[m]);
                     dn[m] = mma<PT, PE, OP>(vf[m], uf, dn[m]);
+                    if constexpr (HALF) dn[m] = mma(lf[m], u1, dn[m]);
                 }
             }
             phase_end();
         }
-        if (EARLY) { load_rest(); phase_end(); }
+        if (!L::ROOM) load_keys();
+        float part[8], anchor;                                // the slices' partial sums, all at once: a loop over them waited for each
         {
-            const int j = 16 * wave + i16;
+            const float* parts = wave == 0 ? a.zpart : a.bpart;      // the other waves load along
+#pragma unroll
+            for (int s = 0; s < 8; ++s) part[s] = parts[(min(s, a.nsl - 1) * nat + at) * kC + l];
+            anchor = a.apart[min(l & 7, a.nsl - 1) * nat + at];
+        }
+        phase_end();
+        if (!L::ROOM) __syncthreads();                        // the matrix takes the values' place
+        {
+            const int j = 16 * wc + i16;
             const float rkj = vec[kRk * kC + j] * vec[kBe * kC + j];
             const double gj = G[j];
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const f32x4 sqi = vec4(vec + kSq * kC, 16 * m), rki = vec4(vec + kRk * kC, 16 * m);
+            for (int m = 0; m < 2; ++m) {
+                const f32x4 sqi = vec4(vec + kSq * kC, r0 + 16 * m), rki = vec4(vec + kRk * kC, r0 + 16 * m);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 16 * m + 4 * g + e;
+                    const int i = r0 + 16 * m + 4 * g + e;
                     const float d = __expf((float)(G[i] - gj)) * rkj;      // above the diagonal it may be infinite: selected away
                     const float p = dp[m][e] * d * sqi[e], n = -dn[m][e] * d * rki[e];
                     dp[m][e] = i >= j ? p : 0.f;
                     dn[m][e] = i > j ? n : 0.f;
                 }
-                plane_write<OP>(M, 16 * m, 16 * wave, dp[m]);
+                plane_write<OP>(M, r0 + 16 * m, 16 * wc, dp[m]);
                 phase_end();
             }
         }
-        __syncthreads();
-        {
-            if (!EARLY) load_rest();
-            if (wave == 0) {      // dg: lane = frame
-                float z = 0.f;
+        if (!L::ROOM) store_keys();
+        if (wave == 0) {      // dg: lane = frame
+            float z = 0.f;
 #pragma unroll
-                for (int s = 0; s < 8; ++s) z += s < a.nsl ? part[s] : 0.f;
-                float an = (l & 7) < a.nsl ? anchor : 0.f;
-                an += __shfl_xor(an, 1);
-                an += __shfl_xor(an, 2);
-                an += __shfl_xor(an, 4);
-                if (p0 + l >= w.len) z = 0.f;
+            for (int s = 0; s < 8; ++s) z += s < a.nsl ? part[s] : 0.f;
+            float an = (l & 7) < a.nsl ? anchor : 0.f;
+            an += __shfl_xor(an, 1);
+            an += __shfl_xor(an, 2);
+            an += __shfl_xor(an, 4);
+            if (p0 + l >= w.len) z = 0.f;
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) { const float u = __shfl_down(z, o); if (l + o < 64) z += u; }
-                if (p0 + l < w.len) {
-                    const int64_t o = w.frame(p0 + l) * gts + bh;
-                    a.gg[o] = a.fresh && p0 + l == 0 ? 0.f : z + an;
-                }
+            for (int o = 1; o < 64; o <<= 1) { const float u = __shfl_down(z, o); if (l + o < 64) z += u; }
+            if (p0 + l < w.len) {
+                const int64_t o = w.frame(p0 + l) * gts + bh;
+                a.gg[o] = a.fresh && p0 + l == 0 ? 0.f : z + an;
             }
-            if (wave == 1) {      // dbeta
-                float be = 0.f;
+        }
+        if (wave == 1) {      // dbeta
+            float be = 0.f;
 #pragma unroll
-                for (int s = 0; s < 8; ++s) be += s < a.nsl ? part[s] : 0.f;
-                if (p0 + l < w.len) a.gbeta[w.frame(p0 + l) * gts + bh] = be;
-            }
-            rk.store(Kl, LDK, a.dk, c * kC, w.len);
-            rq.store(Ql, LDK, a.dk, c * kC, w.len);
+            for (int s = 0; s < 8; ++s) be += s < a.nsl ? part[s] : 0.f;
+            if (p0 + l < w.len) a.gbeta[w.frame(p0 + l) * gts + bh] = be;
         }
         __syncthreads();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int n0 = (wave * NT + n) * 16;
+                const int n0 = (wc * NT + n) * 16;
                 const auto kf = col_frag(Kl, LDK, 32 * kb, n0);
                 const auto qf = col_frag(Ql, LDK, 32 * kb, n0);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    if (kb <= m / 2) tq[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, 16 * m, 32 * kb), kf, tq[m][n]);
-                    if (kb >= m / 2) tk[m][n] = mma<OP, PT, OP>(plane_cols<OP>(M, 32 * kb, 16 * m), qf, tk[m][n]);
+                for (int m = 0; m < 2; ++m) {
+                    if (kb <= wr) tq[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, r0 + 16 * m, 32 * kb), kf, tq[m][n]);
+                    if (kb >= wr) tk[m][n] = mma<OP, PT, OP>(plane_cols<OP>(M, 32 * kb, r0 + 16 * m), qf, tk[m][n]);
                 }
                 phase_end();
             }
         __syncthreads();
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            if (m < wave) continue;
-            if (m > wave) plane_write<OP>(M, 16 * m, 16 * wave, dn[m]);
+        for (int m = 0; m < 2; ++m) {
+            const int bi = 2 * wr + m;
+            if (bi < wc) continue;
+            if (bi > wc) plane_write<OP>(M, 16 * bi, 16 * wc, dn[m]);
             else {      // the diagonal block: its upper half is the transpose of its lower half
                 f32x4 t = dn[m];
 #pragma unroll
@@ -1279,18 +1356,18 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
                     for (int x = 0; x < 4; ++x) { const float v = __shfl(dn[m][x], (i16 >> 2) * 16 + i); if ((i16 & 3) == x) up = v; }
                     if (i < i16) t[e] = up;
                 }
-                plane_write<OP>(M, 16 * m, 16 * wave, t);
+                plane_write<OP>(M, 16 * bi, 16 * wc, t);
             }
-            if (m > wave) plane_write_t<OP>(M, 16 * m, 16 * wave, dn[m]);
+            if (bi > wc) plane_write_t<OP>(M, 16 * bi, 16 * wc, dn[m]);
         }
         __syncthreads();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const auto kf = col_frag(Kl, LDK, 32 * kb, (wave * NT + n) * 16);
+                const auto kf = col_frag(Kl, LDK, 32 * kb, (wc * NT + n) * 16);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) tk[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, 16 * m, 32 * kb), kf, tk[m][n]);
+                for (int m = 0; m < 2; ++m) tk[m][n] = mma<OP, PT, OP>(plane_rows<OP>(M, r0 + 16 * m, 32 * kb), kf, tk[m][n]);
                 phase_end();
             }
     }
@@ -1298,48 +1375,48 @@ __global__ __launch_bounds__(256, Gd<T>::PT == 1 && DK == 64 ? 2 : 1) void gdr_g
     // through the normalisation: dq = tq - q |q|^-2 (q . tq)  (|.|^2 with its epsilon), dk alike
     if (a.norm) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < 2; ++m) {
             f32x4 sq = {0, 0, 0, 0}, sk = {0, 0, 0, 0};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int n0 = (wave * NT + n) * 16;
-                sq += tq[m][n] * tile_read(Ql, LDK, 16 * m, n0);
-                sk += tk[m][n] * tile_read(Kl, LDK, 16 * m, n0);
+                const int n0 = (wc * NT + n) * 16;
+                sq += tq[m][n] * tile_read(Ql, LDK, r0 + 16 * m, n0);
+                sk += tk[m][n] * tile_read(Kl, LDK, r0 + 16 * m, n0);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) { sq[e] = row16_sum(sq[e]); sk[e] = row16_sum(sk[e]); }
             if (i16 == 0) {
-                *reinterpret_cast<f32x4a*>(dots + wave * kC + 16 * m + 4 * g) = sq;
-                *reinterpret_cast<f32x4a*>(dots + (4 + wave) * kC + 16 * m + 4 * g) = sk;
+                *reinterpret_cast<f32x4a*>(dots + wc * kC + r0 + 16 * m + 4 * g) = sq;
+                *reinterpret_cast<f32x4a*>(dots + (4 + wc) * kC + r0 + 16 * m + 4 * g) = sk;
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < 2; ++m) {
             f32x4 sq = {0, 0, 0, 0}, sk = {0, 0, 0, 0};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) { sq += vec4(dots + x * kC, 16 * m); sk += vec4(dots + (4 + x) * kC, 16 * m); }
-            const f32x4 rk = vec4(vec + kRk * kC, 16 * m), rq = vec4(vec + kSq * kC, 16 * m) * (1.f / a.scale);
+            for (int x = 0; x < 4; ++x) { sq += vec4(dots + x * kC, r0 + 16 * m); sk += vec4(dots + (4 + x) * kC, r0 + 16 * m); }
+            const f32x4 rk = vec4(vec + kRk * kC, r0 + 16 * m), rq = vec4(vec + kSq * kC, r0 + 16 * m) * (1.f / a.scale);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int n0 = (wave * NT + n) * 16;
-                tq[m][n] -= sq * rq * rq * tile_read(Ql, LDK, 16 * m, n0);
-                tk[m][n] -= sk * rk * rk * tile_read(Kl, LDK, 16 * m, n0);
+                const int n0 = (wc * NT + n) * 16;
+                tq[m][n] -= sq * rq * rq * tile_read(Ql, LDK, r0 + 16 * m, n0);
+                tk[m][n] -= sk * rk * rk * tile_read(Kl, LDK, r0 + 16 * m, n0);
             }
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            tile_write(Ql, LDK, 16 * m, (wave * NT + n) * 16, tq[m][n]);
-            tile_write(Kl, LDK, 16 * m, (wave * NT + n) * 16, tk[m][n]);
+            tile_write(Ql, LDK, r0 + 16 * m, (wc * NT + n) * 16, tq[m][n]);
+            tile_write(Kl, LDK, r0 + 16 * m, (wc * NT + n) * 16, tk[m][n]);
         }
     __syncthreads();
     constexpr int VE = 16 / sizeof(T);
     const int vpr = a.dk / VE;
-    for (int i = tid; i < kC * vpr; i += 256) {
+    for (int i = tid; i < kC * vpr; i += NTH) {
         const int row = i / vpr, col = (i % vpr) * VE, p = p0 + row;
         if (p >= w.len) continue;
         const int64_t t = w.frame(p);
@@ -1481,13 +1558,13 @@ static GdrLayout gdr_saved(int T, int B, int H, int dk, int dv, bool train) {
     return s;
 }
 struct GdrBwdLayout { size_t dS, E, z, b, a, end; };
-static GdrBwdLayout gdr_bwd_ws(int T, int B, int H, int dk, int dv, int dtype) {
+static GdrBwdLayout gdr_bwd_ws(int T, int B, int H, int dk, int dv) {
     GdrBwdLayout s{};
     const size_t n = (size_t)B * H * ((T + kC - 1) / kC), nsl = (dv + 15) / 16;
     size_t o = 0;
     auto put = [&](size_t bytes) { const size_t at = o; o = align_up(o + bytes, 256); return at; };
     s.dS = put(n * dk * dv * 4);
-    s.E = put(n * kC * dv * (dtype == SP_BF16 ? 2 : 4));
+    s.E = put(n * kC * dv * 4);
     s.z = put(n * nsl * kC * 4);
     s.b = put(n * nsl * kC * 4);
     s.a = put(n * nsl * 4);
@@ -1548,7 +1625,7 @@ template <typename T, int DK> static int gdr_backward(const GdrArgs& a, hipStrea
         return gdr_rscan<T, DK, 4>(a, s);
     };
     if (const int rc = walk()) return rc;
-    return gdr_launch(gdr_grads_kernel<T, DK>, GradLds<T, DK>::bytes, (int64_t)a.B * a.Hk * a.nc, 256, a, s, "gdr_grads_kernel");
+    return gdr_launch(gdr_grads_kernel<T, DK>, GradLds<T, DK>::bytes, (int64_t)a.B * a.Hk * a.nc, 512, a, s, "gdr_grads_kernel");
 }
 
 }  // namespace sp
@@ -1557,7 +1634,7 @@ using namespace sp;
 
 extern "C" size_t sp_gdr_workspace_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype, int backward) {
     if (gdr_check("sp_gdr_workspace_bytes", T, B, Hk, H, dk, dv, 0, dtype)) return 0;
-    return backward ? gdr_bwd_ws(T, B, H, dk, dv, dtype).end : gdr_saved(T, B, H, dk, dv, false).end;
+    return backward ? gdr_bwd_ws(T, B, H, dk, dv).end : gdr_saved(T, B, H, dk, dv, false).end;
 }
 extern "C" size_t sp_gdr_saved_bytes(int T, int B, int Hk, int H, int dk, int dv, int dtype) {
     if (gdr_check("sp_gdr_saved_bytes", T, B, Hk, H, dk, dv, 0, dtype)) return 0;
@@ -1622,7 +1699,7 @@ extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const flo
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype) &&
                      gdr_aligned(go, strides + 15, dtype), "sp_gdr_bwd: q, k, v, go need 16-byte aligned rows and at most 2^23 elements from frame to frame");
     const GdrLayout lay = gdr_saved(T, B, H, dk, dv, true);
-    const GdrBwdLayout ws = gdr_bwd_ws(T, B, H, dk, dv, dtype);
+    const GdrBwdLayout ws = gdr_bwd_ws(T, B, H, dk, dv);
     if (saved_bytes < lay.end || workspace_bytes < ws.end)
         return fail(SP_EWORKSPACE, "sp_gdr_bwd: saved %zu < %zu or workspace %zu < %zu bytes", saved_bytes, lay.end, workspace_bytes, ws.end);
     GdrArgs a{};
@@ -1632,7 +1709,7 @@ extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const flo
     a.go = go; a.gsT = gstate_out;
     for (int i = 0; i < 3; ++i) a.gos[i] = strides[15 + i];
     char* wb = (char*)workspace;
-    a.dS = (float*)(wb + ws.dS); a.E = wb + ws.E; a.zpart = (float*)(wb + ws.z); a.bpart = (float*)(wb + ws.b); a.apart = (float*)(wb + ws.a);
+    a.dS = (float*)(wb + ws.dS); a.E = (uint32_t*)(wb + ws.E); a.zpart = (float*)(wb + ws.z); a.bpart = (float*)(wb + ws.b); a.apart = (float*)(wb + ws.a);
     a.gq = gq; a.gk = gk; a.gv = gv; a.gg = gg; a.gbeta = gbeta; a.gs0 = gstate;
     hipStream_t s = (hipStream_t)stream;
     const bool wide = dk > 64;

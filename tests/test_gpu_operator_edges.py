@@ -29,3 +29,18 @@ def test_delta_output_is_rounded_once(cuda, dtype, T, B, Hk, r, dk, dv, train):
     o, _ = ops.gated_delta_rule(*dev[:5], state=dev[5], normalize=True)
     ro, _ = delta_reference(*(t.double() for t in args), None, dk ** -0.5, True, False)
     rounded_once(o, ro, "o")
+
+
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=ids)
+@pytest.mark.parametrize("T,B,Hk,r,dk,dv", [(200, 1, 2, 2, 64, 128), (200, 1, 1, 2, 128, 72), (70, 9, 16, 1, 16, 72)], ids=str)
+@pytest.mark.parametrize("normalize", [True, False])
+def test_delta_gradients_are_rounded_once(cuda, dtype, T, B, Hk, r, dk, dv, normalize):
+    from speech_amd import ops
+    args, go, gs = delta_inputs(T, B, Hk, r, dk, dv, dtype, 11)
+    dev, ref = [t.to(cuda).requires_grad_(True) for t in args], [t.double().requires_grad_(True) for t in args]
+    o, final = ops.gated_delta_rule(*dev[:5], state=dev[5], normalize=normalize)
+    ro, rf = delta_reference(*ref, None, dk ** -0.5, normalize, False)
+    got = torch.autograd.grad([o, final], dev[:3], [go.to(cuda), gs.to(cuda)])
+    want = torch.autograd.grad([ro, rf], ref[:3], [go.double(), gs.double()])
+    for name, u, w in zip(("dq", "dk", "dv"), got, want):
+        rounded_once(u, w, name)
