@@ -365,7 +365,8 @@ template <int NT> struct TriRegs {
         }
     }
 };
-// the blocks right of the diagonal that products over 32 columns touch: (0, 1) and (2, 3)
+// the blocks right of the diagonal that products over 32 columns touch: (0, 1) and (2, 3).  A loop that ends lane by lane: in front of
+// everything that lives in registers (see gdr_grads_kernel)
 __device__ __forceinline__ void clear_upper(__bf16* t, int planes, int tid, int nt) {
     for (int i = tid; i < planes * 64; i += nt) {
         const int pl = i >> 6, row = (i >> 1) & 31, half = i & 1;
@@ -644,6 +645,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     const int col0 = (sg * NW + wave) * 16;                        // this wave's columns of dv
     const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv;
+    clear_upper(Xl, 3 + OP, tid, NT);
     f32x4 S[KT];
 #pragma unroll
     for (int m = 0; m < KT; ++m) S[m] = f32x4{0, 0, 0, 0};
@@ -668,7 +670,6 @@ __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
     };
-    clear_upper(Xl, 3 + OP, tid, NT);
     if (ncl > 0) fetch(0);
     for (int c = 0; c < ncl; ++c) {
         const int64_t at = (int64_t)bh * a.nc + c;
@@ -820,6 +821,7 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
     const int slice = sg * NW + wave, col0 = slice * 16;
     const int vcols = min(a.dv - sg * NW * 16, NW * 16), mycols = a.dv - col0;
     const int64_t state = (int64_t)bh * a.dk * a.dv, nat = (int64_t)a.B * a.H * a.nc;
+    clear_upper(Xl, 6, tid, NT);
     f32x4 S[KT], s0n[KT];                                   // dS; the next chunk's starting state
 #pragma unroll
     for (int m = 0; m < KT; ++m) S[m] = f32x4{0, 0, 0, 0};
@@ -847,7 +849,6 @@ __global__ __launch_bounds__(NW * 64) void gdr_rscan_kernel(GdrArgs a) {
 #pragma unroll
         for (int i = 0; i < kVec * kC / NT; ++i) rvec[i] = a.vec[at * kVec * kC + i * NT + tid];
     };
-    clear_upper(Xl, 6, tid, NT);
     if (ncl > 0) fetch(ncl - 1);
     for (int c = ncl - 1; c >= 0; --c) {
         const int64_t at = (int64_t)bh * a.nc + c;
