@@ -916,9 +916,16 @@ def _same_device(x, **others):
             raise ValueError(f"{name} is on {t.device}, the input on {dev}")
 
 
+def _dual(*tensors):
+    """Whether a tensor carries a forward-mode tangent (one test of an integer outside forward_ad.dual_level)."""
+    fwd = torch.autograd.forward_ad
+    return fwd._current_level >= 0 and any(t is not None and fwd.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _wants_grad(*tensors):
-    """Whether autograd has to see the call; without, the kernels are called directly (a Function's apply costs a small kernel's time)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether autograd has to see the call; without, the kernels are called directly (a Function's apply costs a small kernel's time).  A
+    tangent has to be seen too: apply refuses it (NotImplementedError), a direct call would drop it, which stands for zero."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or _dual(*tensors)
 
 
 def _once(what):
@@ -1296,6 +1303,8 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None, normalize=False):
         raise ValueError("state must be a contiguous, 16-byte aligned tensor: it is updated in place")
     if state.requires_grad:
         raise ValueError("state requires a gradient: gated_delta_step updates it in place and is not differentiable")
+    if _dual(q, k, v, g, beta, state):
+        raise NotImplementedError("gated_delta_step has no derivative: a forward-mode tangent cannot pass through it")
     scale = dk ** -0.5 if scale is None else float(scale)
     if scale == 0.0 or not math.isfinite(scale):
         raise ValueError(f"scale must be finite and not zero, got {scale}")

@@ -44,3 +44,29 @@ def test_delta_gradients_are_rounded_once(cuda, dtype, T, B, Hk, r, dk, dv, norm
     want = torch.autograd.grad([ro, rf], ref[:3], [go.double(), gs.double()])
     for name, u, w in zip(("dq", "dk", "dv"), got, want):
         rounded_once(u, w, name)
+
+
+# ------------------------------------------------------------------------------------------ calls that are refused
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(cuda, grad):
+    """No operator has a forward-mode derivative: a dual tensor raises, in whichever argument it comes, with and without gradient mode."""
+    import torch.autograd.forward_ad as fwd
+    from speech_amd import ops
+    x, w = torch.randn(4, 6, 16, device=cuda), torch.ones(16, device=cuda)
+    q, g = torch.randn(20, 2, 2, 16, device=cuda), -torch.rand(20, 2, 2, device=cuda)
+    state, rng = torch.zeros(2, 2, 16, 16, device=cuda), ops.dropout_rng(1, cuda)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))      # noqa: E731
+        calls = [lambda: ops.group_norm(dual(x), w, w, 4), lambda: ops.group_norm(x, dual(w), w, 4), lambda: ops.group_norm(x, w, dual(w), 4),
+                 lambda: ops.group_norm(x, w, w, 4, residual=dual(x)), lambda: ops.dropout(dual(x), 0.5, rng), lambda: ops.dropout(x, 0.5, rng, residual=dual(x))]
+        for T in (20, 5):
+            a = (q[:T], q[:T], q[:T], g[:T], -g[:T], state)
+            calls += [lambda a=a, i=i: ops.gated_delta_rule(*(dual(t) if j == i else t for j, t in enumerate(a))) for i in range(6)]
+        a = (q[0], q[0], q[0], g[0], -g[0], state)
+        calls += [lambda i=i: ops.gated_delta_step(*(dual(t) if j == i else t for j, t in enumerate(a))) for i in range(6)]
+        for i, call in enumerate(calls):
+            with pytest.raises(NotImplementedError):
+                call()
+                raise AssertionError(i)
+        # what carries no tangent still runs inside the level
+        assert torch.isfinite(ops.group_norm(x, w, w, 4)).all() and torch.isfinite(ops.gated_delta_step(*a)).all()
