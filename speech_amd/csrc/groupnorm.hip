@@ -6,14 +6,16 @@
 //
 // HBM-bound: forward reads x (and the residual) and writes y; the statistics need x before the first output, so x is read twice -- the
 // second time from the Infinity Cache at the conv stack's size (61 MB).  The backward reads gy, x and the residual twice for the same reason.
-// Measured at [32][40][751][32] bf16 with SiLU and residual: statistics 17 us, apply 32 (5.8 TB/s), backward statistics 44 (5.6), backward
+// Measured at [32][40][751][32] bf16 with SiLU and residual: statistics 18.6 us, apply 32 (5.8 TB/s), backward statistics 44 (5.6), backward
 // apply 43 (5.7); rows, 24032 x 1024 bf16, 8 groups: forward 22 us (4.5 TB/s), backward 36 (4.1) + 7.4 for the parameters' gradients.
 // Two routes, chosen by the shape alone:
 //   rows    one position a sample (F * T == 1): a (sample, group) is a contiguous segment that a team of lanes holds in registers; one
 //           read, one write, two-pass statistics.
 //   blocks  everything else: a statistics kernel over (sample, split) and an apply kernel that merges the splits' partials itself.
-// Statistics: every thread sums differences to its own first value, (count, mean, M2) triples are merged as sums of w * mean and of
-// M2 + w * (mean - mean_all)^2: a large mean or a click in the first frame costs no digits.  All sums are f32 in a fixed order.
+// Statistics: a thread takes kU positions at a time as a triple (count, mean, M2 around that mean) and adds it to its own by Chan's formula;
+// triples of threads and splits are merged as sums of w * mean and of M2 + w * (mean - mean_all)^2.  Every term of M2 is positive and nothing
+// is subtracted from it: a large mean costs no digits, nor does a click, in the first frame or elsewhere.  (One sum of squares of differences to
+// the first value lost them where that value was the click: 1.4e-4 of rstd after 469 positions.)  All sums are f32 in a fixed order.
 #include "common.h"
 
 namespace sp {
@@ -158,10 +160,10 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
     for (int cb = 0; cb < nch; cb += cpb) {
         const int chunk = cb + threadIdx.x % cpb;
         const bool on = row < rows && chunk < nch;
-        float k[VW], sm[VW], sq[VW];
+        float mean[VW], sq[VW];
         int cnt = 0;
 #pragma unroll
-        for (int i = 0; i < VW; ++i) { k[i] = 0.f; sm[i] = 0.f; sq[i] = 0.f; }
+        for (int i = 0; i < VW; ++i) { mean[i] = 0.f; sq[i] = 0.f; }
         if (on) {
             const T* base = x + chunk * VW;
             GnWalk w(lo + row, hi, rows, s.T);
@@ -169,39 +171,51 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
             while (w.more()) {
                 GnRaw<T, VW> raw[kU];
                 bool on[kU];
+                int nb = 0;
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
                     on[u] = w.more() && w.t < len;
+                    nb += on[u];
                     raw[u] = *reinterpret_cast<const GnRaw<T, VW>*>(base + px.at(on[u]));
                     gn_next(w, px);
                 }
+                if (nb == 0) continue;
+                const float rb = 1.f / (float)nb, part = (float)nb / (float)(cnt + nb), rest = (float)cnt * part;
+                cnt += nb;
+                float mb[VW], d[kU][VW];
+#pragma unroll
+                for (int i = 0; i < VW; ++i) mb[i] = 0.f;
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    if (!on[u]) continue;
-                    float v[VW];
-                    gn_get<T, VW>(raw[u], v);
-                    if (cnt == 0) {
+                    gn_get<T, VW>(raw[u], d[u]);
 #pragma unroll
-                        for (int i = 0; i < VW; ++i) k[i] = v[i];
+                    for (int i = 0; i < VW; ++i) {
+                        d[u][i] = on[u] ? d[u][i] : 0.f;
+                        mb[i] += d[u][i];
                     }
-                    ++cnt;
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) { const float d = v[i] - k[i]; sm[i] += d; sq[i] += d * d; }
                 }
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    mb[i] *= rb;
+                    const float away = mb[i] - mean[i];
+                    mean[i] += away * part;
+                    sq[i] += away * away * rest;
+                }
+#pragma unroll
+                for (int u = 0; u < kU; ++u)
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) {
+                        const float e = on[u] ? d[u][i] - mb[i] : 0.f;
+                        sq[i] += e * e;
+                    }
             }
         }
-        const float inv = cnt ? 1.f / (float)cnt : 0.f;
         // positions below p that are counted: whole bands of len frames and the last one's
         const auto counted = [&](int p) { return p / s.T * len + min(p % s.T, len); };
         const float c_all = hi > lo ? (float)(counted(hi) - counted(lo)) : 0.f;
-        float mean[VW], sum[VW];
+        float sum[VW];
 #pragma unroll
-        for (int i = 0; i < VW; ++i) {
-            mean[i] = k[i] + sm[i] * inv;
-            sum[i] = (float)cnt * mean[i];
-            sq[i] -= sm[i] * sm[i] * inv;
-            if (sq[i] < 0.f) sq[i] = 0.f;
-        }
+        for (int i = 0; i < VW; ++i) sum[i] = (float)cnt * mean[i];
         __syncthreads();                                       // the pass before has read its sums
         const int nw = gn_row_sums<VW>(sum, red, cpb, row, rows);
         // channels of this pass: [cb * VW, cb * VW + cpb * VW); a group may span passes only when VW == 1 (C > 256): see below

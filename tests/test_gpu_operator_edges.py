@@ -70,3 +70,29 @@ def test_forward_mode_tangents_are_refused(cuda, grad):
                 raise AssertionError(i)
         # what carries no tangent still runs inside the level
         assert torch.isfinite(ops.group_norm(x, w, w, 4)).all() and torch.isfinite(ops.gated_delta_step(*a)).all()
+
+
+# ------------------------------------------------------------------------------------------ group norm: threads that walk far
+@pytest.mark.parametrize("shape", [(1, 30, 1000, 257), (385, 1, 300, 129)], ids=str)
+@pytest.mark.parametrize("click,offset", [(1e4, 0.0), (-3e4, 50.0)])
+def test_group_norm_click_in_a_long_walk(cuda, shape, click, offset):
+    """One channel a group, the first frame of every sample a click: with 257 and 129 channels a workgroup has one row of threads, a thread walks
+    469 and 300 positions, and its first one is the click.  The variance is a sum of positive terms in a chain of 118 steps of four positions
+    with three roundings each, and rstd halves the relative error: 177 half steps of f32, with fewer than 64 of the merging and the rest 256.
+    The mean of a walk: a step rounds a mean of size |offset| + 8 + K / n twice, and an error made after n of N positions reaches the walk's end
+    as its share n / N: over 118 steps at most 118 half steps of |offset| + 8 and half a half step of the click K, times the walk's share of
+    the sample."""
+    from speech_amd import ops
+    N, F, T, C = shape
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(*shape, generator=g) + offset
+    x[:, 0, 0] = click
+    w, b = torch.ones(C), torch.zeros(C)
+    y = ops.group_norm(x.to(cuda), w.to(cuda), b.to(cuda), C).double().cpu()
+    v = x.double()
+    m = v.mean((1, 2), keepdim=True)
+    rstd = 1 / torch.sqrt(((v - m) ** 2).mean((1, 2), keepdim=True) + 1e-5)
+    want = (v - m) * rstd
+    walk = 469 / 30000 if N == 1 else 1.0
+    bound = 256 * 2.0 ** -24 * want.abs() + 2.0 ** -24 * (128 * (abs(offset) + 8) + abs(click) * walk) * rstd
+    assert ((y - want).abs() <= bound).all(), float(((y - want).abs() / want.abs().clamp_min(1e-6)).max())
