@@ -218,7 +218,8 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(const T* __restric
         for (int i = 0; i < VW; ++i) sum[i] = (float)cnt * mean[i];
         __syncthreads();                                       // the pass before has read its sums
         const int nw = gn_row_sums<VW>(sum, red, cpb, row, rows);
-        // channels of this pass: [cb * VW, cb * VW + cpb * VW); a group may span passes only when VW == 1 (C > 256): see below
+        // channels of this pass: [cb * VW, cb * VW + cpb * VW); with more than 256 chunks (VW 1, 2 and 4 with C > 256, 512 and 1024) a group may lie in
+        // two passes, each of which writes a triple for its part of the channels
         const int c0 = cb * VW, c1 = min(s.C, c0 + cpb * VW);
         const int g0 = c0 / s.Cg, g1 = (c1 - 1) / s.Cg;
         const float winv = c_all > 0.f ? 1.f / c_all : 0.f;

@@ -3,7 +3,7 @@ form, padding that must have no influence, calls that must be refused.  Referenc
 import pytest
 import torch
 
-from test_gpu_operators import DTYPES, delta_inputs, delta_reference, ids
+from test_gpu_operators import DTYPES, close, delta_inputs, delta_reference, gn_inputs, gn_reference, ids
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,98 @@ def test_group_norm_click_in_a_long_walk(cuda, shape, click, offset):
     walk = 469 / 30000 if N == 1 else 1.0
     bound = 256 * 2.0 ** -24 * want.abs() + 2.0 ** -24 * (128 * (abs(offset) + 8) + abs(click) * walk) * rstd
     assert ((y - want).abs() <= bound).all(), float(((y - want).abs() / want.abs().clamp_min(1e-6)).max())
+
+
+def _gn_compare(cuda, x, w, b, r, gy, G, act, lengths=None, xd=None, rd=None, gyd=None, time_major=False):
+    """Values and gradients against the 64-bit statement; xd, rd, gyd: the same tensors on the GPU in another layout."""
+    from speech_amd import ops
+    xd, rd = ((t if d is None else d) for t, d in ((x.to(cuda), xd), (r.to(cuda) if r is not None else None, rd)))
+    gyd = gy.to(cuda) if gyd is None else gyd
+    leaves = [t.detach().requires_grad_(True) for t in (xd, w.to(cuda), b.to(cuda), rd) if t is not None]
+    L = None if lengths is None else torch.tensor(lengths, device=cuda)
+    y = ops.group_norm(*leaves[:3], G, act=act, residual=leaves[3] if rd is not None else None, lengths=L, time_major=time_major)
+    ref = [t.double().requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    ry = gn_reference(*ref[:3], G, act, ref[3] if r is not None else None, lengths)
+    got, want = torch.autograd.grad(y, leaves, gyd), torch.autograd.grad(ry, ref, gy.double())
+    scale = float(ry.detach().abs().max()) + 8
+    # chains: a thread's positions (at most 32 here) four at a time, eight rows of partial results, trees: fewer than 256 roundings
+    close(y, ry, scale, 256, what="y")
+    terms = float(gy.abs().max() * w.abs().max()) * 6 * 2       # rstd is below 2 for these inputs (spread 1.5)
+    close(got[0], want[0], terms, 512, what="dx")
+    m = x[..., 0].numel()
+    for k in (1, 2):      # sums of m terms of size <= 8 gy, in chains of 32 positions, 96 rows a chain behind them and trees
+        close(got[k], want[k], float(gy.abs().max()) * 8 * m ** 0.5 + float(want[k].abs().max()), 512, torch.float32, "parameters")
+    if rd is not None:
+        close(got[3], want[3], float(gy.abs().max()) * 2, 64, what="dres")
+    return y, got
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("layout", ["dense", "gaps", "time_major"])
+def test_group_norm_long_walks(cuda, dtype, ragged, layout):
+    """150 samples of 7 bands of 101 frames, 64 channels: splits of 142 positions, 32 rows of threads, four and a half positions a thread; a walk
+    crosses the ends of bands.  gaps: bands and frames with memory between them; time_major: gradients arrive in the order that the result was
+    written in."""
+    x, w, b, r, gy = gn_inputs((150, 7, 101, 64), dtype, 4, True)
+    lengths = [101 - (n * 37) % 102 if n % 2 else 101 for n in range(150)] if ragged else None
+    kw = {}
+    if layout == "gaps":
+        def spread(t):
+            base = torch.full((150, 9, 104, 80), float("nan"), dtype=dtype, device=cuda)
+            base[:, 1:8, 2:103, 8:72] = t.to(cuda)
+            return base[:, 1:8, 2:103, 8:72]
+        kw = dict(xd=spread(x), rd=spread(r), gyd=spread(gy))
+    elif layout == "time_major":
+        kw = dict(time_major=True, gyd=gy.to(cuda).permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3))
+    y, got = _gn_compare(cuda, x, w, b, r, gy, 8, "silu", lengths, **kw)
+    if layout == "time_major":
+        assert y.permute(2, 0, 1, 3).is_contiguous()
+    if ragged:
+        for n, v in enumerate(lengths):
+            assert not y[n, :, v:].any() and not got[0][n, :, v:].any() and not got[3][n, :, v:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("res,act", [(True, "silu"), (False, "none")])
+def test_group_norm_rows_in_turn(cuda, dtype, res, act):
+    """40000 samples of one position, 256 channels in 8 groups: a team of lanes takes two or three units forwards and six or seven backwards,
+    each one's loads ahead of the one before, the parameters' gradients summed in registers on the way."""
+    x, w, b, r, gy = gn_inputs((40000, 1, 1, 256), dtype, 5, res)
+    _gn_compare_rows(cuda, x, w, b, r, gy, 8, act)
+
+
+def _gn_compare_rows(cuda, x, w, b, r, gy, G, act):
+    from speech_amd import ops
+    leaves = [t.to(cuda).requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    y = ops.group_norm(*leaves[:3], G, act=act, residual=leaves[3] if r is not None else None)
+    ref = [t.double().requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    v = ref[0].unflatten(-1, (G, -1))
+    m = v.mean(-1, keepdim=True)
+    z = ((v - m) / torch.sqrt(((v - m) ** 2).mean(-1, keepdim=True) + 1e-5)).flatten(-2) * ref[1] + ref[2]
+    z = z + ref[3] if r is not None else z
+    ry = z * torch.sigmoid(z) if act == "silu" else z
+    got, want = torch.autograd.grad(y, leaves, gy.to(cuda)), torch.autograd.grad(ry, ref, gy.double())
+    close(y, ry, float(ry.detach().abs().max()) + 8, 128, what="y")
+    rstd = float((1 / torch.sqrt(v.detach().var(-1, unbiased=False) + 1e-5)).max())
+    close(got[0], want[0], rstd * float(gy.abs().max() * w.abs().max()) * 6, 256, what="dx")
+    for k in (1, 2):
+        close(got[k], want[k], float(gy.abs().max()) * 8 * x.shape[0] ** 0.5 + float(want[k].abs().max()), 512, torch.float32, "parameters")
+    if r is not None:
+        close(got[3], want[3], float(gy.abs().max()) * 2, 64, what="dres")
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 40, 2048, 1), (2, 2, 20, 2040, 3), (3, 1, 33, 1026, 2)], ids=str)
+@pytest.mark.parametrize("offset", [2, 4])
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+def test_group_norm_several_passes_of_channels(cuda, dtype, shape, offset):
+    """Tensors aligned to two or four elements only: more chunks of channels than a workgroup has threads, and groups that lie in two passes."""
+    *s, G = shape
+    x, w, b, r, gy = gn_inputs(s, dtype, 6, True)
+
+    def shift(t):
+        base = torch.empty(t.numel() + 8, dtype=dtype, device=cuda)
+        v = base[offset:offset + t.numel()].view(t.shape)
+        v.copy_(t.to(cuda))
+        return v
+    _gn_compare(cuda, x, w, b, r, gy, G, "silu", None, shift(x), shift(r), shift(gy))
