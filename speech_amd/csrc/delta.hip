@@ -1585,8 +1585,14 @@ template <typename K> static int gdr_launch(K kernel, size_t lds, int64_t blocks
 }
 
 // Columns of dv a workgroup of the scans owns: 128 in eight waves (a head's K, Q and matrices are then staged once), or 64 in four where the
-// eight would leave CUs idle that the four fill: up to 128 heads.  T = 751, bf16, dk 64, dv 128, wide against narrow: 160 heads scan 84 us
-// against 126, reverse scan 182 against 245; 256 heads 98 against 141 and 215 against 264; 64 heads 70 against 59 and 147 against 117.
+// eight would leave CUs idle that the four fill: up to 128 heads.  T = 751, dv 128, both directions, wide against narrow in us, forward (prep
+// and scan) and backward (reverse scan and gradients):
+//   heads          128                  136                  256
+//   bf16 dk 64     147/139  338/299     153/194  374/435     171/215  476/536
+//   f16 dk 64      180/157  398/353     183/228  420/530     205/252  538/643
+//   f32 dk 64      210/183  -           215/274  -           268/315  -
+//   bf16 dk 128    182/170  -           188/242  -           225/282  -
+//   f16 dk 128     248/213  -           254/323  -           296/367  -
 // Eight waves have 256 registers each.  Where the tiles do not fit those, the narrow form is the faster one at 256 heads as well: the
 // reverse scan of dk 128 (bf16 400 us against 358, f16 700 against 525) and of f32 (dk 64: 488 against 420; dk 128 exceeds the LDS), the
 // scan of f32 at dk 128 (373 against 358).

@@ -191,3 +191,80 @@ def test_group_norm_several_passes_of_channels(cuda, dtype, shape, offset):
         v.copy_(t.to(cuda))
         return v
     _gn_compare(cuda, x, w, b, r, gy, G, "silu", None, shift(x), shift(r), shift(gy))
+
+
+# ------------------------------------------------------------------------------------------ the scans' wide form
+def heads_reference(args, lengths, bidirectional, go=None, gs=None):
+    """The gated delta rule (q and k normalised) frame by frame in 64 bits, all heads of all utterances at once."""
+    q, k, v, g, beta, S = (t.double().requires_grad_(go is not None) for t in args)
+    leaves = [q, k, v, g, beta, S]
+    T, B, Hk, dk = q.shape
+    H = v.shape[2]
+    n = torch.tensor(lengths)
+    t = torch.arange(T)[:, None]
+    back = torch.where(t < n, n - 1 - t, t)                       # [T, B]: an utterance's own frames backwards
+
+    def turn(x):
+        if not bidirectional:
+            return x
+        h = x.shape[2] // 2
+        at = back.view(T, B, 1, *[1] * (x.dim() - 3)).expand(T, B, h, *x.shape[3:])
+        return torch.cat([x[:, :, :h], torch.gather(x[:, :, h:], 0, at)], 2)
+    qh, kh = (x / torch.sqrt((x * x).sum(-1, keepdim=True) + 1e-6) for x in (q, k))
+    qh, kh = (turn(x).repeat_interleave(H // Hk, 2) for x in (qh * dk ** -0.5, kh))
+    vh, gh, bh = turn(v), turn(g), turn(beta)
+    out = []
+    for i in range(T):
+        on = (i < n).view(B, 1, 1)
+        s1 = torch.exp(gh[i])[..., None, None] * S
+        u = bh[i][..., None] * (vh[i] - (kh[i][..., None] * s1).sum(-2))
+        s1 = s1 + kh[i][..., None] * u[..., None, :]
+        out.append(torch.where(on, (qh[i][..., None] * s1).sum(-2), 0.0))
+        S = torch.where(on[..., None], s1, S)
+    o = turn(torch.stack(out))
+    if go is None:
+        return [o.detach(), S.detach()]
+    clean = torch.where((t < n)[..., None, None], go.double(), 0.0)
+    return [o.detach(), S.detach(), *torch.autograd.grad([o, S], leaves, [clean, gs.double()])]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("dk", [64, 72, 128])
+@pytest.mark.parametrize("dv", [72, 128])
+@pytest.mark.parametrize("train", [False, True])
+def test_delta_wide_scans(cuda, dtype, dk, dv, train):
+    """More than 128 heads and columns: scans of eight waves.  17 utterances of 8 heads, three chunks, ragged, both directions.  Three utterances
+    against the 64-bit statement (bounds as in test_gpu_operators.delta_check, 16-bit results as rounded_once), all of them against the same
+    utterances in two calls of the narrow form: the same sums in the same order but for what the compiler joins to a multiply-add, so
+    within the same f32 bound, and a 16-bit result within two roundings of it."""
+    from speech_amd import ops
+    T, B = 150, 17
+    args, go, gs = delta_inputs(T, B, 8, 1, dk, dv, dtype, 21, unit=False)
+    lengths = [150 - (b * 29) % 151 if b % 3 else 150 for b in range(B)]
+    lengths[1], lengths[16] = 0, 129
+
+    def run(sel):
+        xs = [(t[sel] if i == 5 else t[:, sel]).to(cuda).requires_grad_(train) for i, t in enumerate(args)]
+        o, f = ops.gated_delta_rule(*xs[:5], state=xs[5], lengths=torch.tensor(lengths)[sel].to(cuda), normalize=True, bidirectional=True)
+        out = [o, f]
+        if train:
+            out += torch.autograd.grad([o, f], xs, [go[:, sel].to(cuda), gs[sel].to(cuda)])
+        return [t.detach().cpu() for t in out]
+    wide = run(slice(0, B))
+    halves = [run(slice(0, 8)), run(slice(8, B))]
+    which = lambda i: 0 if i in (1, 7) else 1      # noqa: E731      # the batch dimension: states [B, ..], everything else [T, B, ..]
+    f32 = 64 * 2.0 ** -24
+    names = ["o", "final", "dq", "dk", "dv", "dg", "dbeta", "dstate"]
+    for i, u in enumerate(wide):
+        w = torch.cat([h[i] for h in halves], which(i)).double()
+        bound = 4 * f32 + (0 if u.dtype == torch.float32 else 2 * torch.finfo(dtype).eps / 2)
+        assert torch.isfinite(u).all() and float((u.double() - w).norm() / w.norm()) <= bound, ("narrow", names[i])
+    some = [0, 2, 16]
+    part = [t[some] if i == 5 else t[:, some] for i, t in enumerate(args)]
+    ref = heads_reference(part, [lengths[b] for b in some], True, *((go[:, some], gs[some]) if train else ()))
+    for i, w in enumerate(ref):
+        u = wide[i][some] if which(i) == 0 else wide[i][:, some]
+        if u.dtype == torch.float32:
+            assert float((u.double() - w).norm() / w.norm()) <= (f32 if i < 2 else 4 * f32), (names[i], float((u.double() - w).norm() / w.norm()))
+        else:
+            rounded_once(u, w, names[i])
