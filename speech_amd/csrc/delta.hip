@@ -1695,14 +1695,14 @@ extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const flo
 
 extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const float* g, const float* beta, const int32_t* lengths,
                           const int64_t* strides, int T, int B, int Hk, int H, int dk, int dv, float scale, int flags, int dtype,
-                          const void* o, const void* saved, size_t saved_bytes, const void* go, const float* gstate_out, void* gq, void* gk,
+                          const void* /* o */, const void* saved, size_t saved_bytes, const void* go, const float* gstate_out, void* gq, void* gk,
                           void* gv, float* gg, float* gbeta, float* gstate, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = gdr_check("sp_gdr_bwd", T, B, Hk, H, dk, dv, flags & ~SP_GDR_NO_STATE, dtype);
     if (rc) return rc;
     if (B == 0) return SP_OK;
     SP_CHECK_ARG(scale != 0.f, "sp_gdr_bwd: scale is zero");
     SP_CHECK_ARG(T > 0, "sp_gdr_bwd: T=0 has nothing to differentiate");
-    SP_CHECK_ARG(q && k && v && g && beta && strides && o && saved && go && gq && gk && gv && gg && gbeta && workspace, "sp_gdr_bwd: null pointer");
+    SP_CHECK_ARG(q && k && v && g && beta && strides && saved && go && gq && gk && gv && gg && gbeta && workspace, "sp_gdr_bwd: null pointer");
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype) &&
                      gdr_aligned(go, strides + 15, dtype), "sp_gdr_bwd: q, k, v, go need 16-byte aligned rows and at most 2^23 elements from frame to frame");
     const GdrLayout lay = gdr_saved(T, B, H, dk, dv, true);

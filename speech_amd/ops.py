@@ -1191,7 +1191,7 @@ class _GatedDeltaFn(torch.autograd.Function):
         T, B, Hk, H, dk, dv = dims
         final = g.new_empty((B, H, dk, dv))
         o, saved = _gdr_fwd(q, k, v, g, beta, state, final, lengths, dims, _strides(q, k, v, g, beta), scale, flags, True)
-        ctx.save_for_backward(q, k, v, g, beta, lengths, o, saved)
+        ctx.save_for_backward(q, k, v, g, beta, lengths, saved)      # not o: a caller may change it in place
         ctx.cfg = (dims, scale, flags | (_lib.GDR_NO_STATE if state is None else 0))
         ctx.set_materialize_grads(False)
         return o, final
@@ -1199,11 +1199,11 @@ class _GatedDeltaFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, go, gstate):
         _once("gated_delta_rule")
-        q, k, v, g, beta, lengths, o, saved = ctx.saved_tensors
+        q, k, v, g, beta, lengths, saved = ctx.saved_tensors
         dims, scale, flags = ctx.cfg
         T, B, Hk, H, dk, dv = dims
         code = _CODE[q.dtype]
-        go = _head_rows(go) if go is not None else torch.zeros_like(o)
+        go = _head_rows(go) if go is not None else v.new_zeros((T, B, H, dv))
         gstate = gstate.contiguous() if gstate is not None else None
         gq, gk = q.new_empty((T, B, Hk, dk)), q.new_empty((T, B, Hk, dk))
         gv = v.new_empty((T, B, H, dv))
@@ -1213,7 +1213,7 @@ class _GatedDeltaFn(torch.autograd.Function):
         ws = saved.new_empty(n)
         with on_device(q):
             rc = lib().sp_gdr_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), addr(lengths),
-                                  _strides(q, k, v, g, beta, go), T, B, Hk, H, dk, dv, scale, flags, code, o.data_ptr(), saved.data_ptr(),
+                                  _strides(q, k, v, g, beta, go), T, B, Hk, H, dk, dv, scale, flags, code, None, saved.data_ptr(),
                                   saved.numel(), go.data_ptr(), addr(gstate), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), gg.data_ptr(),
                                   gb.data_ptr(), addr(gs0), ws.data_ptr(), n, raw_stream(q))
         check(rc, "sp_gdr_bwd")

@@ -268,3 +268,19 @@ def test_delta_wide_scans(cuda, dtype, dk, dv, train):
             assert float((u.double() - w).norm() / w.norm()) <= (f32 if i < 2 else 4 * f32), (names[i], float((u.double() - w).norm() / w.norm()))
         else:
             rounded_once(u, w, names[i])
+
+
+# ------------------------------------------------------------------------------------------ what a caller may do with a result
+def test_delta_output_may_be_changed_in_place(cuda):
+    """The backward does not need o: a mask multiplied into it in place is differentiated like one multiplied out of place."""
+    from speech_amd import ops
+    args, go, gs = delta_inputs(70, 2, 2, 2, 16, 24, torch.float32, 12)
+    mask = (torch.rand(70, 2, 4, 24, generator=torch.Generator().manual_seed(0)) > 0.3).float().to(cuda)
+    grads = []
+    for inplace in (True, False):
+        xs = [t.to(cuda).requires_grad_(True) for t in args]
+        o, f = ops.gated_delta_rule(*xs[:5], state=xs[5], normalize=True)
+        o = o.mul_(mask) if inplace else o * mask
+        f = f.mul_(0.5) if inplace else f * 0.5
+        grads.append(torch.autograd.grad([o, f], xs, [go.to(cuda), gs.to(cuda)]))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -1,0 +1,28 @@
+"""Edges of the encoder operators that need no GPU: what the C ABI checks on the host before anything is launched (no address is followed),
+the build's dependencies, the models' arguments."""
+import ctypes
+
+import pytest
+
+P = 4096          # an aligned address that is never read
+
+
+def i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+@pytest.fixture(scope="module")
+def h():
+    from speech_amd import _lib
+    return _lib.lib()
+
+
+STRIDES = i64(*([256, 128, 64] * 2 + [512, 256, 64] + [8, 4, 1] * 2 + [512, 256, 64]))
+
+
+def _gdr_bwd(h, o=P, saved=P, go=P, gq=P, gk=P, gv=P, ws=P, nws=1 << 40):
+    return h.sp_gdr_bwd(P, P, P, P, P, None, STRIDES, 40, 2, 2, 4, 64, 64, 1.0, 0, 2, o, saved, 1 << 40, go, None, gq, gk, gv, P, P, None, ws, nws, None)
+
+
+def test_gated_delta_backward_does_not_ask_for_o(h):
+    assert _gdr_bwd(h, o=None, nws=16) == -2 and b"workspace" in h.sp_last_error()      # past the check of addresses, refused for its workspace
