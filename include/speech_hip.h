@@ -404,7 +404,8 @@ int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period
  * a head, addresses and strides aligned to 16 bytes, frames at most 2^23 elements apart (a forward of up to 12 frames without `saved` takes
  * any); state, state_out, o aligned to 16 bytes.  B * H <= 65536.
  * saved: NULL (inference), or sp_gdr_saved_bytes() device bytes that the forward fills and the backward reads; workspace:
- * sp_gdr_workspace_bytes(.., backward), for an inference forward and for the backward (a forward with `saved` needs none).
+ * sp_gdr_workspace_bytes(.., backward), for an inference forward and for the backward (a forward with `saved` needs none).  T = 0: the state is
+ * copied (or zeros written), `saved` is left as it was.
  * Backward: go = d loss / d o, gstate_out = d loss / d state_out or NULL; writes gq, gk [T][B][Hk][dk], gv [T][B][H][dv] (dense, dtype), gg,
  * gbeta f32 [T][B][H] dense, gstate f32 or NULL; frames behind an utterance's end get zeros.  T >= 1.  Results are bit-reproducible.  o is not
  * read (it is formed again) and may be NULL.

@@ -1664,7 +1664,7 @@ extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const flo
     a.s0 = state; a.sT = state_out; a.o = o;
     hipStream_t s = (hipStream_t)stream;
     const bool train = saved != nullptr;
-    if (!train && T <= kRecurrentMax) {       // T = 0: the state is copied
+    if (T == 0 || (!train && T <= kRecurrentMax)) {       // T = 0: the state is copied, and nothing to save
         const int64_t blocks = (int64_t)B * H * ((dv + 31) / 32);
 #define SP_GDR_REC(T_) return T == 1 ? gdr_launch(gdr_recurrent_kernel<T_, 1>, 0, blocks, 256, a, s, "gdr_recurrent_kernel") \
                                      : gdr_launch(gdr_recurrent_kernel<T_, kRecurrentMax>, 0, blocks, 256, a, s, "gdr_recurrent_kernel")

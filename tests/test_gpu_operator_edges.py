@@ -284,3 +284,18 @@ def test_delta_output_may_be_changed_in_place(cuda):
         f = f.mul_(0.5) if inplace else f * 0.5
         grads.append(torch.autograd.grad([o, f], xs, [go.to(cuda), gs.to(cuda)]))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_delta_without_frames_copies_the_state(cuda, train):
+    """The C ABI with T = 0, with and without a place for what a backward would need."""
+    from speech_amd import _lib, ops
+    h = _lib.lib()
+    state, out, some = torch.randn(2, 4, 16, 24, device=cuda), torch.full((2, 4, 16, 24), 7.0, device=cuda), torch.zeros(64, device=cuda)
+    strides = ops._host_i64([0] * 15)
+    for s0, want in ((state, state), (None, torch.zeros_like(state))):
+        saved = some.data_ptr() if train else None
+        rc = h.sp_gdr_fwd(None, None, None, None, None, None if s0 is None else s0.data_ptr(), None, strides, 0, 2, 2, 4, 16, 24, 1.0, 0, _lib.SP_F32, None,
+                          out.data_ptr(), saved, 256 if train else 0, None, 0, ops.raw_stream(state))
+        assert rc == 0, h.sp_last_error()
+        assert torch.equal(out, want) and not some.any()
