@@ -402,7 +402,7 @@ int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period
  * value heads h >= H / 2 walk each utterance's own frames backwards (Hk even).  o: [T][B][H][dv] dense.
  * strides: HOST array of element strides (t, b, h): fwd q, k, v, g, beta (15); bwd the same and go's (18).  q, k, v, go: unit stride inside
  * a head, addresses and strides aligned to 16 bytes, frames at most 2^23 elements apart (a forward of up to 12 frames without `saved` takes
- * any); state, state_out, o aligned to 16 bytes.  B * H <= 65536.
+ * any); state, state_out, o, saved, workspace, gq, gk, gv aligned to 16 bytes.  B * H <= 65536, and B * H * (ceil(T / 64) + 4) < 2^22.
  * saved: NULL (inference), or sp_gdr_saved_bytes() device bytes that the forward fills and the backward reads; workspace:
  * sp_gdr_workspace_bytes(.., backward), for an inference forward and for the backward (a forward with `saved` needs none).  T = 0: the state is
  * copied (or zeros written), `saved` is left as it was.

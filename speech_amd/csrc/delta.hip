@@ -25,6 +25,7 @@
 // reverse with dS) -> grads (dq, dk, dg, dbeta of a chunk; all chunks at once).  Few frames (streaming, single tokens): one recurrent kernel.
 #include "common.h"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace sp {
@@ -1579,6 +1580,12 @@ static bool gdr_aligned(const void* p, const int64_t* st, int dtype) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st[0] % ve == 0 && st[1] % ve == 0 && st[2] % ve == 0;
 }
 
+// every address that the kernels read or write 16 bytes at a time
+static bool gdr_at16(std::initializer_list<const void*> ps) {
+    for (const void* p : ps) if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+    return true;
+}
+
 template <typename K> static int gdr_launch(K kernel, size_t lds, int64_t blocks, int threads, const GdrArgs& a, hipStream_t s, const char* what) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, s, a);
     return check_launch(what);
@@ -1657,8 +1664,7 @@ extern "C" int sp_gdr_fwd(const void* q, const void* k, const void* v, const flo
     if (B == 0) return SP_OK;
     SP_CHECK_ARG(state_out && strides, "sp_gdr_fwd: null pointer");
     SP_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "sp_gdr_fwd: null pointer");
-    SP_CHECK_ARG(reinterpret_cast<uintptr_t>(state) % 16 == 0 && reinterpret_cast<uintptr_t>(state_out) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0,
-                 "sp_gdr_fwd: state and o must be 16-byte aligned");
+    SP_CHECK_ARG(gdr_at16({state, state_out, o, saved, workspace}), "sp_gdr_fwd: state, state_out, o, saved and workspace must be 16-byte aligned");
     GdrArgs a{};
     gdr_fill(a, q, k, v, g, beta, lengths, strides, T, B, Hk, H, dk, dv, scale, flags);
     a.s0 = state; a.sT = state_out; a.o = o;
@@ -1705,6 +1711,7 @@ extern "C" int sp_gdr_bwd(const void* q, const void* k, const void* v, const flo
     SP_CHECK_ARG(q && k && v && g && beta && strides && saved && go && gq && gk && gv && gg && gbeta && workspace, "sp_gdr_bwd: null pointer");
     SP_CHECK_ARG(gdr_aligned(q, strides, dtype) && gdr_aligned(k, strides + 3, dtype) && gdr_aligned(v, strides + 6, dtype) &&
                      gdr_aligned(go, strides + 15, dtype), "sp_gdr_bwd: q, k, v, go need 16-byte aligned rows and at most 2^23 elements from frame to frame");
+    SP_CHECK_ARG(gdr_at16({saved, gq, gk, gv, workspace}), "sp_gdr_bwd: saved, gq, gk, gv and workspace must be 16-byte aligned");
     const GdrLayout lay = gdr_saved(T, B, H, dk, dv, true);
     const GdrBwdLayout ws = gdr_bwd_ws(T, B, H, dk, dv);
     if (saved_bytes < lay.end || workspace_bytes < ws.end)

@@ -26,3 +26,22 @@ def _gdr_bwd(h, o=P, saved=P, go=P, gq=P, gk=P, gv=P, ws=P, nws=1 << 40):
 
 def test_gated_delta_backward_does_not_ask_for_o(h):
     assert _gdr_bwd(h, o=None, nws=16) == -2 and b"workspace" in h.sp_last_error()      # past the check of addresses, refused for its workspace
+
+
+@pytest.mark.parametrize("name", ["saved", "gq", "gk", "gv", "ws"])
+def test_gated_delta_backward_asks_for_aligned_buffers(h, name):
+    """They are read and written 16 bytes at a time."""
+    assert _gdr_bwd(h, **{name: P + 8}) == -1 and b"aligned" in h.sp_last_error()
+
+
+@pytest.mark.parametrize("name", ["saved", "ws", "state_out", "o"])
+def test_gated_delta_forward_asks_for_aligned_buffers(h, name):
+    a = dict(saved=P if name == "saved" else None, ws=P, state_out=P, o=P)
+    a[name] = P + 4
+    assert h.sp_gdr_fwd(P, P, P, P, P, None, None, STRIDES, 40, 2, 2, 4, 64, 64, 1.0, 0, 2, a["o"], a["state_out"], a["saved"], 1 << 40, a["ws"], 1 << 40,
+                        None) == -1 and b"aligned" in h.sp_last_error()
+
+
+def test_gated_delta_grid_is_limited_as_documented(h):
+    assert h.sp_gdr_workspace_bytes(64 * 59, 8192, 8, 8, 8, 8, 2, 0) > 0        # 65536 * (59 + 4) = 2^22 - 2^16
+    assert h.sp_gdr_workspace_bytes(64 * 60, 8192, 8, 8, 8, 8, 2, 0) == 0 and b"grid" in h.sp_last_error()
