@@ -1,6 +1,8 @@
 """Edges of the encoder operators that need no GPU: what the C ABI checks on the host before anything is launched (no address is followed),
 the build's dependencies, the models' arguments."""
 import ctypes
+import os
+import time
 
 import pytest
 
@@ -45,3 +47,47 @@ def test_gated_delta_forward_asks_for_aligned_buffers(h, name):
 def test_gated_delta_grid_is_limited_as_documented(h):
     assert h.sp_gdr_workspace_bytes(64 * 59, 8192, 8, 8, 8, 8, 2, 0) > 0        # 65536 * (59 + 4) = 2^22 - 2^16
     assert h.sp_gdr_workspace_bytes(64 * 60, 8192, 8, 8, 8, 8, 2, 0) == 0 and b"grid" in h.sp_last_error()
+
+
+def test_build_follows_its_flags(tmp_path, monkeypatch):
+    """An object is built again when its source, a header or the file that holds the compiler's flags is newer."""
+    from speech_amd import build
+    src, obj = tmp_path / "csrc", tmp_path / "build"
+    src.mkdir()
+    files = {n: src / n for n in ("a.hip", "b.hip", "common.h")}
+    flags, lib = tmp_path / "build.py", tmp_path / "lib.so"
+    for p in (*files.values(), flags):
+        p.write_text("x")
+    compiled = []
+
+    def compile_(name):
+        compiled.append(name)
+        (obj / (name[:-4] + ".o")).write_text("o")
+
+    class Done:
+        returncode, stdout, stderr = 0, "", ""
+
+    def link(cmd, **kw):
+        lib.write_text("lib")
+        return Done
+    for name, value in (("CSRC", str(src)), ("OBJDIR", str(obj)), ("LIB", str(lib)), ("SELF", str(flags)), ("_compile", compile_)):
+        monkeypatch.setattr(build, name, value)
+    monkeypatch.setattr(build.subprocess, "run", link)
+
+    def newer(p):
+        t = time.time() + 100 * (len(compiled) + 1)
+        os.utime(p, (t, t))
+
+    def again():
+        n = len(compiled)
+        build.build(verbose=False)
+        return sorted(compiled[n:])
+    assert again() == ["a.hip", "b.hip"]
+    assert again() == []
+    newer(files["a.hip"])
+    assert again() == ["a.hip"]
+    for p in (src / "a.hip", obj / "a.o"):
+        os.utime(p, (time.time(), time.time()))
+    assert again() == []
+    newer(flags)
+    assert again() == ["a.hip", "b.hip"]
