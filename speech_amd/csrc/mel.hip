@@ -94,7 +94,7 @@ __device__ __forceinline__ c2 cmul(c2 a, c2 w) {
 __device__ __forceinline__ c2 cmul_k(c2 a, float wre, float wim) { return cmul(a, c2{wre, wim}); }
 
 // forward 8-point DFT in place (mel_math.h dft8)
-__device__ __forceinline__ void dft8_pk(c2 (&z)[8]) {
+__device__ __forceinline__ void dft8_c2(c2 (&z)[8]) {
     const c2 a0 = z[0] + z[4], a4 = z[0] - z[4], a1 = z[1] + z[5], a5 = z[1] - z[5];
     const c2 a2 = z[2] + z[6], a6 = z[2] - z[6], a3 = z[3] + z[7], a7 = z[3] - z[7];
     const c2 b0 = a0 + a2, b2 = a0 - a2, b1 = a1 + a3, b3 = a1 - a3;
@@ -106,8 +106,8 @@ __device__ __forceinline__ void dft8_pk(c2 (&z)[8]) {
     z[1] = d0 + d1; z[5] = d0 - d1; z[3] = add_mi(d2, d3); z[7] = add_pi(d2, d3);
 }
 
-// forward 5-point DFT (mel_math.h dft5): 18 packed instructions
-__device__ __forceinline__ void dft5_pk(c2 x0, c2 x1, c2 x2, c2 x3, c2 x4, c2& y0, c2& y1, c2& y2, c2& y3, c2& y4) {
+// forward 5-point DFT (mel_math.h dft5): 36 instructions
+__device__ __forceinline__ void dft5_c2(c2 x0, c2 x1, c2 x2, c2 x3, c2 x4, c2& y0, c2& y1, c2& y2, c2& y3, c2& y4) {
     const c2 t1 = x1 + x4, t2 = x2 + x3, t3 = x1 - x4, t4 = x2 - x3;
     y0 = x0 + t1 + t2;
     const c2 a1 = x0 + kC1 * t1 + kC2 * t2, a2 = x0 + kC2 * t1 + kC1 * t2;
@@ -117,23 +117,23 @@ __device__ __forceinline__ void dft5_pk(c2 x0, c2 x1, c2 x2, c2 x3, c2 x4, c2& y
 }
 
 // forward 25-point DFT in place (mel_math.h dft25)
-__device__ __forceinline__ void dft25_pk(c2 (&y)[25]) {
+__device__ __forceinline__ void dft25_c2(c2 (&y)[25]) {
     constexpr float twre[4][4] = SP_TW25_RE;
     constexpr float twim[4][4] = SP_TW25_IM;
     c2 g[5][5];
 #pragma unroll
-    for (int b = 0; b < 5; ++b) dft5_pk(y[b], y[5 + b], y[10 + b], y[15 + b], y[20 + b], g[b][0], g[b][1], g[b][2], g[b][3], g[b][4]);
+    for (int b = 0; b < 5; ++b) dft5_c2(y[b], y[5 + b], y[10 + b], y[15 + b], y[20 + b], g[b][0], g[b][1], g[b][2], g[b][3], g[b][4]);
 #pragma unroll
     for (int b = 1; b < 5; ++b)
 #pragma unroll
         for (int c = 1; c < 5; ++c) g[b][c] = cmul_k(g[b][c], twre[b - 1][c - 1], twim[b - 1][c - 1]);
 #pragma unroll
-    for (int c = 0; c < 5; ++c) dft5_pk(g[0][c], g[1][c], g[2][c], g[3][c], g[4][c], y[c], y[c + 5], y[c + 10], y[c + 15], y[c + 20]);
+    for (int c = 0; c < 5; ++c) dft5_c2(g[0][c], g[1][c], g[2][c], g[3][c], g[4][c], y[c], y[c + 5], y[c + 10], y[c + 15], y[c + 20]);
 }
 
 // real-FFT split for one bin pair (mel_math.h real_post) WITHOUT its two halvings: from Zk = Z[k], Zm = Z[200-k]
 // and w = W400^k, 2|X[k]| and 2|X[200-k]| (the filterbank images carry the factor 1/2, exactly)
-__device__ __forceinline__ void real_post_pk(c2 Zk, c2 Zm, c2 w, float& mag_k, float& mag_m) {
+__device__ __forceinline__ void real_post_c2(c2 Zk, c2 Zm, c2 w, float& mag_k, float& mag_m) {
     const c2 E = add_conj(Zk, Zm), P = cmul(sub_conj(Zk, Zm), w);
     const c2 xa = add_mi(E, P), xb = add_pi(E, P);
     mag_k = __builtin_amdgcn_sqrtf(fmaf(xa.y, xa.y, xa.x * xa.x));
@@ -234,7 +234,7 @@ __device__ __forceinline__ void transform_frames(const S* __restrict__ x, int N,
             c2 z[8];
 #pragma unroll
             for (int n1 = 0; n1 < 8; ++n1) z[n1] = ld2(src + p * (2 * kHop * 4) + n1 * 200) * w[n1];
-            dft8_pk(z);
+            dft8_c2(z);
             if (active) {
                 st2(dst + p * (2 * kZStride * 8), z[0]);
 #pragma unroll
@@ -251,7 +251,7 @@ __device__ __forceinline__ void transform_frames(const S* __restrict__ x, int N,
         c2 y[25];
 #pragma unroll
         for (int n2 = 0; n2 < 25; ++n2) y[n2] = ld2(base + (k1 * 25 + n2) * 8);
-        dft25_pk(y);
+        dft25_c2(y);
 #pragma unroll
         for (int k2 = 0; k2 < 25; ++k2) st2(base + (k1 + 8 * k2) * 8, y[k2]);
     }
@@ -274,8 +274,8 @@ __device__ __forceinline__ void transform_frames(const S* __restrict__ x, int N,
                 zkB = ld2(nb + kB * 8); zmB = ld2(nb + (200 - kB) * 8);
             }
             float m0, m1, m2, m3;
-            real_post_pk(ckA, cmA, twA, m0, m1);
-            real_post_pk(ckB, cmB, twB, m2, m3);
+            real_post_c2(ckA, cmA, twA, m0, m1);
+            real_post_c2(ckB, cmB, twB, m2, m3);
             char* mrow = L + f * (kMagStride * 4);
             st1(mrow + kA * 4, m0);
             st1(mrow + (200 - kA) * 4, m1);
