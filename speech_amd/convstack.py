@@ -317,13 +317,19 @@ class _Conv3x5Fn(torch.autograd.Function):
         return gx, gw
 
 
-def conv_stack_group(spec, cnn, blocks, f32=False):
+def conv_stack_group(spec, cnn, blocks, f32=False, lengths=None):
     """conv_stack for blocks with GroupNorm: same output layout [T', B, F*32], feature index f*32 + c.  f32: the evaluation outside
-    autocast, every convolution on sp_conv2d_f32 (no gradients)."""
+    autocast, every convolution on sp_conv2d_f32 (no gradients).  lengths: int [B], each utterance's frames in spec; what lies behind
+    them is taken as the zeros that an utterance by itself would have there, in front of every convolution, and comes out as zeros."""
     from . import ops
     spec = spec.detach().float().contiguous()
     B, _, Fin, Tin = spec.shape
     F, T = (Fin - 1) // 2 + 1, (Tin - 1) // 2 + 1
+    inside = None
+    if lengths is not None:
+        spec = spec.masked_fill(torch.arange(Tin, device=spec.device) >= lengths.view(B, 1, 1, 1), 0.0)
+        lengths = torch.clamp((lengths + 1) // 2, 0, T)
+        inside = torch.arange(T, device=spec.device).view(1, 1, T, 1) < lengths.view(B, 1, 1, 1)
     chl = (F * T * C, T * C, C)
     if f32:
         ones, zeros = torch.ones(C, dtype=torch.float32, device=spec.device), torch.zeros(C, dtype=torch.float32, device=spec.device)
@@ -336,10 +342,12 @@ def conv_stack_group(spec, cnn, blocks, f32=False):
         x = conv(spec, cnn, 2, (Fin * Tin, Tin, 1), 1, Fin, Tin, _f32(cnn.bias))
     else:
         x = _StemFn.apply(spec, cnn.weight, cnn.bias)
+    if inside is not None:
+        x = x.masked_fill(~inside, 0.0)
     for i, blk in enumerate(blocks):
         g1, g2 = blk.bn1, blk.bn2
         y = conv(x, blk.conv1, 1, chl, C, F, T, zeros) if f32 else _Conv3x5Fn.apply(x, blk.conv1.weight)
-        y = ops.group_norm(y, g1.weight, g1.bias, g1.num_groups, g1.eps, act="relu")
+        y = ops.group_norm(y, g1.weight, g1.bias, g1.num_groups, g1.eps, act="relu", lengths=lengths)
         y = conv(y, blk.conv2, 1, chl, C, F, T, zeros) if f32 else _Conv3x5Fn.apply(y, blk.conv2.weight)
-        x = ops.group_norm(y, g2.weight, g2.bias, g2.num_groups, g2.eps, act="relu", residual=x, time_major=i == len(blocks) - 1)
+        x = ops.group_norm(y, g2.weight, g2.bias, g2.num_groups, g2.eps, act="relu", residual=x, lengths=lengths, time_major=i == len(blocks) - 1)
     return x.permute(2, 0, 1, 3).reshape(T, B, F * C)

@@ -94,14 +94,18 @@ spectrogram_transform = _SpectrogramTransform()
 train_audio_transforms = _TrainTransform()
 
 
-def collate_fn(data, data_type="train", vocab=text):
-    """data.py:160-178: list of (waveform [1,N], utterance str) -> the batch contract."""
+def collate_fn(data, data_type="train", vocab=text, frames=False):
+    """data.py:160-178: list of (waveform [1,N], utterance str) -> the batch contract.  frames=True: a fourth entry, the utterances'
+    own mel frames (int32 [B])."""
     waveforms = [w for (w, _) in data]
     spectrograms = featurize(waveforms, augment=(data_type == "train"))
     label_list = [torch.tensor(vocab.text_to_int(u), dtype=torch.int64) for (_, u) in data]
     label_lengths = [len(x) for x in label_list]
     labels = torch.nn.utils.rnn.pad_sequence(label_list, batch_first=True)
-    return spectrograms, labels, torch.tensor(label_lengths, dtype=torch.int32)
+    batch = spectrograms, labels, torch.tensor(label_lengths, dtype=torch.int32)
+    if frames:
+        batch += (torch.tensor([ops.num_frames(w.numel()) for w in waveforms], dtype=torch.int32),)
+    return batch
 
 
 class SortedDataset(torch.utils.data.Dataset):

@@ -33,9 +33,9 @@ def greedy_decode_ids(output, blank_label=0, frame_lengths=None):
     return _decode_ids(output, blank_label, frame_lengths)
 
 
-def greedy_decoder(output, labels, label_lengths, blank_label=0, vocab=text):
+def greedy_decoder(output, labels, label_lengths, blank_label=0, vocab=text, frame_lengths=None):
     """decoder.py:28-42: (decoded strings, target strings)."""
-    decodes = [vocab.int_to_text(ids) for ids in _decode_ids(output, blank_label)]
+    decodes = [vocab.int_to_text(ids) for ids in _decode_ids(output, blank_label, frame_lengths)]
     labels = torch.as_tensor(labels).cpu()
     label_lengths = torch.as_tensor(label_lengths).cpu().tolist()
     targets = [vocab.int_to_text(labels[i][: label_lengths[i]].tolist()) for i in range(len(decodes))]

@@ -16,8 +16,10 @@ with model.half(), scripts/eval_dataset.py).  ResidualBlock.forward below is the
 torch statement of one block and is used only by tests as the reference of the kernels.
 
 Two variants without a counterpart in the reference: ``norm="group"`` normalises the blocks over groups of channels of each utterance
-instead of over the batch (no coupling between utterances or data-parallel ranks, one form for training and evaluation), and
-``rnn="delta"`` replaces the SRU stack by gated delta rule layers (GatedDeltaLayer).
+instead of over the batch (one form for training and evaluation), and ``rnn="delta"`` replaces the SRU stack by gated delta rule layers
+(GatedDeltaLayer).  Both take the utterances' lengths (``SRModel.forward(x, lengths)``): with both of them an utterance's results are then
+those it has by itself, whatever the batch pads it with.  Without lengths the padding counts as frames, as it always does in the
+default model; with ``rnn="sru"`` the backward direction starts in it in any case.
 """
 import math
 
@@ -305,31 +307,48 @@ class SRModel(nn.Module):
                                         nn.Linear(2 * rnn_dim, n_vocab + 1, bias=False))
         self.compute_dtype = compute_dtype
 
-    def encode(self, x):
-        """[B, 1, F, T] f32 spectrogram -> layer-normed encoder output, time-major [T', B, 2*rnn_dim]."""
+    @property
+    def takes_lengths(self):
+        """Whether the model has a use for the utterances' lengths (either variant)."""
+        return self.norm == "group" or self.rnn == "delta"
+
+    def encode(self, x, lengths=None):
+        """[B, 1, F, T] f32 spectrogram -> layer-normed encoder output, time-major [T', B, 2*rnn_dim].  lengths (variants only): int [B]
+        on x's device, the frames of x that belong to each utterance; rows behind out_frames(lengths[b]) say nothing."""
         cd = self.compute_dtype
+        if lengths is not None:
+            if not self.takes_lengths:
+                raise ValueError("lengths belong to norm='group' and rnn='delta': BatchNorm and the SRU stack take the padding as frames")
+            if tuple(lengths.shape) != x.shape[:1] or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != x.device:
+                raise ValueError(f"lengths must be whole numbers [{x.shape[0]}] on {x.device}")
+            lengths = lengths.long().clamp(0, x.shape[-1])
         if self.norm == "group":
             f32 = cd == torch.float32 and not self.training and not torch.is_grad_enabled()
-            x = convstack.conv_stack_group(x, self.cnn, list(self.resnet_layers), f32)
+            x = convstack.conv_stack_group(x, self.cnn, list(self.resnet_layers), f32, lengths)
         elif cd == torch.float32 and not self.training and not torch.is_grad_enabled():
             # fp32 evaluation (train.py:162-168, outside autocast): the conv stack in f32 as well
             x = convstack.conv_stack_eval_f32(x, self.cnn, list(self.resnet_layers))
         else:
             # conv stack on the channel-last bf16 kernels -> [T', B, (F/2)*32], feature = f*32 + c
             x = convstack.conv_stack(x, self.cnn, list(self.resnet_layers), self.training)
-        x, _ = (self.delta_layers if self.rnn == "delta" else self.sru_layers)(x.to(cd))
+        if self.rnn == "delta":
+            x, _ = self.delta_layers(x.to(cd), None if lengths is None else out_frames(lengths))
+        else:
+            x, _ = self.sru_layers(x.to(cd))
         ln = self.classifier[0]
         return ops.layer_norm(x, ln.weight, ln.bias, ln.eps)
 
-    def forward(self, x):  # [B, 1, F, T] f32 spectrogram -> f32 logits [B, T', V]
-        x = self.encode(x).transpose(0, 1).contiguous()
+    def forward(self, x, lengths=None):  # [B, 1, F, T] f32 spectrogram -> f32 logits [B, T', V]
+        x = self.encode(x, lengths).transpose(0, 1).contiguous()
         return ops.classifier(x, self.classifier[1].weight)
 
-    def ctc_loss(self, x, labels, label_lengths, max_label_len=None):
+    def ctc_loss(self, x, labels, label_lengths, max_label_len=None, lengths=None):
         """The training step's loss, CTCLoss(blank=0)(log_softmax(self(x)), ...) of train.py:69-77, with the
-        classifier and the loss as one node (ops.classifier_ctc_loss)."""
-        return ops.classifier_ctc_loss(self.encode(x), self.classifier[1].weight, labels, label_lengths, 0,
-                                       max_label_len)
+        classifier and the loss as one node (ops.classifier_ctc_loss).  With lengths every utterance is scored over its own frames
+        (score_frames) instead of all T'."""
+        h = self.encode(x, lengths)
+        return ops.classifier_ctc_loss(h, self.classifier[1].weight, labels, label_lengths, 0, max_label_len,
+                                       None if lengths is None else score_frames(lengths, labels, label_lengths, h.shape[0]))
 
     # keys whose presence depends on the version of the `sru` package / torch that wrote the checkpoint and that
     # carry no trained values: sru registers `scale_x` (1.0 unless rescale=True; net.py:66 passes rescale=False)
@@ -359,3 +378,13 @@ class SRModel(nn.Module):
 def out_frames(t):
     """Encoder frames for t mel frames: the stride-2 stem (net.py:56)."""
     return (t - 1) // 2 + 1
+
+
+def score_frames(lengths, labels, label_lengths, t_out):
+    """int32 [B]: the encoder frames that CTC scores of utterances of `lengths` mel frames in a batch of t_out encoder frames.  Their own
+    frames; all t_out where those are fewer than the transcript needs (its labels and a blank between equal neighbours): the loss
+    would be infinite."""
+    own = torch.clamp(out_frames(lengths.long()), 0, t_out)
+    n = label_lengths.view(-1, 1)
+    twice = (labels[:, 1:] == labels[:, :-1]) & (torch.arange(1, max(1, labels.shape[1]), device=labels.device) < n)
+    return torch.where(own < label_lengths + twice.sum(1), t_out, own).to(torch.int32)

@@ -727,14 +727,15 @@ class _HeadCTCFn(torch.autograd.Function):
     dW) instead of a pass over [T'*B, V]."""
 
     @staticmethod
-    def forward(ctx, x_tm, weight, labels, label_lengths, blank, max_label_len):
+    def forward(ctx, x_tm, weight, labels, label_lengths, blank, max_label_len, input_lengths):
         T, B, n = x_tm.shape
         V = weight.shape[0]
         x2d = x_tm.reshape(T * B, n)
         logits, wb = _classifier_logits(x2d, weight)            # [T*B, V] view, row pitch Vp
         Vp = wb.shape[0]
         ctx.weight = weight
-        il = _full_lengths(B, T, x_tm.device)                                  # train.py:72-74: all T' frames
+        # train.py:72-74: all T' frames
+        il = _full_lengths(B, T, x_tm.device) if input_lengths is None else input_lengths
         gbuf, ctx.gkey = _grad_buffer(T * B, V, Vp, x2d.dtype, x2d.device)     # the gradient leaves the kernel in
                                                                                # the GEMMs' dtype, pad columns zero
         loss, _, _ = ctc_fwd_bwd(logits.as_strided((T, B, V), (B * Vp, Vp, 1)), labels, il, label_lengths, blank,
@@ -750,13 +751,14 @@ class _HeadCTCFn(torch.autograd.Function):
         gx = _classifier_dx(gb, wb, g, w32).view(ctx.shape)
         gw = _classifier_dw(gb, x2d, ctx.weight, g)
         _release_grad_buffer(ctx.gkey, gb)
-        return gx, gw, None, None, None, None
+        return gx, gw, None, None, None, None, None
 
 
-def classifier_ctc_loss(x_tm, weight, labels, label_lengths, blank=0, max_label_len=None):
+def classifier_ctc_loss(x_tm, weight, labels, label_lengths, blank=0, max_label_len=None, input_lengths=None):
     """x_tm [T', B, n] (time-major, already layer-normed), weight [V, n] -> scalar CTC loss (mean
-    reduction over the batch of nll / label length, every utterance scored over all T' frames)."""
-    return _HeadCTCFn.apply(x_tm, weight, labels, label_lengths, blank, max_label_len)
+    reduction over the batch of nll / label length, every utterance scored over all T' frames, or over its
+    input_lengths (int32 [B]))."""
+    return _HeadCTCFn.apply(x_tm, weight, labels, label_lengths, blank, max_label_len, input_lengths)
 
 
 def classifier(x, weight):

@@ -34,14 +34,16 @@ def test(dataset_type, batch_size, model, test_loader, beam_decode=False, log=pr
     test_cer, test_wer = [], []
     with torch.no_grad():
         for batch in test_loader:
-            spectrograms, labels, label_lengths = batch
-            logits = model(spectrograms.cuda())                       # [B, T', V]
+            spectrograms, labels, label_lengths, *frames = batch
+            frames = [t.cuda() for t in frames]                       # the utterances' mel frames, for the model's variants
+            logits = model(spectrograms.cuda(), *frames)              # [B, T', V]
+            own = net.out_frames(frames[0]) if frames else None
             # eval_dataset.py:40 takes log_softmax first; the greedy path is invariant to it
             if ctc_decoder is not None:
-                preds = ctc_decoder.decode_batch(None, logits)        # eval_dataset.py:43-51, raw logits
+                preds = ctc_decoder.decode_batch(None, logits, frame_lengths=own)      # eval_dataset.py:43-51, raw logits
                 targets = [text.int_to_text(labels[j][: label_lengths[j]].tolist()) for j in range(len(preds))]
             else:
-                preds, targets = decoder.greedy_decoder(logits, labels, label_lengths)
+                preds, targets = decoder.greedy_decoder(logits, labels, label_lengths, frame_lengths=own)
             for tgt, pred in zip(targets, preds):
                 test_cer.append(decoder.cer(tgt, pred))
                 test_wer.append(decoder.wer(tgt, pred))
@@ -86,12 +88,12 @@ def _clips(batch):
     return batch
 
 
-def build_loader(dataset, loader_batch_size, num_workers=3):
+def build_loader(dataset, loader_batch_size, num_workers=3, frames=False):
     """eval_dataset.py:121-128: shuffle off; the workers decode clips, the featuriser runs on the GPU in this process
-    (train.FeaturizingLoader), since forked workers must not touch it."""
+    (train.FeaturizingLoader), since forked workers must not touch it.  frames: batches carry the utterances' own mel frames."""
     from ..train import FeaturizingLoader
     return FeaturizingLoader(torch.utils.data.DataLoader(dataset=dataset, batch_size=loader_batch_size, shuffle=False,
-                                                         collate_fn=_clips, num_workers=num_workers), "valid")
+                                                         collate_fn=_clips, num_workers=num_workers), "valid", frames)
 
 
 def parse_args(argv=None):
@@ -131,7 +133,7 @@ def main(argv=None, log=print):
         model.load_checkpoint(torch.load(a.model_file, map_location="cpu", weights_only=True))
     elif a.dataset_type != "synthetic":
         raise SystemExit("model_file is required for a real corpus")
-    loader = build_loader(dataset, loader_bs, 0 if a.dataset_type == "synthetic" else a.num_workers)
+    loader = build_loader(dataset, loader_bs, 0 if a.dataset_type == "synthetic" else a.num_workers, model.takes_lengths)
     return test(a.dataset_type, hparams["batch_size"], model, loader, a.beam_decode, log=log, lm_path=a.lm)
 
 

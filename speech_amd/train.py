@@ -271,9 +271,9 @@ class BucketedAllReduce:
 
 
 def train_step(model, optimizer, spectrograms, labels, label_lengths, clip_grad_norm=2.0, dp=None,
-               max_label_len=None):
-    """One optimisation step on a featurised batch (train.py:62-87).  Returns the loss tensor
-    (device, no sync)."""
+               max_label_len=None, lengths=None):
+    """One optimisation step on a featurised batch (train.py:62-87).  lengths: the utterances' mel frames, for models that take them
+    (net.SRModel.takes_lengths).  Returns the loss tensor (device, no sync)."""
     optimizer.zero_grad()
     # FlatAdam: every .grad is a zeroed view of the flat arena, so accumulating backward kernels may
     # write straight into it (ops.GradSink) instead of through a temporary and an add per parameter
@@ -281,7 +281,7 @@ def train_step(model, optimizer, spectrograms, labels, label_lengths, clip_grad_
     ops.set_grad_sink(sink)
     try:
         if hasattr(model, "ctc_loss"):      # SRModel: classifier + CTC as one node, time-major logits
-            loss = model.ctc_loss(spectrograms, labels, label_lengths, max_label_len)
+            loss = model.ctc_loss(spectrograms, labels, label_lengths, max_label_len, **({} if lengths is None else {"lengths": lengths}))
         else:
             output = model(spectrograms)                                   # [B, T', V]
             B, Tp, _ = output.shape
@@ -306,10 +306,10 @@ def train(batch_size, model, train_loader, optimizer, scheduler, epoch, iter_met
     data_len = len(train_loader.dataset) if hasattr(train_loader, "dataset") else len(train_loader)
     start = batch_start = time.time()
     for batch_idx, batch in enumerate(train_loader):
-        spectrograms, labels, label_lengths = batch
+        spectrograms, labels, label_lengths, *frames = batch
         spectrograms = spectrograms.cuda()
         loss = train_step(model, optimizer, spectrograms, labels.cuda(), label_lengths.cuda(),
-                          clip_grad_norm, dp)
+                          clip_grad_norm, dp, lengths=frames[0].cuda() if frames else None)
         scheduler.step()
         iter_meter.step()
         if batch_idx % 100 == 0:
@@ -335,15 +335,19 @@ def eval_dataset(model, loader, name, log=print, dtype=torch.float32, group=None
     eval_loss, eval_cer, eval_wer, n = 0.0, [], [], 0
     try:
         for batch in loader:
-            spectrograms, labels, label_lengths = batch
-            spectrograms, labels, label_lengths = spectrograms.cuda(), labels.cuda(), label_lengths.cuda()
-            output = model(spectrograms).float()
+            spectrograms, labels, label_lengths, *frames = batch
+            spectrograms, labels, label_lengths, *frames = (t.cuda() for t in (spectrograms, labels, label_lengths, *frames))
+            output = model(spectrograms, *frames).float()
             B, Tp, _ = output.shape
-            input_lengths = torch.full((B,), Tp, dtype=torch.int32, device=output.device)
+            if frames:
+                input_lengths = net.score_frames(frames[0], labels, label_lengths, Tp)
+            else:
+                input_lengths = torch.full((B,), Tp, dtype=torch.int32, device=output.device)
             loss, _, _ = ops.ctc_fwd_bwd(output, labels, input_lengths, label_lengths, want_grad=False)
             eval_loss += float(loss)
             n += 1
-            preds, targets = decoder.greedy_decoder(output, labels, label_lengths)
+            preds, targets = decoder.greedy_decoder(output, labels, label_lengths,
+                                                    frame_lengths=net.out_frames(frames[0]) if frames else None)
             for tgt, pred in zip(targets, preds):
                 eval_cer.append(decoder.cer(tgt, pred))
                 eval_wer.append(decoder.wer(tgt, pred))
@@ -460,8 +464,8 @@ class FeaturizingLoader:
     """DataLoader workers read and decode the clips (file IO, as in the reference); the featuriser runs on the
     GPU, which forked workers must not touch, so collate_fn is applied here, in the training process."""
 
-    def __init__(self, loader, data_type):
-        self.loader, self.data_type = loader, data_type
+    def __init__(self, loader, data_type, frames=False):
+        self.loader, self.data_type, self.frames = loader, data_type, frames
         self.dataset = loader.dataset
 
     def __len__(self):
@@ -469,7 +473,7 @@ class FeaturizingLoader:
 
     def __iter__(self):
         for clips in self.loader:
-            yield data.collate_fn(clips, self.data_type)
+            yield data.collate_fn(clips, self.data_type, frames=self.frames)
 
 
 def _clips(batch):
@@ -481,6 +485,7 @@ def build_loaders(hparams, rank, world):
     training, SortedTV for the "tv" evaluation, IBMDataset for the "ibm" one whose CER picks the checkpoint."""
     bs = hparams["batch_size"]
     workers = hparams.get("num_workers", 6)
+    frames = hparams.get("norm") == "group" or hparams.get("rnn") == "delta"      # the variants take the utterances' lengths
     if hparams["synthetic"]:
         train_set = data.SyntheticSorted(hparams["synthetic_clips"], bs, seed=7)
         tv_eval = data.SyntheticSorted(max(bs, hparams["synthetic_clips"] // 8), bs, seed=11, max_s=6.0)
@@ -504,16 +509,16 @@ def build_loaders(hparams, rank, world):
     if hparams["steps"]:
         sampler.n = min(sampler.n, hparams["steps"] * world)
     train_loader = FeaturizingLoader(torch.utils.data.DataLoader(
-        train_set, batch_size=None, sampler=sampler, collate_fn=_clips, num_workers=workers, pin_memory=False), "train")
+        train_set, batch_size=None, sampler=sampler, collate_fn=_clips, num_workers=workers, pin_memory=False), "train", frames)
     # train.py:222-239: the tv evaluation walks its batches shuffled, the ibm one in order; each rank takes every
     # world-th batch / utterance (world 1: exactly the reference's loaders)
     evals = [("tv", FeaturizingLoader(torch.utils.data.DataLoader(
         tv_eval, batch_size=None, sampler=ShardSampler(len(tv_eval), rank, world, shuffle=True), collate_fn=_clips,
-        num_workers=min(workers, 4)), "valid"))]
+        num_workers=min(workers, 4)), "valid", frames))]
     if ibm_eval is not None:
         evals.append(("ibm", FeaturizingLoader(torch.utils.data.DataLoader(
             ibm_eval, batch_size=32 * hparams["multiplier"] * 2, sampler=ShardSampler(len(ibm_eval), rank, world),
-            collate_fn=_clips, num_workers=min(workers, 4)), "valid")))
+            collate_fn=_clips, num_workers=min(workers, 4)), "valid", frames)))
     return train_loader, sampler, evals
 
 

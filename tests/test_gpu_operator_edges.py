@@ -299,3 +299,105 @@ def test_delta_without_frames_copies_the_state(cuda, train):
                           out.data_ptr(), saved, 256 if train else 0, None, 0, ops.raw_stream(state))
         assert rc == 0, h.sp_last_error()
         assert torch.equal(out, want) and not some.any()
+
+
+# ------------------------------------------------------------------------------------------ padding has no influence
+def _variant(cuda, dtype):
+    from speech_amd import net
+    torch.manual_seed(3)
+    m = net.SRModel(2, 64, 28, 80, 0.0, compute_dtype=dtype, norm="group", rnn="delta").to(cuda)
+    with torch.no_grad():
+        for blk in m.resnet_layers:
+            blk.bn2.weight.uniform_(0.5, 1.0)
+            blk.bn1.bias.uniform_(-0.3, 0.3)
+            blk.bn2.bias.uniform_(-0.3, 0.3)
+    return m
+
+
+def test_an_utterance_does_not_see_its_batch(cuda):
+    """Group norm and delta layers, f32 evaluation: an utterance's logits in a padded batch are those that it has by itself.  Both are within
+    f32 rounding of the exact ones: 4096 half steps for the conv stack and 2048 for each layer (test_gpu_operators), twice."""
+    from speech_amd import net
+    m = _variant(cuda, torch.float32).eval()
+    lengths = [90, 61, 40, 3, 0, 90, 1]
+    spec = torch.rand(len(lengths), 1, 80, 90, device=cuda)
+    L = torch.tensor(lengths, device=cuda)
+    with torch.no_grad():
+        batch = m(spec, L)
+        for b, n in enumerate(lengths):
+            if n:
+                alone = m(spec[b:b + 1, :, :, :n], L[b:b + 1])
+                k = net.out_frames(n)
+                assert alone.shape[1] == k
+                assert float((batch[b, :k] - alone[0]).norm() / alone.norm()) <= 2 * (4096 + 2 * 2048) * 2.0 ** -24, n
+        assert torch.isfinite(batch).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+def test_padding_holds_anything(cuda, dtype):
+    """What lies behind the utterances' frames reaches neither loss nor gradients, not even as NaN.  (The layer norms' and the convolutions'
+    parameter gradients are summed with float atomics: 1024 half steps of their largest value.)"""
+    m = _variant(cuda, dtype).train()
+    lengths = torch.tensor([90, 61, 40, 25], dtype=torch.int32, device=cuda)
+    labels = torch.randint(1, 29, (4, 6), generator=torch.Generator().manual_seed(0)).to(cuda)
+    ll = torch.tensor([6, 4, 5, 2], dtype=torch.int32, device=cuda)
+    spec = torch.rand(4, 1, 80, 90, device=cuda)
+    out = []
+    for fill in (0.0, 3.0, float("nan"), float("inf")):
+        x = spec.clone()
+        for b, n in enumerate(lengths.tolist()):
+            x[b, :, :, n:] = fill
+        m.zero_grad()
+        loss = m.ctc_loss(x, labels, ll, lengths=lengths)
+        loss.backward()
+        out.append((loss.detach(), {n: p.grad.clone() for n, p in m.named_parameters()}))
+    for loss, grads in out[1:]:
+        assert torch.equal(loss, out[0][0]) and torch.isfinite(loss)
+        for n, g in grads.items():
+            w = out[0][1][n]
+            assert torch.isfinite(g).all() and float((g - w).abs().max()) <= 1024 * 2.0 ** -24 * float(w.abs().max()), n
+
+
+def test_ctc_scores_own_frames(cuda):
+    """The loss of utterances with lengths is CTC over their own encoder frames, in 64 bits from the model's logits."""
+    from speech_amd import net
+    m = _variant(cuda, torch.float32).eval()
+    lengths = torch.tensor([90, 61, 40, 4], device=cuda)
+    labels = torch.randint(1, 29, (4, 6), generator=torch.Generator().manual_seed(1)).to(cuda)
+    ll = torch.tensor([6, 4, 5, 4], device=cuda)                  # the last one needs more frames than its two: scored over the batch's
+    spec = torch.rand(4, 1, 80, 90, device=cuda)
+    with torch.no_grad():
+        logits = m(spec, lengths).double().cpu()
+        loss = m.ctc_loss(spec, labels, ll.int(), lengths=lengths)
+    own = net.score_frames(lengths, labels, ll, logits.shape[1]).cpu()
+    assert own.tolist() == [45, 31, 20, 45]
+    want = torch.nn.functional.ctc_loss(logits.log_softmax(-1).transpose(0, 1), labels.cpu(), own.long(), ll.cpu(), 0, "mean")
+    assert float(loss) == pytest.approx(float(want), rel=1e-5)
+
+
+def test_commands_hand_the_lengths_on(cuda, monkeypatch):
+    """Loaders of the variants carry the clips' frames, training and evaluation give them to the model; the default model's carry none."""
+    from speech_amd import data, net, ops, train
+    from speech_amd.scripts import eval_dataset as ev
+    clips = data.SyntheticSorted(8, 4, seed=3, max_s=2.0)
+    hp = dict(batch_size=4, synthetic=True, synthetic_clips=8, steps=1, num_workers=0, multiplier=1)
+    for variant in (dict(norm="group", rnn="delta"), dict(norm="batch", rnn="sru")):
+        loader, _, evals = train.build_loaders(dict(hp, **variant), 0, 1)
+        for x in (loader, evals[0][1]):
+            batch = next(iter(x))
+            assert len(batch) == (4 if variant["norm"] == "group" else 3)
+            if len(batch) == 4:
+                assert batch[3].dtype == torch.int32 and int(batch[3].max()) == batch[0].shape[-1]
+    assert data.collate_fn(clips[0], "valid", frames=True)[3].tolist() == [ops.num_frames(n) for n in clips.samples[:4]]
+    m, seen = _variant(cuda, torch.float32), []
+    encode = net.SRModel.encode
+    monkeypatch.setattr(net.SRModel, "encode", lambda self, x, lengths=None: (seen.append(None if lengths is None else lengths.tolist()), encode(self, x, lengths))[1])
+    frames = [ops.num_frames(n) for n in clips.samples]
+    opt = train.FlatAdam(m.parameters(), lr=1e-3)
+    from types import SimpleNamespace
+    pairs = train.FeaturizingLoader(torch.utils.data.DataLoader(clips, batch_size=None, collate_fn=lambda b: b), "valid", True)
+    train.train(4, m, pairs, opt, SimpleNamespace(step=lambda: None), 0, SimpleNamespace(step=lambda: None), 2.0, max_steps=1, log=lambda *a: None)
+    assert seen == [frames[:4]]
+    train.eval_dataset(m, pairs, "valid", log=lambda *a: None)
+    ev.test("synthetic", 4, m, ev.build_loader(clips, None, 0, True), log=lambda *a: None)
+    assert seen[1:] == [frames[:4], frames[4:]] * 2

@@ -91,3 +91,31 @@ def test_build_follows_its_flags(tmp_path, monkeypatch):
     assert again() == []
     newer(flags)
     assert again() == ["a.hip", "b.hip"]
+
+
+def test_the_default_model_takes_no_lengths():
+    import torch
+    from speech_amd import net
+    x = torch.zeros(2, 1, 80, 20)
+    m = net.SRModel(1, 64, 28, 80, 0.0)
+    assert not m.takes_lengths
+    for call in (m.encode, m):
+        with pytest.raises(ValueError, match="padding"):
+            call(x, torch.tensor([20, 10]))
+    for kw in (dict(norm="group"), dict(rnn="delta")):
+        m = net.SRModel(1, 64, 28, 80, 0.0, **kw)
+        assert m.takes_lengths
+        for bad in (torch.tensor([20]), torch.tensor([20.0, 10.0]), torch.tensor([True, False])):
+            with pytest.raises(ValueError, match="whole numbers"):
+                m(x, bad)
+
+
+def test_frames_that_ctc_scores():
+    """Own frames, or the batch's where a transcript needs more: its labels and a blank between equal neighbours."""
+    import torch
+    from speech_amd import net
+    labels = torch.tensor([[1, 1, 2, 2], [1, 2, 3, 9], [4, 4, 4, 0], [5, 0, 0, 0]])
+    n = torch.tensor([4, 3, 3, 1], dtype=torch.int32)                # needs 6, 3, 5, 1
+    assert net.score_frames(torch.tensor([11, 5, 8, 1]), labels, n, 30).tolist() == [6, 3, 30, 1]
+    assert net.score_frames(torch.tensor([10, 4, 9, 0], dtype=torch.int32), labels, n, 30).tolist() == [30, 30, 5, 30]
+    assert net.score_frames(torch.tensor([99, 99], dtype=torch.uint8), labels[:2, :0], n[:2] * 0, 30).tolist() == [30, 30]
