@@ -964,6 +964,8 @@ def _lengths(lengths, n):
     """int32 [n] on the device, or ValueError."""
     if tuple(lengths.shape) != (n,) or lengths.dtype not in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
         raise ValueError(f"lengths must be whole numbers [{n}]")
+    if lengths.dtype == torch.int64:        # the kernels clamp to [0, T], of 32 bits
+        lengths = lengths.clamp(0, 2 ** 31 - 1)
     return lengths.to(torch.int32).contiguous()
 
 

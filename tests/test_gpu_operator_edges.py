@@ -401,3 +401,18 @@ def test_commands_hand_the_lengths_on(cuda, monkeypatch):
     train.eval_dataset(m, pairs, "valid", log=lambda *a: None)
     ev.test("synthetic", 4, m, ev.build_loader(clips, None, 0, True), log=lambda *a: None)
     assert seen[1:] == [frames[:4], frames[4:]] * 2
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.uint8], ids=ids)
+def test_lengths_of_any_type_are_clamped(cuda, dtype):
+    """Values beyond the tensor mean all of its frames, also those that 32 bits do not hold."""
+    from speech_amd import ops
+    x, w = torch.randn(3, 2, 7, 16, device=cuda), torch.ones(16, device=cuda)
+    args, _, _ = delta_inputs(7, 3, 2, 1, 16, 16, torch.float32, 1, state=False)
+    qkv = [t.to(cuda) for t in args[:5]]
+    big = {torch.int64: (1 << 32) + 2, torch.int32: (1 << 31) - 1, torch.uint8: 255}[dtype]
+    low = {torch.int64: -(1 << 32) + 2, torch.int32: -(1 << 31), torch.uint8: 0}[dtype]
+    a, b = torch.tensor([big, 3, low], dtype=dtype, device=cuda), torch.tensor([7, 3, 0], device=cuda)
+    assert torch.equal(ops.group_norm(x, w, w, 4, lengths=a), ops.group_norm(x, w, w, 4, lengths=b))
+    for u, v in zip(ops.gated_delta_rule(*qkv, lengths=a), ops.gated_delta_rule(*qkv, lengths=b)):
+        assert torch.equal(u, v)
