@@ -256,6 +256,8 @@ class GatedDeltaLayer(nn.Module):
         """One frame x [B, n_in] of every session; `state` f32 [B, heads, dk, dv] is updated in place.  Evaluation only."""
         if self.bidirectional:
             raise RuntimeError("a bidirectional layer cannot run frame by frame")
+        if self.training and self.dropout > 0:
+            raise RuntimeError("step is for evaluation: call eval() first (a layer in training mode would drop out)")
         return self._out(ops.gated_delta_step(*self._split(x), state, normalize=True), x, None)
 
 

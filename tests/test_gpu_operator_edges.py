@@ -416,3 +416,15 @@ def test_lengths_of_any_type_are_clamped(cuda, dtype):
     assert torch.equal(ops.group_norm(x, w, w, 4, lengths=a), ops.group_norm(x, w, w, 4, lengths=b))
     for u, v in zip(ops.gated_delta_rule(*qkv, lengths=a), ops.gated_delta_rule(*qkv, lengths=b)):
         assert torch.equal(u, v)
+
+
+def test_layer_step_refuses_before_it_touches_the_state(cuda):
+    """A training-mode layer with dropout has no single-frame form."""
+    from speech_amd import net
+    layer = net.GatedDeltaLayer(64, 64, heads=4, dk=16, dropout=0.1, bidirectional=False).to(cuda).train()
+    state = torch.zeros(2, 4, 16, 16, device=cuda)
+    with pytest.raises(RuntimeError, match="evaluation"):
+        layer.step(torch.randn(2, 64, device=cuda), state)
+    assert not state.any()
+    layer.eval().step(torch.randn(2, 64, device=cuda), state)
+    assert state.any()
