@@ -409,6 +409,8 @@ int sp_dropout(const void* x, const void* residual, int64_t rows, int64_t period
  * Backward: go = d loss / d o, gstate_out = d loss / d state_out or NULL; writes gq, gk [T][B][Hk][dk], gv [T][B][H][dv] (dense, dtype), gg,
  * gbeta f32 [T][B][H] dense, gstate f32 or NULL; frames behind an utterance's end get zeros.  T >= 1.  Results are bit-reproducible.  o is not
  * read (it is formed again) and may be NULL.
+ * A non-finite value stays in its utterance and head; the chunked form (more than 12 frames, or `saved`) may spread it to the earlier frames of its
+ * chunk of 64 frames of the walk.
  * SP_GDR_NO_STATE (backward): the forward had state = NULL; the decay of every walk's first frame then met nothing, and its gradient is
  * written as the exact 0 that it is instead of the rounding of two sums that cancel.
  * --------------------------------------------------------------------------------------- */

@@ -1266,7 +1266,11 @@ def gated_delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None, nor
     128): H a multiple of Hk, H / Hk consecutive value heads share a key head.  g (log decay) and beta [T, B, H] are taken in float32.
     state: the state before the first frame (zeros).  lengths int [B]: frames t >= lengths[b] are not read, leave the state alone and come
     out (and back) as zeros.  scale: default dk ** -0.5.  normalize=True divides q and k by sqrt(|.|^2 + 1e-6) first.  bidirectional=True:
-    the second half of the heads walks each utterance's own frames backwards (Hk even)."""
+    the second half of the heads walks each utterance's own frames backwards (Hk even).
+
+    An infinity or NaN in a frame of an utterance stays in its utterance and head.  Up to 12 frames without gradients it reaches the later
+    frames of the walk only; longer calls take 64 frames of a walk at a time (0-63, 64-127, ...), and all frames of its chunk may become NaN.
+    The gradients of that head and utterance are then not finite either."""
     B, Hk, dk, H, dv = _gdr_check(q, k, v, g, beta, state, ("T", "B"))
     if bidirectional and Hk % 2:
         raise ValueError(f"both directions need an even number of key heads, not {Hk}")
@@ -1301,7 +1305,8 @@ def _step_strides(*strides):
 
 def gated_delta_step(q, k, v, g, beta, state, scale=None, normalize=False):
     """One frame of gated_delta_rule for serving: q, k [B, Hk, dk], v [B, H, dv], g, beta [B, H] -> o [B, H, dv]; `state` (float32,
-    contiguous [B, H, dk, dv]) is updated in place.  Not differentiable."""
+    contiguous [B, H, dk, dv]) is updated in place.  Not differentiable: o carries no gradient whatever requires one; a state that requires
+    one and forward-mode tangents are refused."""
     B, Hk, dk, H, dv = _gdr_check(q, k, v, g, beta, state, ("B",))
     if state is None or not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state must be a contiguous, 16-byte aligned tensor: it is updated in place")

@@ -428,3 +428,39 @@ def test_layer_step_refuses_before_it_touches_the_state(cuda):
     assert not state.any()
     layer.eval().step(torch.randn(2, 64, device=cuda), state)
     assert state.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("T,at,train", [(12, 5, False), (150, 70, False), (150, 70, True)])
+def test_delta_non_finite_values_stay_in_their_head(cuda, dtype, bad, T, at, train):
+    """An infinity or NaN in one frame of one head: other heads and utterances, forwards and backwards, and the chunks in front of its own (few
+    frames: all frames in front of it) are what they are without it, bit for bit; one in a column of v stays in that column of o."""
+    from speech_amd import ops
+    args, go, gs = delta_inputs(T, 3, 4, 1, 16, 24, dtype, 31)
+    lengths = torch.tensor([T, T - 1, T], device=cuda)
+
+    def run(which, index):
+        xs = [t.clone() for t in args]
+        if which is not None:
+            xs[which][index] = bad
+        xs = [t.to(cuda).requires_grad_(train) for t in xs]
+        o, f = ops.gated_delta_rule(*xs[:5], state=xs[5], lengths=lengths, normalize=True, bidirectional=True)
+        g = torch.autograd.grad([o, f], xs, [go.to(cuda), gs.to(cuda)]) if train else ()
+        return o.detach(), f.detach(), g
+    o, f, g = run(None, None)
+    others = [b * 4 + h for b in range(3) for h in range(4) if (b, h) not in ((1, 0), (1, 2))]
+    flat = lambda t: t.flatten(1, 2)[:, others]      # noqa: E731
+    front = at if T <= 12 else 64                      # frames of a forward head that do not meet it
+    behind = at + 1 if T <= 12 else T - 1 - 64         # of a head that walks backwards, from the utterance's end
+    for which, index in ((0, (at, 1, [0, 2])), (1, (at, 1, [0, 2])), (3, (at, 1, [0, 2])), (4, (at, 1, [0, 2]))):
+        if which == 3 and bad > 0:
+            continue                                    # a gate of +inf is no decay
+        p, e, d = run(which, index)
+        assert torch.equal(flat(p), flat(o)) and torch.equal(e.flatten(0, 1)[others], f.flatten(0, 1)[others])
+        assert torch.equal(p[:front, 1, 0], o[:front, 1, 0]) and torch.equal(p[behind:, 1, 2], o[behind:, 1, 2])
+        for x, y in zip(d[:5], g[:5]):
+            assert torch.equal(flat(x), flat(y))
+    p, e, _ = run(2, (at, 1, 0, 7))
+    cols = [c for c in range(24) if c != 7]
+    assert torch.equal(p[..., cols], o[..., cols]) and torch.equal(e[..., cols], f[..., cols])
