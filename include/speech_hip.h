@@ -361,7 +361,7 @@ int sp_layernorm_bwd(const void* gy, const void* x, const float* mean, const flo
  * Tensors are [N][F][T][C] of dtype (SP_F32 / SP_F16 / SP_BF16), element (n, f, t, c) at n*s0 + f*s1 + t*s2 + c; strides (HOST
  * array, elements): fwd x, residual, y; bwd gy, x, residual, gx, gres (three each; those of a NULL tensor are ignored).
  * gamma, beta f32 [C]; C % G == 0, C <= 2048, N <= 2^22.  residual may be NULL.  act: SP_ACT_*.  lengths: DEVICE int32 [N] or NULL;
- * frames t >= lengths[n] are outside: not counted, not read, written as 0 (values outside [0, T] are clamped).  A sample of length
+ * frames t >= lengths[n] are outside: whatever they hold has no influence, they are written as 0 (values outside [0, T] are clamped).  A sample of length
  * 0 is all zeros.  mean, rstd: f32 [N][G], both or neither NULL (the backward needs them).
  * Backward: gx, gres = d loss / d x, d residual (gres may be NULL), dgamma / dbeta f32
  * [C], overwritten or (accumulate != 0) added to.  All reductions are in a fixed order: results are bit-reproducible.

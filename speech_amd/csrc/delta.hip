@@ -20,7 +20,7 @@
 // 3e-6 to 1e-5 instead of 3e-7; the f32 matrix instruction costs 5.3 times a bf16 one, three to six bf16 products at most as much.  What
 // only reaches a 16-bit output (o, dq, dk) takes two parts.  Outputs of 16-bit type are rounded once.
 //
-// Kernels: prep (N, P, X of a chunk; all chunks at once) -> scan (walks the chunks with S in registers; a wave owns 32 columns of dv and
+// Kernels: prep (N, P, X of a chunk; all chunks at once) -> scan (walks the chunks with S in registers; a wave owns 16 columns of dv and
 // never talks to the others: the accumulator layout of one product is the B operand of the next) ; backward: rscan (the same walk in
 // reverse with dS) -> grads (dq, dk, dg, dbeta of a chunk; all chunks at once).  Few frames (streaming, single tokens): one recurrent kernel.
 #include "common.h"
@@ -623,10 +623,10 @@ template <int P> __device__ __forceinline__ void row_operands(Frag<P> (&f)[2], c
 // A wave owns 16 columns of dv: the state's columns, U's, O's.  Only K, Q, X, P and the vectors are shared (LDS, filled a chunk ahead
 // through registers); two barriers a chunk.  A wave whose columns lie behind dv works on zeros and writes nothing: as many steps as the
 // others, and no branch around the matrix instructions.
-// 101 us, 12 chunks in turn: 8.4 us a chunk, of which the matrix pipes are busy 18 %.  P takes two parts: with one, o was off by 1.34 times its own
-// rounding (bf16: 2.2e-3 of the two-norm instead of 1.66e-3) for 2.5 us less.  Bound by the chain of four dependent products a chunk
-// (K S, X, P, K^T U) at two waves a SIMD; the states are the only thing that could be split further, and every split loads K, Q, X and P
-// again.  Inference at dk 128 (T = 1501, 128 heads, one wave a SIMD): 139 us, 24 chunks (132 with one part of P).
+// 100 to 105 us, 12 chunks in turn: 8.5 us a chunk, of which the matrix pipes are busy 18 %.  P takes two parts: with one, o was off by 1.34 times
+// its own rounding (bf16: 2.2e-3 of the two-norm instead of 1.66e-3) for 2.5 us less.  Bound by the chain of three dependent products a chunk
+// (K S, X, K^T U), with Q S and P U, which feed o alone, behind the same waits, at two waves a SIMD; the states are the only thing that could
+// be split further, and every split loads K, Q, X and P again.  Inference at dk 128 (T = 1501, 128 heads, one wave a SIMD): 139 us, 24 chunks (132 with one part of P).
 template <typename T, int DK, int NW, bool TRAIN>
 __global__ __launch_bounds__(NW * 64) void gdr_scan_kernel(GdrArgs a) {
     extern __shared__ __align__(16) char smem[];
@@ -798,8 +798,8 @@ template <typename T> __device__ __forceinline__ float behind(float v, uint32_t 
 
 // E and O are formed again from the state at the chunk's start: 36 + 84 more matrix instructions a wave and chunk instead of 100 KB more
 // traffic a chunk (E in f32 and the rest of O that its rounding dropped, written by the forward and read back).
-// 223 us, 18.6 us a chunk (f32 at 30 heads, dk 40, dv 72, 301 frames: 76 us): 246 matrix instructions a wave and chunk keep the pipes busy 17 %
-// of the time, 425 MB move.  Bound by latency at two waves a SIMD, which 256 registers a lane allow: without the next chunk's loads it took three
+// 223 to 232 us, 19 us a chunk (f32 at 30 heads, dk 40, dv 72, 301 frames: 76 us): 246 matrix instructions a wave and chunk keep the pipes busy 17 %
+// of the time, 439 MB move.  Bound by latency at two waves a SIMD, which 256 registers a lane allow: without the next chunk's loads it took three
 // quarters of the time (they find registers only at the chunk's end).
 // Measured and not kept: those loads earlier (they spill), their lines touched into the L2 cache a chunk ahead (7 % more).
 template <typename T, int DK, int NW>
@@ -1087,8 +1087,8 @@ __device__ __forceinline__ void store_ev(const TileRegs<T, 128, 512>& v, const T
 }
 
 // One workgroup a (key head, chunk), its value heads in turn: shared heads' gradients are sums in registers, in a fixed order.  Eight waves: a
-// wave owns a quarter of dk in the products with the states and 16 columns j of the 64 x 64 products, and half of the rows of both.  219 us (one
-// value head a key head; four: 160): 342 MB at 1.5 TB/s, bound by the waits between its phases.  Two parts of E and of dV take 128 KB of LDS, so one
+// wave owns a quarter of dk in the products with the states and 16 columns j of the 64 x 64 products, and half of the rows of both.  219 to 226 us
+// (one value head a key head; four: 160): 284 MB at 1.3 TB/s, bound by the waits between its phases.  Two parts of E and of dV take 128 KB of LDS, so one
 // workgroup a CU; four waves a workgroup, two of them a CU, held one part of each: 173 us, dq off by 1.34 times its own rounding, dk by 1.47.
 // Other shapes of the same size, eight waves against four: f32 dk 64 302 us / 363, dk 128 451 / 608, f16 dk 64 245 / 272, dk 128 337 / 415,
 // bf16 dk 128 313 / 289 (one part).

@@ -1061,7 +1061,7 @@ def group_norm(x, weight, bias, groups, eps=1e-5, act="none", residual=None, len
 
     x [N, C], [N, T, C] or [N, F, T, C] (float32 / bfloat16 / float16); statistics per sample and group over all positions and the
     C / groups channels (f32, biased variance).  act: "none", "relu" or "silu".  residual: like x.  lengths int [N]: only frames
-    t < lengths[n] of the T dimension belong to sample n; the others are not read and come out (and back) as zeros.  Any strides are
+    t < lengths[n] of the T dimension belong to sample n; what the others hold has no influence, and they come out (and back) as zeros.  Any strides are
     taken as they are, the channel dimension excepted.  time_major=True: the result is the same tensor, laid out in memory as
     [T, N, F, C] (the order the recurrent layers read)."""
     _act_tensor(x, "x")
