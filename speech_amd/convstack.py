@@ -328,7 +328,7 @@ def conv_stack_group(spec, cnn, blocks, f32=False, lengths=None):
     inside = None
     if lengths is not None:
         spec = spec.masked_fill(torch.arange(Tin, device=spec.device) >= lengths.view(B, 1, 1, 1), 0.0)
-        lengths = torch.clamp((lengths + 1) // 2, 0, T)
+        lengths = torch.clamp((lengths + 1) // 2, 0, T).int()
         inside = torch.arange(T, device=spec.device).view(1, 1, T, 1) < lengths.view(B, 1, 1, 1)
     chl = (F * T * C, T * C, C)
     if f32:

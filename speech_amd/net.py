@@ -334,7 +334,7 @@ class SRModel(nn.Module):
             # conv stack on the channel-last bf16 kernels -> [T', B, (F/2)*32], feature = f*32 + c
             x = convstack.conv_stack(x, self.cnn, list(self.resnet_layers), self.training)
         if self.rnn == "delta":
-            x, _ = self.delta_layers(x.to(cd), None if lengths is None else out_frames(lengths))
+            x, _ = self.delta_layers(x.to(cd), None if lengths is None else out_frames(lengths).int())
         else:
             x, _ = self.sru_layers(x.to(cd))
         ln = self.classifier[0]
@@ -386,6 +386,7 @@ def score_frames(lengths, labels, label_lengths, t_out):
     """int32 [B]: the encoder frames that CTC scores of utterances of `lengths` mel frames in a batch of t_out encoder frames.  Their own
     frames; all t_out where those are fewer than the transcript needs (its labels and a blank between equal neighbours): the loss
     would be infinite."""
+    labels, label_lengths = labels.to(lengths.device), label_lengths.to(lengths.device)
     own = torch.clamp(out_frames(lengths.long()), 0, t_out)
     n = label_lengths.view(-1, 1)
     twice = (labels[:, 1:] == labels[:, :-1]) & (torch.arange(1, max(1, labels.shape[1]), device=labels.device) < n)

@@ -369,6 +369,7 @@ def test_ctc_scores_own_frames(cuda):
     with torch.no_grad():
         logits = m(spec, lengths).double().cpu()
         loss = m.ctc_loss(spec, labels, ll.int(), lengths=lengths)
+        assert torch.equal(loss, m.ctc_loss(spec, labels.cpu(), ll.int().cpu(), lengths=lengths))      # labels from wherever they are
     own = net.score_frames(lengths, labels, ll, logits.shape[1]).cpu()
     assert own.tolist() == [45, 31, 20, 45]
     want = torch.nn.functional.ctc_loss(logits.log_softmax(-1).transpose(0, 1), labels.cpu(), own.long(), ll.cpu(), 0, "mean")
