@@ -465,3 +465,29 @@ def test_delta_non_finite_values_stay_in_their_head(cuda, dtype, bad, T, at, tra
     p, e, _ = run(2, (at, 1, 0, 7))
     cols = [c for c in range(24) if c != 7]
     assert torch.equal(p[..., cols], o[..., cols]) and torch.equal(e[..., cols], f[..., cols])
+
+
+@pytest.mark.parametrize("norm,rnn", [("group", "sru"), ("batch", "delta")])
+def test_mixed_variants_take_lengths(cuda, norm, rnn):
+    """Group norm in front of SRU layers clears the padding; delta layers behind BatchNorm walk own frames.  A training pass and an evaluation."""
+    from speech_amd import convstack, net, ops
+    torch.manual_seed(7)
+    m = net.SRModel(2, 64, 28, 80, 0.0, compute_dtype=torch.bfloat16, norm=norm, rnn=rnn).to(cuda)
+    lengths = torch.tensor([60, 31, 0], device=cuda)
+    labels, ll = torch.randint(1, 29, (3, 4), device=cuda), torch.tensor([4, 3, 0], dtype=torch.int32, device=cuda)
+    x = torch.rand(3, 1, 80, 60, device=cuda)
+    m.train()
+    loss = m.ctc_loss(x, labels, ll, lengths=lengths)
+    loss.backward()
+    assert torch.isfinite(loss) and all(torch.isfinite(p.grad).all() for p in m.parameters() if p.grad is not None)
+    m.eval()
+    with torch.no_grad():
+        got = m.encode(x, lengths)
+        if norm == "group":
+            dirty = x.clone()
+            dirty[1, :, :, 31:], dirty[2] = float("nan"), float("inf")
+            assert torch.equal(m.encode(dirty, lengths), got)
+        else:
+            h = convstack.conv_stack(x, m.cnn, list(m.resnet_layers), False).to(torch.bfloat16)
+            h, _ = m.delta_layers(h, torch.tensor([30, 16, 0], device=cuda))
+            assert torch.equal(ops.layer_norm(h, m.classifier[0].weight, m.classifier[0].bias, m.classifier[0].eps), got)
